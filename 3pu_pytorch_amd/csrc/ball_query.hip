@@ -84,7 +84,7 @@ extern "C" int tpu3_ball_query(tpu3_stream_t stream, int b, int n, int m, float 
     if (b > 65535) return TPU3_ELIMIT;
     hipStream_t s = (hipStream_t)stream;
     if (n == 0) {
-        const hipError_t e = hipMemsetAsync(idx, 0, (size_t)b * m * nsample * sizeof(int32_t), s);
+        const hipError_t e = tpu3_fill_u32(idx, 0, (size_t)b * m * nsample, s);
         return e == hipSuccess ? TPU3_OK : (int)e;
     }
     const dim3 g((m + BQ_WAVES - 1) / BQ_WAVES, b);

@@ -908,7 +908,7 @@ int tpu3_fps_cluster_launch(hipStream_t s, int b, int g, const void *fb_args, vo
     const size_t lds = fc_lds_bytes(a0.ntile, g);
     if (lds > 160 * 1024)
         return TPU3_ELIMIT;
-    hipError_t e = hipMemsetAsync(mbox, 0, (size_t)b * tpu3_fps_cluster_mailbox_bytes(g), s);
+    hipError_t e = tpu3_fill_u32(mbox, 0, (size_t)b * tpu3_fps_cluster_mailbox_bytes(g) / 4, s);
     if (e != hipSuccess)
         return (int)e;
     // (the per-phase cycle counters only when somebody asked for the statistics)

@@ -209,6 +209,21 @@ extern "C" int tpu3_denormalize_f32(tpu3_stream_t stream, long patches, int rows
     return tpu3_launch_status();
 }
 
+static __global__ __launch_bounds__(256) void fill_u32_kernel(uint32_t *__restrict__ p, uint32_t v, size_t words)
+{
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (size_t)gridDim.x * 256)
+        p[i] = v;
+}
+
+hipError_t tpu3_fill_u32(void *p, uint32_t v, size_t words, hipStream_t s)
+{
+    if (words == 0)
+        return hipSuccess;
+    const size_t blocks = (words + 255) / 256;
+    hipLaunchKernelGGL(fill_u32_kernel, dim3((unsigned)(blocks > 4096 ? 4096 : blocks)), dim3(256), 0, s, (uint32_t *)p, v, words);
+    return hipGetLastError();
+}
+
 extern "C" int tpu3_fill_f32_i32(tpu3_stream_t stream, float *a, long na, float va, int32_t *c, long nc, int32_t vc)
 {
     if (na < 0 || nc < 0 || (na > 0 && !a) || (nc > 0 && !c)) return TPU3_EINVAL;

@@ -2149,7 +2149,7 @@ extern "C" int tpu3_knn_graph_self_f32(tpu3_stream_t stream, int b, int n, int c
     const size_t need = tpu3_knn_unique_workspace_bytes(b, n);
     if (need == 0 || !workspace || workspace_bytes < need) return TPU3_EINVAL;
     hipStream_t s = (hipStream_t)stream;
-    hipError_t e = hipMemsetAsync(uws, 0, (size_t)TPU3_KNN_UWS_WORDS(groups) * sizeof(uint32_t), s);
+    hipError_t e = tpu3_fill_u32(uws, 0, (size_t)TPU3_KNN_UWS_WORDS(groups), s);
     if (e != hipSuccess) return (int)e;
     KnnArgs a{n, n, c, k, b, 1, x, x, nullptr, nullptr, nullptr, L.grp, dup, uws, 2, 0, idx, 0, nullptr};
     const int threads = kg_graph_threads(b, n);
@@ -2273,7 +2273,7 @@ extern "C" int tpu3_knn_unique_prepare_f32(tpu3_stream_t stream, int b, int m, i
     const int bp = L.pts_of ? L.bp : b;
     const int groups = L.grp ? L.groups : 1;
     if (bp < 0 || groups < 1) return TPU3_EINVAL;
-    hipError_t e = hipMemsetAsync(uws, 0, (size_t)TPU3_KNN_UWS_WORDS(groups) * sizeof(uint32_t), s);
+    hipError_t e = tpu3_fill_u32(uws, 0, (size_t)TPU3_KNN_UWS_WORDS(groups), s);
     if (e != hipSuccess) return (int)e;
     if (b == 0 || bp == 0 || n == 0) return TPU3_OK;
     if (!points) return TPU3_EINVAL;
@@ -2298,7 +2298,7 @@ extern "C" int tpu3_knn_unique_prepare_f32(tpu3_stream_t stream, int b, int m, i
         e = hipMallocAsync(&ws, need, s);
         if (e != hipSuccess) return (int)e;
     }
-    e = hipMemsetAsync(ws, 0xFF, need, s);
+    e = tpu3_fill_u32(ws, 0xFFFFFFFFu, need / 4, s);
     if (e != hipSuccess) return (int)e;
     const int nblk = (n + 255) / 256;
     const dim3 g((unsigned)((long)nblk * bp));

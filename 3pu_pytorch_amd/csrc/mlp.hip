@@ -1842,9 +1842,9 @@ extern "C" int tpu3_linear_wgrad_bias_f32(tpu3_stream_t stream, long m, int cin,
     if (!dw) return TPU3_EINVAL;
     hipStream_t s = (hipStream_t)stream;
     if (m == 0) {
-        hipError_t e = hipMemsetAsync(dw, 0, (size_t)cin * cout * sizeof(float), s);
+        hipError_t e = tpu3_fill_u32(dw, 0, (size_t)cin * cout, s);
         if (e == hipSuccess && db)
-            e = hipMemsetAsync(db, 0, (size_t)cout * sizeof(float), s);
+            e = tpu3_fill_u32(db, 0, (size_t)cout, s);
         return (int)e;
     }
     if (!x || !dy) return TPU3_EINVAL;
@@ -1981,7 +1981,7 @@ extern "C" int tpu3_linear_wgrad_f32(tpu3_stream_t stream, long m, int cin, int 
     if (!dw) return TPU3_EINVAL;
     hipStream_t s = (hipStream_t)stream;
     if (m == 0) {
-        const hipError_t e = hipMemsetAsync(dw, 0, (size_t)cin * cout * sizeof(float), s);
+        const hipError_t e = tpu3_fill_u32(dw, 0, (size_t)cin * cout, s);
         return (int)e;
     }
     if (!x || !dy) return TPU3_EINVAL;

@@ -547,7 +547,7 @@ int tpu3_nmdist_grid_forward(hipStream_t s, int b, int n, int m, const float *xy
     char *ws = nullptr;
     hipError_t err = hipMallocAsync((void **)&ws, total, s);
     if (err != hipSuccess) return (int)err;
-    err = hipMemsetAsync(ws, 0, zero_bytes, s);
+    err = tpu3_fill_u32(ws, 0, zero_bytes / 4, s);
     if (err != hipSuccess) { (void)hipFreeAsync(ws, s); return (int)err; }
     a.bbox = (uint32_t *)(ws + o_bbox);
     a.sbox = (uint32_t *)(ws + o_sbox);

@@ -277,7 +277,7 @@ int nm_dir(hipStream_t s, int b, int n, int m, const float *a, const float *bb, 
         unsigned long long *packed = nullptr;
         hipError_t e = hipMallocAsync((void **)&packed, (size_t)total * 8, s);
         if (e != hipSuccess) return (int)e;
-        e = hipMemsetAsync(packed, 0xFF, (size_t)total * 8, s);
+        e = tpu3_fill_u32(packed, 0xFFFFFFFFu, (size_t)total * 2, s);
         if (e != hipSuccess) return (int)e;
         const dim3 g((n + NM_THREADS * 4 - 1) / (NM_THREADS * 4), (unsigned)splits, b);
         hipLaunchKernelGGL(nmdist_fwd_split_kernel<4>, g, dim3(NM_THREADS), 0, s, n, m, chunk, a, bb, packed);

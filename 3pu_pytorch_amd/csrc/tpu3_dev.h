@@ -228,3 +228,7 @@ static inline int tpu3_launch_status()
 {
     return (int)hipGetLastError();
 }
+
+// p[0 .. words) = v by a kernel (glue.hip).  Every clear that a caller may capture into a graph goes through it: memset
+// nodes of a captured graph have given wrong results on replays after the first.
+hipError_t tpu3_fill_u32(void *p, uint32_t v, size_t words, hipStream_t s);
