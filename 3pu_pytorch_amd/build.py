@@ -14,8 +14,11 @@ OBJ = os.path.join(HERE, "objs")       # per-file objects (git-ignored)
 # -ffp-contract=off: every fused multiply-add in the kernels is an explicit fmaf(), so the
 #   arithmetic is the oracle's operation for operation (bit-exact indices).
 # -munsafe-fp-atomics: fp32 atomicAdd lowers to the hardware global_atomic_add_f32.
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 (hipcc forms them from scalar and float2 code by itself; some of their
+#   forms have given wrong results now and then, without an error).
 HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
-               "-ffp-contract=off", "-munsafe-fp-atomics", "-Wall", "-Wno-unused-function"]
+               "-ffp-contract=off", "-munsafe-fp-atomics", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+               "-Wall", "-Wno-unused-function"]
 
 
 def sources():
