@@ -21,6 +21,19 @@ class KnnLayout(ctypes.Structure):
                 ("tile_pts", _vp), ("tile_idx", _vp), ("tile_box", _vp)]
 
 
+class Heads(ctypes.Structure):
+    """tpu3_heads (include/tpu3.h)."""
+    _fields_ = [("data", _vp), ("sb", ctypes.c_int64), ("sr", ctypes.c_int64), ("sh", ctypes.c_int64), ("heads", _i)]
+
+
+class Positions(ctypes.Structure):
+    """tpu3_positions (include/tpu3.h)."""
+    _fields_ = [("data", _vp), ("sb", ctypes.c_int64), ("sr", ctypes.c_int64), ("sa", ctypes.c_int64), ("type", _i),
+                ("axes", _i), ("pairs", _i), ("freq", _vp), ("freq_type", _i)]
+
+
+_hp, _pp = ctypes.POINTER(Heads), ctypes.POINTER(Positions)
+
 # name -> (restype, argtypes); exactly the functions include/tpu3.h declares
 SIGNATURES = {
     "tpu3_version": (ctypes.c_char_p, []),
@@ -107,7 +120,23 @@ SIGNATURES = {
     "tpu3_dense_edge_conv_pk_f32": (_i, [_vp, _i, _i, _i, _vp, _vp, _i, _i, _i, _vp, _vp, _i]),
     "tpu3_dense_edge_conv_fold_pk_f32": (_i, [_vp, _i, _i, _i, _vp, _vp, _i, _i, _i, _vp, _vp, _i, _i, _vp, _vp, _i, _i,
                                               _i, _vp]),
+    "tpu3_norm_rotate_fwd": (_i, [_vp, _i, _i, _i, _i, _hp, _hp, _vp, _i, _vp, _i, _i, _pp, _f, _i, _vp, _vp]),
+    "tpu3_norm_rotate_bwd": (_i, [_vp, _i, _i, _i, _i, _hp, _hp, _vp, _i, _vp, _i, _i, _pp, _f, _i, _hp, _hp, _vp, _vp, _vp,
+                                  _vp, _vp, _sz]),
+    "tpu3_norm_rotate_bwd_workspace_bytes": (_sz, [_i, _i, _i]),
+    "tpu3_block_means": (_i, [_vp, _i, _i, _i, _i, _hp, _vp, _i, _vp]),
+    "tpu3_block_select": (_i, [_vp, _i, _i, _i, _i, _i, _hp, _i, _vp, _vp, _vp, _i, _i, _vp, _vp, _sz]),
+    "tpu3_block_select_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "tpu3_block_attn_fwd": (_i, [_vp, _i, _i, _i, _i, _i, _hp, _hp, _hp, _vp, _i, _f, _vp, _vp, _i, _vp, _vp, _vp, _sz]),
+    "tpu3_block_attn_fwd_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
+    "tpu3_block_attn_bwd": (_i, [_vp, _i, _i, _i, _i, _i, _hp, _hp, _hp, _hp, _hp, _vp, _i, _f, _vp, _vp, _i, _vp, _vp, _vp,
+                                 _vp, _vp, _sz]),
+    "tpu3_block_attn_bwd_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
 }
+
+TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}                                  # TPU3_TYPE_*
+POSITION_TYPES = {torch.float32: 0, torch.float64: 1, torch.int32: 2, torch.int64: 3}            # TPU3_POS_*
+ATTN_BLOCK, BLOCK_COUNT_MAX, ATTN_BLOCKS_MAX = 64, 64, 65536
 
 MFMA_F32, MFMA_F16 = 0, 1        # TPU3_MFMA_* of include/tpu3.h
 STORE_F32, STORE_F16 = 0, 1      # TPU3_STORE_* of include/tpu3.h

@@ -1,0 +1,978 @@
+// block_attn.hip -- softmax attention of every query over the blocks of 64 keys that were picked for it, and its gradient.
+//
+//   x_ij = scale q_i . k_j  over the live keys j of the picked blocks (causal: j <= n - m + i),
+//   p_ij = exp(x_ij) / sum_j exp(x_ij),   o_i = sum_j p_ij v_j,   nothing to see: o_i = 0
+//   dv_j = sum_i p_ij do_i,   ds_ij = p_ij (do_i . v_j - do_i . o_i),   dq_i = scale sum_j ds_ij k_j,
+//   dk_j = scale sum_i ds_ij q_i
+//
+// Forward and dq: a workgroup takes 64 rows = 64 / group queries of one key head with all heads of the group (they share
+// the picked blocks), forms the UNION of the rows' blocks in LDS with one bit per query, and runs over it once, with the
+// running maximum and sum of the softmax.  A block that no row of a wave picked is skipped by that wave; the mask of the
+// others costs a select a score.  Queries that are near each other pick nearly the same blocks -- points in a spatial
+// order, tokens in a sequence, the heads of a group always -- so the union is a few blocks larger than one query's set,
+// and a block's keys and values are read once for 64 rows.
+// dk, dv: a workgroup per block of keys gathers the rows that picked it (a bit matrix, blocks by queries, written by
+// block_pick_bits_kernel) and runs over them densely.  Nothing is added up with atomics: results do not depend on the order
+// in which workgroups run.
+//
+// Matrix instructions: 16x16x32 on the 16-bit types, 16x16x4 on fp32 (eight of them per 32 channels); accumulators, the
+// softmax and all sums in fp32.  Scores are formed transposed (keys x rows): a lane then holds 16 scores of ONE row, the
+// row's maximum is 15 register operations and two lane exchanges, and the probabilities already sit where the second
+// product wants its B operand -- the order of the 32 keys inside an instruction is free as long as both operands agree.
+// The transposed operand of that product comes out of the row-major LDS tile through the transposing LDS read.
+#include "heads.h"
+
+namespace {
+
+constexpr int BA_BLOCK = TPU3_ATTN_BLOCK;
+constexpr int BA_THREADS = 256;
+constexpr int BA_ROWS = 64;                 // rows of a workgroup, 16 a wave
+
+struct BaArgs {
+    tpu3_heads q, k, v, o, go;              // o, go: backward
+    const int32_t *blocks;                  // (b, m, hk, count)
+    const int32_t *n_arr, *m_arr;
+    void *out, *out2;                       // forward: o; dq pass: dq; dk / dv pass: dk, dv (contiguous)
+    float *lse;                             // (b, hq, m): log2 of the softmax denominator, scaled scores in base 2
+    float *delta;                           // (b, hq, m): do . o
+    float *gmax;                            // (b, hq, m): largest |do| of the row
+    uint64_t *bits;                         // (b, hk, nb, mt): bit = query of the tile of 64 picked the block
+    float *part;                            // split forward: (rows, splits, d + 2)
+    int b, m, n, nb, mt, hq, hk, group, d, count, causal, splits, tiles, qt, cap;
+    float scale, scale2;                    // scale2 = scale * log2(e)
+};
+
+typedef short ba_s4 __attribute__((ext_vector_type(4)));
+
+// ---- operands ----------------------------------------------------------------------------------------------------------
+template <typename T> __device__ __forceinline__ hd_f4 ba_mma(const typename hd_vec<T>::v8 &a, const typename hd_vec<T>::v8 &b, hd_f4 c);
+template <> __device__ __forceinline__ hd_f4 ba_mma<__bf16>(const hd_bf8 &a, const hd_bf8 &b, hd_f4 c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ hd_f4 ba_mma<_Float16>(const hd_h8 &a, const hd_h8 &b, hd_f4 c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ hd_f4 ba_mma<float>(const hd_f8 &a, const hd_f8 &b, hd_f4 c)
+{
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], c, 0, 0, 0);
+    return c;
+}
+
+template <typename T> __device__ __forceinline__ typename hd_vec<T>::v8 ba_zero()
+{
+    typename hd_vec<T>::v8 z;
+    __builtin_memset(&z, 0, sizeof(z));
+    return z;
+}
+
+// LDS rows are padded by 16 bytes (BA_PAD channels): 16 lanes that read 16 bytes of 16 consecutive rows then touch 64
+// different banks for rows of 64, 128 and 256 bytes.
+template <typename T> struct BaPad { static constexpr int v = 16 / sizeof(T); };
+
+// A operand, transposed: lane (l15, g) gets channel c0 + l15 of the rows r0 + g*4 + {0..3} and r0 + 16 + g*4 + {0..3}
+template <typename T, int STRIDE> __device__ __forceinline__ typename hd_vec<T>::v8 ba_column(const T *tile, int r0, int c0)
+{
+    const int lane = threadIdx.x & 63, g = lane >> 4, l15 = lane & 15;
+    typename hd_vec<T>::v8 f;
+    if constexpr (sizeof(T) == 4) {
+        const T *p = tile + (r0 + g * 4) * STRIDE + c0 + l15;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f.v[i] = p[i * STRIDE];
+            f.v[4 + i] = p[(16 + i) * STRIDE];
+        }
+    } else {
+        // 16 lanes read a 4 x 16 piece (8 bytes a lane) and receive its columns
+        typedef __attribute__((address_space(3))) ba_s4 lds_s4;
+        const T *p = tile + (r0 + g * 4 + (l15 >> 2)) * STRIDE + c0 + (l15 & 3) * 4;
+        union {
+            ba_s4 s[2];
+            typename hd_vec<T>::v8 v;
+        } u;
+        u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(p));
+        u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(p + 16 * STRIDE));
+        f = u.v;
+    }
+    return f;
+}
+
+template <typename T> __device__ __forceinline__ typename hd_vec<T>::v8 ba_pack(const hd_f4 &a, const hd_f4 &b)
+{
+    typename hd_vec<T>::v8 f;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            f.v[i] = a[i], f.v[4 + i] = b[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            f[i] = (T)a[i], f[4 + i] = (T)b[i];
+    }
+    return f;
+}
+
+template <typename T> __device__ __forceinline__ void ba_store4(T *p, const hd_f4 &x)
+{
+    typename hd_vec<T>::v4 y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        y[i] = (T)x[i];
+    *(typename hd_vec<T>::v4 *)p = y;
+}
+
+// maximum / sum over the four lane groups that hold a column (lanes l, l+16, l+32, l+48)
+__device__ __forceinline__ float ba_col_max(float v)
+{
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float ba_col_sum(float v)
+{
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
+}
+
+// ---- staging of a 64-row tile ------------------------------------------------------------------------------------------
+template <typename T, int DP> struct BaStage {
+    static constexpr int CHUNKS = DP / 8, PER = BA_ROWS * CHUNKS / BA_THREADS;      // 16-byte pieces of a thread
+    typename hd_vec<T>::v8 r[PER];
+    // rows [row0, row0 + 64) of one head; rows from `end` on and channels from d on read as zero
+    __device__ __forceinline__ void load(const T *base, int64_t stride, int row0, int end, int d)
+    {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int e = i * BA_THREADS + threadIdx.x, row = e / CHUNKS, c = (e % CHUNKS) * 8;
+            if (row0 + row < end && c < d)
+                r[i] = *(const typename hd_vec<T>::v8 *)(base + (int64_t)(row0 + row) * stride + c);
+            else
+                r[i] = ba_zero<T>();
+        }
+    }
+    // the tile with what is not finite as zero; `odd` collects the rows that hold such a value
+    __device__ __forceinline__ void store_finite(T *tile, unsigned long long *odd) const
+    {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int e = i * BA_THREADS + threadIdx.x, row = e / CHUNKS, c = (e % CHUNKS) * 8;
+            bool any = false;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+                const bool fin = fabsf((float)r[i][x]) <= 3.4028235e38f;
+                any |= !fin;
+                tile[row * (DP + BaPad<T>::v) + c + x] = fin ? (T)r[i][x] : (T)0.f;
+            }
+            if (any)
+                atomicOr(odd, 1ull << row);
+        }
+    }
+    __device__ __forceinline__ void store(T *tile) const
+    {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int e = i * BA_THREADS + threadIdx.x, row = e / CHUNKS, c = (e % CHUNKS) * 8;
+            *(typename hd_vec<T>::v8 *)(tile + row * (DP + BaPad<T>::v) + c) = r[i];
+        }
+    }
+};
+
+struct BaTile {                             // which rows a workgroup has
+    int b, h, i0, live, lm, z;              // sequence, key head, first query, live keys and queries, split
+};
+__device__ __forceinline__ BaTile ba_tile(const BaArgs &a, int64_t id)
+{
+    BaTile t;
+    t.z = (int)(id % a.splits);
+    id /= a.splits;
+    const int tile = (int)(id % a.tiles);
+    const int bh = (int)(id / a.tiles);
+    t.h = bh % a.hk;
+    t.b = bh / a.hk;
+    t.i0 = tile * a.qt;
+    t.live = a.n_arr ? min(max(a.n_arr[t.b], 0), a.n) : a.n;
+    t.lm = a.m_arr ? min(max(a.m_arr[t.b], 0), a.m) : a.m;
+    return t;
+}
+// workgroups are dealt to the eight XCDs in turn: give each XCD a contiguous range of ids, so that the tiles of a head,
+// which read the same keys, share an L2
+__device__ __forceinline__ int64_t ba_xcd(int64_t id, int64_t all)
+{
+    const int64_t per = all / 8, cut = per * 8;
+    return id < cut ? (id & 7) * per + (id >> 3) : id;
+}
+
+// keys that query i may see end here
+__device__ __forceinline__ int ba_limit(const BaArgs &a, int live, int lm, int i)
+{
+    if (i >= lm)
+        return 0;
+    return a.causal ? max(0, live - lm + i + 1) : live;
+}
+
+// The union of the blocks of the tile's queries, ascending, with the queries that picked each: list[u], mask[u], u < the
+// return value.  An index outside the live blocks, or behind what the query may see, is nobody's; one that a query names
+// twice counts once.
+__device__ int ba_union(const BaArgs &a, const BaTile &t, uint32_t *list, uint64_t *mask, uint32_t *words, uint32_t *before)
+{
+    __shared__ uint32_t wave_total[4];
+    const int nw = (a.nb + 31) / 32, entries = a.qt * a.count;
+    for (int w = threadIdx.x; w < nw; w += BA_THREADS)
+        words[w] = 0;
+    __syncthreads();
+    const int32_t *idx = a.blocks + (((int64_t)t.b * a.m + t.i0) * a.hk + t.h) * a.count;
+    auto entry = [&](int e, int &q) {
+        q = e / a.count;
+        const int i = t.i0 + q;
+        if (i >= t.lm)
+            return -1;
+        const int blk = idx[(int64_t)q * a.hk * a.count + (e - q * a.count)];
+        return blk >= 0 && blk < a.nb && blk * BA_BLOCK < ba_limit(a, t.live, t.lm, i) ? blk : -1;
+    };
+    for (int e = threadIdx.x; e < entries; e += BA_THREADS) {
+        int q;
+        const int blk = entry(e, q);
+        if (blk >= 0)
+            atomicOr(words + (blk >> 5), 1u << (blk & 31));
+    }
+    __syncthreads();
+    const int per = (nw + BA_THREADS - 1) / BA_THREADS, w0 = min(nw, (int)threadIdx.x * per), w1 = min(nw, w0 + per);
+    uint32_t mine = 0;
+    for (int w = w0; w < w1; ++w)
+        mine += __popc(words[w]);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t inc = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t v = __shfl_up(inc, o, 64);
+        inc += lane >= o ? v : 0u;
+    }
+    if (lane == 63)
+        wave_total[wave] = inc;
+    __syncthreads();
+    uint32_t at = inc - mine, total = 0;
+    for (int w = 0; w < 4; ++w) {
+        at += w < wave ? wave_total[w] : 0u;
+        total += wave_total[w];
+    }
+    for (int w = w0; w < w1; ++w) {
+        before[w] = at;
+        for (uint32_t bitsleft = words[w]; bitsleft; bitsleft &= bitsleft - 1) {
+            list[at] = (uint32_t)(w * 32 + __ffs((int)bitsleft) - 1);
+            mask[at++] = 0;
+        }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < entries; e += BA_THREADS) {
+        int q;
+        const int blk = entry(e, q);
+        if (blk >= 0) {
+            const uint32_t u = before[blk >> 5] + __popc(words[blk >> 5] & ((1u << (blk & 31)) - 1));
+            atomicOr((unsigned long long *)(mask + u), 1ull << q);
+        }
+    }
+    __syncthreads();
+    return (int)total;
+}
+
+template <typename T, int DP> struct BaLds {
+    static constexpr int STRIDE = DP + BaPad<T>::v;
+    static constexpr size_t TILE = (size_t)BA_ROWS * STRIDE * sizeof(T);
+};
+
+// the rows of this lane's column as B operands: channels kk*32 + g*8 .. +8 of row l15
+template <typename T, int DP>
+__device__ __forceinline__ void ba_row_operand(const T *p, bool live, int d, typename hd_vec<T>::v8 *f)
+{
+    const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int kk = 0; kk < DP / 32; ++kk) {
+        const int c = kk * 32 + g * 8;
+        f[kk] = live && c < d ? *(const typename hd_vec<T>::v8 *)(p + c) : ba_zero<T>();
+    }
+}
+
+// ---- forward -----------------------------------------------------------------------------------------------------------
+template <typename T, int DP>
+__global__ __launch_bounds__(BA_THREADS) void block_attn_fwd_kernel(BaArgs a, int64_t all)
+{
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    __shared__ unsigned long long odd;      // careful pass: rows of the tile that hold a value that is not finite
+    constexpr int STRIDE = BaLds<T, DP>::STRIDE;
+    T *Ks = (T *)smem, *Vs = (T *)(smem + BaLds<T, DP>::TILE);
+    uint64_t *mask = (uint64_t *)(smem + 2 * BaLds<T, DP>::TILE);
+    uint32_t *list = (uint32_t *)(mask + a.cap), *words = list + a.cap, *before = words + (a.nb + 31) / 32;
+
+    const int64_t id = ba_xcd(blockIdx.x, all);
+    const BaTile t = ba_tile(a, id);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
+    const int row = wave * 16 + l15, ql = row / a.group, hg = row - ql * a.group, i = t.i0 + ql;
+    const bool mine = ql < a.qt && i < t.lm;
+    const int head = t.h * a.group + hg;
+    const int limit = mine ? ba_limit(a, t.live, t.lm, i) : 0;
+
+    typename hd_vec<T>::v8 qf[DP / 32];
+    ba_row_operand<T, DP>((const T *)a.q.data + t.b * a.q.sb + (int64_t)i * a.q.sr + (int64_t)head * a.q.sh, mine, a.d, qf);
+    const int count = ba_union(a, t, list, mask, words, before);
+    const T *K = (const T *)a.k.data + t.b * a.k.sb + t.h * a.k.sh, *V = (const T *)a.v.data + t.b * a.v.sb + t.h * a.v.sh;
+
+    hd_f4 acc[DP / 16];
+    float top, sum;                         // running maximum of the column; this lane's share of its sum
+    // A value that is not finite, times the probability 0 of a row that does not see it, is not 0: in the matrix product it
+    // would reach every row of the wave.  A workgroup that ends with such an output runs a second, careful pass, which
+    // leaves these values out of the matrix product and adds them to the rows that see them one by one.
+    for (int careful = 0;; careful = 1) {
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c)
+            acc[c] = hd_f4{0.f, 0.f, 0.f, 0.f};
+        top = -INFINITY, sum = 0.f;
+
+        BaStage<T, DP> kr, vr;
+        if (t.z < count) {
+            const int r0 = (int)list[t.z] * BA_BLOCK;
+            kr.load(K, a.k.sr, r0, t.live, a.d);
+            vr.load(V, a.v.sr, r0, t.live, a.d);
+        }
+        for (int u = t.z; u < count; u += a.splits) {
+            const int k0 = (int)list[u] * BA_BLOCK;
+            const bool bit = mine && ((mask[u] >> ql) & 1);
+            __syncthreads();
+            kr.store(Ks);
+            if (careful) {
+                if (threadIdx.x == 0)
+                    odd = 0;
+                __syncthreads();
+                vr.store_finite(Vs, &odd);
+            } else {
+                vr.store(Vs);
+            }
+            __syncthreads();
+            if (u + a.splits < count) {
+                const int r0 = (int)list[u + a.splits] * BA_BLOCK;
+                kr.load(K, a.k.sr, r0, t.live, a.d);
+                vr.load(V, a.v.sr, r0, t.live, a.d);
+            }
+            if (!__any(bit))
+                continue;                   // (wave-uniform; the barriers are at the head of the loop)
+            hd_f4 s[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                s[x] = hd_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int kk = 0; kk < DP / 32; ++kk)
+                    s[x] = ba_mma<T>(*(const typename hd_vec<T>::v8 *)(Ks + (x * 16 + l15) * STRIDE + kk * 32 + g * 8), qf[kk], s[x]);
+            }
+            float mx = -INFINITY;
+            if (__any(bit && k0 + BA_BLOCK > limit)) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        s[x][r] = k0 + x * 16 + g * 4 + r < limit ? s[x][r] : -INFINITY;
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    mx = fmaxf(mx, s[x][r]);
+            mx = ba_col_max(mx) * a.scale2;
+            const float next = bit ? fmaxf(top, mx) : top;
+            const float base = next == -INFINITY ? 0.f : next;
+            const float keep = __builtin_amdgcn_exp2f(top - base);     // top = -inf: 0
+            top = next;
+            sum *= keep;
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][r], a.scale2, -base));
+                    s[x][r] = bit ? p : 0.f;
+                    sum += s[x][r];
+                }
+            if (__any(keep != 1.f)) {
+#pragma unroll
+                for (int c = 0; c < DP / 16; ++c)
+                    acc[c] *= keep;
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const typename hd_vec<T>::v8 pf = ba_pack<T>(s[2 * j], s[2 * j + 1]);
+#pragma unroll
+                for (int c = 0; c < DP / 16; ++c)
+                    acc[c] = ba_mma<T>(ba_column<T, STRIDE>(Vs, j * 32, c * 16), pf, acc[c]);
+            }
+            if (careful) {
+                for (unsigned long long left = odd; left; left &= left - 1) {
+                    const int kk = __ffsll(left) - 1;               // the key's place in the block: score register and lane group
+                    float p = 0.f;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            p = (kk >> 4) == x && (kk & 3) == r ? s[x][r] : p;
+                    p = __shfl(p, ((kk >> 2) & 3) * 16 + l15, 64);
+                    const bool sees = bit && k0 + kk < limit;
+#pragma unroll
+                    for (int c = 0; c < DP / 16; ++c)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int ch = c * 16 + g * 4 + r;
+                            const float val = sees && ch < a.d ? (float)V[(int64_t)(k0 + kk) * a.v.sr + ch] : 0.f;
+                            if (!(fabsf(val) <= 3.4028235e38f))
+                                acc[c][r] = __builtin_fmaf(p, val, acc[c][r]);
+                        }
+                }
+            }
+        }
+        bool finite = true;
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                finite &= fabsf(acc[c][r]) <= 3.4028235e38f;
+        if (careful || !__syncthreads_or(!finite))
+            break;
+    }
+    sum = ba_col_sum(sum);
+    const bool row_there = ql < a.qt && i < a.m;
+    if (!row_there)
+        return;
+    if (a.splits > 1) {
+        float *P = a.part + ((((int64_t)t.b * a.hq + head) * a.m + i) * a.splits + t.z) * (DP + 4);
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c)
+            *(hd_f4 *)(P + c * 16 + g * 4) = acc[c];
+        if (g == 0)
+            P[DP] = top, P[DP + 1] = sum;
+        return;
+    }
+    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
+    T *O = (T *)a.out + (((int64_t)t.b * a.m + i) * a.hq + head) * a.d;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c)
+        if (c * 16 + g * 4 < a.d)
+            ba_store4<T>(O + c * 16 + g * 4, acc[c] * inv);
+    if (a.lse && g == 0)
+        a.lse[((int64_t)t.b * a.hq + head) * a.m + i] = sum > 0.f ? top + log2f(sum) : -INFINITY;
+}
+
+// Joins the splits of a row: 16 lanes a row, each a few channels.
+template <typename T, int DP>
+__global__ __launch_bounds__(BA_THREADS) void block_attn_join_kernel(BaArgs a, int64_t rows)
+{
+    const int64_t row = (int64_t)blockIdx.x * (BA_THREADS / 16) + (threadIdx.x >> 4);
+    if (row >= rows)
+        return;
+    const int l = threadIdx.x & 15;
+    const float *P = a.part + row * a.splits * (DP + 4);
+    float top = -INFINITY;
+    for (int z = 0; z < a.splits; ++z)
+        top = fmaxf(top, P[z * (DP + 4) + DP]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, y[DP / 16] = {};
+    for (int z = 0; z < a.splits; ++z) {
+        const float *Z = P + z * (DP + 4);
+        const float f = __builtin_amdgcn_exp2f(Z[DP] - base);
+        sum = __builtin_fmaf(Z[DP + 1], f, sum);
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c)
+            y[c] = __builtin_fmaf(Z[l * (DP / 16) + c], f, y[c]);
+    }
+    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
+    const int64_t i = row % a.m, bh = row / a.m, h = bh % a.hq, b = bh / a.hq;
+    T *O = (T *)a.out + ((b * a.m + i) * a.hq + h) * a.d;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c)
+        if (l * (DP / 16) + c < a.d)
+            O[l * (DP / 16) + c] = (T)(y[c] * inv);
+    if (a.lse && l == 0)
+        a.lse[row] = sum > 0.f ? top + log2f(sum) : -INFINITY;
+}
+
+// ---- backward: dq, and the rows' do . o ----------------------------------------------------------------------------------
+// fp16: ds is scaled by a power of two that brings the row's largest |do| to [1, 2) before it is rounded, and the
+// accumulated row is scaled back: ds of a small gradient would fall below fp16's normal numbers otherwise.
+__device__ __forceinline__ float ba_pow2_inverse(float x)
+{
+    const int e = (int)((__float_as_uint(x) >> 23) & 255u);
+    return e == 0 || e >= 253 ? 1.f : __uint_as_float((uint32_t)(254 - e) << 23);
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(BA_THREADS) void block_attn_dq_kernel(BaArgs a, int64_t all)
+{
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    __shared__ unsigned long long odd;
+    constexpr int STRIDE = BaLds<T, DP>::STRIDE;
+    constexpr bool HALF = __is_same(T, _Float16);
+    T *Ks = (T *)smem, *Vs = (T *)(smem + BaLds<T, DP>::TILE);
+    uint64_t *mask = (uint64_t *)(smem + 2 * BaLds<T, DP>::TILE);
+    uint32_t *list = (uint32_t *)(mask + a.cap), *words = list + a.cap, *before = words + (a.nb + 31) / 32;
+
+    const int64_t id = ba_xcd(blockIdx.x, all);
+    const BaTile t = ba_tile(a, id);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
+    const int row = wave * 16 + l15, ql = row / a.group, hg = row - ql * a.group, i = t.i0 + ql;
+    const bool mine = ql < a.qt && i < t.lm;
+    const int head = t.h * a.group + hg;
+    const int limit = mine ? ba_limit(a, t.live, t.lm, i) : 0;
+    const int64_t at = ((int64_t)t.b * a.hq + head) * a.m + i;
+
+    typename hd_vec<T>::v8 qf[DP / 32], gf[DP / 32];
+    ba_row_operand<T, DP>((const T *)a.q.data + t.b * a.q.sb + (int64_t)i * a.q.sr + (int64_t)head * a.q.sh, mine, a.d, qf);
+    ba_row_operand<T, DP>((const T *)a.go.data + t.b * a.go.sb + (int64_t)i * a.go.sr + (int64_t)head * a.go.sh, mine, a.d, gf);
+    float delta = 0.f, gmax = 0.f;
+    {
+        typename hd_vec<T>::v8 of[DP / 32];
+        ba_row_operand<T, DP>((const T *)a.o.data + t.b * a.o.sb + (int64_t)i * a.o.sr + (int64_t)head * a.o.sh, mine, a.d, of);
+#pragma unroll
+        for (int kk = 0; kk < DP / 32; ++kk)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                delta = __builtin_fmaf((float)gf[kk][c], (float)of[kk][c], delta);
+                gmax = fmaxf(gmax, fabsf((float)gf[kk][c]));
+            }
+    }
+    delta = ba_col_sum(delta);
+    const float lse = mine ? a.lse[at] : 0.f;
+    float up = 1.f;
+    if (HALF) {
+        gmax = ba_col_max(gmax);
+        up = ba_pow2_inverse(gmax);
+    }
+    if (mine && g == 0) {
+        a.delta[at] = delta;
+        if (HALF)
+            a.gmax[at] = gmax;
+    }
+    const int count = ba_union(a, t, list, mask, words, before);
+    const T *K = (const T *)a.k.data + t.b * a.k.sb + t.h * a.k.sh, *V = (const T *)a.v.data + t.b * a.v.sb + t.h * a.v.sh;
+    hd_f4 acc[DP / 16];
+    // as in the forward kernel: a second, careful pass where a key that is not finite may have reached rows that do not see
+    // it; those that do are not numbers
+    bool poison = false;
+    for (int careful = 0;; careful = 1) {
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c)
+            acc[c] = hd_f4{0.f, 0.f, 0.f, 0.f};
+        BaStage<T, DP> kr, vr;
+        if (count > 0) {
+            const int r0 = (int)list[0] * BA_BLOCK;
+            kr.load(K, a.k.sr, r0, t.live, a.d);
+            vr.load(V, a.v.sr, r0, t.live, a.d);
+        }
+        for (int u = 0; u < count; ++u) {
+            const int k0 = (int)list[u] * BA_BLOCK;
+            const bool bit = mine && ((mask[u] >> ql) & 1);
+            __syncthreads();
+            vr.store(Vs);
+            if (careful) {
+                if (threadIdx.x == 0)
+                    odd = 0;
+                __syncthreads();
+                kr.store_finite(Ks, &odd);
+            } else {
+                kr.store(Ks);
+            }
+            __syncthreads();
+            if (careful && bit)
+                poison |= (odd & (limit - k0 >= BA_BLOCK ? ~0ull : (1ull << max(0, limit - k0)) - 1)) != 0;
+            if (u + 1 < count) {
+                const int r0 = (int)list[u + 1] * BA_BLOCK;
+                kr.load(K, a.k.sr, r0, t.live, a.d);
+                vr.load(V, a.v.sr, r0, t.live, a.d);
+            }
+            if (!__any(bit))
+                continue;
+            hd_f4 s[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                hd_f4 p = {0.f, 0.f, 0.f, 0.f}, dp = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int kk = 0; kk < DP / 32; ++kk) {
+                    const int off = (x * 16 + l15) * STRIDE + kk * 32 + g * 8;
+                    p = ba_mma<T>(*(const typename hd_vec<T>::v8 *)(Ks + off), qf[kk], p);
+                    dp = ba_mma<T>(*(const typename hd_vec<T>::v8 *)(Vs + off), gf[kk], dp);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(p[r], a.scale2, -lse)) * (dp[r] - delta);
+                    s[x][r] = bit && k0 + x * 16 + g * 4 + r < limit ? (HALF ? e * up : e) : 0.f;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const typename hd_vec<T>::v8 sf = ba_pack<T>(s[2 * j], s[2 * j + 1]);
+#pragma unroll
+                for (int c = 0; c < DP / 16; ++c)
+                    acc[c] = ba_mma<T>(ba_column<T, STRIDE>(Ks, j * 32, c * 16), sf, acc[c]);
+            }
+        }
+        bool finite = true;
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                finite &= fabsf(acc[c][r]) <= 3.4028235e38f;
+        if (careful || !__syncthreads_or(!finite))
+            break;
+    }
+    if (!(ql < a.qt && i < a.m))
+        return;
+    T *O = (T *)a.out + (((int64_t)t.b * a.m + i) * a.hq + head) * a.d;
+    const float back = poison ? NAN : HALF ? a.scale / up : a.scale;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c)
+        if (c * 16 + g * 4 < a.d)
+            ba_store4<T>(O + c * 16 + g * 4, acc[c] * back);
+}
+
+// ---- backward: which queries picked a block ------------------------------------------------------------------------------
+// bits[(b, h, blk), tile of 64 queries]: a workgroup per (sequence, key head, tile) collects the tile's words in LDS.
+constexpr int BP_WORDS = 2048;
+__global__ __launch_bounds__(BA_THREADS) void block_pick_bits_kernel(BaArgs a)
+{
+    __shared__ unsigned long long w[BP_WORDS];
+    const int tile = (int)(blockIdx.x % a.mt), bh = (int)(blockIdx.x / a.mt), h = bh % a.hk, b = bh / a.hk;
+    const int live = a.n_arr ? min(max(a.n_arr[b], 0), a.n) : a.n, lm = a.m_arr ? min(max(a.m_arr[b], 0), a.m) : a.m;
+    const int i0 = tile * 64, entries = min(64, a.m - i0) * a.count;
+    const int32_t *idx = a.blocks + (((int64_t)b * a.m + i0) * a.hk + h) * a.count;
+    for (int b0 = 0; b0 < a.nb; b0 += BP_WORDS) {
+        const int words = min(BP_WORDS, a.nb - b0);
+        for (int x = threadIdx.x; x < words; x += BA_THREADS)
+            w[x] = 0;
+        __syncthreads();
+        for (int e = threadIdx.x; e < entries; e += BA_THREADS) {
+            const int q = e / a.count, blk = idx[(int64_t)q * a.hk * a.count + (e - q * a.count)];
+            if (blk >= b0 && blk < b0 + words && blk * BA_BLOCK < ba_limit(a, live, lm, i0 + q))
+                atomicOr(w + (blk - b0), 1ull << q);
+        }
+        __syncthreads();
+        for (int x = threadIdx.x; x < words; x += BA_THREADS)
+            a.bits[((int64_t)bh * a.nb + b0 + x) * a.mt + tile] = w[x];
+        __syncthreads();
+    }
+}
+
+// ---- backward: dk, dv ----------------------------------------------------------------------------------------------------
+// A workgroup per block of keys; a wave owns 16 of its keys.  Scores are formed as rows x keys here, so that P and dS come
+// out with a key per lane: the B operand of dv^T = do^T P and dk^T = q^T dS.
+constexpr int BD_WORDS = 64;                // tiles of queries looked through at a time
+
+template <typename T, int DP> struct BaDkv {
+    static constexpr int STRIDE = BaLds<T, DP>::STRIDE;
+    T *Qs, *Gs;
+    float *lse, *delta, *gmax;
+    int *limit, *list;
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__(BA_THREADS) void block_attn_dkv_kernel(BaArgs a, int64_t all)
+{
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    __shared__ int wave_total[4];
+    constexpr int STRIDE = BaLds<T, DP>::STRIDE;
+    constexpr bool HALF = __is_same(T, _Float16);
+    T *Qs = (T *)smem, *Gs = (T *)(smem + BaLds<T, DP>::TILE);
+    float *lse_s = (float *)(smem + 2 * BaLds<T, DP>::TILE), *delta_s = lse_s + 64, *gmax_s = delta_s + 64;
+    int *limit_s = (int *)(gmax_s + 64), *list = limit_s + 64;              // list: BD_WORDS * 64 queries
+
+    const int64_t id = ba_xcd(blockIdx.x, all);
+    const int blk = (int)(id % a.nb), bh = (int)(id / a.nb), h = bh % a.hk, b = bh / a.hk;
+    const int live = a.n_arr ? min(max(a.n_arr[b], 0), a.n) : a.n, lm = a.m_arr ? min(max(a.m_arr[b], 0), a.m) : a.m;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
+    const int key = blk * BA_BLOCK + wave * 16 + l15;
+    typename hd_vec<T>::v8 kf[DP / 32], vf[DP / 32];
+    ba_row_operand<T, DP>((const T *)a.k.data + b * a.k.sb + (int64_t)key * a.k.sr + h * a.k.sh, key < live, a.d, kf);
+    ba_row_operand<T, DP>((const T *)a.v.data + b * a.v.sb + (int64_t)key * a.v.sr + h * a.v.sh, key < live, a.d, vf);
+    hd_f4 dk[DP / 16], dv[DP / 16];
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c)
+        dk[c] = dv[c] = hd_f4{0.f, 0.f, 0.f, 0.f};
+    float up = 1.f;                         // fp16: dk is accumulated times this power of two
+    bool first = true;
+    const uint64_t *bits = a.bits + ((int64_t)bh * a.nb + blk) * a.mt;
+
+    for (int w0 = 0; w0 < a.mt; w0 += BD_WORDS) {
+        // the queries of the next 64 tiles that picked this block, in order
+        const int words = min(BD_WORDS, a.mt - w0);
+        uint64_t word = 0;
+        int at = 0, total = 0;
+        if (wave == 0) {
+            word = lane < words ? bits[w0 + lane] : 0ull;
+            int inc = __popcll(word);
+            at = -inc;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int v = __shfl_up(inc, o, 64);
+                inc += lane >= o ? v : 0;
+            }
+            at += inc;
+            if (lane == 63)
+                wave_total[0] = inc;
+            for (; word; word &= word - 1)
+                list[at++] = (w0 + lane) * 64 + __ffsll((unsigned long long)word) - 1;
+        }
+        __syncthreads();
+        total = wave_total[0];
+        const int rows = total * a.group;
+        for (int r0 = 0; r0 < rows; r0 += BA_ROWS) {
+            constexpr int CHUNKS = DP / 8, PER = BA_ROWS * CHUNKS / BA_THREADS;
+            typename hd_vec<T>::v8 qr[PER], gr[PER];
+#pragma unroll
+            for (int x = 0; x < PER; ++x) {
+                const int e = x * BA_THREADS + threadIdx.x, r = r0 + e / CHUNKS, c = (e % CHUNKS) * 8;
+                if (r < rows && c < a.d) {
+                    const int q = r / a.group, head = h * a.group + (r - q * a.group);
+                    const int64_t i = list[q];
+                    qr[x] = *(const typename hd_vec<T>::v8 *)((const T *)a.q.data + b * a.q.sb + i * a.q.sr + (int64_t)head * a.q.sh + c);
+                    gr[x] = *(const typename hd_vec<T>::v8 *)((const T *)a.go.data + b * a.go.sb + i * a.go.sr + (int64_t)head * a.go.sh + c);
+                } else {
+                    qr[x] = ba_zero<T>();
+                    gr[x] = ba_zero<T>();
+                }
+            }
+            float row_lse = 0.f, row_delta = 0.f, row_gmax = 0.f;
+            int row_limit = 0;
+            if (threadIdx.x < BA_ROWS && r0 + (int)threadIdx.x < rows) {
+                const int r = r0 + threadIdx.x, q = r / a.group, head = h * a.group + (r - q * a.group), i = list[q];
+                const int64_t p = ((int64_t)b * a.hq + head) * a.m + i;
+                row_lse = a.lse[p], row_delta = a.delta[p], row_limit = ba_limit(a, live, lm, i);
+                if (HALF)
+                    row_gmax = a.gmax[p];
+            }
+            __syncthreads();                // the previous tile has been read
+#pragma unroll
+            for (int x = 0; x < PER; ++x) {
+                const int e = x * BA_THREADS + threadIdx.x, r = e / CHUNKS, c = (e % CHUNKS) * 8;
+                *(typename hd_vec<T>::v8 *)(Qs + r * STRIDE + c) = qr[x];
+                *(typename hd_vec<T>::v8 *)(Gs + r * STRIDE + c) = gr[x];
+            }
+            if (threadIdx.x < BA_ROWS) {
+                lse_s[threadIdx.x] = row_lse, delta_s[threadIdx.x] = row_delta, limit_s[threadIdx.x] = row_limit;
+                if (HALF)
+                    gmax_s[threadIdx.x] = row_gmax;
+            }
+            __syncthreads();
+            if (HALF) {
+                // the largest |do| of the rows so far decides the power of two (every wave finds the same)
+                float m = gmax_s[lane];
+#pragma unroll
+                for (int o = 32; o > 0; o >>= 1)
+                    m = fmaxf(m, __shfl_xor(m, o, 64));
+                const float want = ba_pow2_inverse(m);
+                if (m > 0.f && (first || want < up)) {
+                    if (!first)
+#pragma unroll
+                        for (int c = 0; c < DP / 16; ++c)
+                            dk[c] *= want / up;
+                    up = want;
+                    first = false;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {   // 32 rows at a time
+                hd_f4 p[2], ds[2];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    hd_f4 s = {0.f, 0.f, 0.f, 0.f}, dp = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int kk = 0; kk < DP / 32; ++kk) {
+                        const int off = (j * 32 + x * 16 + l15) * STRIDE + kk * 32 + g * 8;
+                        s = ba_mma<T>(*(const typename hd_vec<T>::v8 *)(Qs + off), kf[kk], s);
+                        dp = ba_mma<T>(*(const typename hd_vec<T>::v8 *)(Gs + off), vf[kk], dp);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int rr = j * 32 + x * 16 + g * 4 + r;
+                        const bool see = key < limit_s[rr];
+                        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.scale2, -lse_s[rr]));
+                        const float f = e * (dp[r] - delta_s[rr]);
+                        p[x][r] = see ? e : 0.f;
+                        ds[x][r] = see ? (HALF ? f * up : f) : 0.f;
+                    }
+                }
+                const typename hd_vec<T>::v8 pf = ba_pack<T>(p[0], p[1]), sf = ba_pack<T>(ds[0], ds[1]);
+#pragma unroll
+                for (int c = 0; c < DP / 16; ++c) {
+                    dv[c] = ba_mma<T>(ba_column<T, STRIDE>(Gs, j * 32, c * 16), pf, dv[c]);
+                    dk[c] = ba_mma<T>(ba_column<T, STRIDE>(Qs, j * 32, c * 16), sf, dk[c]);
+                }
+            }
+        }
+        __syncthreads();                    // the list is rebuilt
+    }
+    if (key >= a.n)
+        return;
+    const int64_t at = (((int64_t)b * a.n + key) * a.hk + h) * a.d;
+    const float back = HALF ? a.scale / up : a.scale;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c)
+        if (c * 16 + g * 4 < a.d) {
+            ba_store4<T>((T *)a.out + at + c * 16 + g * 4, dk[c] * back);
+            ba_store4<T>((T *)a.out2 + at + c * 16 + g * 4, dv[c]);
+        }
+}
+
+// ---- host --------------------------------------------------------------------------------------------------------------
+int ba_fill(BaArgs &a, int type, int b, int m, int n, int d, const tpu3_heads *q, const tpu3_heads *k, const tpu3_heads *v,
+            const int32_t *blocks, int count, float scale, const int32_t *n_arr, const int32_t *m_arr, int causal)
+{
+    if (b < 0 || m < 0 || n < 0 || d <= 0 || !hd_type_ok(type) || !q || !k || !v || q->heads <= 0 || k->heads <= 0 ||
+        q->heads % k->heads || v->heads != k->heads || count <= 0 || !(scale > 0.f) || scale > 3e38f)
+        return TPU3_EINVAL;
+    if (d % 8 || d > 128 || count > TPU3_BLOCK_COUNT_MAX || q->heads / k->heads > BA_ROWS ||
+        (n > 0 && (n - 1) / BA_BLOCK + 1 > TPU3_ATTN_BLOCKS_MAX))
+        return TPU3_ELIMIT;
+    a.q = *q, a.k = *k, a.v = *v, a.blocks = blocks, a.n_arr = n_arr, a.m_arr = m_arr;
+    a.b = b, a.m = m, a.n = n, a.nb = n > 0 ? (n - 1) / BA_BLOCK + 1 : 0, a.mt = (m + 63) / 64;
+    a.hq = q->heads, a.hk = k->heads, a.group = a.hq / a.hk, a.d = d, a.count = count, a.causal = causal != 0;
+    a.scale = scale, a.scale2 = scale * 1.44269504088896340736f;
+    a.qt = BA_ROWS / a.group;
+    a.tiles = m > 0 ? (m - 1) / a.qt + 1 : 0;
+    a.cap = a.qt * count < a.nb ? a.qt * count : a.nb;
+    a.splits = 1;
+    if (b == 0 || m == 0)
+        return TPU3_OK;
+    if (!hd_rows_ok(q, type) || !blocks || (n > 0 && (!hd_rows_ok(k, type) || !hd_rows_ok(v, type))))
+        return TPU3_EINVAL;
+    if ((int64_t)b * a.hk * a.tiles > 0x7FFFFFFFLL / 64 || (int64_t)b * a.hk * a.nb > 0x7FFFFFFFLL || (int64_t)b * a.hk * a.mt > 0x7FFFFFFFLL)
+        return TPU3_ELIMIT;
+    return 1;
+}
+
+// Splits of a tile's blocks: where the tiles alone do not fill the chip (two workgroups a compute unit).
+int ba_splits(int b, int m, int n, int hq, int hk, int count)
+{
+    if (b <= 0 || m <= 0 || n <= 0 || hk <= 0 || hq < hk || count <= 0)
+        return 1;
+    const int qt = BA_ROWS / (hq / hk);
+    if (qt < 1)
+        return 1;
+    const int64_t tiles = (int64_t)b * hk * ((m - 1) / qt + 1);
+    const int64_t used = (int64_t)(m < qt ? m : qt) * count, nb = (n - 1) / BA_BLOCK + 1;
+    int64_t s = 512 / tiles, most = used < nb ? used : nb;
+    s = s < most ? s : most;
+    return s < 1 ? 1 : s > 64 ? 64 : (int)s;
+}
+
+int ba_dp(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
+
+size_t ba_lds(const BaArgs &a, size_t tile) { return 2 * tile + (size_t)a.cap * 12 + (size_t)((a.nb + 31) / 32) * 8; }
+
+template <typename K> int ba_allow(K kernel, size_t lds)
+{
+    return (int)hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+}
+
+template <typename T, int DP> int ba_forward(const BaArgs &a, hipStream_t s)
+{
+    const int64_t all = (int64_t)a.b * a.hk * a.tiles * a.splits;
+    const size_t lds = ba_lds(a, BaLds<T, DP>::TILE);
+    int rc = ba_allow(block_attn_fwd_kernel<T, DP>, lds);
+    if (rc)
+        return rc;
+    hipLaunchKernelGGL((block_attn_fwd_kernel<T, DP>), dim3((unsigned)all), dim3(BA_THREADS), lds, s, a, all);
+    if (a.splits > 1) {
+        const int64_t rows = (int64_t)a.b * a.hq * a.m, per = BA_THREADS / 16;
+        hipLaunchKernelGGL((block_attn_join_kernel<T, DP>), dim3((unsigned)((rows + per - 1) / per)), dim3(BA_THREADS), 0, s, a, rows);
+    }
+    return tpu3_launch_status();
+}
+
+template <typename T, int DP> int ba_backward(BaArgs a, void *dq, void *dk, void *dv, hipStream_t s)
+{
+    int rc = TPU3_OK;
+    // dq also leaves the rows' do . o for the pass over the keys
+    const int64_t all = (int64_t)a.b * a.hk * a.tiles;
+    const size_t lds = ba_lds(a, BaLds<T, DP>::TILE);
+    rc = ba_allow(block_attn_dq_kernel<T, DP>, lds);
+    if (rc)
+        return rc;
+    a.out = dq;
+    hipLaunchKernelGGL((block_attn_dq_kernel<T, DP>), dim3((unsigned)all), dim3(BA_THREADS), lds, s, a, all);
+    if (a.nb == 0)
+        return tpu3_launch_status();
+    hipLaunchKernelGGL(block_pick_bits_kernel, dim3((unsigned)(a.b * a.hk * a.mt)), dim3(BA_THREADS), 0, s, a);
+    const size_t lds2 = 2 * BaLds<T, DP>::TILE + 4 * 64 * 4 + (size_t)BD_WORDS * 64 * 4;
+    rc = ba_allow(block_attn_dkv_kernel<T, DP>, lds2);
+    if (rc)
+        return rc;
+    a.out = dk, a.out2 = dv;
+    const int64_t blocks = (int64_t)a.b * a.hk * a.nb;
+    hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP>), dim3((unsigned)blocks), dim3(BA_THREADS), lds2, s, a, blocks);
+    return tpu3_launch_status();
+}
+
+template <typename T> int ba_forward_d(const BaArgs &a, hipStream_t s)
+{
+    const int dp = ba_dp(a.d);
+    return dp == 32 ? ba_forward<T, 32>(a, s) : dp == 64 ? ba_forward<T, 64>(a, s) : ba_forward<T, 128>(a, s);
+}
+template <typename T> int ba_backward_d(const BaArgs &a, void *dq, void *dk, void *dv, hipStream_t s)
+{
+    const int dp = ba_dp(a.d);
+    return dp == 32 ? ba_backward<T, 32>(a, dq, dk, dv, s) : dp == 64 ? ba_backward<T, 64>(a, dq, dk, dv, s) : ba_backward<T, 128>(a, dq, dk, dv, s);
+}
+
+}  // namespace
+
+extern "C" size_t tpu3_block_attn_fwd_workspace_bytes(int b, int m, int n, int hq, int hk, int d, int count)
+{
+    const int s = ba_splits(b, m, n, hq, hk, count);
+    return s == 1 ? 0 : (size_t)b * m * hq * s * (ba_dp(d) + 4) * 4;
+}
+
+extern "C" int tpu3_block_attn_fwd(tpu3_stream_t stream, int type, int b, int m, int n, int d, const tpu3_heads *q,
+                                   const tpu3_heads *k, const tpu3_heads *v, const int32_t *blocks, int count, float scale,
+                                   const int32_t *n_arr, const int32_t *m_arr, int causal, void *out, float *lse,
+                                   void *workspace, size_t workspace_bytes)
+{
+    BaArgs a = {};
+    const int rc = ba_fill(a, type, b, m, n, d, q, k, v, blocks, count, scale, n_arr, m_arr, causal);
+    if (rc <= 0)
+        return rc;
+    if (!out || ((uintptr_t)out & 15))
+        return TPU3_EINVAL;
+    a.out = out, a.lse = lse;
+    a.splits = ba_splits(b, m, n, a.hq, a.hk, count);
+    if (a.splits > 1) {
+        if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < (size_t)b * m * a.hq * a.splits * (ba_dp(d) + 4) * 4)
+            return TPU3_EINVAL;
+        a.part = (float *)workspace;
+    }
+    const hipStream_t s = (hipStream_t)stream;
+    return type == TPU3_TYPE_F32 ? ba_forward_d<float>(a, s) : type == TPU3_TYPE_F16 ? ba_forward_d<_Float16>(a, s) : ba_forward_d<__bf16>(a, s);
+}
+
+extern "C" size_t tpu3_block_attn_bwd_workspace_bytes(int b, int m, int n, int hq, int hk)
+{
+    if (b <= 0 || m <= 0 || hq <= 0 || hk <= 0)
+        return 0;
+    const size_t nb = n > 0 ? (size_t)(n - 1) / BA_BLOCK + 1 : 0, mt = ((size_t)m + 63) / 64;
+    return (size_t)b * hk * nb * mt * 8 + (size_t)b * hq * m * 8;
+}
+
+extern "C" int tpu3_block_attn_bwd(tpu3_stream_t stream, int type, int b, int m, int n, int d, const tpu3_heads *q,
+                                   const tpu3_heads *k, const tpu3_heads *v, const tpu3_heads *o, const tpu3_heads *go,
+                                   const int32_t *blocks, int count, float scale, const int32_t *n_arr, const int32_t *m_arr,
+                                   int causal, const float *lse, void *dq, void *dk, void *dv, void *workspace,
+                                   size_t workspace_bytes)
+{
+    BaArgs a = {};
+    const int rc = ba_fill(a, type, b, m, n, d, q, k, v, blocks, count, scale, n_arr, m_arr, causal);
+    if (rc <= 0)
+        return rc;
+    if (!hd_rows_ok(o, type) || !hd_rows_ok(go, type) || o->heads != a.hq || go->heads != a.hq || !lse || !dq ||
+        ((uintptr_t)dq & 15) || (n > 0 && (!dk || !dv || ((uintptr_t)dk & 15) || ((uintptr_t)dv & 15))) || !workspace ||
+        ((uintptr_t)workspace & 7) || workspace_bytes < tpu3_block_attn_bwd_workspace_bytes(b, m, n, a.hq, a.hk))
+        return TPU3_EINVAL;
+    a.o = *o, a.go = *go, a.lse = (float *)lse;
+    a.bits = (uint64_t *)workspace;
+    a.delta = (float *)(a.bits + (size_t)b * a.hk * a.nb * a.mt);
+    a.gmax = a.delta + (size_t)b * a.hq * m;
+    const hipStream_t s = (hipStream_t)stream;
+    return type == TPU3_TYPE_F32 ? ba_backward_d<float>(a, dq, dk, dv, s) : type == TPU3_TYPE_F16 ? ba_backward_d<_Float16>(a, dq, dk, dv, s) : ba_backward_d<__bf16>(a, dq, dk, dv, s);
+}

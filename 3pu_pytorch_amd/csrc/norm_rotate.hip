@@ -1,0 +1,480 @@
+// norm_rotate.hip -- per-head RMS norm of queries and keys with the position rotation in the same pass, and its gradient.
+//
+//   r = 1 / sqrt(mean_c x_c^2 + eps),  u = x r,  y = u w,  then every pair (one, two) of the rotated channels turns by the
+//   angle position[axis] * freq[axis][f]:  (y_one c - y_two s,  y_one s + y_two c);  channels behind the pairs pass.
+//   Backward, with h = the gradient turned back by the same angle:
+//   dx = r (h w - u mean_c(h w u)),  dw = sum over rows of h u.
+//
+// Bound by memory: a row is read once and written once (backward: read twice, written once), ~20 flops a channel.  A lane
+// holds eight consecutive channels (one 16-byte access for the 16-bit types); 4 .. 32 lanes hold a row, so that the sums
+// of a row are a few lane exchanges.  The turns are shared by all heads of a token: a workgroup takes a few tokens,
+// computes their cosines and sines once into LDS and then runs over the tokens' rows.  Angles are formed and reduced in
+// 64 bits (a position of 1e5 times a frequency of 1 leaves 7 of fp32's 24 bits for the fraction of a turn), the sine and
+// cosine of the fraction in 32.  The partner of a channel in the half-split order sits in another lane: the normed row
+// goes through the workgroup's LDS (four times the HBM bytes, at an aggregate LDS rate of ten times HBM's).
+#include "heads.h"
+
+namespace {
+
+constexpr int NR_THREADS = 256;
+constexpr int NR_MAX_WG = 1024;             // backward: persistent workgroups, one partial weight gradient each
+
+struct NrArgs {
+    tpu3_heads x[2];                        // queries, keys (heads 0: none)
+    tpu3_heads g[2];                        // backward: gradients of the outputs
+    const void *w[2];
+    int w_head[2];                          // channels between two heads' weights (0: one set for all heads)
+    void *out[2];                           // contiguous (b, n, heads, d)
+    float *part;                            // backward: (workgroups, rows of weights, d)
+    int want_w[2];
+    const void *pos, *freq;
+    int64_t pos_sb, pos_sn, pos_sa;
+    int64_t tokens;
+    int n, d, axes, pairs, total_pairs, w_type, pos_type, freq_type, interleaved, tok;
+    float eps, inv_d;
+};
+
+__device__ __forceinline__ float nr_weight(const void *w, int type, int i)
+{
+    if (type == TPU3_TYPE_F32)
+        return ((const float *)w)[i];
+    if (type == TPU3_TYPE_F16)
+        return (float)((const _Float16 *)w)[i];
+    return (float)((const __bf16 *)w)[i];
+}
+__device__ __forceinline__ double nr_position(const void *p, int type, int64_t i)
+{
+    if (type == TPU3_POS_F32)
+        return (double)((const float *)p)[i];
+    if (type == TPU3_POS_F64)
+        return ((const double *)p)[i];
+    if (type == TPU3_POS_I32)
+        return (double)((const int32_t *)p)[i];
+    return (double)((const int64_t *)p)[i];
+}
+
+// cosines and sines of the workgroup's tokens: cs[t * total_pairs + p]
+__device__ __forceinline__ void nr_turns(const NrArgs &a, int64_t t0, int count, float2 *cs)
+{
+    const int all = count * a.total_pairs;
+    for (int i = threadIdx.x; i < all; i += NR_THREADS) {
+        const int t = i / a.total_pairs, p = i - t * a.total_pairs, ax = p / a.pairs;
+        const int64_t tok = t0 + t, e = tok / a.n, r = tok - e * a.n;
+        const double pos = nr_position(a.pos, a.pos_type, e * a.pos_sb + r * a.pos_sn + ax * a.pos_sa);
+        const double f = a.freq_type == TPU3_POS_F64 ? ((const double *)a.freq)[p] : (double)((const float *)a.freq)[p];
+        double turn = pos * f * 0.15915494309189533577;         // 1 / (2 pi)
+        turn -= rint(turn);
+        float s, c;
+        sincospif(2.f * (float)turn, &s, &c);
+        cs[i] = make_float2(c, s);
+    }
+}
+
+template <int LPR> __device__ __forceinline__ float nr_row_sum(float v)
+{
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1)
+        v += __shfl_xor(v, o, 64);
+    return v;
+}
+
+// eight channels from c0 on turned by (c, sign * s); `row` is this row's slice of the exchange buffer
+__device__ __forceinline__ void nr_turn(const NrArgs &a, const float2 *cs, float *row, int c0, float sign, float *y)
+{
+    const int P = a.total_pairs;
+    if (a.interleaved) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const int p = (c0 + i) >> 1;
+            if (p < P) {
+                const float2 t = cs[p];
+                const float s = sign * t.y, u = y[i], v = y[i + 1];
+                y[i] = __builtin_fmaf(u, t.x, -v * s);
+                y[i + 1] = __builtin_fmaf(u, s, v * t.x);
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i += 4)
+        *(hd_f4 *)(row + c0 + i) = hd_f4{y[i], y[i + 1], y[i + 2], y[i + 3]};
+    __builtin_amdgcn_wave_barrier();        // the row's lanes are in one wave, whose LDS accesses complete in order
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (c0 + 8 <= P && (P & 3) == 0) {                          // all eight are first partners
+        const float *o = row + c0 + P;
+        const hd_f4 o0 = *(const hd_f4 *)o, o1 = *(const hd_f4 *)(o + 4);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float2 t = cs[c0 + i];
+            y[i] = __builtin_fmaf(y[i], t.x, -(i < 4 ? o0[i & 3] : o1[i & 3]) * (sign * t.y));
+        }
+    } else if (c0 >= P && c0 + 8 <= 2 * P && (P & 3) == 0) {    // all eight are second partners
+        const float *o = row + c0 - P;
+        const hd_f4 o0 = *(const hd_f4 *)o, o1 = *(const hd_f4 *)(o + 4);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float2 t = cs[c0 - P + i];
+            y[i] = __builtin_fmaf(i < 4 ? o0[i & 3] : o1[i & 3], sign * t.y, y[i] * t.x);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int c = c0 + i;
+            if (c < P) {
+                const float2 t = cs[c];
+                y[i] = __builtin_fmaf(y[i], t.x, -row[c + P] * (sign * t.y));
+            } else if (c < 2 * P) {
+                const float2 t = cs[c - P];
+                y[i] = __builtin_fmaf(row[c - P], sign * t.y, y[i] * t.x);
+            }
+        }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+template <typename T, int LPR>
+__global__ __launch_bounds__(NR_THREADS) void norm_rotate_kernel(NrArgs a)
+{
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    constexpr int GROUPS = NR_THREADS / LPR, ROW = LPR * 8 + 4;
+    float *ex = (float *)smem;                                  // (GROUPS, ROW) exchange rows
+    float2 *cs = (float2 *)(ex + GROUPS * ROW);                 // (tok, total_pairs)
+    const int64_t t0 = (int64_t)blockIdx.x * a.tok;
+    const int count = (int)min((int64_t)a.tok, a.tokens - t0);
+    const int grp = threadIdx.x / LPR, c0 = (threadIdx.x % LPR) * 8;
+    const bool live = c0 < a.d;
+    nr_turns(a, t0, count, cs);
+    __syncthreads();
+    for (int side = 0; side < 2; ++side) {
+        const int heads = a.x[side].heads;
+        const T *X = (const T *)a.x[side].data;
+        T *Y = (T *)a.out[side];
+        for (int r = grp; r < count * heads; r += GROUPS) {
+            const int t = r / heads, h = r - t * heads;
+            const int64_t tok = t0 + t, e = tok / a.n, i = tok - e * a.n;
+            float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (live)
+                hd_load8(X + e * a.x[side].sb + i * a.x[side].sr + h * a.x[side].sh + c0, y);
+            float ss = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                ss = __builtin_fmaf(y[j], y[j], ss);
+            const float inv = 1.f / sqrtf(__builtin_fmaf(nr_row_sum<LPR>(ss), a.inv_d, a.eps));
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                y[j] *= inv;
+            if (a.w[side] && live) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    y[j] *= nr_weight(a.w[side], a.w_type, h * a.w_head[side] + c0 + j);
+            }
+            nr_turn(a, cs + t * a.total_pairs, ex + grp * ROW, c0, 1.f, y);
+            if (live)
+                hd_store8(Y + (tok * heads + h) * a.d + c0, y);
+        }
+    }
+}
+
+// The weight gradients: a lane adds up h u of its eight channels over the rows that its wave takes.  One set of weights for
+// all heads: in registers over the whole kernel.  A set per head: a wave takes whole (head, token part) units, adds its
+// lanes up after each and keeps the unit's row in LDS.  Either way a workgroup leaves one partial sum per weight, in an
+// order that the sizes alone decide; norm_rotate_wsum_kernel adds the workgroups' in 64 bits.
+template <typename T, int LPR>
+__global__ __launch_bounds__(NR_THREADS) void norm_rotate_bwd_kernel(NrArgs a, int split)
+{
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    constexpr int GROUPS = NR_THREADS / LPR, ROW = LPR * 8 + 4, PER = 64 / LPR;
+    const int heads_all = a.x[0].heads + a.x[1].heads;
+    float *ex = (float *)smem;
+    float *acc = ex + GROUPS * ROW;                             // (units, d) per-head sums
+    const bool per_head = a.w_head[0] != 0 || a.w_head[1] != 0;
+    const bool want = a.want_w[0] || a.want_w[1];
+    const int units = heads_all * split;
+    float2 *cs = (float2 *)(acc + (want ? (per_head ? units : 8) * a.d : 0));
+    const int grp = threadIdx.x / LPR, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c0 = (threadIdx.x % LPR) * 8;
+    const bool live = c0 < a.d;
+    const int part_tok = (a.tok + split - 1) / split;
+    float ws[2][8] = {};
+    if (want && per_head)
+        for (int i = threadIdx.x; i < units * a.d; i += NR_THREADS)
+            acc[i] = 0.f;
+    for (int64_t t0 = (int64_t)blockIdx.x * a.tok; t0 < a.tokens; t0 += (int64_t)gridDim.x * a.tok) {
+        const int count = (int)min((int64_t)a.tok, a.tokens - t0);
+        __syncthreads();
+        nr_turns(a, t0, count, cs);
+        __syncthreads();
+        for (int u = wave; u < units; u += 4) {
+            const int hu = u / split, s = u - hu * split;
+            const int side = hu < a.x[0].heads ? 0 : 1, h = side ? hu - a.x[0].heads : hu, heads = a.x[side].heads;
+            const T *X = (const T *)a.x[side].data + h * a.x[side].sh + c0;
+            const T *G = (const T *)a.g[side].data + h * a.g[side].sh + c0;
+            T *Y = (T *)a.out[side];
+            const int last = min(count, (s + 1) * part_tok);
+            float w[8], wg[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                w[j] = a.w[side] && live ? nr_weight(a.w[side], a.w_type, h * a.w_head[side] + c0 + j) : 1.f;
+            // (whole waves run the loop: the lanes of a row exchange values inside)
+            for (int tb = s * part_tok; tb < last; tb += PER) {
+                const int t = tb + lane / LPR;
+                const bool row = t < last && live;
+                const int tc = min(t, last - 1);
+                const int64_t tok = t0 + tc, e = tok / a.n, i = tok - e * a.n;
+                float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, g[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                if (row) {
+                    hd_load8(X + e * a.x[side].sb + i * a.x[side].sr, x);
+                    hd_load8(G + e * a.g[side].sb + i * a.g[side].sr, g);
+                }
+                nr_turn(a, cs + tc * a.total_pairs, ex + grp * ROW, c0, -1.f, g);
+                float ss = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    ss = __builtin_fmaf(x[j], x[j], ss);
+                const float inv = 1.f / sqrtf(__builtin_fmaf(nr_row_sum<LPR>(ss), a.inv_d, a.eps));
+                float dot = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    x[j] *= inv;
+                    wg[j] = __builtin_fmaf(g[j], x[j], wg[j]);
+                    g[j] *= w[j];
+                    dot = __builtin_fmaf(g[j], x[j], dot);
+                }
+                dot = nr_row_sum<LPR>(dot) * a.inv_d;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    g[j] = inv * __builtin_fmaf(-x[j], dot, g[j]);
+                if (row)
+                    hd_store8(Y + (tok * heads + h) * a.d + c0, g);
+            }
+            if (!want)
+                continue;
+            if (per_head) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+#pragma unroll
+                    for (int o = LPR; o < 64; o <<= 1)
+                        wg[j] += __shfl_xor(wg[j], o, 64);
+                }
+                if (lane < LPR && live)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        acc[u * a.d + c0 + j] += wg[j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    ws[0][j] += side ? 0.f : wg[j], ws[1][j] += side ? wg[j] : 0.f;
+            }
+        }
+    }
+    if (!want)
+        return;
+    if (!per_head) {
+#pragma unroll
+        for (int side = 0; side < 2; ++side)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float v = ws[side][j];
+#pragma unroll
+                for (int o = LPR; o < 64; o <<= 1)
+                    v += __shfl_xor(v, o, 64);
+                if (lane < LPR && live)
+                    acc[(side * 4 + wave) * a.d + c0 + j] = v;
+            }
+    }
+    __syncthreads();
+    const int rows = per_head ? heads_all : 2, terms = per_head ? split : 4;
+    for (int i = threadIdx.x; i < rows * a.d; i += NR_THREADS) {
+        const int r = i / a.d, c = i - r * a.d;
+        float v = 0.f;
+        for (int s = 0; s < terms; ++s)
+            v += acc[(r * terms + s) * a.d + c];
+        a.part[(int64_t)blockIdx.x * rows * a.d + i] = v;
+    }
+}
+
+// out[i] = sum over the workgroups' partial sums of column i, in 64 bits and in a fixed order
+__global__ __launch_bounds__(1024) void norm_rotate_wsum_kernel(int wgs, int cols, int first, int count, int w_type,
+                                                               const float *__restrict__ part, void *__restrict__ out)
+{
+    __shared__ double s[32][33];
+    const int c = threadIdx.x & 31, g = threadIdx.x >> 5, i = blockIdx.x * 32 + c;
+    double v = 0.0;
+    if (i < count)
+        for (int r = g; r < wgs; r += 32)
+            v += (double)part[(int64_t)r * cols + first + i];
+    s[g][c] = v;
+    __syncthreads();
+    if (g == 0 && i < count) {
+        v = 0.0;
+        for (int r = 0; r < 32; ++r)
+            v += s[r][c];
+        if (w_type == TPU3_TYPE_F32)
+            ((float *)out)[i] = (float)v;
+        else if (w_type == TPU3_TYPE_F16)
+            ((_Float16 *)out)[i] = (_Float16)(float)v;
+        else
+            ((__bf16 *)out)[i] = (__bf16)(float)v;
+    }
+}
+
+struct NrPlan {
+    int lpr, tok, split, wgs;
+    size_t lds;
+};
+
+// Tokens of a workgroup: enough rows to fill its 256 threads, few enough that the chip's 256 compute units all get some.
+NrPlan nr_plan(int64_t tokens, int heads, int d, int pairs, bool bwd, bool per_head, bool want)
+{
+    NrPlan p;
+    p.lpr = d <= 32 ? 4 : d <= 64 ? 8 : d <= 128 ? 16 : 32;
+    p.tok = bwd ? 64 : 16;
+    while (p.tok > 1 && (tokens + p.tok - 1) / p.tok < 1024)
+        p.tok >>= 1;
+    while (p.tok > 1 && (size_t)p.tok * pairs * 8 > 32768)
+        p.tok >>= 1;
+    const int64_t tiles = (tokens + p.tok - 1) / p.tok;
+    p.split = bwd && heads % 4 ? (p.tok >= 4 ? 4 : 1) : 1;
+    p.wgs = bwd ? (int)(tiles < NR_MAX_WG ? tiles : NR_MAX_WG) : 0;
+    p.lds = (size_t)(NR_THREADS / p.lpr) * (p.lpr * 8 + 4) * 4 + (size_t)p.tok * pairs * 8;
+    if (bwd && want)
+        p.lds += (size_t)(per_head ? heads * p.split : 8) * d * 4;
+    return p;
+}
+
+int nr_fill(NrArgs &a, int type, int b, int n, int d, const tpu3_heads *q, const tpu3_heads *k, const void *wq, int wq_head,
+            const void *wk, int wk_head, int w_type, const tpu3_positions *pos, float eps, int interleaved)
+{
+    if (b < 0 || n < 0 || d <= 0 || !hd_type_ok(type) || !hd_type_ok(w_type) || !q || !k || !pos || !(eps >= 0.f))
+        return TPU3_EINVAL;
+    if (d % 8 || d > 256 || q->heads > 1024 || k->heads > 1024)
+        return TPU3_ELIMIT;
+    if (q->heads <= 0 || k->heads < 0 || pos->axes < 1 || pos->pairs < 0 || (wq_head != 0 && wq_head != d) ||
+        (wk_head != 0 && wk_head != d) || pos->type < TPU3_POS_F32 || pos->type > TPU3_POS_I64 ||
+        (pos->freq_type != TPU3_POS_F32 && pos->freq_type != TPU3_POS_F64))
+        return TPU3_EINVAL;
+    if (pos->axes > d || pos->pairs > d || 2L * pos->axes * pos->pairs > d)
+        return TPU3_EINVAL;
+    if (b == 0 || n == 0)
+        return TPU3_OK;
+    if (!hd_rows_ok(q, type) || (k->heads && !hd_rows_ok(k, type)))
+        return TPU3_EINVAL;
+    if (pos->pairs && (!pos->data || !pos->freq))
+        return TPU3_EINVAL;
+    a.x[0] = *q, a.x[1] = *k;
+    a.w[0] = wq, a.w[1] = wk, a.w_head[0] = wq_head, a.w_head[1] = wk_head, a.w_type = w_type;
+    a.pos = pos->data, a.pos_type = pos->type, a.pos_sb = pos->sb, a.pos_sn = pos->sr, a.pos_sa = pos->sa;
+    a.freq = pos->freq, a.freq_type = pos->freq_type, a.axes = pos->axes, a.pairs = pos->pairs > 0 ? pos->pairs : 1;
+    a.total_pairs = pos->axes * pos->pairs;
+    a.tokens = (int64_t)b * n, a.n = n, a.d = d, a.interleaved = interleaved != 0;
+    a.eps = eps, a.inv_d = 1.f / (float)d;
+    return 1;
+}
+
+template <typename T> int nr_forward(const NrArgs &a, const NrPlan &p, hipStream_t s)
+{
+    const dim3 grid((unsigned)((a.tokens + p.tok - 1) / p.tok));
+#define NR_GO(L) hipLaunchKernelGGL((norm_rotate_kernel<T, L>), grid, dim3(NR_THREADS), p.lds, s, a)
+    if (p.lpr == 4)
+        NR_GO(4);
+    else if (p.lpr == 8)
+        NR_GO(8);
+    else if (p.lpr == 16)
+        NR_GO(16);
+    else
+        NR_GO(32);
+#undef NR_GO
+    return tpu3_launch_status();
+}
+
+template <typename T> int nr_backward(const NrArgs &a, const NrPlan &p, hipStream_t s)
+{
+    const void *f = p.lpr == 4   ? (const void *)norm_rotate_bwd_kernel<T, 4>
+                    : p.lpr == 8 ? (const void *)norm_rotate_bwd_kernel<T, 8>
+                    : p.lpr == 16 ? (const void *)norm_rotate_bwd_kernel<T, 16>
+                                  : (const void *)norm_rotate_bwd_kernel<T, 32>;
+    const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds);
+    if (e != hipSuccess)
+        return (int)e;
+#define NR_GO(L) hipLaunchKernelGGL((norm_rotate_bwd_kernel<T, L>), dim3(p.wgs), dim3(NR_THREADS), p.lds, s, a, p.split)
+    if (p.lpr == 4)
+        NR_GO(4);
+    else if (p.lpr == 8)
+        NR_GO(8);
+    else if (p.lpr == 16)
+        NR_GO(16);
+    else
+        NR_GO(32);
+#undef NR_GO
+    return tpu3_launch_status();
+}
+
+}  // namespace
+
+extern "C" int tpu3_norm_rotate_fwd(tpu3_stream_t stream, int type, int b, int n, int d, const tpu3_heads *q,
+                                    const tpu3_heads *k, const void *wq, int wq_head, const void *wk, int wk_head, int w_type,
+                                    const tpu3_positions *pos, float eps, int interleaved, void *oq, void *ok)
+{
+    NrArgs a = {};
+    const int rc = nr_fill(a, type, b, n, d, q, k, wq, wq_head, wk, wk_head, w_type, pos, eps, interleaved);
+    if (rc <= 0)
+        return rc;
+    if (!oq || ((uintptr_t)oq & 15) || (k->heads && (!ok || ((uintptr_t)ok & 15))))
+        return TPU3_EINVAL;
+    a.out[0] = oq, a.out[1] = ok;
+    const NrPlan p = nr_plan(a.tokens, q->heads + k->heads, d, a.total_pairs, false, false, false);
+    if ((a.tokens + p.tok - 1) / p.tok > 0x7FFFFFFFLL)
+        return TPU3_ELIMIT;
+    a.tok = p.tok;
+    const hipStream_t s = (hipStream_t)stream;
+    return type == TPU3_TYPE_F32 ? nr_forward<float>(a, p, s) : type == TPU3_TYPE_F16 ? nr_forward<_Float16>(a, p, s) : nr_forward<__bf16>(a, p, s);
+}
+
+extern "C" size_t tpu3_norm_rotate_bwd_workspace_bytes(int heads, int d, int per_head)
+{
+    if (heads <= 0 || d <= 0)
+        return 0;
+    return (size_t)NR_MAX_WG * (per_head ? heads : 2) * d * 4;
+}
+
+extern "C" int tpu3_norm_rotate_bwd(tpu3_stream_t stream, int type, int b, int n, int d, const tpu3_heads *q,
+                                    const tpu3_heads *k, const void *wq, int wq_head, const void *wk, int wk_head, int w_type,
+                                    const tpu3_positions *pos, float eps, int interleaved, const tpu3_heads *gq,
+                                    const tpu3_heads *gk, void *dq, void *dk, void *dwq, void *dwk, void *workspace,
+                                    size_t workspace_bytes)
+{
+    NrArgs a = {};
+    const int rc = nr_fill(a, type, b, n, d, q, k, wq, wq_head, wk, wk_head, w_type, pos, eps, interleaved);
+    if (rc <= 0)
+        return rc;
+    if (!hd_rows_ok(gq, type) || gq->heads != q->heads || !dq || ((uintptr_t)dq & 15))
+        return TPU3_EINVAL;
+    if (k->heads && (!hd_rows_ok(gk, type) || gk->heads != k->heads || !dk || ((uintptr_t)dk & 15)))
+        return TPU3_EINVAL;
+    a.g[0] = *gq;
+    if (k->heads)
+        a.g[1] = *gk;
+    a.out[0] = dq, a.out[1] = dk;
+    a.want_w[0] = dwq && wq, a.want_w[1] = dwk && wk && k->heads;
+    const bool want = a.want_w[0] || a.want_w[1], per_head = wq_head != 0 || wk_head != 0;
+    const int heads = q->heads + k->heads;
+    if (want && (!workspace || ((uintptr_t)workspace & 3) || workspace_bytes < tpu3_norm_rotate_bwd_workspace_bytes(heads, d, per_head)))
+        return TPU3_EINVAL;
+    a.part = (float *)workspace;
+    const NrPlan p = nr_plan(a.tokens, heads, d, a.total_pairs, true, per_head, want);
+    if (p.lds > 160 * 1024)
+        return TPU3_ELIMIT;
+    a.tok = p.tok;
+    const hipStream_t s = (hipStream_t)stream;
+    int st = type == TPU3_TYPE_F32 ? nr_backward<float>(a, p, s) : type == TPU3_TYPE_F16 ? nr_backward<_Float16>(a, p, s) : nr_backward<__bf16>(a, p, s);
+    if (st || !want)
+        return st;
+    // columns of a partial row: per head, all query heads' weights then all key heads'; else one set each.  Where only one
+    // side has a set per head, the other side's heads are added up here too: that mixture is refused above the C ABI.
+    const int cols = (per_head ? heads : 2) * d, nq = (per_head ? q->heads : 1) * d, nk = (per_head ? k->heads : 1) * d;
+    if (a.want_w[0])
+        hipLaunchKernelGGL(norm_rotate_wsum_kernel, dim3((nq + 31) / 32), dim3(1024), 0, s, p.wgs, cols, 0, nq, w_type, a.part, dwq);
+    if (a.want_w[1])
+        hipLaunchKernelGGL(norm_rotate_wsum_kernel, dim3((nk + 31) / 32), dim3(1024), 0, s, p.wgs, cols, nq, nk, w_type, a.part, dwk);
+    return tpu3_launch_status();
+}

@@ -17,6 +17,8 @@ import torch
 
 from .. import _lib as L
 from .. import sampling
+from .attention import (block_attention, block_means, norm_rotate, rotation_frequencies, select_blocks,  # noqa: F401
+                        sparse_attention)
 
 
 import collections

@@ -522,6 +522,86 @@ int tpu3_gather_rows_f32(tpu3_stream_t stream, int b, int n, long m, int c, cons
 int tpu3_scatter_add_rows_f32(tpu3_stream_t stream, int b, int n, long m, int c, const float *g, const void *idx,
                               int idx_elem_size, float *dx);
 
+/* ---- attention between points (csrc/norm_rotate.hip, block_select.hip, block_attn.hip) -------------------------------------
+ * The learned form of what the inter-level skip does with a fixed kernel (network/upsampler.py:317-347: a cheap search, weights
+ * that are normalised, a weighted sum of the rows found); the reference has no such operator.
+ * All tensors of heads are (b, rows, heads, d) with unit channel stride: d % 8 == 0, 16-byte aligned rows (strides in
+ * elements; a stride may be 0).  `type` is the element type of every such tensor of a call. */
+#define TPU3_TYPE_F32 0
+#define TPU3_TYPE_F16 1
+#define TPU3_TYPE_BF16 2
+typedef struct {
+    void *data;
+    int64_t sb, sr, sh;     /* elements between sequences, rows and heads */
+    int heads;              /* 0: absent (keys of tpu3_norm_rotate_*) */
+} tpu3_heads;
+
+/* Positions of the rows and the frequencies of the rotated pairs: pair p = axis * pairs + f turns by
+ * position[axis] * freq[axis * pairs + f] (64 bits).  data (b, rows, axes) by strides, freq contiguous. */
+#define TPU3_POS_F32 0
+#define TPU3_POS_F64 1
+#define TPU3_POS_I32 2
+#define TPU3_POS_I64 3
+typedef struct {
+    const void *data;
+    int64_t sb, sr, sa;
+    int type;               /* TPU3_POS_* of data */
+    int axes, pairs;        /* 2 * axes * pairs <= d; pairs = 0: no rotation */
+    const void *freq;
+    int freq_type;          /* TPU3_POS_F32 / TPU3_POS_F64 */
+} tpu3_positions;
+
+/* Norm of every head's row and its rotation in one pass: y = x / sqrt(mean(x^2) + eps) * w, then pair p of the first
+ * 2 * axes * pairs channels turned: (one c - two s, one s + two c); partners are channels (p, p + axes * pairs), or
+ * (2p, 2p + 1) with interleaved != 0; channels behind them pass.  w*: d weights for all heads (w*_head = 0), d a head
+ * (w*_head = d), or NULL (ones); both sides alike.  oq / ok contiguous, 16-byte aligned.  d <= 256 (else TPU3_ELIMIT).
+ *   bwd: gq / gk = gradients of oq / ok -> dq, dk, and dwq / dwk (NULL: not wanted) in the weights' type and shape;
+ *   workspace = tpu3_norm_rotate_bwd_workspace_bytes(all heads, d, a set of weights per head) bytes when a weight's
+ *   gradient is wanted.  Deterministic: no atomics. */
+int tpu3_norm_rotate_fwd(tpu3_stream_t stream, int type, int b, int n, int d, const tpu3_heads *q, const tpu3_heads *k,
+                         const void *wq, int wq_head, const void *wk, int wk_head, int w_type, const tpu3_positions *pos,
+                         float eps, int interleaved, void *oq, void *ok);
+int tpu3_norm_rotate_bwd(tpu3_stream_t stream, int type, int b, int n, int d, const tpu3_heads *q, const tpu3_heads *k,
+                         const void *wq, int wq_head, const void *wk, int wk_head, int w_type, const tpu3_positions *pos,
+                         float eps, int interleaved, const tpu3_heads *gq, const tpu3_heads *gk, void *dq, void *dk, void *dwq,
+                         void *dwk, void *workspace, size_t workspace_bytes);
+size_t tpu3_norm_rotate_bwd_workspace_bytes(int heads, int d, int per_head);
+
+/* Attention over picked blocks of TPU3_ATTN_BLOCK consecutive keys.  n_arr / m_arr: live keys / queries of each sequence
+ * (NULL: all n / m).  causal: query i stands at key position live keys - live queries + i and sees the keys up to it. */
+#define TPU3_ATTN_BLOCK 64
+#define TPU3_BLOCK_COUNT_MAX 64
+#define TPU3_ATTN_BLOCKS_MAX 65536
+/* means (b, ceil(n / 64), k->heads, d) f32, 16-byte aligned: the mean of every block's live rows, summed in 64 bits and
+ * rounded once (no live row: 0).  last < 0: every block; last >= 0: only the blocks that hold the last `last` live rows (a
+ * cache that has grown), the others are left as they are.  d <= 128. */
+int tpu3_block_means(tpu3_stream_t stream, int type, int b, int n, int d, const tpu3_heads *k, const int32_t *n_arr, int last,
+                     float *means);
+/* blocks (b, m, hk, count) i32: per query and key head the `count` blocks with the largest (sum of the group's query rows) .
+ * mean, in 64 bits (not a number: behind every number; equal ones to the lowest block), ascending, -1 behind them.  causal:
+ * the block of the query's own position always, the others among those before it.  A query behind m_arr, or one that sees
+ * nothing: all -1.  d <= 128, count <= 64; workspace = tpu3_block_select_workspace_bytes bytes, 8-byte aligned (0: NULL). */
+int tpu3_block_select(tpu3_stream_t stream, int type, int b, int m, int n, int d, const tpu3_heads *q, int hk,
+                      const float *means, const int32_t *n_arr, const int32_t *m_arr, int causal, int count, int32_t *blocks,
+                      void *workspace, size_t workspace_bytes);
+size_t tpu3_block_select_workspace_bytes(int b, int m, int n, int hk, int count);
+/* out (b, m, q->heads, d) contiguous = softmax(scale q k^T) v over the live keys of the blocks (b, m, k->heads, count) that a
+ * query names (shared by the heads of a group; an index outside the live blocks, or behind what the query may see, counts
+ * for nothing, one named twice counts once); a row that sees nothing: 0.  lse (b, q->heads, m) f32 or NULL: log2 of the
+ * denominator, what the backward pass needs.  q->heads / k->heads <= 64, d <= 128; workspace =
+ * tpu3_block_attn_fwd_workspace_bytes bytes, 16-byte aligned (0: NULL). */
+int tpu3_block_attn_fwd(tpu3_stream_t stream, int type, int b, int m, int n, int d, const tpu3_heads *q, const tpu3_heads *k,
+                        const tpu3_heads *v, const int32_t *blocks, int count, float scale, const int32_t *n_arr,
+                        const int32_t *m_arr, int causal, void *out, float *lse, void *workspace, size_t workspace_bytes);
+size_t tpu3_block_attn_fwd_workspace_bytes(int b, int m, int n, int hq, int hk, int d, int count);
+/* Its gradient: o / lse of the forward call, go = the gradient of o -> dq, dk, dv contiguous (rows behind the live ones: 0).
+ * Deterministic: no floating-point atomics.  workspace = tpu3_block_attn_bwd_workspace_bytes bytes, 16-byte aligned. */
+int tpu3_block_attn_bwd(tpu3_stream_t stream, int type, int b, int m, int n, int d, const tpu3_heads *q, const tpu3_heads *k,
+                        const tpu3_heads *v, const tpu3_heads *o, const tpu3_heads *go, const int32_t *blocks, int count,
+                        float scale, const int32_t *n_arr, const int32_t *m_arr, int causal, const float *lse, void *dq,
+                        void *dk, void *dv, void *workspace, size_t workspace_bytes);
+size_t tpu3_block_attn_bwd_workspace_bytes(int b, int m, int n, int hq, int hk);
+
 /* ---- measurement hooks (bench.py and tools/ only; a caller of the path never needs them) ------------
  * tpu3_debug_fps_bucket_events: the NEXT bucketed-FPS call (n beyond the register-resident limit)
  * records `start` / `stop` (hipEvent_t created by the caller) on ITS stream immediately before / after
