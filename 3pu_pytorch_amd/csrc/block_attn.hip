@@ -33,6 +33,7 @@ struct BaArgs {
     const int32_t *blocks;                  // (b, m, hk, count)
     const int32_t *n_arr, *m_arr;
     void *out, *out2;                       // forward: o; dq pass: dq; dk / dv pass: dk, dv (contiguous)
+    void *rest;                             // 16-bit types, contiguous like o: what the rounding of o took, for do . o
     float *lse;                             // (b, hq, m): log2 of the softmax denominator, scaled scores in base 2
     float *delta;                           // (b, hq, m): do . o
     float *gmax;                            // (b, hq, m): largest |do| of the row
@@ -122,6 +123,19 @@ template <typename T> __device__ __forceinline__ void ba_store4(T *p, const hd_f
     for (int i = 0; i < 4; ++i)
         y[i] = (T)x[i];
     *(typename hd_vec<T>::v4 *)p = y;
+}
+
+// the same, and what the rounding took
+template <typename T> __device__ __forceinline__ void ba_store_rest(T *p, T *rest, bool want, int at, const hd_f4 &x)
+{
+    ba_store4<T>(p + at, x);
+    if (sizeof(T) == 2 && want) {
+        hd_f4 r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            r[i] = x[i] - (float)(T)x[i];
+        ba_store4<T>(rest + at, r);
+    }
 }
 
 // maximum / sum over the four lane groups that hold a column (lanes l, l+16, l+32, l+48)
@@ -453,7 +467,7 @@ __global__ __launch_bounds__(BA_THREADS) void block_attn_fwd_kernel(BaArgs a, in
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c)
         if (c * 16 + g * 4 < a.d)
-            ba_store4<T>(O + c * 16 + g * 4, acc[c] * inv);
+            ba_store_rest<T>(O, (T *)a.rest + (O - (T *)a.out), a.rest != nullptr, c * 16 + g * 4, acc[c] * inv);
     if (a.lse && g == 0)
         a.lse[((int64_t)t.b * a.hq + head) * a.m + i] = sum > 0.f ? top + log2f(sum) : -INFINITY;
 }
@@ -485,8 +499,12 @@ __global__ __launch_bounds__(BA_THREADS) void block_attn_join_kernel(BaArgs a, i
     T *O = (T *)a.out + ((b * a.m + i) * a.hq + h) * a.d;
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c)
-        if (l * (DP / 16) + c < a.d)
-            O[l * (DP / 16) + c] = (T)(y[c] * inv);
+        if (l * (DP / 16) + c < a.d) {
+            const T v = (T)(y[c] * inv);
+            O[l * (DP / 16) + c] = v;
+            if (a.rest)
+                ((T *)a.rest)[O - (T *)a.out + l * (DP / 16) + c] = (T)(y[c] * inv - (float)v);
+        }
     if (a.lse && l == 0)
         a.lse[row] = sum > 0.f ? top + log2f(sum) : -INFINITY;
 }
@@ -525,13 +543,15 @@ __global__ __launch_bounds__(BA_THREADS) void block_attn_dq_kernel(BaArgs a, int
     ba_row_operand<T, DP>((const T *)a.go.data + t.b * a.go.sb + (int64_t)i * a.go.sr + (int64_t)head * a.go.sh, mine, a.d, gf);
     float delta = 0.f, gmax = 0.f;
     {
-        typename hd_vec<T>::v8 of[DP / 32];
+        // the rounding of o, times a gradient, would move all of a row's ds one way: it goes back in
+        typename hd_vec<T>::v8 of[DP / 32], rf[DP / 32];
         ba_row_operand<T, DP>((const T *)a.o.data + t.b * a.o.sb + (int64_t)i * a.o.sr + (int64_t)head * a.o.sh, mine, a.d, of);
+        ba_row_operand<T, DP>((const T *)a.rest + (((int64_t)t.b * a.m + i) * a.hq + head) * a.d, mine && a.rest, a.d, rf);
 #pragma unroll
         for (int kk = 0; kk < DP / 32; ++kk)
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
-                delta = __builtin_fmaf((float)gf[kk][c], (float)of[kk][c], delta);
+                delta = __builtin_fmaf((float)gf[kk][c], (float)of[kk][c] + (float)rf[kk][c], delta);
                 gmax = fmaxf(gmax, fabsf((float)gf[kk][c]));
             }
     }
@@ -928,15 +948,15 @@ extern "C" size_t tpu3_block_attn_fwd_workspace_bytes(int b, int m, int n, int h
 extern "C" int tpu3_block_attn_fwd(tpu3_stream_t stream, int type, int b, int m, int n, int d, const tpu3_heads *q,
                                    const tpu3_heads *k, const tpu3_heads *v, const int32_t *blocks, int count, float scale,
                                    const int32_t *n_arr, const int32_t *m_arr, int causal, void *out, float *lse,
-                                   void *workspace, size_t workspace_bytes)
+                                   void *rest, void *workspace, size_t workspace_bytes)
 {
     BaArgs a = {};
     const int rc = ba_fill(a, type, b, m, n, d, q, k, v, blocks, count, scale, n_arr, m_arr, causal);
     if (rc <= 0)
         return rc;
-    if (!out || ((uintptr_t)out & 15))
+    if (!out || ((uintptr_t)out & 15) || ((uintptr_t)rest & 15))
         return TPU3_EINVAL;
-    a.out = out, a.lse = lse;
+    a.out = out, a.lse = lse, a.rest = type == TPU3_TYPE_F32 ? nullptr : rest;
     a.splits = ba_splits(b, m, n, a.hq, a.hk, count);
     if (a.splits > 1) {
         if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < (size_t)b * m * a.hq * a.splits * (ba_dp(d) + 4) * 4)
@@ -958,18 +978,18 @@ extern "C" size_t tpu3_block_attn_bwd_workspace_bytes(int b, int m, int n, int h
 extern "C" int tpu3_block_attn_bwd(tpu3_stream_t stream, int type, int b, int m, int n, int d, const tpu3_heads *q,
                                    const tpu3_heads *k, const tpu3_heads *v, const tpu3_heads *o, const tpu3_heads *go,
                                    const int32_t *blocks, int count, float scale, const int32_t *n_arr, const int32_t *m_arr,
-                                   int causal, const float *lse, void *dq, void *dk, void *dv, void *workspace,
-                                   size_t workspace_bytes)
+                                   int causal, const float *lse, const void *rest, void *dq, void *dk, void *dv,
+                                   void *workspace, size_t workspace_bytes)
 {
     BaArgs a = {};
     const int rc = ba_fill(a, type, b, m, n, d, q, k, v, blocks, count, scale, n_arr, m_arr, causal);
     if (rc <= 0)
         return rc;
-    if (!hd_rows_ok(o, type) || !hd_rows_ok(go, type) || o->heads != a.hq || go->heads != a.hq || !lse || !dq ||
+    if (!hd_rows_ok(o, type) || !hd_rows_ok(go, type) || o->heads != a.hq || go->heads != a.hq || !lse || !dq || ((uintptr_t)rest & 15) ||
         ((uintptr_t)dq & 15) || (n > 0 && (!dk || !dv || ((uintptr_t)dk & 15) || ((uintptr_t)dv & 15))) || !workspace ||
         ((uintptr_t)workspace & 7) || workspace_bytes < tpu3_block_attn_bwd_workspace_bytes(b, m, n, a.hq, a.hk))
         return TPU3_EINVAL;
-    a.o = *o, a.go = *go, a.lse = (float *)lse;
+    a.o = *o, a.go = *go, a.lse = (float *)lse, a.rest = type == TPU3_TYPE_F32 ? nullptr : (void *)rest;
     a.bits = (uint64_t *)workspace;
     a.delta = (float *)(a.bits + (size_t)b * a.hk * a.nb * a.mt);
     a.gmax = a.delta + (size_t)b * a.hq * m;

@@ -16,7 +16,6 @@ Rows near each other should hold points near each other (a space-filling order, 
 
 Device tensors only; everything runs on the current stream of the tensors' device and can be captured into a graph.  Results
 do not depend on the order in which workgroups run."""
-import ctypes
 import math
 
 import torch
@@ -43,6 +42,8 @@ def _rows(t, name, like=None):
 
 
 def _taken(t):
+    if t is None or (t.is_contiguous() and not t.data_ptr() & 15):
+        return t                                        # (rows of a multiple of 8 channels: 16 bytes)
     per = 16 // t.element_size()
     if t.stride(3) != 1 or t.data_ptr() & 15 or any(t.size(i) > 1 and t.stride(i) % per for i in range(3)):
         t = t.contiguous()
@@ -51,12 +52,32 @@ def _taken(t):
     return t
 
 
+_ABSENT = L.Heads(None, 0, 0, 0, 0)
+
+
 def _heads(t):
     """tpu3_heads of a tensor that _taken returned; None: absent."""
     if t is None:
-        return L.Heads(None, 0, 0, 0, 0)
-    s = [t.stride(i) if t.size(i) > 1 else 0 for i in range(3)]
-    return L.Heads(t.data_ptr() or None, s[0], s[1], s[2], t.size(2))
+        return _ABSENT
+    size, stride = t.shape, t.stride()
+    return L.Heads(t.data_ptr() or None, stride[0] if size[0] > 1 else 0, stride[1] if size[1] > 1 else 0,
+                   stride[2] if size[2] > 1 else 0, size[2])
+
+
+def _launch(name, t, *args):
+    """A C entry point on the current stream of the tensor's device (which is made the current device if it is not)."""
+    dev = t.get_device()
+    if torch.cuda.current_device() == dev:
+        rc = getattr(L.lib(), name)(torch.cuda.current_stream().cuda_stream, *args)
+    else:
+        with torch.cuda.device(dev):
+            rc = getattr(L.lib(), name)(torch.cuda.current_stream().cuda_stream, *args)
+    if rc:
+        L.check(rc, name)
+
+
+def _workspace(need, t):
+    return torch.empty((need,), dtype=torch.uint8, device=t.device) if need else None
 
 
 def _lengths(t, name, b, device):
@@ -76,61 +97,55 @@ def rotation_frequencies(axes, pairs, base=10000.0, device=None):
     return f.repeat(axes, 1)
 
 
+def _rotation(q, position, freq):
+    s = position.stride()
+    return L.Positions(position.data_ptr(), s[0], s[1], s[2], L.POSITION_TYPES[position.dtype], freq.size(0), freq.size(1),
+                       freq.data_ptr() or None, L.POSITION_TYPES[freq.dtype])
+
+
+def _weights(wq, wk, d):
+    some = wq if wq is not None else wk
+    return (L.ptr(wq), d if wq is not None and wq.dim() == 2 else 0, L.ptr(wk), d if wk is not None and wk.dim() == 2 else 0,
+            L.TYPES[some.dtype] if some is not None else 0)
+
+
+def _norm_rotate_forward(q, k, wq, wk, position, freq, eps, interleaved):
+    q, k = _taken(q), _taken(k)
+    oq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ok = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    b, n, _, d = q.shape
+    _launch("tpu3_norm_rotate_fwd", q, L.TYPES[q.dtype], b, n, d, _heads(q), _heads(k), *_weights(wq, wk, d),
+            _rotation(q, position, freq), eps, interleaved, oq.data_ptr(), L.ptr(ok))
+    return oq, ok
+
+
 class _NormRotate(torch.autograd.Function):
-    @staticmethod
-    def _call(q, k, position, freq):
-        d, p = q.size(3), position
-        pos = L.Positions(p.data_ptr(), p.stride(0), p.stride(1), p.stride(2), L.POSITION_TYPES[p.dtype], freq.size(0),
-                          freq.size(1), freq.data_ptr() or None, L.POSITION_TYPES[freq.dtype])
-        return L.TYPES[q.dtype], q.size(0), q.size(1), d, pos
-
-    @staticmethod
-    def _weights(wq, wk, d):
-        some = wq if wq is not None else wk
-        return (L.ptr(wq), d if wq is not None and wq.dim() == 2 else 0, L.ptr(wk), d if wk is not None and wk.dim() == 2 else 0,
-                L.TYPES[some.dtype] if some is not None else 0)
-
     @staticmethod
     def forward(ctx, q, k, wq, wk, position, freq, eps, interleaved):
         ctx.save_for_backward(q, k, wq, wk, position, freq)
         ctx.eps, ctx.interleaved = eps, interleaved
-        ctx.set_materialize_grads(True)
-        q, k = _taken(q), None if k is None else _taken(k)
-        oq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        ok = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        typ, b, n, d, pos = _NormRotate._call(q, k, position, freq)
-        hq, hk = _heads(q), _heads(k)
-        with torch.cuda.device(q.device):
-            L.check(L.lib().tpu3_norm_rotate_fwd(L.stream_of(q), typ, b, n, d, ctypes.byref(hq), ctypes.byref(hk),
-                                                 *_NormRotate._weights(wq, wk, d), ctypes.byref(pos), eps, interleaved,
-                                                 L.ptr(oq), L.ptr(ok)), "tpu3_norm_rotate_fwd")
-        return oq, ok
+        return _norm_rotate_forward(q, k, wq, wk, position, freq, eps, interleaved)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gq, gk):
         q, k, wq, wk, position, freq = ctx.saved_tensors
-        q, k = _taken(q), None if k is None else _taken(k)
-        gq = _taken(gq)
+        q, k, gq = _taken(q), _taken(k), _taken(gq)
         gk = None if k is None else _taken(gk)
+        b, n, hq, d = q.shape
         dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         dk = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        typ, b, n, d, pos = _NormRotate._call(q, k, position, freq)
         make = torch.zeros if b * n == 0 else torch.empty            # (no rows: the kernels do not run)
         dwq, dwk = (make(w.shape, dtype=w.dtype, device=w.device) if w is not None and need else None
                     for w, need in ((wq, ctx.needs_input_grad[2]), (wk, ctx.needs_input_grad[3])))
-        ws, need = None, 0
-        lib = L.lib()
+        need = 0
         if dwq is not None or dwk is not None:
             per_head = int((wq if wq is not None else wk).dim() == 2)
-            need = lib.tpu3_norm_rotate_bwd_workspace_bytes(q.size(2) + (0 if k is None else k.size(2)), d, per_head)
-            ws = torch.empty((need,), dtype=torch.uint8, device=q.device)
-        h = [_heads(t) for t in (q, k, gq, gk)]
-        with torch.cuda.device(q.device):
-            L.check(lib.tpu3_norm_rotate_bwd(L.stream_of(q), typ, b, n, d, ctypes.byref(h[0]), ctypes.byref(h[1]),
-                                             *_NormRotate._weights(wq, wk, d), ctypes.byref(pos), ctx.eps, ctx.interleaved,
-                                             ctypes.byref(h[2]), ctypes.byref(h[3]), L.ptr(dq), L.ptr(dk), L.ptr(dwq),
-                                             L.ptr(dwk), L.ptr(ws), need), "tpu3_norm_rotate_bwd")
+            need = L.lib().tpu3_norm_rotate_bwd_workspace_bytes(hq + (0 if k is None else k.size(2)), d, per_head)
+        ws = _workspace(need, q)
+        _launch("tpu3_norm_rotate_bwd", q, L.TYPES[q.dtype], b, n, d, _heads(q), _heads(k), *_weights(wq, wk, d),
+                _rotation(q, position, freq), ctx.eps, ctx.interleaved, _heads(gq), _heads(gk), dq.data_ptr(), L.ptr(dk),
+                L.ptr(dwq), L.ptr(dwk), L.ptr(ws), need)
         return dq, dk, dwq, dwk, None, None, None, None
 
 
@@ -192,7 +207,9 @@ def norm_rotate(q, k, q_weight, k_weight, position, freq, eps=1e-6, interleaved=
                            % (tuple(position.shape), tuple(freq.shape), b, n))
     if 2 * freq.numel() > d:
         raise RuntimeError("norm_rotate: %d pairs need more than %d channels" % (freq.numel(), d))
-    return _NormRotate.apply(q, k, wq, wk, position, freq.contiguous(), float(eps), int(bool(interleaved)))
+    args = (q, k, wq, wk, position, freq.contiguous(), float(eps), int(bool(interleaved)))
+    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4])
+    return _NormRotate.apply(*args) if grad else _norm_rotate_forward(*args)
 
 
 # ---- blocks ------------------------------------------------------------------------------------------------------------
@@ -238,10 +255,8 @@ def block_means(k, n_arr=None, out=None, last=None):
     if last is not None and int(last) < 0:
         raise RuntimeError("block_means: last must not be negative, got %s" % last)
     k = _taken(k)
-    h = _heads(k)
-    with torch.cuda.device(k.device):
-        L.check(L.lib().tpu3_block_means(L.stream_of(k), L.TYPES[k.dtype], b, n, d, ctypes.byref(h), L.ptr(n_arr),
-                                         -1 if last is None else min(int(last), n), L.ptr(out)), "tpu3_block_means")
+    _launch("tpu3_block_means", k, L.TYPES[k.dtype], b, n, d, _heads(k), L.ptr(n_arr),
+            -1 if last is None else min(int(last), n), out.data_ptr())
     return out
 
 
@@ -276,59 +291,58 @@ def select_blocks(q, means, keys, count, n_arr=None, m_arr=None, causal=False):
         means = means.clone()
     blocks = torch.empty((b, m, hk, count), dtype=torch.int32, device=q.device)
     q = _taken(q)
-    h = _heads(q)
-    lib = L.lib()
-    need = lib.tpu3_block_select_workspace_bytes(b, m, keys, hk, count)
-    ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
-    with torch.cuda.device(q.device):
-        L.check(lib.tpu3_block_select(L.stream_of(q), L.TYPES[q.dtype], b, m, keys, d, ctypes.byref(h), hk, L.ptr(means),
-                                      L.ptr(n_arr), L.ptr(m_arr), int(bool(causal)), count, L.ptr(blocks), L.ptr(ws), need),
-                "tpu3_block_select")
+    need = L.lib().tpu3_block_select_workspace_bytes(b, m, keys, hk, count)
+    ws = _workspace(need, q)
+    _launch("tpu3_block_select", q, L.TYPES[q.dtype], b, m, keys, d, _heads(q), hk, means.data_ptr(), L.ptr(n_arr),
+            L.ptr(m_arr), int(bool(causal)), count, blocks.data_ptr(), L.ptr(ws), need)
     return blocks
+
+
+def _attention_forward(q, k, v, blocks, scale, n_arr, m_arr, causal, grad=False):
+    """-> o, and for the backward pass lse and what the rounding of a 16-bit o took (else None)."""
+    q, k, v = _taken(q), _taken(k), _taken(v)
+    b, m, hq, d = q.shape
+    n, hk, count = k.size(1), k.size(2), blocks.size(3)
+    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty((b, hq, m), dtype=torch.float32, device=q.device) if grad else None
+    rest = torch.empty(q.shape, dtype=q.dtype, device=q.device) if grad and q.dtype != torch.float32 else None
+    need = L.lib().tpu3_block_attn_fwd_workspace_bytes(b, m, n, hq, hk, d, count)
+    ws = _workspace(need, q)
+    _launch("tpu3_block_attn_fwd", q, L.TYPES[q.dtype], b, m, n, d, _heads(q), _heads(k), _heads(v), blocks.data_ptr(), count,
+            scale, L.ptr(n_arr), L.ptr(m_arr), causal, o.data_ptr(), L.ptr(lse), L.ptr(rest), L.ptr(ws), need)
+    return o, lse, rest
 
 
 class _BlockAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, blocks, scale, n_arr, m_arr, causal):
-        grad = any(ctx.needs_input_grad[:3])
-        tq, tk, tv = _taken(q), _taken(k), _taken(v)
-        b, m, hq, d = q.shape
-        n, hk, count = k.size(1), k.size(2), blocks.size(3)
-        o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        lse = torch.empty((b, hq, m), dtype=torch.float32, device=q.device) if grad else None
-        lib = L.lib()
-        need = lib.tpu3_block_attn_fwd_workspace_bytes(b, m, n, hq, hk, d, count)
-        ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
-        h = [_heads(t) for t in (tq, tk, tv)]
-        with torch.cuda.device(q.device):
-            L.check(lib.tpu3_block_attn_fwd(L.stream_of(q), L.TYPES[q.dtype], b, m, n, d, *[ctypes.byref(t) for t in h],
-                                            L.ptr(blocks), count, scale, L.ptr(n_arr), L.ptr(m_arr), causal, L.ptr(o),
-                                            L.ptr(lse), L.ptr(ws), need), "tpu3_block_attn_fwd")
-        if grad:
-            ctx.save_for_backward(q, k, v, o, lse, blocks, n_arr, m_arr)
-            ctx.scale, ctx.causal = scale, causal
+        o, lse, rest = _attention_forward(q, k, v, blocks, scale, n_arr, m_arr, causal, True)
+        ctx.save_for_backward(q, k, v, o, lse, rest, blocks, n_arr, m_arr)
+        ctx.scale, ctx.causal = scale, causal
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, go):
-        q, k, v, o, lse, blocks, n_arr, m_arr = ctx.saved_tensors
+        q, k, v, o, lse, rest, blocks, n_arr, m_arr = ctx.saved_tensors
         q, k, v, o, go = (_taken(t) for t in (q, k, v, o, go))
         b, m, hq, d = q.shape
         n, hk, count = k.size(1), k.size(2), blocks.size(3)
         dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         make = torch.zeros if m == 0 else torch.empty                # (no queries: the kernels do not run)
         dk, dv = (make(t.shape, dtype=t.dtype, device=t.device) for t in (k, v))
-        lib = L.lib()
-        need = lib.tpu3_block_attn_bwd_workspace_bytes(b, m, n, hq, hk)
-        ws = torch.empty((need,), dtype=torch.uint8, device=q.device)
-        h = [_heads(t) for t in (q, k, v, o, go)]
-        with torch.cuda.device(q.device):
-            L.check(lib.tpu3_block_attn_bwd(L.stream_of(q), L.TYPES[q.dtype], b, m, n, d, *[ctypes.byref(t) for t in h],
-                                            L.ptr(blocks), count, ctx.scale, L.ptr(n_arr), L.ptr(m_arr), ctx.causal,
-                                            L.ptr(lse), L.ptr(dq), L.ptr(dk), L.ptr(dv), L.ptr(ws), need),
-                    "tpu3_block_attn_bwd")
+        need = L.lib().tpu3_block_attn_bwd_workspace_bytes(b, m, n, hq, hk)
+        ws = _workspace(need, q)
+        _launch("tpu3_block_attn_bwd", q, L.TYPES[q.dtype], b, m, n, d, _heads(q), _heads(k), _heads(v), _heads(o), _heads(go),
+                blocks.data_ptr(), count, ctx.scale, L.ptr(n_arr), L.ptr(m_arr), ctx.causal, lse.data_ptr(), L.ptr(rest),
+                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), L.ptr(ws), need)
         return dq, dk, dv, None, None, None, None, None
+
+
+def _attention(q, k, v, *args):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _BlockAttention.apply(q, k, v, *args)
+    return _attention_forward(q, k, v, *args)[0]
 
 
 def _check_attention(q, k, v, scale, n_arr, m_arr):
@@ -370,7 +384,7 @@ def block_attention(q, k, v, blocks, scale=None, n_arr=None, m_arr=None, causal=
     _count(blocks.size(3))
     if blocks.dtype == torch.int64:
         blocks = blocks.clamp(-1, L.ATTN_BLOCKS_MAX).to(torch.int32)
-    return _BlockAttention.apply(q, k, v, blocks.contiguous(), scale, n_arr, m_arr, int(bool(causal)))
+    return _attention(q, k, v, blocks.contiguous(), scale, n_arr, m_arr, int(bool(causal)))
 
 
 def sparse_attention(q, k, v, count, scale=None, n_arr=None, m_arr=None, causal=False, means=None):
@@ -383,4 +397,4 @@ def sparse_attention(q, k, v, count, scale=None, n_arr=None, m_arr=None, causal=
     blocks = select_blocks(q, means, k.size(1), count, n_arr, m_arr, causal)
     if means.size(2) != k.size(2):
         raise RuntimeError("means have %d heads, k has %d" % (means.size(2), k.size(2)))
-    return _BlockAttention.apply(q, k, v, blocks, scale, n_arr, m_arr, int(bool(causal)))
+    return _attention(q, k, v, blocks, scale, n_arr, m_arr, int(bool(causal)))

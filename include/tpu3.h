@@ -587,19 +587,20 @@ int tpu3_block_select(tpu3_stream_t stream, int type, int b, int m, int n, int d
 size_t tpu3_block_select_workspace_bytes(int b, int m, int n, int hk, int count);
 /* out (b, m, q->heads, d) contiguous = softmax(scale q k^T) v over the live keys of the blocks (b, m, k->heads, count) that a
  * query names (shared by the heads of a group; an index outside the live blocks, or behind what the query may see, counts
- * for nothing, one named twice counts once); a row that sees nothing: 0.  lse (b, q->heads, m) f32 or NULL: log2 of the
- * denominator, what the backward pass needs.  q->heads / k->heads <= 64, d <= 128; workspace =
- * tpu3_block_attn_fwd_workspace_bytes bytes, 16-byte aligned (0: NULL). */
+ * for nothing, one named twice counts once); a row that sees nothing: 0.  For the backward pass, or NULL: lse
+ * (b, q->heads, m) f32, log2 of the denominator, and rest, like out, what the rounding of a 16-bit out took.
+ * q->heads / k->heads <= 64, d <= 128; workspace = tpu3_block_attn_fwd_workspace_bytes bytes, 16-byte aligned (0: NULL). */
 int tpu3_block_attn_fwd(tpu3_stream_t stream, int type, int b, int m, int n, int d, const tpu3_heads *q, const tpu3_heads *k,
                         const tpu3_heads *v, const int32_t *blocks, int count, float scale, const int32_t *n_arr,
-                        const int32_t *m_arr, int causal, void *out, float *lse, void *workspace, size_t workspace_bytes);
+                        const int32_t *m_arr, int causal, void *out, float *lse, void *rest, void *workspace,
+                        size_t workspace_bytes);
 size_t tpu3_block_attn_fwd_workspace_bytes(int b, int m, int n, int hq, int hk, int d, int count);
-/* Its gradient: o / lse of the forward call, go = the gradient of o -> dq, dk, dv contiguous (rows behind the live ones: 0).
- * Deterministic: no floating-point atomics.  workspace = tpu3_block_attn_bwd_workspace_bytes bytes, 16-byte aligned. */
+/* Its gradient: o / lse / rest (NULL: do . o from the rounded o) of the forward call, go = the gradient of o -> dq, dk, dv
+ * contiguous (rows behind the live ones: 0).  Deterministic: no floating-point atomics.  workspace = tpu3_block_attn_bwd_workspace_bytes bytes, 16-byte aligned. */
 int tpu3_block_attn_bwd(tpu3_stream_t stream, int type, int b, int m, int n, int d, const tpu3_heads *q, const tpu3_heads *k,
                         const tpu3_heads *v, const tpu3_heads *o, const tpu3_heads *go, const int32_t *blocks, int count,
-                        float scale, const int32_t *n_arr, const int32_t *m_arr, int causal, const float *lse, void *dq,
-                        void *dk, void *dv, void *workspace, size_t workspace_bytes);
+                        float scale, const int32_t *n_arr, const int32_t *m_arr, int causal, const float *lse,
+                        const void *rest, void *dq, void *dk, void *dv, void *workspace, size_t workspace_bytes);
 size_t tpu3_block_attn_bwd_workspace_bytes(int b, int m, int n, int hq, int hk);
 
 /* ---- measurement hooks (bench.py and tools/ only; a caller of the path never needs them) ------------
