@@ -38,7 +38,8 @@ struct BaArgs {
     float *delta;                           // (b, hq, m): do . o
     float *gmax;                            // (b, hq, m): largest |do| of the row
     uint64_t *bits;                         // (b, hk, nb, mt): bit = query of the tile of 64 picked the block
-    float *part;                            // split forward: (rows, splits, d + 2)
+    float *part;                            // split forward: (rows, splits, d + 4); split dk / dv: (splits, blocks, 2, 64, d)
+    int32_t *used;                          // split dk / dv: (splits, blocks), the part holds something
     int b, m, n, nb, mt, hq, hk, group, d, count, causal, splits, tiles, qt, cap;
     float scale, scale2;                    // scale2 = scale * log2(e)
 };
@@ -116,6 +117,18 @@ template <typename T> __device__ __forceinline__ typename hd_vec<T>::v8 ba_pack(
     return f;
 }
 
+template <typename T> __device__ __forceinline__ typename hd_vec<T>::v8 ba_ones()
+{
+    typename hd_vec<T>::v8 f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if constexpr (sizeof(T) == 4)
+            f.v[i] = 1.f;
+        else
+            f[i] = (T)1.f;
+    return f;
+}
+
 template <typename T> __device__ __forceinline__ void ba_store4(T *p, const hd_f4 &x)
 {
     typename hd_vec<T>::v4 y;
@@ -138,16 +151,21 @@ template <typename T> __device__ __forceinline__ void ba_store_rest(T *p, T *res
     }
 }
 
-// maximum / sum over the four lane groups that hold a column (lanes l, l+16, l+32, l+48)
+// maximum / sum over the four lane groups that hold a column (lanes l, l+16, l+32, l+48): swapping a register with itself
+// between halves (rows) of the wave gives both sides' values, without a trip through LDS
 __device__ __forceinline__ float ba_col_max(float v)
 {
-    v = fmaxf(v, __shfl_xor(v, 16, 64));
-    return fmaxf(v, __shfl_xor(v, 32, 64));
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
 }
 __device__ __forceinline__ float ba_col_sum(float v)
 {
-    v += __shfl_xor(v, 16, 64);
-    return v + __shfl_xor(v, 32, 64);
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
 // ---- staging of a 64-row tile ------------------------------------------------------------------------------------------
@@ -191,6 +209,12 @@ template <typename T, int DP> struct BaStage {
             *(typename hd_vec<T>::v8 *)(tile + row * (DP + BaPad<T>::v) + c) = r[i];
         }
     }
+};
+
+// waves a SIMD that the register allocation aims at
+template <typename T, int DP> struct BaWaves {
+    static constexpr int v = sizeof(T) == 4 ? (DP == 128 ? 1 : DP == 64 ? 2 : 3) : DP == 128 ? 2 : 3;
+    static constexpr int dkv = sizeof(T) == 4 ? (DP == 128 ? 1 : 2) : DP == 128 ? 2 : 3;
 };
 
 struct BaTile {                             // which rows a workgroup has
@@ -310,7 +334,7 @@ __device__ __forceinline__ void ba_row_operand(const T *p, bool live, int d, typ
 
 // ---- forward -----------------------------------------------------------------------------------------------------------
 template <typename T, int DP>
-__global__ __launch_bounds__(BA_THREADS) void block_attn_fwd_kernel(BaArgs a, int64_t all)
+__global__ __launch_bounds__(BA_THREADS, (BaWaves<T, DP>::v)) void block_attn_fwd_kernel(BaArgs a, int64_t all)
 {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ unsigned long long odd;      // careful pass: rows of the tile that hold a value that is not finite
@@ -333,7 +357,8 @@ __global__ __launch_bounds__(BA_THREADS) void block_attn_fwd_kernel(BaArgs a, in
     const T *K = (const T *)a.k.data + t.b * a.k.sb + t.h * a.k.sh, *V = (const T *)a.v.data + t.b * a.v.sb + t.h * a.v.sh;
 
     hd_f4 acc[DP / 16];
-    float top, sum;                         // running maximum of the column; this lane's share of its sum
+    hd_f4 sums;                             // running sum of the column, in every register
+    float top;                              // running maximum of the column
     // A value that is not finite, times the probability 0 of a row that does not see it, is not 0: in the matrix product it
     // would reach every row of the wave.  A workgroup that ends with such an output runs a second, careful pass, which
     // leaves these values out of the matrix product and adds them to the rows that see them one by one.
@@ -341,7 +366,7 @@ __global__ __launch_bounds__(BA_THREADS) void block_attn_fwd_kernel(BaArgs a, in
 #pragma unroll
         for (int c = 0; c < DP / 16; ++c)
             acc[c] = hd_f4{0.f, 0.f, 0.f, 0.f};
-        top = -INFINITY, sum = 0.f;
+        top = -INFINITY, sums = hd_f4{0.f, 0.f, 0.f, 0.f};
 
         BaStage<T, DP> kr, vr;
         if (t.z < count) {
@@ -396,16 +421,17 @@ __global__ __launch_bounds__(BA_THREADS) void block_attn_fwd_kernel(BaArgs a, in
             const float base = next == -INFINITY ? 0.f : next;
             const float keep = __builtin_amdgcn_exp2f(top - base);     // top = -inf: 0
             top = next;
-            sum *= keep;
+            // a row that did not pick the block: exp2(x - inf) = 0 (a score that is not finite is left to the careful pass)
+            const float off = bit ? base : INFINITY;
 #pragma unroll
             for (int x = 0; x < 4; ++x)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][r], a.scale2, -base));
-                    s[x][r] = bit ? p : 0.f;
-                    sum += s[x][r];
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][r], a.scale2, -off));
+                    s[x][r] = careful ? (bit ? p : 0.f) : p;
                 }
             if (__any(keep != 1.f)) {
+                sums *= keep;
 #pragma unroll
                 for (int c = 0; c < DP / 16; ++c)
                     acc[c] *= keep;
@@ -413,6 +439,8 @@ __global__ __launch_bounds__(BA_THREADS) void block_attn_fwd_kernel(BaArgs a, in
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const typename hd_vec<T>::v8 pf = ba_pack<T>(s[2 * j], s[2 * j + 1]);
+                // the denominator as one more row of the product: ones times the probabilities, as rounded as they are there
+                sums = ba_mma<T>(ba_ones<T>(), pf, sums);
 #pragma unroll
                 for (int c = 0; c < DP / 16; ++c)
                     acc[c] = ba_mma<T>(ba_column<T, STRIDE>(Vs, j * 32, c * 16), pf, acc[c]);
@@ -446,10 +474,11 @@ __global__ __launch_bounds__(BA_THREADS) void block_attn_fwd_kernel(BaArgs a, in
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 finite &= fabsf(acc[c][r]) <= 3.4028235e38f;
+        finite &= fabsf(sums[0]) <= 3.4028235e38f;
         if (careful || !__syncthreads_or(!finite))
             break;
     }
-    sum = ba_col_sum(sum);
+    const float sum = sums[0];
     const bool row_there = ql < a.qt && i < a.m;
     if (!row_there)
         return;
@@ -519,7 +548,7 @@ __device__ __forceinline__ float ba_pow2_inverse(float x)
 }
 
 template <typename T, int DP>
-__global__ __launch_bounds__(BA_THREADS) void block_attn_dq_kernel(BaArgs a, int64_t all)
+__global__ __launch_bounds__(BA_THREADS, (BaWaves<T, DP>::v)) void block_attn_dq_kernel(BaArgs a, int64_t all)
 {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ unsigned long long odd;
@@ -681,15 +710,8 @@ __global__ __launch_bounds__(BA_THREADS) void block_pick_bits_kernel(BaArgs a)
 // out with a key per lane: the B operand of dv^T = do^T P and dk^T = q^T dS.
 constexpr int BD_WORDS = 64;                // tiles of queries looked through at a time
 
-template <typename T, int DP> struct BaDkv {
-    static constexpr int STRIDE = BaLds<T, DP>::STRIDE;
-    T *Qs, *Gs;
-    float *lse, *delta, *gmax;
-    int *limit, *list;
-};
-
 template <typename T, int DP>
-__global__ __launch_bounds__(BA_THREADS) void block_attn_dkv_kernel(BaArgs a, int64_t all)
+__global__ __launch_bounds__(BA_THREADS, (BaWaves<T, DP>::dkv)) void block_attn_dkv_kernel(BaArgs a, int64_t all)
 {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ int wave_total[4];
@@ -700,7 +722,7 @@ __global__ __launch_bounds__(BA_THREADS) void block_attn_dkv_kernel(BaArgs a, in
     int *limit_s = (int *)(gmax_s + 64), *list = limit_s + 64;              // list: BD_WORDS * 64 queries
 
     const int64_t id = ba_xcd(blockIdx.x, all);
-    const int blk = (int)(id % a.nb), bh = (int)(id / a.nb), h = bh % a.hk, b = bh / a.hk;
+    const int z = (int)(id % a.splits), blk = (int)(id / a.splits % a.nb), bh = (int)(id / a.splits / a.nb), h = bh % a.hk, b = bh / a.hk;
     const int live = a.n_arr ? min(max(a.n_arr[b], 0), a.n) : a.n, lm = a.m_arr ? min(max(a.m_arr[b], 0), a.m) : a.m;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
     const int key = blk * BA_BLOCK + wave * 16 + l15;
@@ -714,10 +736,43 @@ __global__ __launch_bounds__(BA_THREADS) void block_attn_dkv_kernel(BaArgs a, in
     float up = 1.f;                         // fp16: dk is accumulated times this power of two
     bool first = true;
     const uint64_t *bits = a.bits + ((int64_t)bh * a.nb + blk) * a.mt;
+    const int per = (a.mt + a.splits - 1) / a.splits, end = min(a.mt, (z + 1) * per);
+    bool any = false;
 
-    for (int w0 = 0; w0 < a.mt; w0 += BD_WORDS) {
+    constexpr int CHUNKS = DP / 8, PER = BA_ROWS * CHUNKS / BA_THREADS;
+    typename hd_vec<T>::v8 qr[PER], gr[PER];
+    float row_lse = 0.f, row_delta = 0.f, row_gmax = 0.f;
+    int row_limit = 0;
+    // rows r0 .. r0 + 63 of the list (query by query, all heads of the group) to registers; rows behind the last are zeros
+    // that see nothing
+    auto fetch = [&](int r0, int rows) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < PER; ++x) {
+            const int e = x * BA_THREADS + threadIdx.x, r = r0 + e / CHUNKS, c = (e % CHUNKS) * 8;
+            if (r < rows && c < a.d) {
+                const int q = r / a.group, head = h * a.group + (r - q * a.group);
+                const int64_t i = list[q];
+                qr[x] = *(const typename hd_vec<T>::v8 *)((const T *)a.q.data + b * a.q.sb + i * a.q.sr + (int64_t)head * a.q.sh + c);
+                gr[x] = *(const typename hd_vec<T>::v8 *)((const T *)a.go.data + b * a.go.sb + i * a.go.sr + (int64_t)head * a.go.sh + c);
+            } else {
+                qr[x] = ba_zero<T>();
+                gr[x] = ba_zero<T>();
+            }
+        }
+        row_lse = row_delta = row_gmax = 0.f;
+        row_limit = 0;
+        if (threadIdx.x < BA_ROWS && r0 + (int)threadIdx.x < rows) {
+            const int r = r0 + threadIdx.x, q = r / a.group, head = h * a.group + (r - q * a.group), i = list[q];
+            const int64_t p = ((int64_t)b * a.hq + head) * a.m + i;
+            row_lse = a.lse[p], row_delta = a.delta[p], row_limit = ba_limit(a, live, lm, i);
+            if (HALF)
+                row_gmax = a.gmax[p];
+        }
+    };
+
+    for (int w0 = z * per; w0 < end; w0 += BD_WORDS) {
         // the queries of the next 64 tiles that picked this block, in order
-        const int words = min(BD_WORDS, a.mt - w0);
+        const int words = min(BD_WORDS, end - w0);
         uint64_t word = 0;
         int at = 0, total = 0;
         if (wave == 0) {
@@ -738,31 +793,10 @@ __global__ __launch_bounds__(BA_THREADS) void block_attn_dkv_kernel(BaArgs a, in
         __syncthreads();
         total = wave_total[0];
         const int rows = total * a.group;
+        any |= rows > 0;
+        if (rows > 0)
+            fetch(0, rows);
         for (int r0 = 0; r0 < rows; r0 += BA_ROWS) {
-            constexpr int CHUNKS = DP / 8, PER = BA_ROWS * CHUNKS / BA_THREADS;
-            typename hd_vec<T>::v8 qr[PER], gr[PER];
-#pragma unroll
-            for (int x = 0; x < PER; ++x) {
-                const int e = x * BA_THREADS + threadIdx.x, r = r0 + e / CHUNKS, c = (e % CHUNKS) * 8;
-                if (r < rows && c < a.d) {
-                    const int q = r / a.group, head = h * a.group + (r - q * a.group);
-                    const int64_t i = list[q];
-                    qr[x] = *(const typename hd_vec<T>::v8 *)((const T *)a.q.data + b * a.q.sb + i * a.q.sr + (int64_t)head * a.q.sh + c);
-                    gr[x] = *(const typename hd_vec<T>::v8 *)((const T *)a.go.data + b * a.go.sb + i * a.go.sr + (int64_t)head * a.go.sh + c);
-                } else {
-                    qr[x] = ba_zero<T>();
-                    gr[x] = ba_zero<T>();
-                }
-            }
-            float row_lse = 0.f, row_delta = 0.f, row_gmax = 0.f;
-            int row_limit = 0;
-            if (threadIdx.x < BA_ROWS && r0 + (int)threadIdx.x < rows) {
-                const int r = r0 + threadIdx.x, q = r / a.group, head = h * a.group + (r - q * a.group), i = list[q];
-                const int64_t p = ((int64_t)b * a.hq + head) * a.m + i;
-                row_lse = a.lse[p], row_delta = a.delta[p], row_limit = ba_limit(a, live, lm, i);
-                if (HALF)
-                    row_gmax = a.gmax[p];
-            }
             __syncthreads();                // the previous tile has been read
 #pragma unroll
             for (int x = 0; x < PER; ++x) {
@@ -776,6 +810,8 @@ __global__ __launch_bounds__(BA_THREADS) void block_attn_dkv_kernel(BaArgs a, in
                     gmax_s[threadIdx.x] = row_gmax;
             }
             __syncthreads();
+            if (r0 + BA_ROWS < rows)
+                fetch(r0 + BA_ROWS, rows);
             if (HALF) {
                 // the largest |do| of the rows so far decides the power of two (every wave finds the same)
                 float m = gmax_s[lane];
@@ -824,16 +860,48 @@ __global__ __launch_bounds__(BA_THREADS) void block_attn_dkv_kernel(BaArgs a, in
         }
         __syncthreads();                    // the list is rebuilt
     }
+    const float back = HALF ? a.scale / up : a.scale;
+    if (a.splits > 1) {                     // a part of the queries: joined by block_attn_dkv_join_kernel
+        const int64_t tile = ((int64_t)z * a.b * a.hk + bh) * a.nb + blk;
+        if (threadIdx.x == 0)
+            a.used[tile] = any;
+        if (!any)
+            return;
+        float *P = a.part + (tile * 2 * BA_BLOCK + wave * 16 + l15) * DP;
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) {
+            *(hd_f4 *)(P + c * 16 + g * 4) = dk[c] * back;
+            *(hd_f4 *)(P + BA_BLOCK * DP + c * 16 + g * 4) = dv[c];
+        }
+        return;
+    }
     if (key >= a.n)
         return;
     const int64_t at = (((int64_t)b * a.n + key) * a.hk + h) * a.d;
-    const float back = HALF ? a.scale / up : a.scale;
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c)
         if (c * 16 + g * 4 < a.d) {
             ba_store4<T>((T *)a.out + at + c * 16 + g * 4, dk[c] * back);
             ba_store4<T>((T *)a.out2 + at + c * 16 + g * 4, dv[c]);
         }
+}
+
+// dk and dv of a block from its parts, in the parts' order
+template <typename T, int DP> __global__ __launch_bounds__(BA_THREADS) void block_attn_dkv_join_kernel(BaArgs a)
+{
+    const int blk = (int)(blockIdx.x % a.nb), bh = (int)(blockIdx.x / a.nb), h = bh % a.hk, b = bh / a.hk;
+    const int64_t parts = (int64_t)a.b * a.hk * a.nb, tile = (int64_t)bh * a.nb + blk;
+    for (int e = threadIdx.x; e < 2 * BA_BLOCK * DP / 4; e += BA_THREADS) {
+        const int row = e / (DP / 4), c = (e % (DP / 4)) * 4, key = blk * BA_BLOCK + row % BA_BLOCK;
+        if (key >= a.n || c >= a.d)
+            continue;
+        hd_f4 y = {0.f, 0.f, 0.f, 0.f};
+        for (int z = 0; z < a.splits; ++z)
+            if (a.used[z * parts + tile])
+                y += *(const hd_f4 *)(a.part + ((z * parts + tile) * 2 * BA_BLOCK + row) * DP + c);
+        T *O = (T *)(row < BA_BLOCK ? a.out : a.out2);
+        ba_store4<T>(O + (((int64_t)b * a.n + key) * a.hk + h) * a.d + c, y);
+    }
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------
@@ -876,6 +944,19 @@ int ba_splits(int b, int m, int n, int hq, int hk, int count)
     int64_t s = 512 / tiles, most = used < nb ? used : nb;
     s = s < most ? s : most;
     return s < 1 ? 1 : s > 64 ? 64 : (int)s;
+}
+
+// Parts of the queries for dk and dv: some blocks are picked by many more queries than others (the first of a sequence by
+// nearly all), and few blocks leave the chip waiting for the longest one.  A part holds 512 queries at least.
+int ba_dkv_splits(int b, int m, int hk, int nb)
+{
+    const int64_t blocks = (int64_t)b * hk * nb;
+    if (blocks <= 0 || blocks >= 1024)
+        return 1;
+    int64_t s = (2047 + blocks) / blocks;
+    const int64_t most = ((int64_t)m + 511) / 512;
+    s = s < most ? s : most;
+    return s > 8 ? 8 : s < 1 ? 1 : (int)s;
 }
 
 int ba_dp(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
@@ -922,7 +1003,10 @@ template <typename T, int DP> int ba_backward(BaArgs a, void *dq, void *dk, void
         return rc;
     a.out = dk, a.out2 = dv;
     const int64_t blocks = (int64_t)a.b * a.hk * a.nb;
-    hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP>), dim3((unsigned)blocks), dim3(BA_THREADS), lds2, s, a, blocks);
+    a.splits = ba_dkv_splits(a.b, a.m, a.hk, a.nb);
+    hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP>), dim3((unsigned)(blocks * a.splits)), dim3(BA_THREADS), lds2, s, a, blocks * a.splits);
+    if (a.splits > 1)
+        hipLaunchKernelGGL((block_attn_dkv_join_kernel<T, DP>), dim3((unsigned)blocks), dim3(BA_THREADS), 0, s, a);
     return tpu3_launch_status();
 }
 
@@ -967,12 +1051,31 @@ extern "C" int tpu3_block_attn_fwd(tpu3_stream_t stream, int type, int b, int m,
     return type == TPU3_TYPE_F32 ? ba_forward_d<float>(a, s) : type == TPU3_TYPE_F16 ? ba_forward_d<_Float16>(a, s) : ba_forward_d<__bf16>(a, s);
 }
 
-extern "C" size_t tpu3_block_attn_bwd_workspace_bytes(int b, int m, int n, int hq, int hk)
+namespace {
+// the parts of the backward workspace: bits, delta, gmax, used, part
+struct BaBwdLayout {
+    size_t delta, gmax, used, part, bytes;
+};
+BaBwdLayout ba_bwd_layout(int b, int m, int n, int hq, int hk, int d)
 {
-    if (b <= 0 || m <= 0 || hq <= 0 || hk <= 0)
+    const size_t nb = n > 0 ? (size_t)(n - 1) / BA_BLOCK + 1 : 0, mt = ((size_t)m + 63) / 64, blocks = (size_t)b * hk * nb;
+    const size_t splits = (size_t)ba_dkv_splits(b, m, hk, (int)nb);
+    auto up = [](size_t x) { return (x + 15) / 16 * 16; };
+    BaBwdLayout l;
+    l.delta = up(blocks * mt * 8);
+    l.gmax = l.delta + up((size_t)b * hq * m * 4);
+    l.used = l.gmax + up((size_t)b * hq * m * 4);
+    l.part = l.used + (splits > 1 ? up(splits * blocks * 4) : 0);
+    l.bytes = l.part + (splits > 1 ? splits * blocks * 2 * BA_BLOCK * ba_dp(d) * 4 : 0);
+    return l;
+}
+}  // namespace
+
+extern "C" size_t tpu3_block_attn_bwd_workspace_bytes(int b, int m, int n, int hq, int hk, int d)
+{
+    if (b <= 0 || m <= 0 || hq <= 0 || hk <= 0 || d <= 0)
         return 0;
-    const size_t nb = n > 0 ? (size_t)(n - 1) / BA_BLOCK + 1 : 0, mt = ((size_t)m + 63) / 64;
-    return (size_t)b * hk * nb * mt * 8 + (size_t)b * hq * m * 8;
+    return ba_bwd_layout(b, m, n, hq, hk, d).bytes;
 }
 
 extern "C" int tpu3_block_attn_bwd(tpu3_stream_t stream, int type, int b, int m, int n, int d, const tpu3_heads *q,
@@ -987,12 +1090,15 @@ extern "C" int tpu3_block_attn_bwd(tpu3_stream_t stream, int type, int b, int m,
         return rc;
     if (!hd_rows_ok(o, type) || !hd_rows_ok(go, type) || o->heads != a.hq || go->heads != a.hq || !lse || !dq || ((uintptr_t)rest & 15) ||
         ((uintptr_t)dq & 15) || (n > 0 && (!dk || !dv || ((uintptr_t)dk & 15) || ((uintptr_t)dv & 15))) || !workspace ||
-        ((uintptr_t)workspace & 7) || workspace_bytes < tpu3_block_attn_bwd_workspace_bytes(b, m, n, a.hq, a.hk))
+        ((uintptr_t)workspace & 15) || workspace_bytes < tpu3_block_attn_bwd_workspace_bytes(b, m, n, a.hq, a.hk, d))
         return TPU3_EINVAL;
     a.o = *o, a.go = *go, a.lse = (float *)lse, a.rest = type == TPU3_TYPE_F32 ? nullptr : (void *)rest;
+    const BaBwdLayout l = ba_bwd_layout(b, m, n, a.hq, a.hk, d);
     a.bits = (uint64_t *)workspace;
-    a.delta = (float *)(a.bits + (size_t)b * a.hk * a.nb * a.mt);
-    a.gmax = a.delta + (size_t)b * a.hq * m;
+    a.delta = (float *)((char *)workspace + l.delta);
+    a.gmax = (float *)((char *)workspace + l.gmax);
+    a.used = (int32_t *)((char *)workspace + l.used);
+    a.part = (float *)((char *)workspace + l.part);
     const hipStream_t s = (hipStream_t)stream;
     return type == TPU3_TYPE_F32 ? ba_backward_d<float>(a, dq, dk, dv, s) : type == TPU3_TYPE_F16 ? ba_backward_d<_Float16>(a, dq, dk, dv, s) : ba_backward_d<__bf16>(a, dq, dk, dv, s);
 }

@@ -10,8 +10,11 @@
 // of a row are a few lane exchanges.  The turns are shared by all heads of a token: a workgroup takes a few tokens,
 // computes their cosines and sines once into LDS and then runs over the tokens' rows.  Angles are formed and reduced in
 // 64 bits (a position of 1e5 times a frequency of 1 leaves 7 of fp32's 24 bits for the fraction of a turn), the sine and
-// cosine of the fraction in 32.  The partner of a channel in the half-split order sits in another lane: the normed row
-// goes through the workgroup's LDS (four times the HBM bytes, at an aggregate LDS rate of ten times HBM's).
+// cosine of the fraction in 32.  Both pair orders use one expression, z[c] = y[c] C[c] + y[partner(c)] S[c], with the sign
+// folded into S and C = 1, S = 0 behind the pairs.  In the half-split order the partner sits in another lane: the normed row
+// goes through LDS with its first half stored a second time behind the second, so that the partner of channel c is
+// always c + P places from the start (P pairs) and every lane reads eight consecutive floats.
+// The next row is requested before the current one is worked on (a wave otherwise has 1 KB in flight, and the chip 7 MB).
 #include "heads.h"
 
 namespace {
@@ -34,13 +37,19 @@ struct NrArgs {
     float eps, inv_d;
 };
 
-__device__ __forceinline__ float nr_weight(const void *w, int type, int i)
+__device__ __forceinline__ void nr_weights(const void *w, int type, int i, float *y)
 {
-    if (type == TPU3_TYPE_F32)
-        return ((const float *)w)[i];
-    if (type == TPU3_TYPE_F16)
-        return (float)((const _Float16 *)w)[i];
-    return (float)((const __bf16 *)w)[i];
+    if (!w) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            y[j] = 1.f;
+    } else if (type == TPU3_TYPE_F32) {
+        hd_load8((const float *)w + i, y);
+    } else if (type == TPU3_TYPE_F16) {
+        hd_load8((const _Float16 *)w + i, y);
+    } else {
+        hd_load8((const __bf16 *)w + i, y);
+    }
 }
 __device__ __forceinline__ double nr_position(const void *p, int type, int64_t i)
 {
@@ -53,12 +62,12 @@ __device__ __forceinline__ double nr_position(const void *p, int type, int64_t i
     return (double)((const int64_t *)p)[i];
 }
 
-// cosines and sines of the workgroup's tokens: cs[t * total_pairs + p]
-__device__ __forceinline__ void nr_turns(const NrArgs &a, int64_t t0, int count, float2 *cs)
+// C and S of the workgroup's tokens: cs[(t * 2 + which) * d + c]
+__device__ __forceinline__ void nr_turns(const NrArgs &a, int64_t t0, int count, float sign, float *cs)
 {
-    const int all = count * a.total_pairs;
-    for (int i = threadIdx.x; i < all; i += NR_THREADS) {
-        const int t = i / a.total_pairs, p = i - t * a.total_pairs, ax = p / a.pairs;
+    const int P = a.total_pairs, rest = a.d - 2 * P;
+    for (int i = threadIdx.x; i < count * P; i += NR_THREADS) {
+        const int t = i / P, p = i - t * P, ax = p / a.pairs;
         const int64_t tok = t0 + t, e = tok / a.n, r = tok - e * a.n;
         const double pos = nr_position(a.pos, a.pos_type, e * a.pos_sb + r * a.pos_sn + ax * a.pos_sa);
         const double f = a.freq_type == TPU3_POS_F64 ? ((const double *)a.freq)[p] : (double)((const float *)a.freq)[p];
@@ -66,7 +75,16 @@ __device__ __forceinline__ void nr_turns(const NrArgs &a, int64_t t0, int count,
         turn -= rint(turn);
         float s, c;
         sincospif(2.f * (float)turn, &s, &c);
-        cs[i] = make_float2(c, s);
+        const int one = a.interleaved ? 2 * p : p, two = a.interleaved ? 2 * p + 1 : p + P;
+        float *C = cs + t * 2 * a.d, *S = C + a.d;
+        C[one] = C[two] = c;
+        S[one] = -sign * s;
+        S[two] = sign * s;
+    }
+    for (int i = threadIdx.x; i < count * rest; i += NR_THREADS) {
+        const int t = i / rest, c = 2 * P + (i - t * rest);
+        cs[t * 2 * a.d + c] = 1.f;
+        cs[(t * 2 + 1) * a.d + c] = 0.f;
     }
 }
 
@@ -78,101 +96,117 @@ template <int LPR> __device__ __forceinline__ float nr_row_sum(float v)
     return v;
 }
 
-// eight channels from c0 on turned by (c, sign * s); `row` is this row's slice of the exchange buffer
-__device__ __forceinline__ void nr_turn(const NrArgs &a, const float2 *cs, float *row, int c0, float sign, float *y)
+// floats of an exchange row: the channels, the first half again, and zeros up to the last place that is read
+__host__ __device__ __forceinline__ int nr_row(int d, int pairs, int interleaved) { return interleaved ? 0 : d + (pairs + 3) / 4 * 4 + 4; }
+
+// eight channels from c0 on turned; `row` is this row's exchange slice
+__device__ __forceinline__ void nr_turn(const NrArgs &a, const float *cs, float *row, int c0, float *y)
 {
-    const int P = a.total_pairs;
+    float o[8];
     if (a.interleaved) {
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-            const int p = (c0 + i) >> 1;
-            if (p < P) {
-                const float2 t = cs[p];
-                const float s = sign * t.y, u = y[i], v = y[i + 1];
-                y[i] = __builtin_fmaf(u, t.x, -v * s);
-                y[i + 1] = __builtin_fmaf(u, s, v * t.x);
-            }
-        }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; i += 4)
-        *(hd_f4 *)(row + c0 + i) = hd_f4{y[i], y[i + 1], y[i + 2], y[i + 3]};
-    __builtin_amdgcn_wave_barrier();        // the row's lanes are in one wave, whose LDS accesses complete in order
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (c0 + 8 <= P && (P & 3) == 0) {                          // all eight are first partners
-        const float *o = row + c0 + P;
-        const hd_f4 o0 = *(const hd_f4 *)o, o1 = *(const hd_f4 *)(o + 4);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float2 t = cs[c0 + i];
-            y[i] = __builtin_fmaf(y[i], t.x, -(i < 4 ? o0[i & 3] : o1[i & 3]) * (sign * t.y));
-        }
-    } else if (c0 >= P && c0 + 8 <= 2 * P && (P & 3) == 0) {    // all eight are second partners
-        const float *o = row + c0 - P;
-        const hd_f4 o0 = *(const hd_f4 *)o, o1 = *(const hd_f4 *)(o + 4);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float2 t = cs[c0 - P + i];
-            y[i] = __builtin_fmaf(i < 4 ? o0[i & 3] : o1[i & 3], sign * t.y, y[i] * t.x);
-        }
+        for (int i = 0; i < 8; ++i)
+            o[i] = y[i ^ 1];
     } else {
+        const int P = a.total_pairs;
+        if (c0 + 8 <= 2 * P) {
+            *(hd_f4 *)(row + c0) = hd_f4{y[0], y[1], y[2], y[3]};
+            *(hd_f4 *)(row + c0 + 4) = hd_f4{y[4], y[5], y[6], y[7]};
+        } else if (c0 < 2 * P) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int c = c0 + i;
-            if (c < P) {
-                const float2 t = cs[c];
-                y[i] = __builtin_fmaf(y[i], t.x, -row[c + P] * (sign * t.y));
-            } else if (c < 2 * P) {
-                const float2 t = cs[c - P];
-                y[i] = __builtin_fmaf(row[c - P], sign * t.y, y[i] * t.x);
-            }
+            for (int i = 0; i < 8; ++i)
+                if (c0 + i < 2 * P)
+                    row[c0 + i] = y[i];
         }
+        if (c0 + 8 <= P) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                row[2 * P + c0 + i] = y[i];
+        } else if (c0 < P) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c0 + i < P)
+                    row[2 * P + c0 + i] = y[i];
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();    // the row's lanes are in one wave, whose LDS accesses complete in order
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            o[i] = row[P + c0 + i];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    const hd_f4 c_0 = *(const hd_f4 *)(cs + c0), c_1 = *(const hd_f4 *)(cs + c0 + 4);
+    const hd_f4 s_0 = *(const hd_f4 *)(cs + a.d + c0), s_1 = *(const hd_f4 *)(cs + a.d + c0 + 4);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        y[i] = __builtin_fmaf(o[i], i < 4 ? s_0[i & 3] : s_1[i & 3], y[i] * (i < 4 ? c_0[i & 3] : c_1[i & 3]));
+}
+
+// the exchange rows' places behind the second half's copy stay zero (read by channels that do not turn, times S = 0)
+__device__ __forceinline__ void nr_clear(float *ex, int all)
+{
+    for (int i = threadIdx.x; i < all; i += NR_THREADS)
+        ex[i] = 0.f;
 }
 
 template <typename T, int LPR>
 __global__ __launch_bounds__(NR_THREADS) void norm_rotate_kernel(NrArgs a)
 {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    constexpr int GROUPS = NR_THREADS / LPR, ROW = LPR * 8 + 4;
-    float *ex = (float *)smem;                                  // (GROUPS, ROW) exchange rows
-    float2 *cs = (float2 *)(ex + GROUPS * ROW);                 // (tok, total_pairs)
+    constexpr int GROUPS = NR_THREADS / LPR;
+    typedef typename hd_vec<T>::v8 V8;
+    const int len = nr_row(a.d, a.total_pairs, a.interleaved);
+    float *ex = (float *)smem, *cs = ex + GROUPS * len;         // (GROUPS, len) exchange rows, (tok, 2, d) turns
     const int64_t t0 = (int64_t)blockIdx.x * a.tok;
     const int count = (int)min((int64_t)a.tok, a.tokens - t0);
     const int grp = threadIdx.x / LPR, c0 = (threadIdx.x % LPR) * 8;
     const bool live = c0 < a.d;
-    nr_turns(a, t0, count, cs);
+    const int cr = live ? c0 : 0;           // (idle lanes of a row work on channel 0's addresses and write nothing)
+    nr_clear(ex, GROUPS * len);
+    nr_turns(a, t0, count, 1.f, cs);
     __syncthreads();
-    for (int side = 0; side < 2; ++side) {
+    const int hq = a.x[0].heads, rows = count * (hq + a.x[1].heads);
+    auto place = [&](int r, int &side, int &t, int &h) __attribute__((always_inline)) {
+        side = r < count * hq ? 0 : 1;
         const int heads = a.x[side].heads;
-        const T *X = (const T *)a.x[side].data;
-        T *Y = (T *)a.out[side];
-        for (int r = grp; r < count * heads; r += GROUPS) {
-            const int t = r / heads, h = r - t * heads;
+        r -= side ? count * hq : 0;
+        t = r / heads;
+        h = r - t * heads;
+    };
+    auto load = [&](int r, V8 &v) __attribute__((always_inline)) {
+        if (r < rows && live) {
+            int side, t, h;
+            place(r, side, t, h);
             const int64_t tok = t0 + t, e = tok / a.n, i = tok - e * a.n;
-            float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (live)
-                hd_load8(X + e * a.x[side].sb + i * a.x[side].sr + h * a.x[side].sh + c0, y);
-            float ss = 0.f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                ss = __builtin_fmaf(y[j], y[j], ss);
-            const float inv = 1.f / sqrtf(__builtin_fmaf(nr_row_sum<LPR>(ss), a.inv_d, a.eps));
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                y[j] *= inv;
-            if (a.w[side] && live) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    y[j] *= nr_weight(a.w[side], a.w_type, h * a.w_head[side] + c0 + j);
-            }
-            nr_turn(a, cs + t * a.total_pairs, ex + grp * ROW, c0, 1.f, y);
-            if (live)
-                hd_store8(Y + (tok * heads + h) * a.d + c0, y);
+            v = *(const V8 *)((const T *)a.x[side].data + e * a.x[side].sb + i * a.x[side].sr + h * a.x[side].sh + c0);
         }
+    };
+    V8 cur = {}, next = {};
+    load(grp, cur);
+    for (int r = grp; r < rows; r += GROUPS) {
+        load(r + GROUPS, next);
+        int side, t, h;
+        place(r, side, t, h);
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            y[j] = (float)cur[j];
+        float ss = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            ss = __builtin_fmaf(y[j], y[j], ss);
+        const float inv = 1.f / sqrtf(__builtin_fmaf(nr_row_sum<LPR>(ss), a.inv_d, a.eps));
+        float w[8];
+        nr_weights(a.w[side], a.w_type, h * a.w_head[side] + cr, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            y[j] = y[j] * inv * w[j];
+        if (live) {
+            nr_turn(a, cs + t * 2 * a.d, ex + grp * len, c0, y);
+            hd_store8((T *)a.out[side] + ((t0 + t) * a.x[side].heads + h) * a.d + c0, y);
+        }
+        cur = next;
     }
 }
 
@@ -184,25 +218,28 @@ template <typename T, int LPR>
 __global__ __launch_bounds__(NR_THREADS) void norm_rotate_bwd_kernel(NrArgs a, int split)
 {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    constexpr int GROUPS = NR_THREADS / LPR, ROW = LPR * 8 + 4, PER = 64 / LPR;
-    const int heads_all = a.x[0].heads + a.x[1].heads;
+    constexpr int GROUPS = NR_THREADS / LPR, PER = 64 / LPR;
+    typedef typename hd_vec<T>::v8 V8;
+    const int heads_all = a.x[0].heads + a.x[1].heads, len = nr_row(a.d, a.total_pairs, a.interleaved);
     float *ex = (float *)smem;
-    float *acc = ex + GROUPS * ROW;                             // (units, d) per-head sums
-    const bool per_head = a.w_head[0] != 0 || a.w_head[1] != 0;
+    float *acc = ex + GROUPS * len;                             // (units, d) per-head sums
+    const bool per_head = (a.w[0] && a.w_head[0]) || (a.w[1] && a.w_head[1]);
     const bool want = a.want_w[0] || a.want_w[1];
     const int units = heads_all * split;
-    float2 *cs = (float2 *)(acc + (want ? (per_head ? units : 8) * a.d : 0));
+    float *cs = acc + (want ? (per_head ? units : 8) * a.d : 0);
     const int grp = threadIdx.x / LPR, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c0 = (threadIdx.x % LPR) * 8;
     const bool live = c0 < a.d;
+    const int cr = live ? c0 : 0;
     const int part_tok = (a.tok + split - 1) / split;
     float ws[2][8] = {};
+    nr_clear(ex, GROUPS * len);
     if (want && per_head)
         for (int i = threadIdx.x; i < units * a.d; i += NR_THREADS)
             acc[i] = 0.f;
     for (int64_t t0 = (int64_t)blockIdx.x * a.tok; t0 < a.tokens; t0 += (int64_t)gridDim.x * a.tok) {
         const int count = (int)min((int64_t)a.tok, a.tokens - t0);
         __syncthreads();
-        nr_turns(a, t0, count, cs);
+        nr_turns(a, t0, count, -1.f, cs);
         __syncthreads();
         for (int u = wave; u < units; u += 4) {
             const int hu = u / split, s = u - hu * split;
@@ -212,21 +249,28 @@ __global__ __launch_bounds__(NR_THREADS) void norm_rotate_bwd_kernel(NrArgs a, i
             T *Y = (T *)a.out[side];
             const int last = min(count, (s + 1) * part_tok);
             float w[8], wg[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                w[j] = a.w[side] && live ? nr_weight(a.w[side], a.w_type, h * a.w_head[side] + c0 + j) : 1.f;
+            nr_weights(a.w[side], a.w_type, h * a.w_head[side] + cr, w);
+            V8 xc = {}, gc = {}, xn = {}, gn = {};
+            auto load = [&](int t, V8 &x, V8 &g) __attribute__((always_inline)) {
+                if (t < last && live) {
+                    const int64_t tok = t0 + t, e = tok / a.n, i = tok - e * a.n;
+                    x = *(const V8 *)(X + e * a.x[side].sb + i * a.x[side].sr);
+                    g = *(const V8 *)(G + e * a.g[side].sb + i * a.g[side].sr);
+                }
+            };
+            const int tl = lane / LPR;
+            load(s * part_tok + tl, xc, gc);
             // (whole waves run the loop: the lanes of a row exchange values inside)
             for (int tb = s * part_tok; tb < last; tb += PER) {
-                const int t = tb + lane / LPR;
+                const int t = tb + tl, tc = min(t, last - 1);
                 const bool row = t < last && live;
-                const int tc = min(t, last - 1);
-                const int64_t tok = t0 + tc, e = tok / a.n, i = tok - e * a.n;
-                float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, g[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                if (row) {
-                    hd_load8(X + e * a.x[side].sb + i * a.x[side].sr, x);
-                    hd_load8(G + e * a.g[side].sb + i * a.g[side].sr, g);
-                }
-                nr_turn(a, cs + tc * a.total_pairs, ex + grp * ROW, c0, -1.f, g);
+                load(t + PER, xn, gn);
+                float x[8], g[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    x[j] = row ? (float)xc[j] : 0.f, g[j] = row ? (float)gc[j] : 0.f;
+                if (live)
+                    nr_turn(a, cs + tc * 2 * a.d, ex + grp * len, c0, g);
                 float ss = 0.f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
@@ -236,7 +280,7 @@ __global__ __launch_bounds__(NR_THREADS) void norm_rotate_bwd_kernel(NrArgs a, i
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     x[j] *= inv;
-                    wg[j] = __builtin_fmaf(g[j], x[j], wg[j]);
+                    wg[j] = row ? __builtin_fmaf(g[j], x[j], wg[j]) : wg[j];
                     g[j] *= w[j];
                     dot = __builtin_fmaf(g[j], x[j], dot);
                 }
@@ -245,7 +289,8 @@ __global__ __launch_bounds__(NR_THREADS) void norm_rotate_bwd_kernel(NrArgs a, i
                 for (int j = 0; j < 8; ++j)
                     g[j] = inv * __builtin_fmaf(-x[j], dot, g[j]);
                 if (row)
-                    hd_store8(Y + (tok * heads + h) * a.d + c0, g);
+                    hd_store8(Y + ((t0 + t) * heads + h) * a.d + c0, g);
+                xc = xn, gc = gn;
             }
             if (!want)
                 continue;
@@ -324,19 +369,19 @@ struct NrPlan {
 };
 
 // Tokens of a workgroup: enough rows to fill its 256 threads, few enough that the chip's 256 compute units all get some.
-NrPlan nr_plan(int64_t tokens, int heads, int d, int pairs, bool bwd, bool per_head, bool want)
+NrPlan nr_plan(int64_t tokens, int heads, int d, int pairs, int interleaved, bool bwd, bool per_head, bool want)
 {
     NrPlan p;
     p.lpr = d <= 32 ? 4 : d <= 64 ? 8 : d <= 128 ? 16 : 32;
     p.tok = bwd ? 64 : 16;
     while (p.tok > 1 && (tokens + p.tok - 1) / p.tok < 1024)
         p.tok >>= 1;
-    while (p.tok > 1 && (size_t)p.tok * pairs * 8 > 32768)
+    while (p.tok > 1 && (size_t)p.tok * d * 8 > 32768)
         p.tok >>= 1;
     const int64_t tiles = (tokens + p.tok - 1) / p.tok;
     p.split = bwd && heads % 4 ? (p.tok >= 4 ? 4 : 1) : 1;
     p.wgs = bwd ? (int)(tiles < NR_MAX_WG ? tiles : NR_MAX_WG) : 0;
-    p.lds = (size_t)(NR_THREADS / p.lpr) * (p.lpr * 8 + 4) * 4 + (size_t)p.tok * pairs * 8;
+    p.lds = (size_t)(NR_THREADS / p.lpr) * nr_row(d, pairs, interleaved) * 4 + (size_t)p.tok * d * 8;
     if (bwd && want)
         p.lds += (size_t)(per_head ? heads * p.split : 8) * d * 4;
     return p;
@@ -361,8 +406,10 @@ int nr_fill(NrArgs &a, int type, int b, int n, int d, const tpu3_heads *q, const
         return TPU3_EINVAL;
     if (pos->pairs && (!pos->data || !pos->freq))
         return TPU3_EINVAL;
+    if (((uintptr_t)wq & 15) || ((uintptr_t)wk & 15) || (wq && wk && k->heads && (wq_head == 0) != (wk_head == 0)))
+        return TPU3_EINVAL;
     a.x[0] = *q, a.x[1] = *k;
-    a.w[0] = wq, a.w[1] = wk, a.w_head[0] = wq_head, a.w_head[1] = wk_head, a.w_type = w_type;
+    a.w[0] = wq, a.w[1] = k->heads ? wk : nullptr, a.w_head[0] = wq_head, a.w_head[1] = wk_head, a.w_type = w_type;
     a.pos = pos->data, a.pos_type = pos->type, a.pos_sb = pos->sb, a.pos_sn = pos->sr, a.pos_sa = pos->sa;
     a.freq = pos->freq, a.freq_type = pos->freq_type, a.axes = pos->axes, a.pairs = pos->pairs > 0 ? pos->pairs : 1;
     a.total_pairs = pos->axes * pos->pairs;
@@ -422,7 +469,7 @@ extern "C" int tpu3_norm_rotate_fwd(tpu3_stream_t stream, int type, int b, int n
     if (!oq || ((uintptr_t)oq & 15) || (k->heads && (!ok || ((uintptr_t)ok & 15))))
         return TPU3_EINVAL;
     a.out[0] = oq, a.out[1] = ok;
-    const NrPlan p = nr_plan(a.tokens, q->heads + k->heads, d, a.total_pairs, false, false, false);
+    const NrPlan p = nr_plan(a.tokens, q->heads + k->heads, d, a.total_pairs, a.interleaved, false, false, false);
     if ((a.tokens + p.tok - 1) / p.tok > 0x7FFFFFFFLL)
         return TPU3_ELIMIT;
     a.tok = p.tok;
@@ -456,12 +503,12 @@ extern "C" int tpu3_norm_rotate_bwd(tpu3_stream_t stream, int type, int b, int n
         a.g[1] = *gk;
     a.out[0] = dq, a.out[1] = dk;
     a.want_w[0] = dwq && wq, a.want_w[1] = dwk && wk && k->heads;
-    const bool want = a.want_w[0] || a.want_w[1], per_head = wq_head != 0 || wk_head != 0;
+    const bool want = a.want_w[0] || a.want_w[1], per_head = (wq && wq_head) || (wk && k->heads && wk_head);
     const int heads = q->heads + k->heads;
     if (want && (!workspace || ((uintptr_t)workspace & 3) || workspace_bytes < tpu3_norm_rotate_bwd_workspace_bytes(heads, d, per_head)))
         return TPU3_EINVAL;
     a.part = (float *)workspace;
-    const NrPlan p = nr_plan(a.tokens, heads, d, a.total_pairs, true, per_head, want);
+    const NrPlan p = nr_plan(a.tokens, heads, d, a.total_pairs, a.interleaved, true, per_head, want);
     if (p.lds > 160 * 1024)
         return TPU3_ELIMIT;
     a.tok = p.tok;
@@ -469,8 +516,7 @@ extern "C" int tpu3_norm_rotate_bwd(tpu3_stream_t stream, int type, int b, int n
     int st = type == TPU3_TYPE_F32 ? nr_backward<float>(a, p, s) : type == TPU3_TYPE_F16 ? nr_backward<_Float16>(a, p, s) : nr_backward<__bf16>(a, p, s);
     if (st || !want)
         return st;
-    // columns of a partial row: per head, all query heads' weights then all key heads'; else one set each.  Where only one
-    // side has a set per head, the other side's heads are added up here too: that mixture is refused above the C ABI.
+    // columns of a partial row: per head, all query heads' weights then all key heads'; else one set each
     const int cols = (per_head ? heads : 2) * d, nq = (per_head ? q->heads : 1) * d, nk = (per_head ? k->heads : 1) * d;
     if (a.want_w[0])
         hipLaunchKernelGGL(norm_rotate_wsum_kernel, dim3((nq + 31) / 32), dim3(1024), 0, s, p.wgs, cols, 0, nq, w_type, a.part, dwq);

@@ -68,10 +68,10 @@ def _launch(name, t, *args):
     """A C entry point on the current stream of the tensor's device (which is made the current device if it is not)."""
     dev = t.get_device()
     if torch.cuda.current_device() == dev:
-        rc = getattr(L.lib(), name)(torch.cuda.current_stream().cuda_stream, *args)
+        rc = getattr(L.lib(), name)(torch.cuda.current_stream(dev).cuda_stream, *args)
     else:
         with torch.cuda.device(dev):
-            rc = getattr(L.lib(), name)(torch.cuda.current_stream().cuda_stream, *args)
+            rc = getattr(L.lib(), name)(torch.cuda.current_stream(dev).cuda_stream, *args)
     if rc:
         L.check(rc, name)
 
@@ -191,7 +191,7 @@ def norm_rotate(q, k, q_weight, k_weight, position, freq, eps=1e-6, interleaved=
             wq, wk = wq.float(), wk.float()              # (32 bits: the heads' gradients of a shared set are added up)
         if wq.dim() != wk.dim():
             wq, wk = wq.expand(hq, d), wk.expand(k.size(2), d)
-    wq, wk = (None if w is None else w.contiguous() for w in (wq, wk))
+    wq, wk = (w if w is None or (w.is_contiguous() and not w.data_ptr() & 15) else w.contiguous().clone() for w in (wq, wk))
     if not position.is_cuda or not freq.is_cuda or position.device != q.device or freq.device != q.device:
         raise RuntimeError("position and freq must be CUDA tensors on %s" % q.device)
     if position.dtype not in L.POSITION_TYPES:
@@ -331,7 +331,7 @@ class _BlockAttention(torch.autograd.Function):
         dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         make = torch.zeros if m == 0 else torch.empty                # (no queries: the kernels do not run)
         dk, dv = (make(t.shape, dtype=t.dtype, device=t.device) for t in (k, v))
-        need = L.lib().tpu3_block_attn_bwd_workspace_bytes(b, m, n, hq, hk)
+        need = L.lib().tpu3_block_attn_bwd_workspace_bytes(b, m, n, hq, hk, d)
         ws = _workspace(need, q)
         _launch("tpu3_block_attn_bwd", q, L.TYPES[q.dtype], b, m, n, d, _heads(q), _heads(k), _heads(v), _heads(o), _heads(go),
                 blocks.data_ptr(), count, ctx.scale, L.ptr(n_arr), L.ptr(m_arr), ctx.causal, lse.data_ptr(), L.ptr(rest),

@@ -596,12 +596,13 @@ int tpu3_block_attn_fwd(tpu3_stream_t stream, int type, int b, int m, int n, int
                         size_t workspace_bytes);
 size_t tpu3_block_attn_fwd_workspace_bytes(int b, int m, int n, int hq, int hk, int d, int count);
 /* Its gradient: o / lse / rest (NULL: do . o from the rounded o) of the forward call, go = the gradient of o -> dq, dk, dv
- * contiguous (rows behind the live ones: 0).  Deterministic: no floating-point atomics.  workspace = tpu3_block_attn_bwd_workspace_bytes bytes, 16-byte aligned. */
+ * contiguous (rows behind the live ones: 0).  Deterministic: no floating-point atomics.  workspace =
+ * tpu3_block_attn_bwd_workspace_bytes bytes, 16-byte aligned. */
 int tpu3_block_attn_bwd(tpu3_stream_t stream, int type, int b, int m, int n, int d, const tpu3_heads *q, const tpu3_heads *k,
                         const tpu3_heads *v, const tpu3_heads *o, const tpu3_heads *go, const int32_t *blocks, int count,
                         float scale, const int32_t *n_arr, const int32_t *m_arr, int causal, const float *lse,
                         const void *rest, void *dq, void *dk, void *dv, void *workspace, size_t workspace_bytes);
-size_t tpu3_block_attn_bwd_workspace_bytes(int b, int m, int n, int hq, int hk);
+size_t tpu3_block_attn_bwd_workspace_bytes(int b, int m, int n, int hq, int hk, int d);
 
 /* ---- measurement hooks (bench.py and tools/ only; a caller of the path never needs them) ------------
  * tpu3_debug_fps_bucket_events: the NEXT bucketed-FPS call (n beyond the register-resident limit)

@@ -101,10 +101,13 @@ def attention(q, k, v, blocks, scale=None, n_arr=None, m_arr=None, causal=False,
     xe = torch.where(see, scale * (qf.abs() @ kf.abs().transpose(2, 3)), torch.zeros_like(x))
     xe = (xe.amax(dim=3, keepdim=True) if n else torch.zeros_like(top)) * (d + 8) * F32
     pe = 2 * xe + (terms + 16) * F32                                       # relative error of a probability
+    # (16-bit types: the denominator adds up the rounded probabilities, each w off, so it is w off itself: o is off by w |o|
+    # more, and the probabilities that the backward pass forms with it by w)
     u, w = unit(dt), unit(dt) if dt != torch.float32 else 0.0
     mag = p @ vf.abs()
-    t_o = u * o.abs() + (w + pe + terms * F32) * mag + tiny(dt) * (1 + (see.double() @ vf.abs()))
+    t_o = (u + w) * o.abs() + (w + pe + terms * F32) * mag + tiny(dt) * (1 + (see.double() @ vf.abs()))
     back = lambda t: t.transpose(1, 2)                                     # noqa: E731
+    pe = pe + w
     out = dict(o=back(o), t_o=1.05 * back(t_o) + 1e-30)
     if go is None:
         return out
