@@ -41,6 +41,7 @@ struct BaArgs {
     float *part;                            // split forward: (rows, splits, d + 4); split dk / dv: (splits, blocks, 2, 64, d)
     int32_t *used;                          // split dk / dv: (splits, blocks), the part holds something
     int b, m, n, nb, mt, hq, hk, group, d, count, causal, splits, tiles, qt, cap;
+    unsigned group_inverse;                 // ceil(2^32 / group): r / group = umulhi(r, it) for r * group < 2^32, group > 1
     float scale, scale2;                    // scale2 = scale * log2(e)
 };
 
@@ -71,36 +72,67 @@ template <typename T> __device__ __forceinline__ typename hd_vec<T>::v8 ba_zero(
     return z;
 }
 
-// LDS rows are padded by 16 bytes (BA_PAD channels): 16 lanes that read 16 bytes of 16 consecutive rows then touch 64
-// different banks for rows of 64, 128 and 256 bytes.
-template <typename T> struct BaPad { static constexpr int v = 16 / sizeof(T); };
-
-// A operand, transposed: lane (l15, g) gets channel c0 + l15 of the rows r0 + g*4 + {0..3} and r0 + 16 + g*4 + {0..3}
-template <typename T, int STRIDE> __device__ __forceinline__ typename hd_vec<T>::v8 ba_column(const T *tile, int r0, int c0)
-{
-    const int lane = threadIdx.x & 63, g = lane >> 4, l15 = lane & 15;
-    typename hd_vec<T>::v8 f;
-    if constexpr (sizeof(T) == 4) {
-        const T *p = tile + (r0 + g * 4) * STRIDE + c0 + l15;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            f.v[i] = p[i * STRIDE];
-            f.v[4 + i] = p[(16 + i) * STRIDE];
-        }
-    } else {
-        // 16 lanes read a 4 x 16 piece (8 bytes a lane) and receive its columns
-        typedef __attribute__((address_space(3))) ba_s4 lds_s4;
-        const T *p = tile + (r0 + g * 4 + (l15 >> 2)) * STRIDE + c0 + (l15 & 3) * 4;
-        union {
-            ba_s4 s[2];
-            typename hd_vec<T>::v8 v;
-        } u;
-        u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(p));
-        u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(p + 16 * STRIDE));
-        f = u.v;
+// A tile of 64 rows in LDS, unpadded; the 16-byte pieces of a row are permuted by its number (piece ^ f(row), f below) so that
+// both kinds of reads hit 64 different banks: 16 lanes that read one piece of 16 consecutive rows, and 32 lanes that read
+// 32 bytes of 8 consecutive rows (the transposing read).  256 bytes hold 1, 2 or 4 rows: f runs through the even numbers
+// over rows 0 .. 7 (of different 256-byte lines) and through the odd ones over rows 8 .. 15.
+template <typename T, int DP> struct BaLds {
+    static constexpr int ROWB = DP * (int)sizeof(T), PIECE = 16 / (int)sizeof(T);
+    static constexpr size_t TILE = (size_t)BA_ROWS * ROWB;
+    static __device__ __forceinline__ int f(int row)
+    {
+        const int low = ROWB >= 256 ? (row & 7) : ROWB == 128 ? ((row >> 1) & 3) : ((row >> 2) & 1);
+        return (low << 1) | ((row >> 3) & 1);
     }
-    return f;
-}
+    // place of a row's piece, in elements
+    static __device__ __forceinline__ int at(int row, int piece) { return row * DP + ((piece ^ f(row)) * PIECE); }
+    // eight channels from 8 * part on
+    static __device__ __forceinline__ typename hd_vec<T>::v8 row8(const T *tile, int row, int part)
+    {
+        if constexpr (sizeof(T) == 2) {
+            return *(const typename hd_vec<T>::v8 *)(tile + at(row, part));
+        } else {
+            hd_f8 r;
+            *(hd_f4 *)(r.v) = *(const hd_f4 *)(tile + at(row, 2 * part));
+            *(hd_f4 *)(r.v + 4) = *(const hd_f4 *)(tile + at(row, 2 * part + 1));
+            return r;
+        }
+    }
+    static __device__ __forceinline__ void put8(T *tile, int row, int part, const typename hd_vec<T>::v8 &x)
+    {
+        if constexpr (sizeof(T) == 2) {
+            *(typename hd_vec<T>::v8 *)(tile + at(row, part)) = x;
+        } else {
+            *(hd_f4 *)(tile + at(row, 2 * part)) = hd_f4{x.v[0], x.v[1], x.v[2], x.v[3]};
+            *(hd_f4 *)(tile + at(row, 2 * part + 1)) = hd_f4{x.v[4], x.v[5], x.v[6], x.v[7]};
+        }
+    }
+    // A operand, transposed: lane (l15, g) gets channel 16 * c + l15 of the rows r0 + g*4 + {0..3} and r0 + 16 + g*4 + {0..3}
+    static __device__ __forceinline__ typename hd_vec<T>::v8 column(const T *tile, int r0, int c)
+    {
+        const int lane = threadIdx.x & 63, g = lane >> 4, l15 = lane & 15;
+        typename hd_vec<T>::v8 o;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                o.v[i] = tile[at(r0 + g * 4 + i, c * 4 + (l15 >> 2)) + (l15 & 3)];
+                o.v[4 + i] = tile[at(r0 + 16 + g * 4 + i, c * 4 + (l15 >> 2)) + (l15 & 3)];
+            }
+        } else {
+            // 16 lanes read a 4 x 16 piece (8 bytes a lane) and receive its columns
+            typedef __attribute__((address_space(3))) ba_s4 lds_s4;
+            const T *p = tile + at(r0 + g * 4 + (l15 >> 2), c * 2 + ((l15 >> 1) & 1)) + (l15 & 1) * 4;
+            union {
+                ba_s4 s[2];
+                typename hd_vec<T>::v8 v;
+            } u;
+            u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(p));
+            u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(p + 16 * DP));
+            o = u.v;
+        }
+        return o;
+    }
+};
 
 template <typename T> __device__ __forceinline__ typename hd_vec<T>::v8 ba_pack(const hd_f4 &a, const hd_f4 &b)
 {
@@ -169,17 +201,24 @@ __device__ __forceinline__ float ba_col_sum(float v)
 }
 
 // ---- staging of a 64-row tile ------------------------------------------------------------------------------------------
-template <typename T, int DP> struct BaStage {
-    static constexpr int CHUNKS = DP / 8, PER = BA_ROWS * CHUNKS / BA_THREADS;      // 16-byte pieces of a thread
+template <typename T, int DP, int NT> struct BaStage {
+    typedef BaLds<T, DP> L;
+    static constexpr int PARTS = DP / 8, PER = BA_ROWS * PARTS / NT;                // eight-channel parts of a thread
     typename hd_vec<T>::v8 r[PER];
-    // rows [row0, row0 + 64) of one head; rows from `end` on and channels from d on read as zero
-    __device__ __forceinline__ void load(const T *base, int64_t stride, int row0, int end, int d)
+    static constexpr int STEP = NT / PARTS;
+    static __device__ __forceinline__ int row(int i) { return (int)threadIdx.x / PARTS + i * STEP; }
+    static __device__ __forceinline__ int part(int) { return (int)threadIdx.x % PARTS; }
+    // rows [row0, row0 + 64) of one head; rows from `end` on and channels from d on read as zero.  `lane`: this thread's
+    // place in row 0's tile (BaStage::lane), so that a tile costs one pointer and steps that are the same for all threads
+    static __device__ __forceinline__ const T *lane(const T *base, int64_t stride) { return base + row(0) * stride + part(0) * 8; }
+    __device__ __forceinline__ void load(const T *lane, int64_t stride, int row0, int end, int d)
     {
+        const T *p = lane + row0 * stride;
+        const int left = part(0) * 8 < d ? end - row0 - row(0) : 0;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int e = i * BA_THREADS + threadIdx.x, row = e / CHUNKS, c = (e % CHUNKS) * 8;
-            if (row0 + row < end && c < d)
-                r[i] = *(const typename hd_vec<T>::v8 *)(base + (int64_t)(row0 + row) * stride + c);
+            if (i * STEP < left)
+                r[i] = *(const typename hd_vec<T>::v8 *)(p + i * STEP * stride);
             else
                 r[i] = ba_zero<T>();
         }
@@ -189,32 +228,44 @@ template <typename T, int DP> struct BaStage {
     {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int e = i * BA_THREADS + threadIdx.x, row = e / CHUNKS, c = (e % CHUNKS) * 8;
+            typename hd_vec<T>::v8 x = r[i];
             bool any = false;
 #pragma unroll
-            for (int x = 0; x < 8; ++x) {
-                const bool fin = fabsf((float)r[i][x]) <= 3.4028235e38f;
+            for (int c = 0; c < 8; ++c) {
+                const bool fin = fabsf((float)r[i][c]) <= 3.4028235e38f;
                 any |= !fin;
-                tile[row * (DP + BaPad<T>::v) + c + x] = fin ? (T)r[i][x] : (T)0.f;
+                if constexpr (sizeof(T) == 4)
+                    x.v[c] = fin ? x.v[c] : 0.f;
+                else
+                    x[c] = fin ? x[c] : (T)0.f;
             }
+            L::put8(tile, row(i), part(i), x);
             if (any)
-                atomicOr(odd, 1ull << row);
+                atomicOr(odd, 1ull << row(i));
         }
     }
     __device__ __forceinline__ void store(T *tile) const
     {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int e = i * BA_THREADS + threadIdx.x, row = e / CHUNKS, c = (e % CHUNKS) * 8;
-            *(typename hd_vec<T>::v8 *)(tile + row * (DP + BaPad<T>::v) + c) = r[i];
-        }
+        for (int i = 0; i < PER; ++i)
+            L::put8(tile, row(i), part(i), r[i]);
     }
 };
 
-// waves a SIMD that the register allocation aims at
-template <typename T, int DP> struct BaWaves {
-    static constexpr int v = sizeof(T) == 4 ? (DP == 128 ? 1 : DP == 64 ? 2 : 3) : DP == 128 ? 2 : 3;
-    static constexpr int dkv = sizeof(T) == 4 ? (DP == 128 ? 1 : 2) : DP == 128 ? 2 : 3;
+// CT, KT: columns (rows of the forward and dq kernels, keys of the dk / dv kernel) of a wave in units of 16.  One: with two,
+// every operand read from LDS feeds two matrix instructions, but half as many waves hide the latencies (attend clouds:
+// 188 us with two, 146 with one).  w, kw: waves a SIMD that the register allocation aims at.
+#ifndef BW64
+#define BW64 3
+#define BW128 3
+#define BK64 3
+#define BK128 2
+#endif
+template <typename T, int DP> struct BaShape {
+    static constexpr int CT = 1, NT = BA_THREADS / CT;
+    static constexpr int w = sizeof(T) == 4 ? (DP == 128 ? 1 : DP == 64 ? 2 : 3) : DP == 128 ? BW128 : BW64;
+    static constexpr int KT = 1, KNT = BA_THREADS / KT;
+    static constexpr int kw = sizeof(T) == 4 ? (DP == 128 ? 1 : 2) : DP == 128 ? BK128 : BK64;
 };
 
 struct BaTile {                             // which rows a workgroup has
@@ -253,11 +304,11 @@ __device__ __forceinline__ int ba_limit(const BaArgs &a, int live, int lm, int i
 // The union of the blocks of the tile's queries, ascending, with the queries that picked each: list[u], mask[u], u < the
 // return value.  An index outside the live blocks, or behind what the query may see, is nobody's; one that a query names
 // twice counts once.
-__device__ int ba_union(const BaArgs &a, const BaTile &t, uint32_t *list, uint64_t *mask, uint32_t *words, uint32_t *before)
+template <int NT> __device__ int ba_union(const BaArgs &a, const BaTile &t, uint32_t *list, uint64_t *mask, uint32_t *words, uint32_t *before)
 {
     __shared__ uint32_t wave_total[4];
     const int nw = (a.nb + 31) / 32, entries = a.qt * a.count;
-    for (int w = threadIdx.x; w < nw; w += BA_THREADS)
+    for (int w = threadIdx.x; w < nw; w += NT)
         words[w] = 0;
     __syncthreads();
     const int32_t *idx = a.blocks + (((int64_t)t.b * a.m + t.i0) * a.hk + t.h) * a.count;
@@ -269,14 +320,29 @@ __device__ int ba_union(const BaArgs &a, const BaTile &t, uint32_t *list, uint64
         const int blk = idx[(int64_t)q * a.hk * a.count + (e - q * a.count)];
         return blk >= 0 && blk < a.nb && blk * BA_BLOCK < ba_limit(a, t.live, t.lm, i) ? blk : -1;
     };
-    for (int e = threadIdx.x; e < entries; e += BA_THREADS) {
+    constexpr int KEPT = 4;                 // of a thread's entries, in registers between the two passes
+    int kept[KEPT];
+#pragma unroll
+    for (int x = 0; x < KEPT; ++x) {
+        const int e = x * NT + threadIdx.x;
         int q;
-        const int blk = entry(e, q);
-        if (blk >= 0)
-            atomicOr(words + (blk >> 5), 1u << (blk & 31));
+        kept[x] = e < entries ? entry(e, q) : -1;
     }
+    auto all_entries = [&](auto &&f) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < KEPT; ++x)
+            if (kept[x] >= 0)
+                f(kept[x], (x * NT + (int)threadIdx.x) / a.count);
+        for (int e = KEPT * NT + threadIdx.x; e < entries; e += NT) {
+            int q;
+            const int blk = entry(e, q);
+            if (blk >= 0)
+                f(blk, q);
+        }
+    };
+    all_entries([&](int blk, int) { atomicOr(words + (blk >> 5), 1u << (blk & 31)); });
     __syncthreads();
-    const int per = (nw + BA_THREADS - 1) / BA_THREADS, w0 = min(nw, (int)threadIdx.x * per), w1 = min(nw, w0 + per);
+    const int per = (nw + NT - 1) / NT, w0 = min(nw, (int)threadIdx.x * per), w1 = min(nw, w0 + per);
     uint32_t mine = 0;
     for (int w = w0; w < w1; ++w)
         mine += __popc(words[w]);
@@ -291,34 +357,26 @@ __device__ int ba_union(const BaArgs &a, const BaTile &t, uint32_t *list, uint64
         wave_total[wave] = inc;
     __syncthreads();
     uint32_t at = inc - mine, total = 0;
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < NT / 64; ++w) {
         at += w < wave ? wave_total[w] : 0u;
         total += wave_total[w];
     }
     for (int w = w0; w < w1; ++w) {
         before[w] = at;
-        for (uint32_t bitsleft = words[w]; bitsleft; bitsleft &= bitsleft - 1) {
-            list[at] = (uint32_t)(w * 32 + __ffs((int)bitsleft) - 1);
-            mask[at++] = 0;
-        }
+        at += __popc(words[w]);
     }
+    for (uint32_t u = threadIdx.x; u < total; u += NT)
+        mask[u] = 0;
     __syncthreads();
-    for (int e = threadIdx.x; e < entries; e += BA_THREADS) {
-        int q;
-        const int blk = entry(e, q);
-        if (blk >= 0) {
-            const uint32_t u = before[blk >> 5] + __popc(words[blk >> 5] & ((1u << (blk & 31)) - 1));
-            atomicOr((unsigned long long *)(mask + u), 1ull << q);
-        }
-    }
+    auto slot = [&](int blk) { return before[blk >> 5] + __popc(words[blk >> 5] & ((1u << (blk & 31)) - 1)); };
+    all_entries([&](int blk, int q) {
+        const uint32_t u = slot(blk);
+        list[u] = (uint32_t)blk;            // (all that name the block write the same)
+        atomicOr((unsigned long long *)(mask + u), 1ull << q);
+    });
     __syncthreads();
     return (int)total;
 }
-
-template <typename T, int DP> struct BaLds {
-    static constexpr int STRIDE = DP + BaPad<T>::v;
-    static constexpr size_t TILE = (size_t)BA_ROWS * STRIDE * sizeof(T);
-};
 
 // the rows of this lane's column as B operands: channels kk*32 + g*8 .. +8 of row l15
 template <typename T, int DP>
@@ -333,50 +391,88 @@ __device__ __forceinline__ void ba_row_operand(const T *p, bool live, int d, typ
 }
 
 // ---- forward -----------------------------------------------------------------------------------------------------------
+// The rows of a workgroup and this lane's columns of it, for the forward and the dq kernel.
+template <typename T, int DP> struct BaRows {
+    static constexpr int CT = BaShape<T, DP>::CT;
+    int ql[CT], i[CT], head[CT], limit[CT];
+    bool mine[CT], there[CT];
+    __device__ __forceinline__ BaRows(const BaArgs &a, const BaTile &t)
+    {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15;
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+            const int row = (wave * CT + c) * 16 + l15;
+            ql[c] = row / a.group;
+            i[c] = t.i0 + ql[c];
+            head[c] = t.h * a.group + (row - ql[c] * a.group);
+            there[c] = ql[c] < a.qt && i[c] < a.m;
+            mine[c] = there[c] && i[c] < t.lm;
+            limit[c] = mine[c] ? ba_limit(a, t.live, t.lm, i[c]) : 0;
+        }
+    }
+    __device__ __forceinline__ const T *at(const tpu3_heads &x, int b, int c) const
+    {
+        return (const T *)x.data + b * x.sb + (int64_t)i[c] * x.sr + (int64_t)head[c] * x.sh;
+    }
+    __device__ __forceinline__ int64_t flat(const BaArgs &a, int b, int c) const { return ((int64_t)b * a.hq + head[c]) * a.m + i[c]; }
+    __device__ __forceinline__ int64_t out(const BaArgs &a, int b, int c) const { return (((int64_t)b * a.m + i[c]) * a.hq + head[c]) * a.d; }
+};
+
 template <typename T, int DP>
-__global__ __launch_bounds__(BA_THREADS, (BaWaves<T, DP>::v)) void block_attn_fwd_kernel(BaArgs a, int64_t all)
+__global__ __launch_bounds__((BaShape<T, DP>::NT), (BaShape<T, DP>::w)) void block_attn_fwd_kernel(BaArgs a, int64_t all)
 {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ unsigned long long odd;      // careful pass: rows of the tile that hold a value that is not finite
-    constexpr int STRIDE = BaLds<T, DP>::STRIDE;
-    T *Ks = (T *)smem, *Vs = (T *)(smem + BaLds<T, DP>::TILE);
-    uint64_t *mask = (uint64_t *)(smem + 2 * BaLds<T, DP>::TILE);
+    typedef BaLds<T, DP> L;
+    typedef typename hd_vec<T>::v8 V8;
+    constexpr int CT = BaShape<T, DP>::CT, NT = BaShape<T, DP>::NT;
+    T *Ks = (T *)smem, *Vs = (T *)(smem + L::TILE);
+    uint64_t *mask = (uint64_t *)(smem + 2 * L::TILE);
     uint32_t *list = (uint32_t *)(mask + a.cap), *words = list + a.cap, *before = words + (a.nb + 31) / 32;
 
     const int64_t id = ba_xcd(blockIdx.x, all);
     const BaTile t = ba_tile(a, id);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
-    const int row = wave * 16 + l15, ql = row / a.group, hg = row - ql * a.group, i = t.i0 + ql;
-    const bool mine = ql < a.qt && i < t.lm;
-    const int head = t.h * a.group + hg;
-    const int limit = mine ? ba_limit(a, t.live, t.lm, i) : 0;
+    const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
+    const BaRows<T, DP> R(a, t);
 
-    typename hd_vec<T>::v8 qf[DP / 32];
-    ba_row_operand<T, DP>((const T *)a.q.data + t.b * a.q.sb + (int64_t)i * a.q.sr + (int64_t)head * a.q.sh, mine, a.d, qf);
-    const int count = ba_union(a, t, list, mask, words, before);
+    V8 qf[CT][DP / 32];
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+        ba_row_operand<T, DP>(R.at(a.q, t.b, c), R.mine[c], a.d, qf[c]);
+    const int count = ba_union<NT>(a, t, list, mask, words, before);
     const T *K = (const T *)a.k.data + t.b * a.k.sb + t.h * a.k.sh, *V = (const T *)a.v.data + t.b * a.v.sb + t.h * a.v.sh;
+    const T *Kl = BaStage<T, DP, NT>::lane(K, a.k.sr), *Vl = BaStage<T, DP, NT>::lane(V, a.v.sr);
 
-    hd_f4 acc[DP / 16];
-    hd_f4 sums;                             // running sum of the column, in every register
-    float top;                              // running maximum of the column
+    hd_f4 acc[CT][DP / 16];
+    hd_f4 sums[CT];                         // running sum of the column, in every register
+    float top[CT];                          // running maximum of the column
     // A value that is not finite, times the probability 0 of a row that does not see it, is not 0: in the matrix product it
     // would reach every row of the wave.  A workgroup that ends with such an output runs a second, careful pass, which
     // leaves these values out of the matrix product and adds them to the rows that see them one by one.
     for (int careful = 0;; careful = 1) {
 #pragma unroll
-        for (int c = 0; c < DP / 16; ++c)
-            acc[c] = hd_f4{0.f, 0.f, 0.f, 0.f};
-        top = -INFINITY, sums = hd_f4{0.f, 0.f, 0.f, 0.f};
-
-        BaStage<T, DP> kr, vr;
+        for (int c = 0; c < CT; ++c) {
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d)
+                acc[c][d] = hd_f4{0.f, 0.f, 0.f, 0.f};
+            top[c] = -INFINITY, sums[c] = hd_f4{0.f, 0.f, 0.f, 0.f};
+        }
+        BaStage<T, DP, NT> kr, vr;
         if (t.z < count) {
             const int r0 = (int)list[t.z] * BA_BLOCK;
-            kr.load(K, a.k.sr, r0, t.live, a.d);
-            vr.load(V, a.v.sr, r0, t.live, a.d);
+            kr.load(Kl, a.k.sr, r0, t.live, a.d);
+            vr.load(Vl, a.v.sr, r0, t.live, a.d);
         }
         for (int u = t.z; u < count; u += a.splits) {
             const int k0 = (int)list[u] * BA_BLOCK;
-            const bool bit = mine && ((mask[u] >> ql) & 1);
+            const uint64_t who = mask[u];
+            bool bit[CT], some = false, edge = false;
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+                bit[c] = R.mine[c] && ((who >> R.ql[c]) & 1);
+                some |= bit[c];
+                edge |= bit[c] && k0 + BA_BLOCK > R.limit[c];
+            }
             __syncthreads();
             kr.store(Ks);
             if (careful) {
@@ -390,115 +486,148 @@ __global__ __launch_bounds__(BA_THREADS, (BaWaves<T, DP>::v)) void block_attn_fw
             __syncthreads();
             if (u + a.splits < count) {
                 const int r0 = (int)list[u + a.splits] * BA_BLOCK;
-                kr.load(K, a.k.sr, r0, t.live, a.d);
-                vr.load(V, a.v.sr, r0, t.live, a.d);
+                kr.load(Kl, a.k.sr, r0, t.live, a.d);
+                vr.load(Vl, a.v.sr, r0, t.live, a.d);
             }
-            if (!__any(bit))
+            if (!__any(some))
                 continue;                   // (wave-uniform; the barriers are at the head of the loop)
-            hd_f4 s[4];
+            hd_f4 s[CT][4];
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                s[x] = hd_f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int kk = 0; kk < DP / 32; ++kk)
-                    s[x] = ba_mma<T>(*(const typename hd_vec<T>::v8 *)(Ks + (x * 16 + l15) * STRIDE + kk * 32 + g * 8), qf[kk], s[x]);
-            }
-            float mx = -INFINITY;
-            if (__any(bit && k0 + BA_BLOCK > limit)) {
+                for (int c = 0; c < CT; ++c)
+                    s[c][x] = hd_f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int x = 0; x < 4; ++x)
+                for (int kk = 0; kk < DP / 32; ++kk) {
+                    const V8 kf = L::row8(Ks, x * 16 + l15, kk * 4 + g);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        s[x][r] = k0 + x * 16 + g * 4 + r < limit ? s[x][r] : -INFINITY;
-            }
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    mx = fmaxf(mx, s[x][r]);
-            mx = ba_col_max(mx) * a.scale2;
-            const float next = bit ? fmaxf(top, mx) : top;
-            const float base = next == -INFINITY ? 0.f : next;
-            const float keep = __builtin_amdgcn_exp2f(top - base);     // top = -inf: 0
-            top = next;
-            // a row that did not pick the block: exp2(x - inf) = 0 (a score that is not finite is left to the careful pass)
-            const float off = bit ? base : INFINITY;
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][r], a.scale2, -off));
-                    s[x][r] = careful ? (bit ? p : 0.f) : p;
+                    for (int c = 0; c < CT; ++c)
+                        s[c][x] = ba_mma<T>(kf, qf[c][kk], s[c][x]);
                 }
-            if (__any(keep != 1.f)) {
-                sums *= keep;
-#pragma unroll
-                for (int c = 0; c < DP / 16; ++c)
-                    acc[c] *= keep;
             }
+            if (__any(edge)) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const typename hd_vec<T>::v8 pf = ba_pack<T>(s[2 * j], s[2 * j + 1]);
-                // the denominator as one more row of the product: ones times the probabilities, as rounded as they are there
-                sums = ba_mma<T>(ba_ones<T>(), pf, sums);
-#pragma unroll
-                for (int c = 0; c < DP / 16; ++c)
-                    acc[c] = ba_mma<T>(ba_column<T, STRIDE>(Vs, j * 32, c * 16), pf, acc[c]);
-            }
-            if (careful) {
-                for (unsigned long long left = odd; left; left &= left - 1) {
-                    const int kk = __ffsll(left) - 1;               // the key's place in the block: score register and lane group
-                    float p = 0.f;
+                for (int c = 0; c < CT; ++c)
 #pragma unroll
                     for (int x = 0; x < 4; ++x)
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
-                            p = (kk >> 4) == x && (kk & 3) == r ? s[x][r] : p;
-                    p = __shfl(p, ((kk >> 2) & 3) * 16 + l15, 64);
-                    const bool sees = bit && k0 + kk < limit;
+                            s[c][x][r] = k0 + x * 16 + g * 4 + r < R.limit[c] ? s[c][x][r] : -INFINITY;
+            }
+            float keep[CT];
+            bool moved = false;
 #pragma unroll
-                    for (int c = 0; c < DP / 16; ++c)
+            for (int c = 0; c < CT; ++c) {
+                float mx = -INFINITY;
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const int ch = c * 16 + g * 4 + r;
-                            const float val = sees && ch < a.d ? (float)V[(int64_t)(k0 + kk) * a.v.sr + ch] : 0.f;
-                            if (!(fabsf(val) <= 3.4028235e38f))
-                                acc[c][r] = __builtin_fmaf(p, val, acc[c][r]);
-                        }
+                for (int x = 0; x < 4; ++x)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        mx = fmaxf(mx, s[c][x][r]);
+                mx = ba_col_max(mx) * a.scale2;
+                const float next = bit[c] ? fmaxf(top[c], mx) : top[c];
+                const float base = next == -INFINITY ? 0.f : next;
+                keep[c] = __builtin_amdgcn_exp2f(top[c] - base);        // top = -inf: 0
+                moved |= keep[c] != 1.f;
+                top[c] = next;
+                // a row that did not pick the block: exp2(x - inf) = 0 (a score that is not finite is left to the careful pass)
+                const float off = bit[c] ? base : INFINITY;
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][x][r], a.scale2, -off));
+                        s[c][x][r] = careful ? (bit[c] ? p : 0.f) : p;
+                    }
+            }
+            if (__any(moved)) {
+#pragma unroll
+                for (int c = 0; c < CT; ++c) {
+                    sums[c] *= keep[c];
+#pragma unroll
+                    for (int d = 0; d < DP / 16; ++d)
+                        acc[c][d] *= keep[c];
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                V8 pf[CT];
+#pragma unroll
+                for (int c = 0; c < CT; ++c) {
+                    pf[c] = ba_pack<T>(s[c][2 * j], s[c][2 * j + 1]);
+                    // the denominator as one more row of the product: ones times the probabilities, as rounded as they are there
+                    sums[c] = ba_mma<T>(ba_ones<T>(), pf[c], sums[c]);
+                }
+#pragma unroll
+                for (int d = 0; d < DP / 16; ++d) {
+                    const V8 vf = L::column(Vs, j * 32, d);
+#pragma unroll
+                    for (int c = 0; c < CT; ++c)
+                        acc[c][d] = ba_mma<T>(vf, pf[c], acc[c][d]);
+                }
+            }
+            if (careful) {
+                for (unsigned long long left = odd; left; left &= left - 1) {
+                    const int kk = __ffsll(left) - 1;               // the key's place in the block: score register and lane group
+#pragma unroll
+                    for (int c = 0; c < CT; ++c) {
+                        float p = 0.f;
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                p = (kk >> 4) == x && (kk & 3) == r ? s[c][x][r] : p;
+                        p = __shfl(p, ((kk >> 2) & 3) * 16 + l15, 64);
+                        const bool sees = bit[c] && k0 + kk < R.limit[c];
+#pragma unroll
+                        for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const int ch = d * 16 + g * 4 + r;
+                                const float val = sees && ch < a.d ? (float)V[(int64_t)(k0 + kk) * a.v.sr + ch] : 0.f;
+                                if (!(fabsf(val) <= 3.4028235e38f))
+                                    acc[c][d][r] = __builtin_fmaf(p, val, acc[c][d][r]);
+                            }
+                    }
                 }
             }
         }
         bool finite = true;
 #pragma unroll
-        for (int c = 0; c < DP / 16; ++c)
+        for (int c = 0; c < CT; ++c) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                finite &= fabsf(acc[c][r]) <= 3.4028235e38f;
-        finite &= fabsf(sums[0]) <= 3.4028235e38f;
+            for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    finite &= fabsf(acc[c][d][r]) <= 3.4028235e38f;
+            finite &= fabsf(sums[c][0]) <= 3.4028235e38f;
+        }
         if (careful || !__syncthreads_or(!finite))
             break;
     }
-    const float sum = sums[0];
-    const bool row_there = ql < a.qt && i < a.m;
-    if (!row_there)
-        return;
-    if (a.splits > 1) {
-        float *P = a.part + ((((int64_t)t.b * a.hq + head) * a.m + i) * a.splits + t.z) * (DP + 4);
 #pragma unroll
-        for (int c = 0; c < DP / 16; ++c)
-            *(hd_f4 *)(P + c * 16 + g * 4) = acc[c];
-        if (g == 0)
-            P[DP] = top, P[DP + 1] = sum;
-        return;
+    for (int c = 0; c < CT; ++c) {
+        if (!R.there[c])
+            continue;
+        const float sum = sums[c][0];
+        if (a.splits > 1) {
+            float *P = a.part + (R.flat(a, t.b, c) * a.splits + t.z) * (DP + 4);
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d)
+                *(hd_f4 *)(P + d * 16 + g * 4) = acc[c][d];
+            if (g == 0)
+                P[DP] = top[c], P[DP + 1] = sum;
+            continue;
+        }
+        const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
+        const int64_t at = R.out(a, t.b, c);
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d)
+            if (d * 16 + g * 4 < a.d)
+                ba_store_rest<T>((T *)a.out + at, (T *)a.rest + at, a.rest != nullptr, d * 16 + g * 4, acc[c][d] * inv);
+        if (a.lse && g == 0)
+            a.lse[R.flat(a, t.b, c)] = sum > 0.f ? top[c] + log2f(sum) : -INFINITY;
     }
-    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
-    T *O = (T *)a.out + (((int64_t)t.b * a.m + i) * a.hq + head) * a.d;
-#pragma unroll
-    for (int c = 0; c < DP / 16; ++c)
-        if (c * 16 + g * 4 < a.d)
-            ba_store_rest<T>(O, (T *)a.rest + (O - (T *)a.out), a.rest != nullptr, c * 16 + g * 4, acc[c] * inv);
-    if (a.lse && g == 0)
-        a.lse[((int64_t)t.b * a.hq + head) * a.m + i] = sum > 0.f ? top + log2f(sum) : -INFINITY;
 }
 
 // Joins the splits of a row: 16 lanes a row, each a few channels.
@@ -548,73 +677,86 @@ __device__ __forceinline__ float ba_pow2_inverse(float x)
 }
 
 template <typename T, int DP>
-__global__ __launch_bounds__(BA_THREADS, (BaWaves<T, DP>::v)) void block_attn_dq_kernel(BaArgs a, int64_t all)
+__global__ __launch_bounds__((BaShape<T, DP>::NT), (BaShape<T, DP>::w)) void block_attn_dq_kernel(BaArgs a, int64_t all)
 {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ unsigned long long odd;
-    constexpr int STRIDE = BaLds<T, DP>::STRIDE;
+    typedef BaLds<T, DP> L;
+    typedef typename hd_vec<T>::v8 V8;
+    constexpr int CT = BaShape<T, DP>::CT, NT = BaShape<T, DP>::NT;
     constexpr bool HALF = __is_same(T, _Float16);
-    T *Ks = (T *)smem, *Vs = (T *)(smem + BaLds<T, DP>::TILE);
-    uint64_t *mask = (uint64_t *)(smem + 2 * BaLds<T, DP>::TILE);
+    T *Ks = (T *)smem, *Vs = (T *)(smem + L::TILE);
+    uint64_t *mask = (uint64_t *)(smem + 2 * L::TILE);
     uint32_t *list = (uint32_t *)(mask + a.cap), *words = list + a.cap, *before = words + (a.nb + 31) / 32;
 
     const int64_t id = ba_xcd(blockIdx.x, all);
     const BaTile t = ba_tile(a, id);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
-    const int row = wave * 16 + l15, ql = row / a.group, hg = row - ql * a.group, i = t.i0 + ql;
-    const bool mine = ql < a.qt && i < t.lm;
-    const int head = t.h * a.group + hg;
-    const int limit = mine ? ba_limit(a, t.live, t.lm, i) : 0;
-    const int64_t at = ((int64_t)t.b * a.hq + head) * a.m + i;
+    const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
+    const BaRows<T, DP> R(a, t);
 
-    typename hd_vec<T>::v8 qf[DP / 32], gf[DP / 32];
-    ba_row_operand<T, DP>((const T *)a.q.data + t.b * a.q.sb + (int64_t)i * a.q.sr + (int64_t)head * a.q.sh, mine, a.d, qf);
-    ba_row_operand<T, DP>((const T *)a.go.data + t.b * a.go.sb + (int64_t)i * a.go.sr + (int64_t)head * a.go.sh, mine, a.d, gf);
-    float delta = 0.f, gmax = 0.f;
-    {
+    V8 qf[CT][DP / 32], gf[CT][DP / 32];
+    float delta[CT], lse[CT], up[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+        ba_row_operand<T, DP>(R.at(a.q, t.b, c), R.mine[c], a.d, qf[c]);
+        ba_row_operand<T, DP>(R.at(a.go, t.b, c), R.mine[c], a.d, gf[c]);
         // the rounding of o, times a gradient, would move all of a row's ds one way: it goes back in
-        typename hd_vec<T>::v8 of[DP / 32], rf[DP / 32];
-        ba_row_operand<T, DP>((const T *)a.o.data + t.b * a.o.sb + (int64_t)i * a.o.sr + (int64_t)head * a.o.sh, mine, a.d, of);
-        ba_row_operand<T, DP>((const T *)a.rest + (((int64_t)t.b * a.m + i) * a.hq + head) * a.d, mine && a.rest, a.d, rf);
+        V8 of[DP / 32], rf[DP / 32];
+        ba_row_operand<T, DP>(R.at(a.o, t.b, c), R.mine[c], a.d, of);
+        ba_row_operand<T, DP>((const T *)a.rest + R.out(a, t.b, c), R.mine[c] && a.rest, a.d, rf);
+        float sum = 0.f, gmax = 0.f;
 #pragma unroll
         for (int kk = 0; kk < DP / 32; ++kk)
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                delta = __builtin_fmaf((float)gf[kk][c], (float)of[kk][c] + (float)rf[kk][c], delta);
-                gmax = fmaxf(gmax, fabsf((float)gf[kk][c]));
+            for (int x = 0; x < 8; ++x) {
+                sum = __builtin_fmaf((float)gf[c][kk][x], (float)of[kk][x] + (float)rf[kk][x], sum);
+                gmax = fmaxf(gmax, fabsf((float)gf[c][kk][x]));
             }
+        delta[c] = ba_col_sum(sum);
+        up[c] = 1.f;
+        if (HALF) {
+            gmax = ba_col_max(gmax);
+            up[c] = ba_pow2_inverse(gmax);
+        }
+        lse[c] = 0.f;
+        if (R.mine[c]) {
+            const int64_t at = R.flat(a, t.b, c);
+            lse[c] = a.lse[at];
+            if (g == 0) {
+                a.delta[at] = delta[c];
+                if (HALF)
+                    a.gmax[at] = gmax;
+            }
+        }
     }
-    delta = ba_col_sum(delta);
-    const float lse = mine ? a.lse[at] : 0.f;
-    float up = 1.f;
-    if (HALF) {
-        gmax = ba_col_max(gmax);
-        up = ba_pow2_inverse(gmax);
-    }
-    if (mine && g == 0) {
-        a.delta[at] = delta;
-        if (HALF)
-            a.gmax[at] = gmax;
-    }
-    const int count = ba_union(a, t, list, mask, words, before);
+    const int count = ba_union<NT>(a, t, list, mask, words, before);
     const T *K = (const T *)a.k.data + t.b * a.k.sb + t.h * a.k.sh, *V = (const T *)a.v.data + t.b * a.v.sb + t.h * a.v.sh;
-    hd_f4 acc[DP / 16];
+    const T *Kl = BaStage<T, DP, NT>::lane(K, a.k.sr), *Vl = BaStage<T, DP, NT>::lane(V, a.v.sr);
+    hd_f4 acc[CT][DP / 16];
     // as in the forward kernel: a second, careful pass where a key that is not finite may have reached rows that do not see
     // it; those that do are not numbers
-    bool poison = false;
+    bool poison[CT] = {};
     for (int careful = 0;; careful = 1) {
 #pragma unroll
-        for (int c = 0; c < DP / 16; ++c)
-            acc[c] = hd_f4{0.f, 0.f, 0.f, 0.f};
-        BaStage<T, DP> kr, vr;
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d)
+                acc[c][d] = hd_f4{0.f, 0.f, 0.f, 0.f};
+        BaStage<T, DP, NT> kr, vr;
         if (count > 0) {
             const int r0 = (int)list[0] * BA_BLOCK;
-            kr.load(K, a.k.sr, r0, t.live, a.d);
-            vr.load(V, a.v.sr, r0, t.live, a.d);
+            kr.load(Kl, a.k.sr, r0, t.live, a.d);
+            vr.load(Vl, a.v.sr, r0, t.live, a.d);
         }
         for (int u = 0; u < count; ++u) {
             const int k0 = (int)list[u] * BA_BLOCK;
-            const bool bit = mine && ((mask[u] >> ql) & 1);
+            const uint64_t who = mask[u];
+            bool bit[CT], some = false;
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+                bit[c] = R.mine[c] && ((who >> R.ql[c]) & 1);
+                some |= bit[c];
+            }
             __syncthreads();
             vr.store(Vs);
             if (careful) {
@@ -626,56 +768,78 @@ __global__ __launch_bounds__(BA_THREADS, (BaWaves<T, DP>::v)) void block_attn_dq
                 kr.store(Ks);
             }
             __syncthreads();
-            if (careful && bit)
-                poison |= (odd & (limit - k0 >= BA_BLOCK ? ~0ull : (1ull << max(0, limit - k0)) - 1)) != 0;
+            if (careful)
+#pragma unroll
+                for (int c = 0; c < CT; ++c)
+                    poison[c] |= bit[c] && (odd & (R.limit[c] - k0 >= BA_BLOCK ? ~0ull : (1ull << max(0, R.limit[c] - k0)) - 1)) != 0;
             if (u + 1 < count) {
                 const int r0 = (int)list[u + 1] * BA_BLOCK;
-                kr.load(K, a.k.sr, r0, t.live, a.d);
-                vr.load(V, a.v.sr, r0, t.live, a.d);
+                kr.load(Kl, a.k.sr, r0, t.live, a.d);
+                vr.load(Vl, a.v.sr, r0, t.live, a.d);
             }
-            if (!__any(bit))
+            if (!__any(some))
                 continue;
-            hd_f4 s[4];
+            hd_f4 s[CT][4];
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                hd_f4 p = {0.f, 0.f, 0.f, 0.f}, dp = {0.f, 0.f, 0.f, 0.f};
+                hd_f4 p[CT], dp[CT];
+#pragma unroll
+                for (int c = 0; c < CT; ++c)
+                    p[c] = dp[c] = hd_f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int kk = 0; kk < DP / 32; ++kk) {
-                    const int off = (x * 16 + l15) * STRIDE + kk * 32 + g * 8;
-                    p = ba_mma<T>(*(const typename hd_vec<T>::v8 *)(Ks + off), qf[kk], p);
-                    dp = ba_mma<T>(*(const typename hd_vec<T>::v8 *)(Vs + off), gf[kk], dp);
+                    const V8 kf = L::row8(Ks, x * 16 + l15, kk * 4 + g), vf = L::row8(Vs, x * 16 + l15, kk * 4 + g);
+#pragma unroll
+                    for (int c = 0; c < CT; ++c) {
+                        p[c] = ba_mma<T>(kf, qf[c][kk], p[c]);
+                        dp[c] = ba_mma<T>(vf, gf[c][kk], dp[c]);
+                    }
                 }
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(p[r], a.scale2, -lse)) * (dp[r] - delta);
-                    s[x][r] = bit && k0 + x * 16 + g * 4 + r < limit ? (HALF ? e * up : e) : 0.f;
-                }
+                for (int c = 0; c < CT; ++c)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(p[c][r], a.scale2, -lse[c])) * (dp[c][r] - delta[c]);
+                        s[c][x][r] = bit[c] && k0 + x * 16 + g * 4 + r < R.limit[c] ? (HALF ? e * up[c] : e) : 0.f;
+                    }
             }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const typename hd_vec<T>::v8 sf = ba_pack<T>(s[2 * j], s[2 * j + 1]);
+                V8 sf[CT];
 #pragma unroll
-                for (int c = 0; c < DP / 16; ++c)
-                    acc[c] = ba_mma<T>(ba_column<T, STRIDE>(Ks, j * 32, c * 16), sf, acc[c]);
+                for (int c = 0; c < CT; ++c)
+                    sf[c] = ba_pack<T>(s[c][2 * j], s[c][2 * j + 1]);
+#pragma unroll
+                for (int d = 0; d < DP / 16; ++d) {
+                    const V8 kf = L::column(Ks, j * 32, d);
+#pragma unroll
+                    for (int c = 0; c < CT; ++c)
+                        acc[c][d] = ba_mma<T>(kf, sf[c], acc[c][d]);
+                }
             }
         }
         bool finite = true;
 #pragma unroll
-        for (int c = 0; c < DP / 16; ++c)
+        for (int c = 0; c < CT; ++c)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                finite &= fabsf(acc[c][r]) <= 3.4028235e38f;
+            for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    finite &= fabsf(acc[c][d][r]) <= 3.4028235e38f;
         if (careful || !__syncthreads_or(!finite))
             break;
     }
-    if (!(ql < a.qt && i < a.m))
-        return;
-    T *O = (T *)a.out + (((int64_t)t.b * a.m + i) * a.hq + head) * a.d;
-    const float back = poison ? NAN : HALF ? a.scale / up : a.scale;
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c)
-        if (c * 16 + g * 4 < a.d)
-            ba_store4<T>(O + c * 16 + g * 4, acc[c] * back);
+    for (int c = 0; c < CT; ++c) {
+        if (!R.there[c])
+            continue;
+        T *O = (T *)a.out + R.out(a, t.b, c);
+        const float back = poison[c] ? NAN : HALF ? a.scale / up[c] : a.scale;
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d)
+            if (d * 16 + g * 4 < a.d)
+                ba_store4<T>(O + d * 16 + g * 4, acc[c][d] * back);
+    }
 }
 
 // ---- backward: which queries picked a block ------------------------------------------------------------------------------
@@ -711,52 +875,58 @@ __global__ __launch_bounds__(BA_THREADS) void block_pick_bits_kernel(BaArgs a)
 constexpr int BD_WORDS = 64;                // tiles of queries looked through at a time
 
 template <typename T, int DP>
-__global__ __launch_bounds__(BA_THREADS, (BaWaves<T, DP>::dkv)) void block_attn_dkv_kernel(BaArgs a, int64_t all)
+__global__ __launch_bounds__((BaShape<T, DP>::KNT), (BaShape<T, DP>::kw)) void block_attn_dkv_kernel(BaArgs a, int64_t all)
 {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    __shared__ int wave_total[4];
-    constexpr int STRIDE = BaLds<T, DP>::STRIDE;
+    __shared__ int list_rows;
+    typedef BaLds<T, DP> L;
+    typedef typename hd_vec<T>::v8 V8;
+    constexpr int KT = BaShape<T, DP>::KT, NT = BaShape<T, DP>::KNT;
     constexpr bool HALF = __is_same(T, _Float16);
-    T *Qs = (T *)smem, *Gs = (T *)(smem + BaLds<T, DP>::TILE);
-    float *lse_s = (float *)(smem + 2 * BaLds<T, DP>::TILE), *delta_s = lse_s + 64, *gmax_s = delta_s + 64;
+    T *Qs = (T *)smem, *Gs = (T *)(smem + L::TILE);
+    float *lse_s = (float *)(smem + 2 * L::TILE), *delta_s = lse_s + 64, *gmax_s = delta_s + 64;
     int *limit_s = (int *)(gmax_s + 64), *list = limit_s + 64;              // list: BD_WORDS * 64 queries
 
     const int64_t id = ba_xcd(blockIdx.x, all);
     const int z = (int)(id % a.splits), blk = (int)(id / a.splits % a.nb), bh = (int)(id / a.splits / a.nb), h = bh % a.hk, b = bh / a.hk;
     const int live = a.n_arr ? min(max(a.n_arr[b], 0), a.n) : a.n, lm = a.m_arr ? min(max(a.m_arr[b], 0), a.m) : a.m;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
-    const int key = blk * BA_BLOCK + wave * 16 + l15;
-    typename hd_vec<T>::v8 kf[DP / 32], vf[DP / 32];
-    ba_row_operand<T, DP>((const T *)a.k.data + b * a.k.sb + (int64_t)key * a.k.sr + h * a.k.sh, key < live, a.d, kf);
-    ba_row_operand<T, DP>((const T *)a.v.data + b * a.v.sb + (int64_t)key * a.v.sr + h * a.v.sh, key < live, a.d, vf);
-    hd_f4 dk[DP / 16], dv[DP / 16];
+    int key[KT];
+    V8 kf[KT][DP / 32], vf[KT][DP / 32];
+    hd_f4 dk[KT][DP / 16], dv[KT][DP / 16];
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c)
-        dk[c] = dv[c] = hd_f4{0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < KT; ++c) {
+        key[c] = blk * BA_BLOCK + (wave * KT + c) * 16 + l15;
+        ba_row_operand<T, DP>((const T *)a.k.data + b * a.k.sb + (int64_t)key[c] * a.k.sr + h * a.k.sh, key[c] < live, a.d, kf[c]);
+        ba_row_operand<T, DP>((const T *)a.v.data + b * a.v.sb + (int64_t)key[c] * a.v.sr + h * a.v.sh, key[c] < live, a.d, vf[c]);
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d)
+            dk[c][d] = dv[c][d] = hd_f4{0.f, 0.f, 0.f, 0.f};
+    }
     float up = 1.f;                         // fp16: dk is accumulated times this power of two
-    bool first = true;
+    bool first = true, any = false;
     const uint64_t *bits = a.bits + ((int64_t)bh * a.nb + blk) * a.mt;
     const int per = (a.mt + a.splits - 1) / a.splits, end = min(a.mt, (z + 1) * per);
-    bool any = false;
 
-    constexpr int CHUNKS = DP / 8, PER = BA_ROWS * CHUNKS / BA_THREADS;
-    typename hd_vec<T>::v8 qr[PER], gr[PER];
+    typedef BaStage<T, DP, NT> S;
+    V8 qr[S::PER], gr[S::PER];
     float row_lse = 0.f, row_delta = 0.f, row_gmax = 0.f;
     int row_limit = 0;
+    const T *Q = (const T *)a.q.data + b * a.q.sb + (int64_t)h * a.group * a.q.sh;
+    const T *G = (const T *)a.go.data + b * a.go.sb + (int64_t)h * a.group * a.go.sh;
     // rows r0 .. r0 + 63 of the list (query by query, all heads of the group) to registers; rows behind the last are zeros
     // that see nothing
     auto fetch = [&](int r0, int rows) __attribute__((always_inline)) {
 #pragma unroll
-        for (int x = 0; x < PER; ++x) {
-            const int e = x * BA_THREADS + threadIdx.x, r = r0 + e / CHUNKS, c = (e % CHUNKS) * 8;
+        for (int x = 0; x < S::PER; ++x) {
+            const int r = r0 + S::row(x), c = S::part(x) * 8;
+            qr[x] = ba_zero<T>();
+            gr[x] = ba_zero<T>();
             if (r < rows && c < a.d) {
-                const int q = r / a.group, head = h * a.group + (r - q * a.group);
+                const int q = a.group == 1 ? r : (int)__umulhi((unsigned)r, a.group_inverse), e = r - q * a.group;
                 const int64_t i = list[q];
-                qr[x] = *(const typename hd_vec<T>::v8 *)((const T *)a.q.data + b * a.q.sb + i * a.q.sr + (int64_t)head * a.q.sh + c);
-                gr[x] = *(const typename hd_vec<T>::v8 *)((const T *)a.go.data + b * a.go.sb + i * a.go.sr + (int64_t)head * a.go.sh + c);
-            } else {
-                qr[x] = ba_zero<T>();
-                gr[x] = ba_zero<T>();
+                qr[x] = *(const V8 *)(Q + i * a.q.sr + e * a.q.sh + c);
+                gr[x] = *(const V8 *)(G + i * a.go.sr + e * a.go.sh + c);
             }
         }
         row_lse = row_delta = row_gmax = 0.f;
@@ -772,13 +942,9 @@ __global__ __launch_bounds__(BA_THREADS, (BaWaves<T, DP>::dkv)) void block_attn_
 
     for (int w0 = z * per; w0 < end; w0 += BD_WORDS) {
         // the queries of the next 64 tiles that picked this block, in order
-        const int words = min(BD_WORDS, end - w0);
-        uint64_t word = 0;
-        int at = 0, total = 0;
         if (wave == 0) {
-            word = lane < words ? bits[w0 + lane] : 0ull;
-            int inc = __popcll(word);
-            at = -inc;
+            uint64_t word = w0 + lane < min(end, w0 + BD_WORDS) ? bits[w0 + lane] : 0ull;
+            int inc = __popcll(word), at = -inc;
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
                 const int v = __shfl_up(inc, o, 64);
@@ -786,23 +952,21 @@ __global__ __launch_bounds__(BA_THREADS, (BaWaves<T, DP>::dkv)) void block_attn_
             }
             at += inc;
             if (lane == 63)
-                wave_total[0] = inc;
+                list_rows = inc * a.group;
             for (; word; word &= word - 1)
                 list[at++] = (w0 + lane) * 64 + __ffsll((unsigned long long)word) - 1;
         }
         __syncthreads();
-        total = wave_total[0];
-        const int rows = total * a.group;
+        const int rows = list_rows;
         any |= rows > 0;
         if (rows > 0)
             fetch(0, rows);
         for (int r0 = 0; r0 < rows; r0 += BA_ROWS) {
             __syncthreads();                // the previous tile has been read
 #pragma unroll
-            for (int x = 0; x < PER; ++x) {
-                const int e = x * BA_THREADS + threadIdx.x, r = e / CHUNKS, c = (e % CHUNKS) * 8;
-                *(typename hd_vec<T>::v8 *)(Qs + r * STRIDE + c) = qr[x];
-                *(typename hd_vec<T>::v8 *)(Gs + r * STRIDE + c) = gr[x];
+            for (int x = 0; x < S::PER; ++x) {
+                L::put8(Qs, S::row(x), S::part(x), qr[x]);
+                L::put8(Gs, S::row(x), S::part(x), gr[x]);
             }
             if (threadIdx.x < BA_ROWS) {
                 lse_s[threadIdx.x] = row_lse, delta_s[threadIdx.x] = row_delta, limit_s[threadIdx.x] = row_limit;
@@ -822,68 +986,94 @@ __global__ __launch_bounds__(BA_THREADS, (BaWaves<T, DP>::dkv)) void block_attn_
                 if (m > 0.f && (first || want < up)) {
                     if (!first)
 #pragma unroll
-                        for (int c = 0; c < DP / 16; ++c)
-                            dk[c] *= want / up;
+                        for (int c = 0; c < KT; ++c)
+#pragma unroll
+                            for (int d = 0; d < DP / 16; ++d)
+                                dk[c][d] *= want / up;
                     up = want;
                     first = false;
                 }
             }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {   // 32 rows at a time
-                hd_f4 p[2], ds[2];
+                hd_f4 p[KT][2], ds[KT][2];
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    hd_f4 s = {0.f, 0.f, 0.f, 0.f}, dp = {0.f, 0.f, 0.f, 0.f};
+                    hd_f4 s[KT], dp[KT];
+#pragma unroll
+                    for (int c = 0; c < KT; ++c)
+                        s[c] = dp[c] = hd_f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int kk = 0; kk < DP / 32; ++kk) {
-                        const int off = (j * 32 + x * 16 + l15) * STRIDE + kk * 32 + g * 8;
-                        s = ba_mma<T>(*(const typename hd_vec<T>::v8 *)(Qs + off), kf[kk], s);
-                        dp = ba_mma<T>(*(const typename hd_vec<T>::v8 *)(Gs + off), vf[kk], dp);
-                    }
+                        const int row = j * 32 + x * 16 + l15;
+                        const V8 qa = L::row8(Qs, row, kk * 4 + g), ga = L::row8(Gs, row, kk * 4 + g);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int rr = j * 32 + x * 16 + g * 4 + r;
-                        const bool see = key < limit_s[rr];
-                        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.scale2, -lse_s[rr]));
-                        const float f = e * (dp[r] - delta_s[rr]);
-                        p[x][r] = see ? e : 0.f;
-                        ds[x][r] = see ? (HALF ? f * up : f) : 0.f;
+                        for (int c = 0; c < KT; ++c) {
+                            s[c] = ba_mma<T>(qa, kf[c][kk], s[c]);
+                            dp[c] = ba_mma<T>(ga, vf[c][kk], dp[c]);
+                        }
                     }
+                    const int r4 = j * 32 + x * 16 + g * 4;
+                    const hd_f4 le = *(const hd_f4 *)(lse_s + r4), de = *(const hd_f4 *)(delta_s + r4);
+                    const int4 li = *(const int4 *)(limit_s + r4);
+                    const int lim[4] = {li.x, li.y, li.z, li.w};
+#pragma unroll
+                    for (int c = 0; c < KT; ++c)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const bool see = key[c] < lim[r];
+                            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][r], a.scale2, -le[r]));
+                            const float f = e * (dp[c][r] - de[r]);
+                            p[c][x][r] = see ? e : 0.f;
+                            ds[c][x][r] = see ? (HALF ? f * up : f) : 0.f;
+                        }
                 }
-                const typename hd_vec<T>::v8 pf = ba_pack<T>(p[0], p[1]), sf = ba_pack<T>(ds[0], ds[1]);
+                V8 pf[KT], sf[KT];
 #pragma unroll
-                for (int c = 0; c < DP / 16; ++c) {
-                    dv[c] = ba_mma<T>(ba_column<T, STRIDE>(Gs, j * 32, c * 16), pf, dv[c]);
-                    dk[c] = ba_mma<T>(ba_column<T, STRIDE>(Qs, j * 32, c * 16), sf, dk[c]);
+                for (int c = 0; c < KT; ++c)
+                    pf[c] = ba_pack<T>(p[c][0], p[c][1]), sf[c] = ba_pack<T>(ds[c][0], ds[c][1]);
+#pragma unroll
+                for (int d = 0; d < DP / 16; ++d) {
+                    const V8 gc = L::column(Gs, j * 32, d), qc = L::column(Qs, j * 32, d);
+#pragma unroll
+                    for (int c = 0; c < KT; ++c) {
+                        dv[c][d] = ba_mma<T>(gc, pf[c], dv[c][d]);
+                        dk[c][d] = ba_mma<T>(qc, sf[c], dk[c][d]);
+                    }
                 }
             }
         }
         __syncthreads();                    // the list is rebuilt
     }
     const float back = HALF ? a.scale / up : a.scale;
+    const int64_t tile = ((int64_t)z * a.b * a.hk + bh) * a.nb + blk;
     if (a.splits > 1) {                     // a part of the queries: joined by block_attn_dkv_join_kernel
-        const int64_t tile = ((int64_t)z * a.b * a.hk + bh) * a.nb + blk;
         if (threadIdx.x == 0)
             a.used[tile] = any;
         if (!any)
             return;
-        float *P = a.part + (tile * 2 * BA_BLOCK + wave * 16 + l15) * DP;
-#pragma unroll
-        for (int c = 0; c < DP / 16; ++c) {
-            *(hd_f4 *)(P + c * 16 + g * 4) = dk[c] * back;
-            *(hd_f4 *)(P + BA_BLOCK * DP + c * 16 + g * 4) = dv[c];
-        }
-        return;
     }
-    if (key >= a.n)
-        return;
-    const int64_t at = (((int64_t)b * a.n + key) * a.hk + h) * a.d;
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c)
-        if (c * 16 + g * 4 < a.d) {
-            ba_store4<T>((T *)a.out + at + c * 16 + g * 4, dk[c] * back);
-            ba_store4<T>((T *)a.out2 + at + c * 16 + g * 4, dv[c]);
+    for (int c = 0; c < KT; ++c) {
+        if (a.splits > 1) {
+            float *P = a.part + (tile * 2 * BA_BLOCK + (wave * KT + c) * 16 + l15) * DP;
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d) {
+                *(hd_f4 *)(P + d * 16 + g * 4) = dk[c][d] * back;
+                *(hd_f4 *)(P + BA_BLOCK * DP + d * 16 + g * 4) = dv[c][d];
+            }
+            continue;
         }
+        if (key[c] >= a.n)
+            continue;
+        const int64_t at = (((int64_t)b * a.n + key[c]) * a.hk + h) * a.d;
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d)
+            if (d * 16 + g * 4 < a.d) {
+                ba_store4<T>((T *)a.out + at + d * 16 + g * 4, dk[c][d] * back);
+                ba_store4<T>((T *)a.out2 + at + d * 16 + g * 4, dv[c][d]);
+            }
+    }
 }
 
 // dk and dv of a block from its parts, in the parts' order
@@ -918,6 +1108,7 @@ int ba_fill(BaArgs &a, int type, int b, int m, int n, int d, const tpu3_heads *q
     a.b = b, a.m = m, a.n = n, a.nb = n > 0 ? (n - 1) / BA_BLOCK + 1 : 0, a.mt = (m + 63) / 64;
     a.hq = q->heads, a.hk = k->heads, a.group = a.hq / a.hk, a.d = d, a.count = count, a.causal = causal != 0;
     a.scale = scale, a.scale2 = scale * 1.44269504088896340736f;
+    a.group_inverse = a.group > 1 ? (unsigned)(((1ull << 32) + a.group - 1) / a.group) : 0u;
     a.qt = BA_ROWS / a.group;
     a.tiles = m > 0 ? (m - 1) / a.qt + 1 : 0;
     a.cap = a.qt * count < a.nb ? a.qt * count : a.nb;
@@ -975,7 +1166,7 @@ template <typename T, int DP> int ba_forward(const BaArgs &a, hipStream_t s)
     int rc = ba_allow(block_attn_fwd_kernel<T, DP>, lds);
     if (rc)
         return rc;
-    hipLaunchKernelGGL((block_attn_fwd_kernel<T, DP>), dim3((unsigned)all), dim3(BA_THREADS), lds, s, a, all);
+    hipLaunchKernelGGL((block_attn_fwd_kernel<T, DP>), dim3((unsigned)all), dim3(BaShape<T, DP>::NT), lds, s, a, all);
     if (a.splits > 1) {
         const int64_t rows = (int64_t)a.b * a.hq * a.m, per = BA_THREADS / 16;
         hipLaunchKernelGGL((block_attn_join_kernel<T, DP>), dim3((unsigned)((rows + per - 1) / per)), dim3(BA_THREADS), 0, s, a, rows);
@@ -993,7 +1184,7 @@ template <typename T, int DP> int ba_backward(BaArgs a, void *dq, void *dk, void
     if (rc)
         return rc;
     a.out = dq;
-    hipLaunchKernelGGL((block_attn_dq_kernel<T, DP>), dim3((unsigned)all), dim3(BA_THREADS), lds, s, a, all);
+    hipLaunchKernelGGL((block_attn_dq_kernel<T, DP>), dim3((unsigned)all), dim3(BaShape<T, DP>::NT), lds, s, a, all);
     if (a.nb == 0)
         return tpu3_launch_status();
     hipLaunchKernelGGL(block_pick_bits_kernel, dim3((unsigned)(a.b * a.hk * a.mt)), dim3(BA_THREADS), 0, s, a);
@@ -1004,7 +1195,7 @@ template <typename T, int DP> int ba_backward(BaArgs a, void *dq, void *dk, void
     a.out = dk, a.out2 = dv;
     const int64_t blocks = (int64_t)a.b * a.hk * a.nb;
     a.splits = ba_dkv_splits(a.b, a.m, a.hk, a.nb);
-    hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP>), dim3((unsigned)(blocks * a.splits)), dim3(BA_THREADS), lds2, s, a, blocks * a.splits);
+    hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP>), dim3((unsigned)(blocks * a.splits)), dim3(BaShape<T, DP>::KNT), lds2, s, a, blocks * a.splits);
     if (a.splits > 1)
         hipLaunchKernelGGL((block_attn_dkv_join_kernel<T, DP>), dim3((unsigned)blocks), dim3(BA_THREADS), 0, s, a);
     return tpu3_launch_status();
