@@ -201,27 +201,21 @@ __device__ __forceinline__ float ba_col_sum(float v)
 }
 
 // ---- staging of a 64-row tile ------------------------------------------------------------------------------------------
-template <typename T, int DP, int NT> struct BaStage {
+template <typename T, int DP> struct BaStage {
     typedef BaLds<T, DP> L;
-    static constexpr int PARTS = DP / 8, PER = BA_ROWS * PARTS / NT;                // eight-channel parts of a thread
+    static constexpr int PARTS = DP / 8, PER = BA_ROWS * PARTS / BA_THREADS;                // eight-channel parts of a thread
     typename hd_vec<T>::v8 r[PER];
-    static constexpr int STEP = NT / PARTS;
+    static constexpr int STEP = BA_THREADS / PARTS;
     static __device__ __forceinline__ int row(int i) { return (int)threadIdx.x / PARTS + i * STEP; }
     static __device__ __forceinline__ int part(int) { return (int)threadIdx.x % PARTS; }
-    // rows [row0, row0 + 64) of one head; rows from `end` on and channels from d on read as zero.  `lane`: this thread's
-    // place in row 0's tile (BaStage::lane), so that a tile costs one pointer and steps that are the same for all threads
-    static __device__ __forceinline__ const T *lane(const T *base, int64_t stride) { return base + row(0) * stride + part(0) * 8; }
-    __device__ __forceinline__ void load(const T *lane, int64_t stride, int row0, int end, int d)
+    // Rows [row0, row0 + 64) of one head.  Rows from `end` on are the last one's copies and channels from d on channel 0's:
+    // real numbers, whose scores are masked or meet zeros.  `lane`: this thread's place in the head (BaStage::lane).
+    static __device__ __forceinline__ const T *lane(const T *base, int d) { return base + (part(0) * 8 < d ? part(0) * 8 : 0); }
+    __device__ __forceinline__ void load(const T *lane, int64_t stride, int row0, int end)
     {
-        const T *p = lane + row0 * stride;
-        const int left = part(0) * 8 < d ? end - row0 - row(0) : 0;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            if (i * STEP < left)
-                r[i] = *(const typename hd_vec<T>::v8 *)(p + i * STEP * stride);
-            else
-                r[i] = ba_zero<T>();
-        }
+        for (int i = 0; i < PER; ++i)
+            r[i] = *(const typename hd_vec<T>::v8 *)(lane + min(row0 + row(i), end - 1) * stride);
     }
     // the tile with what is not finite as zero; `odd` collects the rows that hold such a value
     __device__ __forceinline__ void store_finite(T *tile, unsigned long long *odd) const
@@ -252,21 +246,23 @@ template <typename T, int DP, int NT> struct BaStage {
     }
 };
 
-// CT, KT: columns (rows of the forward and dq kernels, keys of the dk / dv kernel) of a wave in units of 16.  One: with two,
+// w, kw: waves a SIMD that the register allocation aims at (forward and dq, dk / dv).  A wave has 16 rows (keys): with 32,
 // every operand read from LDS feeds two matrix instructions, but half as many waves hide the latencies (attend clouds:
-// 188 us with two, 146 with one).  w, kw: waves a SIMD that the register allocation aims at.
+// 188 us instead of 146).
 #ifndef BW64
 #define BW64 3
-#define BW128 3
+#define BW128 2
 #define BK64 3
 #define BK128 2
 #endif
 template <typename T, int DP> struct BaShape {
-    static constexpr int CT = 1, NT = BA_THREADS / CT;
     static constexpr int w = sizeof(T) == 4 ? (DP == 128 ? 1 : DP == 64 ? 2 : 3) : DP == 128 ? BW128 : BW64;
-    static constexpr int KT = 1, KNT = BA_THREADS / KT;
     static constexpr int kw = sizeof(T) == 4 ? (DP == 128 ? 1 : 2) : DP == 128 ? BK128 : BK64;
+    // 16-row tiles whose row operands are read together (fp32 rows are twice as wide)
+    static constexpr int TOGETHER = DP * sizeof(T) >= 512 ? 1 : DP * sizeof(T) >= 256 ? 2 : 4;
 };
+// LDS reads above stay above: the compiler otherwise sinks each to its matrix instruction and waits for it there
+__device__ __forceinline__ void ba_issue() { __builtin_amdgcn_sched_barrier(0); }
 
 struct BaTile {                             // which rows a workgroup has
     int b, h, i0, live, lm, z;              // sequence, key head, first query, live keys and queries, split
@@ -304,11 +300,11 @@ __device__ __forceinline__ int ba_limit(const BaArgs &a, int live, int lm, int i
 // The union of the blocks of the tile's queries, ascending, with the queries that picked each: list[u], mask[u], u < the
 // return value.  An index outside the live blocks, or behind what the query may see, is nobody's; one that a query names
 // twice counts once.
-template <int NT> __device__ int ba_union(const BaArgs &a, const BaTile &t, uint32_t *list, uint64_t *mask, uint32_t *words, uint32_t *before)
+__device__ int ba_union(const BaArgs &a, const BaTile &t, uint32_t *list, uint64_t *mask, uint32_t *words, uint32_t *before)
 {
     __shared__ uint32_t wave_total[4];
     const int nw = (a.nb + 31) / 32, entries = a.qt * a.count;
-    for (int w = threadIdx.x; w < nw; w += NT)
+    for (int w = threadIdx.x; w < nw; w += BA_THREADS)
         words[w] = 0;
     __syncthreads();
     const int32_t *idx = a.blocks + (((int64_t)t.b * a.m + t.i0) * a.hk + t.h) * a.count;
@@ -324,7 +320,7 @@ template <int NT> __device__ int ba_union(const BaArgs &a, const BaTile &t, uint
     int kept[KEPT];
 #pragma unroll
     for (int x = 0; x < KEPT; ++x) {
-        const int e = x * NT + threadIdx.x;
+        const int e = x * BA_THREADS + threadIdx.x;
         int q;
         kept[x] = e < entries ? entry(e, q) : -1;
     }
@@ -332,8 +328,8 @@ template <int NT> __device__ int ba_union(const BaArgs &a, const BaTile &t, uint
 #pragma unroll
         for (int x = 0; x < KEPT; ++x)
             if (kept[x] >= 0)
-                f(kept[x], (x * NT + (int)threadIdx.x) / a.count);
-        for (int e = KEPT * NT + threadIdx.x; e < entries; e += NT) {
+                f(kept[x], (x * BA_THREADS + (int)threadIdx.x) / a.count);
+        for (int e = KEPT * BA_THREADS + threadIdx.x; e < entries; e += BA_THREADS) {
             int q;
             const int blk = entry(e, q);
             if (blk >= 0)
@@ -342,7 +338,7 @@ template <int NT> __device__ int ba_union(const BaArgs &a, const BaTile &t, uint
     };
     all_entries([&](int blk, int) { atomicOr(words + (blk >> 5), 1u << (blk & 31)); });
     __syncthreads();
-    const int per = (nw + NT - 1) / NT, w0 = min(nw, (int)threadIdx.x * per), w1 = min(nw, w0 + per);
+    const int per = (nw + BA_THREADS - 1) / BA_THREADS, w0 = min(nw, (int)threadIdx.x * per), w1 = min(nw, w0 + per);
     uint32_t mine = 0;
     for (int w = w0; w < w1; ++w)
         mine += __popc(words[w]);
@@ -357,7 +353,7 @@ template <int NT> __device__ int ba_union(const BaArgs &a, const BaTile &t, uint
         wave_total[wave] = inc;
     __syncthreads();
     uint32_t at = inc - mine, total = 0;
-    for (int w = 0; w < NT / 64; ++w) {
+    for (int w = 0; w < BA_THREADS / 64; ++w) {
         at += w < wave ? wave_total[w] : 0u;
         total += wave_total[w];
     }
@@ -365,7 +361,7 @@ template <int NT> __device__ int ba_union(const BaArgs &a, const BaTile &t, uint
         before[w] = at;
         at += __popc(words[w]);
     }
-    for (uint32_t u = threadIdx.x; u < total; u += NT)
+    for (uint32_t u = threadIdx.x; u < total; u += BA_THREADS)
         mask[u] = 0;
     __syncthreads();
     auto slot = [&](int blk) { return before[blk >> 5] + __popc(words[blk >> 5] & ((1u << (blk & 31)) - 1)); };
@@ -391,243 +387,233 @@ __device__ __forceinline__ void ba_row_operand(const T *p, bool live, int d, typ
 }
 
 // ---- forward -----------------------------------------------------------------------------------------------------------
-// The rows of a workgroup and this lane's columns of it, for the forward and the dq kernel.
-template <typename T, int DP> struct BaRows {
-    static constexpr int CT = BaShape<T, DP>::CT;
-    int ql[CT], i[CT], head[CT], limit[CT];
-    bool mine[CT], there[CT];
-    __device__ __forceinline__ BaRows(const BaArgs &a, const BaTile &t)
+// This lane's row (column of the transposed scores) in the forward and the dq kernel.
+struct BaRow {
+    int ql, i, head, limit;
+    bool mine, there;
+    __device__ __forceinline__ BaRow(const BaArgs &a, const BaTile &t)
     {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15;
-#pragma unroll
-        for (int c = 0; c < CT; ++c) {
-            const int row = (wave * CT + c) * 16 + l15;
-            ql[c] = row / a.group;
-            i[c] = t.i0 + ql[c];
-            head[c] = t.h * a.group + (row - ql[c] * a.group);
-            there[c] = ql[c] < a.qt && i[c] < a.m;
-            mine[c] = there[c] && i[c] < t.lm;
-            limit[c] = mine[c] ? ba_limit(a, t.live, t.lm, i[c]) : 0;
-        }
+        const int row = (threadIdx.x >> 6) * 16 + (threadIdx.x & 15);
+        ql = row / a.group;
+        i = t.i0 + ql;
+        head = t.h * a.group + (row - ql * a.group);
+        there = ql < a.qt && i < a.m;
+        mine = there && i < t.lm;
+        limit = mine ? ba_limit(a, t.live, t.lm, i) : 0;
     }
-    __device__ __forceinline__ const T *at(const tpu3_heads &x, int b, int c) const
+    template <typename T> __device__ __forceinline__ const T *at(const tpu3_heads &x, int b) const
     {
-        return (const T *)x.data + b * x.sb + (int64_t)i[c] * x.sr + (int64_t)head[c] * x.sh;
+        return (const T *)x.data + b * x.sb + (int64_t)i * x.sr + (int64_t)head * x.sh;
     }
-    __device__ __forceinline__ int64_t flat(const BaArgs &a, int b, int c) const { return ((int64_t)b * a.hq + head[c]) * a.m + i[c]; }
-    __device__ __forceinline__ int64_t out(const BaArgs &a, int b, int c) const { return (((int64_t)b * a.m + i[c]) * a.hq + head[c]) * a.d; }
+    __device__ __forceinline__ int64_t flat(const BaArgs &a, int b) const { return ((int64_t)b * a.hq + head) * a.m + i; }
+    __device__ __forceinline__ int64_t out(const BaArgs &a, int b) const { return (((int64_t)b * a.m + i) * a.hq + head) * a.d; }
 };
 
+// scores (keys x rows) of the tile: s[x] = 16 keys x 16 rows
 template <typename T, int DP>
-__global__ __launch_bounds__((BaShape<T, DP>::NT), (BaShape<T, DP>::w)) void block_attn_fwd_kernel(BaArgs a, int64_t all)
+__device__ __forceinline__ void ba_scores(const T *tile, const typename hd_vec<T>::v8 *f, hd_f4 *s)
+{
+    typedef BaLds<T, DP> L;
+    constexpr int TG = BaShape<T, DP>::TOGETHER;
+    const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int x0 = 0; x0 < 4; x0 += TG) {
+        typename hd_vec<T>::v8 kf[TG][DP / 32];
+#pragma unroll
+        for (int x = 0; x < TG; ++x)
+#pragma unroll
+            for (int kk = 0; kk < DP / 32; ++kk)
+                kf[x][kk] = L::row8(tile, (x0 + x) * 16 + l15, kk * 4 + g);
+        ba_issue();
+#pragma unroll
+        for (int x = 0; x < TG; ++x)
+            s[x0 + x] = hd_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < DP / 32; ++kk)
+#pragma unroll
+            for (int x = 0; x < TG; ++x)
+                s[x0 + x] = ba_mma<T>(kf[x][kk], f[kk], s[x0 + x]);
+    }
+}
+// the tile's columns of 32 keys, all channels
+template <typename T, int DP> __device__ __forceinline__ void ba_columns(const T *tile, int r0, typename hd_vec<T>::v8 *f)
+{
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d)
+        f[d] = BaLds<T, DP>::column(tile, r0, d);
+}
+__device__ __forceinline__ bool ba_finite(float x) { return fabsf(x) <= 3.4028235e38f; }
+
+// A value that is not finite, times the probability 0 of a row that does not see it, is not 0: in the matrix product it would
+// reach every row of the wave.  A workgroup that ends with such an output runs its blocks a second time, carefully: these
+// values stay out of the matrix product and are added to the rows that see them one by one.
+template <typename T, int DP, bool CAREFUL>
+__device__ __forceinline__ void ba_fwd_pass(const BaArgs &a, const BaTile &t, const BaRow &R, const typename hd_vec<T>::v8 *qf, char *smem,
+                                            const uint64_t *mask, const uint32_t *list, int count, unsigned long long *odd,
+                                            hd_f4 *acc, hd_f4 &sums, float &top)
+{
+    typedef BaLds<T, DP> L;
+    typedef BaStage<T, DP> S;
+    typedef typename hd_vec<T>::v8 V8;
+    T *Ks = (T *)smem, *Vs = (T *)(smem + L::TILE);
+    const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
+    const T *K = (const T *)a.k.data + t.b * a.k.sb + t.h * a.k.sh, *V = (const T *)a.v.data + t.b * a.v.sb + t.h * a.v.sh;
+    const T *Kl = S::lane(K, a.d), *Vl = S::lane(V, a.d);
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d)
+        acc[d] = hd_f4{0.f, 0.f, 0.f, 0.f};
+    top = -INFINITY, sums = hd_f4{0.f, 0.f, 0.f, 0.f};
+    S kr, vr;
+    if (t.z < count) {
+        const int r0 = (int)list[t.z] * BA_BLOCK;
+        kr.load(Kl, a.k.sr, r0, t.live);
+        vr.load(Vl, a.v.sr, r0, t.live);
+    }
+    for (int u = t.z; u < count; u += a.splits) {
+        const int k0 = (int)list[u] * BA_BLOCK;
+        const bool bit = R.mine && ((mask[u] >> R.ql) & 1);
+        __syncthreads();
+        kr.store(Ks);
+        if constexpr (CAREFUL) {
+            if (threadIdx.x == 0)
+                *odd = 0;
+            __syncthreads();
+            vr.store_finite(Vs, odd);
+        } else {
+            vr.store(Vs);
+        }
+        __syncthreads();
+        if (u + a.splits < count) {
+            const int r0 = (int)list[u + a.splits] * BA_BLOCK;
+            kr.load(Kl, a.k.sr, r0, t.live);
+            vr.load(Vl, a.v.sr, r0, t.live);
+        }
+        if (!__any(bit))
+            continue;                       // (wave-uniform; the barriers are at the head of the loop)
+        hd_f4 s[4];
+        ba_scores<T, DP>(Ks, qf, s);
+        V8 vf[DP / 16];
+        ba_columns<T, DP>(Vs, 0, vf);
+        ba_issue();
+        if (__any(bit && k0 + BA_BLOCK > R.limit)) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    s[x][r] = k0 + x * 16 + g * 4 + r < R.limit ? s[x][r] : -INFINITY;
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                mx = fmaxf(mx, s[x][r]);
+        mx = ba_col_max(mx) * a.scale2;
+        const float next = bit ? fmaxf(top, mx) : top;
+        const float base = next == -INFINITY ? 0.f : next;
+        const float keep = __builtin_amdgcn_exp2f(top - base);          // top = -inf: 0
+        top = next;
+        if (__any(keep != 1.f)) {
+            sums *= keep;
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d)
+                acc[d] *= keep;
+        }
+        // a row that did not pick the block: exp2(x - inf) = 0 (a score that is not finite is left to the careful pass)
+        const float off = bit ? base : INFINITY;
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                s[x][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][r], a.scale2, -off));
+                if (CAREFUL)
+                    s[x][r] = bit ? s[x][r] : 0.f;
+            }
+        V8 vn[DP / 16];
+        ba_columns<T, DP>(Vs, 32, vn);
+        ba_issue();
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const V8 pf = ba_pack<T>(s[2 * j], s[2 * j + 1]);
+            // the denominator as one more row of the product: ones times the probabilities, as rounded as they are there
+            sums = ba_mma<T>(ba_ones<T>(), pf, sums);
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d)
+                acc[d] = ba_mma<T>(j ? vn[d] : vf[d], pf, acc[d]);
+        }
+        if constexpr (CAREFUL) {
+            for (unsigned long long left = *odd; left; left &= left - 1) {
+                const int kk = __ffsll(left) - 1;                   // the key's place in the block: score register and lane group
+                float p = 0.f;
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        p = (kk >> 4) == x && (kk & 3) == r ? s[x][r] : p;
+                p = __shfl(p, ((kk >> 2) & 3) * 16 + l15, 64);
+                const bool sees = bit && k0 + kk < R.limit;
+#pragma unroll
+                for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int ch = d * 16 + g * 4 + r;
+                        const float val = sees && ch < a.d ? (float)V[(int64_t)(k0 + kk) * a.v.sr + ch] : 0.f;
+                        if (!ba_finite(val))
+                            acc[d][r] = __builtin_fmaf(p, val, acc[d][r]);
+                    }
+            }
+        }
+    }
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(BA_THREADS, (BaShape<T, DP>::w)) void block_attn_fwd_kernel(BaArgs a, int64_t all)
 {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ unsigned long long odd;      // careful pass: rows of the tile that hold a value that is not finite
     typedef BaLds<T, DP> L;
-    typedef typename hd_vec<T>::v8 V8;
-    constexpr int CT = BaShape<T, DP>::CT, NT = BaShape<T, DP>::NT;
-    T *Ks = (T *)smem, *Vs = (T *)(smem + L::TILE);
     uint64_t *mask = (uint64_t *)(smem + 2 * L::TILE);
     uint32_t *list = (uint32_t *)(mask + a.cap), *words = list + a.cap, *before = words + (a.nb + 31) / 32;
 
     const int64_t id = ba_xcd(blockIdx.x, all);
     const BaTile t = ba_tile(a, id);
-    const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
-    const BaRows<T, DP> R(a, t);
+    const int g = (threadIdx.x & 63) >> 4;
+    const BaRow R(a, t);
+    typename hd_vec<T>::v8 qf[DP / 32];
+    ba_row_operand<T, DP>(R.at<T>(a.q, t.b), R.mine, a.d, qf);
+    const int count = ba_union(a, t, list, mask, words, before);
 
-    V8 qf[CT][DP / 32];
+    hd_f4 acc[DP / 16], sums;               // sums: running sum of the row, in every register
+    float top;                              // running maximum of the row, scaled
+    ba_fwd_pass<T, DP, false>(a, t, R, qf, smem, mask, list, count, &odd, acc, sums, top);
+    bool finite = ba_finite(sums[0]);
 #pragma unroll
-    for (int c = 0; c < CT; ++c)
-        ba_row_operand<T, DP>(R.at(a.q, t.b, c), R.mine[c], a.d, qf[c]);
-    const int count = ba_union<NT>(a, t, list, mask, words, before);
-    const T *K = (const T *)a.k.data + t.b * a.k.sb + t.h * a.k.sh, *V = (const T *)a.v.data + t.b * a.v.sb + t.h * a.v.sh;
-    const T *Kl = BaStage<T, DP, NT>::lane(K, a.k.sr), *Vl = BaStage<T, DP, NT>::lane(V, a.v.sr);
-
-    hd_f4 acc[CT][DP / 16];
-    hd_f4 sums[CT];                         // running sum of the column, in every register
-    float top[CT];                          // running maximum of the column
-    // A value that is not finite, times the probability 0 of a row that does not see it, is not 0: in the matrix product it
-    // would reach every row of the wave.  A workgroup that ends with such an output runs a second, careful pass, which
-    // leaves these values out of the matrix product and adds them to the rows that see them one by one.
-    for (int careful = 0;; careful = 1) {
+    for (int d = 0; d < DP / 16; ++d)
 #pragma unroll
-        for (int c = 0; c < CT; ++c) {
-#pragma unroll
-            for (int d = 0; d < DP / 16; ++d)
-                acc[c][d] = hd_f4{0.f, 0.f, 0.f, 0.f};
-            top[c] = -INFINITY, sums[c] = hd_f4{0.f, 0.f, 0.f, 0.f};
-        }
-        BaStage<T, DP, NT> kr, vr;
-        if (t.z < count) {
-            const int r0 = (int)list[t.z] * BA_BLOCK;
-            kr.load(Kl, a.k.sr, r0, t.live, a.d);
-            vr.load(Vl, a.v.sr, r0, t.live, a.d);
-        }
-        for (int u = t.z; u < count; u += a.splits) {
-            const int k0 = (int)list[u] * BA_BLOCK;
-            const uint64_t who = mask[u];
-            bool bit[CT], some = false, edge = false;
-#pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                bit[c] = R.mine[c] && ((who >> R.ql[c]) & 1);
-                some |= bit[c];
-                edge |= bit[c] && k0 + BA_BLOCK > R.limit[c];
-            }
-            __syncthreads();
-            kr.store(Ks);
-            if (careful) {
-                if (threadIdx.x == 0)
-                    odd = 0;
-                __syncthreads();
-                vr.store_finite(Vs, &odd);
-            } else {
-                vr.store(Vs);
-            }
-            __syncthreads();
-            if (u + a.splits < count) {
-                const int r0 = (int)list[u + a.splits] * BA_BLOCK;
-                kr.load(Kl, a.k.sr, r0, t.live, a.d);
-                vr.load(Vl, a.v.sr, r0, t.live, a.d);
-            }
-            if (!__any(some))
-                continue;                   // (wave-uniform; the barriers are at the head of the loop)
-            hd_f4 s[CT][4];
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-#pragma unroll
-                for (int c = 0; c < CT; ++c)
-                    s[c][x] = hd_f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int kk = 0; kk < DP / 32; ++kk) {
-                    const V8 kf = L::row8(Ks, x * 16 + l15, kk * 4 + g);
-#pragma unroll
-                    for (int c = 0; c < CT; ++c)
-                        s[c][x] = ba_mma<T>(kf, qf[c][kk], s[c][x]);
-                }
-            }
-            if (__any(edge)) {
-#pragma unroll
-                for (int c = 0; c < CT; ++c)
-#pragma unroll
-                    for (int x = 0; x < 4; ++x)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            s[c][x][r] = k0 + x * 16 + g * 4 + r < R.limit[c] ? s[c][x][r] : -INFINITY;
-            }
-            float keep[CT];
-            bool moved = false;
-#pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                float mx = -INFINITY;
-#pragma unroll
-                for (int x = 0; x < 4; ++x)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        mx = fmaxf(mx, s[c][x][r]);
-                mx = ba_col_max(mx) * a.scale2;
-                const float next = bit[c] ? fmaxf(top[c], mx) : top[c];
-                const float base = next == -INFINITY ? 0.f : next;
-                keep[c] = __builtin_amdgcn_exp2f(top[c] - base);        // top = -inf: 0
-                moved |= keep[c] != 1.f;
-                top[c] = next;
-                // a row that did not pick the block: exp2(x - inf) = 0 (a score that is not finite is left to the careful pass)
-                const float off = bit[c] ? base : INFINITY;
-#pragma unroll
-                for (int x = 0; x < 4; ++x)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][x][r], a.scale2, -off));
-                        s[c][x][r] = careful ? (bit[c] ? p : 0.f) : p;
-                    }
-            }
-            if (__any(moved)) {
-#pragma unroll
-                for (int c = 0; c < CT; ++c) {
-                    sums[c] *= keep[c];
-#pragma unroll
-                    for (int d = 0; d < DP / 16; ++d)
-                        acc[c][d] *= keep[c];
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                V8 pf[CT];
-#pragma unroll
-                for (int c = 0; c < CT; ++c) {
-                    pf[c] = ba_pack<T>(s[c][2 * j], s[c][2 * j + 1]);
-                    // the denominator as one more row of the product: ones times the probabilities, as rounded as they are there
-                    sums[c] = ba_mma<T>(ba_ones<T>(), pf[c], sums[c]);
-                }
-#pragma unroll
-                for (int d = 0; d < DP / 16; ++d) {
-                    const V8 vf = L::column(Vs, j * 32, d);
-#pragma unroll
-                    for (int c = 0; c < CT; ++c)
-                        acc[c][d] = ba_mma<T>(vf, pf[c], acc[c][d]);
-                }
-            }
-            if (careful) {
-                for (unsigned long long left = odd; left; left &= left - 1) {
-                    const int kk = __ffsll(left) - 1;               // the key's place in the block: score register and lane group
-#pragma unroll
-                    for (int c = 0; c < CT; ++c) {
-                        float p = 0.f;
-#pragma unroll
-                        for (int x = 0; x < 4; ++x)
-#pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                p = (kk >> 4) == x && (kk & 3) == r ? s[c][x][r] : p;
-                        p = __shfl(p, ((kk >> 2) & 3) * 16 + l15, 64);
-                        const bool sees = bit[c] && k0 + kk < R.limit[c];
-#pragma unroll
-                        for (int d = 0; d < DP / 16; ++d)
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                const int ch = d * 16 + g * 4 + r;
-                                const float val = sees && ch < a.d ? (float)V[(int64_t)(k0 + kk) * a.v.sr + ch] : 0.f;
-                                if (!(fabsf(val) <= 3.4028235e38f))
-                                    acc[c][d][r] = __builtin_fmaf(p, val, acc[c][d][r]);
-                            }
-                    }
-                }
-            }
-        }
-        bool finite = true;
-#pragma unroll
-        for (int c = 0; c < CT; ++c) {
-#pragma unroll
-            for (int d = 0; d < DP / 16; ++d)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    finite &= fabsf(acc[c][d][r]) <= 3.4028235e38f;
-            finite &= fabsf(sums[c][0]) <= 3.4028235e38f;
-        }
-        if (careful || !__syncthreads_or(!finite))
-            break;
-    }
-#pragma unroll
-    for (int c = 0; c < CT; ++c) {
-        if (!R.there[c])
-            continue;
-        const float sum = sums[c][0];
-        if (a.splits > 1) {
-            float *P = a.part + (R.flat(a, t.b, c) * a.splits + t.z) * (DP + 4);
-#pragma unroll
-            for (int d = 0; d < DP / 16; ++d)
-                *(hd_f4 *)(P + d * 16 + g * 4) = acc[c][d];
-            if (g == 0)
-                P[DP] = top[c], P[DP + 1] = sum;
-            continue;
-        }
-        const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
-        const int64_t at = R.out(a, t.b, c);
+        for (int r = 0; r < 4; ++r)
+            finite &= ba_finite(acc[d][r]);
+    if (__syncthreads_or(!finite))
+        ba_fwd_pass<T, DP, true>(a, t, R, qf, smem, mask, list, count, &odd, acc, sums, top);
+    if (!R.there)
+        return;
+    const float sum = sums[0];
+    if (a.splits > 1) {
+        float *P = a.part + (R.flat(a, t.b) * a.splits + t.z) * (DP + 4);
 #pragma unroll
         for (int d = 0; d < DP / 16; ++d)
-            if (d * 16 + g * 4 < a.d)
-                ba_store_rest<T>((T *)a.out + at, (T *)a.rest + at, a.rest != nullptr, d * 16 + g * 4, acc[c][d] * inv);
-        if (a.lse && g == 0)
-            a.lse[R.flat(a, t.b, c)] = sum > 0.f ? top[c] + log2f(sum) : -INFINITY;
+            *(hd_f4 *)(P + d * 16 + g * 4) = acc[d];
+        if (g == 0)
+            P[DP] = top, P[DP + 1] = sum;
+        return;
     }
+    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
+    const int64_t at = R.out(a, t.b);
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d)
+        if (d * 16 + g * 4 < a.d)
+            ba_store_rest<T>((T *)a.out + at, (T *)a.rest + at, a.rest != nullptr, d * 16 + g * 4, acc[d] * inv);
+    if (a.lse && g == 0)
+        a.lse[R.flat(a, t.b)] = sum > 0.f ? top + log2f(sum) : -INFINITY;
 }
 
 // Joins the splits of a row: 16 lanes a row, each a few channels.
@@ -676,170 +662,160 @@ __device__ __forceinline__ float ba_pow2_inverse(float x)
     return e == 0 || e >= 253 ? 1.f : __uint_as_float((uint32_t)(254 - e) << 23);
 }
 
+// As in the forward kernel, CAREFUL is the second pass of a workgroup in which a key that is not finite may have reached rows
+// that do not see it; those that do are not numbers (poison).
+template <typename T, int DP, bool CAREFUL>
+__device__ __forceinline__ void ba_dq_pass(const BaArgs &a, const BaTile &t, const BaRow &R, const typename hd_vec<T>::v8 *qf,
+                                           const typename hd_vec<T>::v8 *gf, float lse, float delta, float up, char *smem,
+                                           const uint64_t *mask, const uint32_t *list, int count, unsigned long long *odd,
+                                           hd_f4 *acc, bool &poison)
+{
+    typedef BaLds<T, DP> L;
+    typedef BaStage<T, DP> S;
+    typedef typename hd_vec<T>::v8 V8;
+    constexpr bool HALF = __is_same(T, _Float16);
+    T *Ks = (T *)smem, *Vs = (T *)(smem + L::TILE);
+    const int g = (threadIdx.x & 63) >> 4;
+    const T *Kl = S::lane((const T *)a.k.data + t.b * a.k.sb + t.h * a.k.sh, a.d);
+    const T *Vl = S::lane((const T *)a.v.data + t.b * a.v.sb + t.h * a.v.sh, a.d);
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d)
+        acc[d] = hd_f4{0.f, 0.f, 0.f, 0.f};
+    S kr, vr;
+    if (count > 0) {
+        const int r0 = (int)list[0] * BA_BLOCK;
+        kr.load(Kl, a.k.sr, r0, t.live);
+        vr.load(Vl, a.v.sr, r0, t.live);
+    }
+    for (int u = 0; u < count; ++u) {
+        const int k0 = (int)list[u] * BA_BLOCK;
+        const bool bit = R.mine && ((mask[u] >> R.ql) & 1);
+        __syncthreads();
+        vr.store(Vs);
+        if constexpr (CAREFUL) {
+            if (threadIdx.x == 0)
+                *odd = 0;
+            __syncthreads();
+            kr.store_finite(Ks, odd);
+        } else {
+            kr.store(Ks);
+        }
+        __syncthreads();
+        if constexpr (CAREFUL)
+            poison |= bit && (*odd & (R.limit - k0 >= BA_BLOCK ? ~0ull : (1ull << max(0, R.limit - k0)) - 1)) != 0;
+        if (u + 1 < count) {
+            const int r0 = (int)list[u + 1] * BA_BLOCK;
+            kr.load(Kl, a.k.sr, r0, t.live);
+            vr.load(Vl, a.v.sr, r0, t.live);
+        }
+        if (!__any(bit))
+            continue;
+        hd_f4 s[4], dp[4];
+        ba_scores<T, DP>(Ks, qf, s);
+        ba_scores<T, DP>(Vs, gf, dp);
+        V8 kf[DP / 16];
+        ba_columns<T, DP>(Ks, 0, kf);
+        ba_issue();
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][r], a.scale2, -lse)) * (dp[x][r] - delta);
+                s[x][r] = HALF ? e * up : e;
+            }
+        if (__any(bit && k0 + BA_BLOCK > R.limit)) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    s[x][r] = k0 + x * 16 + g * 4 + r < R.limit ? s[x][r] : 0.f;
+        }
+        if (!__all(bit)) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    s[x][r] = bit ? s[x][r] : 0.f;
+        }
+        V8 kn[DP / 16];
+        ba_columns<T, DP>(Ks, 32, kn);
+        ba_issue();
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const V8 sf = ba_pack<T>(s[2 * j], s[2 * j + 1]);
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d)
+                acc[d] = ba_mma<T>(j ? kn[d] : kf[d], sf, acc[d]);
+        }
+    }
+}
+
 template <typename T, int DP>
-__global__ __launch_bounds__((BaShape<T, DP>::NT), (BaShape<T, DP>::w)) void block_attn_dq_kernel(BaArgs a, int64_t all)
+__global__ __launch_bounds__(BA_THREADS, (BaShape<T, DP>::w)) void block_attn_dq_kernel(BaArgs a, int64_t all)
 {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ unsigned long long odd;
     typedef BaLds<T, DP> L;
     typedef typename hd_vec<T>::v8 V8;
-    constexpr int CT = BaShape<T, DP>::CT, NT = BaShape<T, DP>::NT;
     constexpr bool HALF = __is_same(T, _Float16);
-    T *Ks = (T *)smem, *Vs = (T *)(smem + L::TILE);
     uint64_t *mask = (uint64_t *)(smem + 2 * L::TILE);
     uint32_t *list = (uint32_t *)(mask + a.cap), *words = list + a.cap, *before = words + (a.nb + 31) / 32;
 
     const int64_t id = ba_xcd(blockIdx.x, all);
     const BaTile t = ba_tile(a, id);
-    const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
-    const BaRows<T, DP> R(a, t);
-
-    V8 qf[CT][DP / 32], gf[CT][DP / 32];
-    float delta[CT], lse[CT], up[CT];
-#pragma unroll
-    for (int c = 0; c < CT; ++c) {
-        ba_row_operand<T, DP>(R.at(a.q, t.b, c), R.mine[c], a.d, qf[c]);
-        ba_row_operand<T, DP>(R.at(a.go, t.b, c), R.mine[c], a.d, gf[c]);
+    const int g = (threadIdx.x & 63) >> 4;
+    const BaRow R(a, t);
+    V8 qf[DP / 32], gf[DP / 32];
+    ba_row_operand<T, DP>(R.at<T>(a.q, t.b), R.mine, a.d, qf);
+    ba_row_operand<T, DP>(R.at<T>(a.go, t.b), R.mine, a.d, gf);
+    float delta = 0.f, gmax = 0.f, lse = 0.f, up = 1.f;
+    {
         // the rounding of o, times a gradient, would move all of a row's ds one way: it goes back in
         V8 of[DP / 32], rf[DP / 32];
-        ba_row_operand<T, DP>(R.at(a.o, t.b, c), R.mine[c], a.d, of);
-        ba_row_operand<T, DP>((const T *)a.rest + R.out(a, t.b, c), R.mine[c] && a.rest, a.d, rf);
-        float sum = 0.f, gmax = 0.f;
+        ba_row_operand<T, DP>(R.at<T>(a.o, t.b), R.mine, a.d, of);
+        ba_row_operand<T, DP>((const T *)a.rest + R.out(a, t.b), R.mine && a.rest, a.d, rf);
 #pragma unroll
         for (int kk = 0; kk < DP / 32; ++kk)
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
-                sum = __builtin_fmaf((float)gf[c][kk][x], (float)of[kk][x] + (float)rf[kk][x], sum);
-                gmax = fmaxf(gmax, fabsf((float)gf[c][kk][x]));
+                delta = __builtin_fmaf((float)gf[kk][x], (float)of[kk][x] + (float)rf[kk][x], delta);
+                gmax = fmaxf(gmax, fabsf((float)gf[kk][x]));
             }
-        delta[c] = ba_col_sum(sum);
-        up[c] = 1.f;
+        delta = ba_col_sum(delta);
         if (HALF) {
             gmax = ba_col_max(gmax);
-            up[c] = ba_pow2_inverse(gmax);
+            up = ba_pow2_inverse(gmax);
         }
-        lse[c] = 0.f;
-        if (R.mine[c]) {
-            const int64_t at = R.flat(a, t.b, c);
-            lse[c] = a.lse[at];
+        if (R.mine) {
+            const int64_t at = R.flat(a, t.b);
+            lse = a.lse[at];
             if (g == 0) {
-                a.delta[at] = delta[c];
+                a.delta[at] = delta;
                 if (HALF)
                     a.gmax[at] = gmax;
             }
         }
     }
-    const int count = ba_union<NT>(a, t, list, mask, words, before);
-    const T *K = (const T *)a.k.data + t.b * a.k.sb + t.h * a.k.sh, *V = (const T *)a.v.data + t.b * a.v.sb + t.h * a.v.sh;
-    const T *Kl = BaStage<T, DP, NT>::lane(K, a.k.sr), *Vl = BaStage<T, DP, NT>::lane(V, a.v.sr);
-    hd_f4 acc[CT][DP / 16];
-    // as in the forward kernel: a second, careful pass where a key that is not finite may have reached rows that do not see
-    // it; those that do are not numbers
-    bool poison[CT] = {};
-    for (int careful = 0;; careful = 1) {
+    const int count = ba_union(a, t, list, mask, words, before);
+    hd_f4 acc[DP / 16];
+    bool poison = false;
+    ba_dq_pass<T, DP, false>(a, t, R, qf, gf, lse, delta, up, smem, mask, list, count, &odd, acc, poison);
+    bool finite = true;
 #pragma unroll
-        for (int c = 0; c < CT; ++c)
+    for (int d = 0; d < DP / 16; ++d)
 #pragma unroll
-            for (int d = 0; d < DP / 16; ++d)
-                acc[c][d] = hd_f4{0.f, 0.f, 0.f, 0.f};
-        BaStage<T, DP, NT> kr, vr;
-        if (count > 0) {
-            const int r0 = (int)list[0] * BA_BLOCK;
-            kr.load(Kl, a.k.sr, r0, t.live, a.d);
-            vr.load(Vl, a.v.sr, r0, t.live, a.d);
-        }
-        for (int u = 0; u < count; ++u) {
-            const int k0 = (int)list[u] * BA_BLOCK;
-            const uint64_t who = mask[u];
-            bool bit[CT], some = false;
+        for (int r = 0; r < 4; ++r)
+            finite &= ba_finite(acc[d][r]);
+    if (__syncthreads_or(!finite))
+        ba_dq_pass<T, DP, true>(a, t, R, qf, gf, lse, delta, up, smem, mask, list, count, &odd, acc, poison);
+    if (!R.there)
+        return;
+    T *O = (T *)a.out + R.out(a, t.b);
+    const float back = poison ? NAN : HALF ? a.scale / up : a.scale;
 #pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                bit[c] = R.mine[c] && ((who >> R.ql[c]) & 1);
-                some |= bit[c];
-            }
-            __syncthreads();
-            vr.store(Vs);
-            if (careful) {
-                if (threadIdx.x == 0)
-                    odd = 0;
-                __syncthreads();
-                kr.store_finite(Ks, &odd);
-            } else {
-                kr.store(Ks);
-            }
-            __syncthreads();
-            if (careful)
-#pragma unroll
-                for (int c = 0; c < CT; ++c)
-                    poison[c] |= bit[c] && (odd & (R.limit[c] - k0 >= BA_BLOCK ? ~0ull : (1ull << max(0, R.limit[c] - k0)) - 1)) != 0;
-            if (u + 1 < count) {
-                const int r0 = (int)list[u + 1] * BA_BLOCK;
-                kr.load(Kl, a.k.sr, r0, t.live, a.d);
-                vr.load(Vl, a.v.sr, r0, t.live, a.d);
-            }
-            if (!__any(some))
-                continue;
-            hd_f4 s[CT][4];
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                hd_f4 p[CT], dp[CT];
-#pragma unroll
-                for (int c = 0; c < CT; ++c)
-                    p[c] = dp[c] = hd_f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int kk = 0; kk < DP / 32; ++kk) {
-                    const V8 kf = L::row8(Ks, x * 16 + l15, kk * 4 + g), vf = L::row8(Vs, x * 16 + l15, kk * 4 + g);
-#pragma unroll
-                    for (int c = 0; c < CT; ++c) {
-                        p[c] = ba_mma<T>(kf, qf[c][kk], p[c]);
-                        dp[c] = ba_mma<T>(vf, gf[c][kk], dp[c]);
-                    }
-                }
-#pragma unroll
-                for (int c = 0; c < CT; ++c)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(p[c][r], a.scale2, -lse[c])) * (dp[c][r] - delta[c]);
-                        s[c][x][r] = bit[c] && k0 + x * 16 + g * 4 + r < R.limit[c] ? (HALF ? e * up[c] : e) : 0.f;
-                    }
-            }
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                V8 sf[CT];
-#pragma unroll
-                for (int c = 0; c < CT; ++c)
-                    sf[c] = ba_pack<T>(s[c][2 * j], s[c][2 * j + 1]);
-#pragma unroll
-                for (int d = 0; d < DP / 16; ++d) {
-                    const V8 kf = L::column(Ks, j * 32, d);
-#pragma unroll
-                    for (int c = 0; c < CT; ++c)
-                        acc[c][d] = ba_mma<T>(kf, sf[c], acc[c][d]);
-                }
-            }
-        }
-        bool finite = true;
-#pragma unroll
-        for (int c = 0; c < CT; ++c)
-#pragma unroll
-            for (int d = 0; d < DP / 16; ++d)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    finite &= fabsf(acc[c][d][r]) <= 3.4028235e38f;
-        if (careful || !__syncthreads_or(!finite))
-            break;
-    }
-#pragma unroll
-    for (int c = 0; c < CT; ++c) {
-        if (!R.there[c])
-            continue;
-        T *O = (T *)a.out + R.out(a, t.b, c);
-        const float back = poison[c] ? NAN : HALF ? a.scale / up[c] : a.scale;
-#pragma unroll
-        for (int d = 0; d < DP / 16; ++d)
-            if (d * 16 + g * 4 < a.d)
-                ba_store4<T>(O + d * 16 + g * 4, acc[c][d] * back);
-    }
+    for (int d = 0; d < DP / 16; ++d)
+        if (d * 16 + g * 4 < a.d)
+            ba_store4<T>(O + d * 16 + g * 4, acc[d] * back);
 }
 
 // ---- backward: which queries picked a block ------------------------------------------------------------------------------
@@ -875,13 +851,12 @@ __global__ __launch_bounds__(BA_THREADS) void block_pick_bits_kernel(BaArgs a)
 constexpr int BD_WORDS = 64;                // tiles of queries looked through at a time
 
 template <typename T, int DP>
-__global__ __launch_bounds__((BaShape<T, DP>::KNT), (BaShape<T, DP>::kw)) void block_attn_dkv_kernel(BaArgs a, int64_t all)
+__global__ __launch_bounds__(BA_THREADS, (BaShape<T, DP>::kw)) void block_attn_dkv_kernel(BaArgs a, int64_t all)
 {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ int list_rows;
     typedef BaLds<T, DP> L;
     typedef typename hd_vec<T>::v8 V8;
-    constexpr int KT = BaShape<T, DP>::KT, NT = BaShape<T, DP>::KNT;
     constexpr bool HALF = __is_same(T, _Float16);
     T *Qs = (T *)smem, *Gs = (T *)(smem + L::TILE);
     float *lse_s = (float *)(smem + 2 * L::TILE), *delta_s = lse_s + 64, *gmax_s = delta_s + 64;
@@ -891,43 +866,35 @@ __global__ __launch_bounds__((BaShape<T, DP>::KNT), (BaShape<T, DP>::kw)) void b
     const int z = (int)(id % a.splits), blk = (int)(id / a.splits % a.nb), bh = (int)(id / a.splits / a.nb), h = bh % a.hk, b = bh / a.hk;
     const int live = a.n_arr ? min(max(a.n_arr[b], 0), a.n) : a.n, lm = a.m_arr ? min(max(a.m_arr[b], 0), a.m) : a.m;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
-    int key[KT];
-    V8 kf[KT][DP / 32], vf[KT][DP / 32];
-    hd_f4 dk[KT][DP / 16], dv[KT][DP / 16];
+    const int key = blk * BA_BLOCK + wave * 16 + l15;
+    V8 kf[DP / 32], vf[DP / 32];
+    hd_f4 dk[DP / 16], dv[DP / 16];
+    ba_row_operand<T, DP>((const T *)a.k.data + b * a.k.sb + (int64_t)key * a.k.sr + h * a.k.sh, key < live, a.d, kf);
+    ba_row_operand<T, DP>((const T *)a.v.data + b * a.v.sb + (int64_t)key * a.v.sr + h * a.v.sh, key < live, a.d, vf);
 #pragma unroll
-    for (int c = 0; c < KT; ++c) {
-        key[c] = blk * BA_BLOCK + (wave * KT + c) * 16 + l15;
-        ba_row_operand<T, DP>((const T *)a.k.data + b * a.k.sb + (int64_t)key[c] * a.k.sr + h * a.k.sh, key[c] < live, a.d, kf[c]);
-        ba_row_operand<T, DP>((const T *)a.v.data + b * a.v.sb + (int64_t)key[c] * a.v.sr + h * a.v.sh, key[c] < live, a.d, vf[c]);
-#pragma unroll
-        for (int d = 0; d < DP / 16; ++d)
-            dk[c][d] = dv[c][d] = hd_f4{0.f, 0.f, 0.f, 0.f};
-    }
+    for (int d = 0; d < DP / 16; ++d)
+        dk[d] = dv[d] = hd_f4{0.f, 0.f, 0.f, 0.f};
     float up = 1.f;                         // fp16: dk is accumulated times this power of two
     bool first = true, any = false;
     const uint64_t *bits = a.bits + ((int64_t)bh * a.nb + blk) * a.mt;
     const int per = (a.mt + a.splits - 1) / a.splits, end = min(a.mt, (z + 1) * per);
 
-    typedef BaStage<T, DP, NT> S;
+    typedef BaStage<T, DP> S;
     V8 qr[S::PER], gr[S::PER];
     float row_lse = 0.f, row_delta = 0.f, row_gmax = 0.f;
     int row_limit = 0;
-    const T *Q = (const T *)a.q.data + b * a.q.sb + (int64_t)h * a.group * a.q.sh;
-    const T *G = (const T *)a.go.data + b * a.go.sb + (int64_t)h * a.group * a.go.sh;
-    // rows r0 .. r0 + 63 of the list (query by query, all heads of the group) to registers; rows behind the last are zeros
-    // that see nothing
+    const T *Q = S::lane((const T *)a.q.data + b * a.q.sb + (int64_t)h * a.group * a.q.sh, a.d);
+    const T *G = S::lane((const T *)a.go.data + b * a.go.sb + (int64_t)h * a.group * a.go.sh, a.d);
+    // rows r0 .. r0 + 63 of the list (query by query, all heads of the group) to registers; rows behind the last are its
+    // copies that see nothing
     auto fetch = [&](int r0, int rows) __attribute__((always_inline)) {
 #pragma unroll
         for (int x = 0; x < S::PER; ++x) {
-            const int r = r0 + S::row(x), c = S::part(x) * 8;
-            qr[x] = ba_zero<T>();
-            gr[x] = ba_zero<T>();
-            if (r < rows && c < a.d) {
-                const int q = a.group == 1 ? r : (int)__umulhi((unsigned)r, a.group_inverse), e = r - q * a.group;
-                const int64_t i = list[q];
-                qr[x] = *(const V8 *)(Q + i * a.q.sr + e * a.q.sh + c);
-                gr[x] = *(const V8 *)(G + i * a.go.sr + e * a.go.sh + c);
-            }
+            const int r = min(r0 + S::row(x), rows - 1);
+            const int q = a.group == 1 ? r : (int)__umulhi((unsigned)r, a.group_inverse), e = r - q * a.group;
+            const int64_t i = list[q];
+            qr[x] = *(const V8 *)(Q + i * a.q.sr + e * a.q.sh);
+            gr[x] = *(const V8 *)(G + i * a.go.sr + e * a.go.sh);
         }
         row_lse = row_delta = row_gmax = 0.f;
         row_limit = 0;
@@ -986,59 +953,58 @@ __global__ __launch_bounds__((BaShape<T, DP>::KNT), (BaShape<T, DP>::kw)) void b
                 if (m > 0.f && (first || want < up)) {
                     if (!first)
 #pragma unroll
-                        for (int c = 0; c < KT; ++c)
-#pragma unroll
-                            for (int d = 0; d < DP / 16; ++d)
-                                dk[c][d] *= want / up;
+                        for (int d = 0; d < DP / 16; ++d)
+                            dk[d] *= want / up;
                     up = want;
                     first = false;
                 }
             }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {   // 32 rows at a time
-                hd_f4 p[KT][2], ds[KT][2];
+                hd_f4 p[2], ds[2];
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    hd_f4 s[KT], dp[KT];
-#pragma unroll
-                    for (int c = 0; c < KT; ++c)
-                        s[c] = dp[c] = hd_f4{0.f, 0.f, 0.f, 0.f};
+                    V8 qa[DP / 32], ga[DP / 32];
 #pragma unroll
                     for (int kk = 0; kk < DP / 32; ++kk) {
-                        const int row = j * 32 + x * 16 + l15;
-                        const V8 qa = L::row8(Qs, row, kk * 4 + g), ga = L::row8(Gs, row, kk * 4 + g);
-#pragma unroll
-                        for (int c = 0; c < KT; ++c) {
-                            s[c] = ba_mma<T>(qa, kf[c][kk], s[c]);
-                            dp[c] = ba_mma<T>(ga, vf[c][kk], dp[c]);
-                        }
+                        qa[kk] = L::row8(Qs, j * 32 + x * 16 + l15, kk * 4 + g);
+                        ga[kk] = L::row8(Gs, j * 32 + x * 16 + l15, kk * 4 + g);
                     }
                     const int r4 = j * 32 + x * 16 + g * 4;
                     const hd_f4 le = *(const hd_f4 *)(lse_s + r4), de = *(const hd_f4 *)(delta_s + r4);
                     const int4 li = *(const int4 *)(limit_s + r4);
                     const int lim[4] = {li.x, li.y, li.z, li.w};
+                    ba_issue();
+                    hd_f4 s = {0.f, 0.f, 0.f, 0.f}, dp = s;
 #pragma unroll
-                    for (int c = 0; c < KT; ++c)
+                    for (int kk = 0; kk < DP / 32; ++kk) {
+                        s = ba_mma<T>(qa[kk], kf[kk], s);
+                        dp = ba_mma<T>(ga[kk], vf[kk], dp);
+                    }
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const bool see = key[c] < lim[r];
-                            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][r], a.scale2, -le[r]));
-                            const float f = e * (dp[c][r] - de[r]);
-                            p[c][x][r] = see ? e : 0.f;
-                            ds[c][x][r] = see ? (HALF ? f * up : f) : 0.f;
-                        }
+                    for (int r = 0; r < 4; ++r) {
+                        const bool see = key < lim[r];
+                        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.scale2, -le[r]));
+                        const float f = e * (dp[r] - de[r]);
+                        p[x][r] = see ? e : 0.f;
+                        ds[x][r] = see ? (HALF ? f * up : f) : 0.f;
+                    }
                 }
-                V8 pf[KT], sf[KT];
+                const V8 pf = ba_pack<T>(p[0], p[1]), sf = ba_pack<T>(ds[0], ds[1]);
+                constexpr int TG = DP / 16 < 4 ? DP / 16 : 4;
 #pragma unroll
-                for (int c = 0; c < KT; ++c)
-                    pf[c] = ba_pack<T>(p[c][0], p[c][1]), sf[c] = ba_pack<T>(ds[c][0], ds[c][1]);
+                for (int d0 = 0; d0 < DP / 16; d0 += TG) {
+                    V8 gc[TG], qc[TG];
 #pragma unroll
-                for (int d = 0; d < DP / 16; ++d) {
-                    const V8 gc = L::column(Gs, j * 32, d), qc = L::column(Qs, j * 32, d);
+                    for (int d = 0; d < TG; ++d) {
+                        gc[d] = L::column(Gs, j * 32, d0 + d);
+                        qc[d] = L::column(Qs, j * 32, d0 + d);
+                    }
+                    ba_issue();
 #pragma unroll
-                    for (int c = 0; c < KT; ++c) {
-                        dv[c][d] = ba_mma<T>(gc, pf[c], dv[c][d]);
-                        dk[c][d] = ba_mma<T>(qc, sf[c], dk[c][d]);
+                    for (int d = 0; d < TG; ++d) {
+                        dv[d0 + d] = ba_mma<T>(gc[d], pf, dv[d0 + d]);
+                        dk[d0 + d] = ba_mma<T>(qc[d], sf, dk[d0 + d]);
                     }
                 }
             }
@@ -1053,27 +1019,24 @@ __global__ __launch_bounds__((BaShape<T, DP>::KNT), (BaShape<T, DP>::kw)) void b
         if (!any)
             return;
     }
+    if (a.splits > 1) {
+        float *P = a.part + (tile * 2 * BA_BLOCK + wave * 16 + l15) * DP;
 #pragma unroll
-    for (int c = 0; c < KT; ++c) {
-        if (a.splits > 1) {
-            float *P = a.part + (tile * 2 * BA_BLOCK + (wave * KT + c) * 16 + l15) * DP;
-#pragma unroll
-            for (int d = 0; d < DP / 16; ++d) {
-                *(hd_f4 *)(P + d * 16 + g * 4) = dk[c][d] * back;
-                *(hd_f4 *)(P + BA_BLOCK * DP + d * 16 + g * 4) = dv[c][d];
-            }
-            continue;
+        for (int d = 0; d < DP / 16; ++d) {
+            *(hd_f4 *)(P + d * 16 + g * 4) = dk[d] * back;
+            *(hd_f4 *)(P + BA_BLOCK * DP + d * 16 + g * 4) = dv[d];
         }
-        if (key[c] >= a.n)
-            continue;
-        const int64_t at = (((int64_t)b * a.n + key[c]) * a.hk + h) * a.d;
-#pragma unroll
-        for (int d = 0; d < DP / 16; ++d)
-            if (d * 16 + g * 4 < a.d) {
-                ba_store4<T>((T *)a.out + at + d * 16 + g * 4, dk[c][d] * back);
-                ba_store4<T>((T *)a.out2 + at + d * 16 + g * 4, dv[c][d]);
-            }
+        return;
     }
+    if (key >= a.n)
+        return;
+    const int64_t at = (((int64_t)b * a.n + key) * a.hk + h) * a.d;
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d)
+        if (d * 16 + g * 4 < a.d) {
+            ba_store4<T>((T *)a.out + at + d * 16 + g * 4, dk[d] * back);
+            ba_store4<T>((T *)a.out2 + at + d * 16 + g * 4, dv[d]);
+        }
 }
 
 // dk and dv of a block from its parts, in the parts' order
@@ -1166,7 +1129,7 @@ template <typename T, int DP> int ba_forward(const BaArgs &a, hipStream_t s)
     int rc = ba_allow(block_attn_fwd_kernel<T, DP>, lds);
     if (rc)
         return rc;
-    hipLaunchKernelGGL((block_attn_fwd_kernel<T, DP>), dim3((unsigned)all), dim3(BaShape<T, DP>::NT), lds, s, a, all);
+    hipLaunchKernelGGL((block_attn_fwd_kernel<T, DP>), dim3((unsigned)all), dim3(BA_THREADS), lds, s, a, all);
     if (a.splits > 1) {
         const int64_t rows = (int64_t)a.b * a.hq * a.m, per = BA_THREADS / 16;
         hipLaunchKernelGGL((block_attn_join_kernel<T, DP>), dim3((unsigned)((rows + per - 1) / per)), dim3(BA_THREADS), 0, s, a, rows);
@@ -1184,7 +1147,7 @@ template <typename T, int DP> int ba_backward(BaArgs a, void *dq, void *dk, void
     if (rc)
         return rc;
     a.out = dq;
-    hipLaunchKernelGGL((block_attn_dq_kernel<T, DP>), dim3((unsigned)all), dim3(BaShape<T, DP>::NT), lds, s, a, all);
+    hipLaunchKernelGGL((block_attn_dq_kernel<T, DP>), dim3((unsigned)all), dim3(BA_THREADS), lds, s, a, all);
     if (a.nb == 0)
         return tpu3_launch_status();
     hipLaunchKernelGGL(block_pick_bits_kernel, dim3((unsigned)(a.b * a.hk * a.mt)), dim3(BA_THREADS), 0, s, a);
@@ -1195,7 +1158,7 @@ template <typename T, int DP> int ba_backward(BaArgs a, void *dq, void *dk, void
     a.out = dk, a.out2 = dv;
     const int64_t blocks = (int64_t)a.b * a.hk * a.nb;
     a.splits = ba_dkv_splits(a.b, a.m, a.hk, a.nb);
-    hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP>), dim3((unsigned)(blocks * a.splits)), dim3(BaShape<T, DP>::KNT), lds2, s, a, blocks * a.splits);
+    hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP>), dim3((unsigned)(blocks * a.splits)), dim3(BA_THREADS), lds2, s, a, blocks * a.splits);
     if (a.splits > 1)
         hipLaunchKernelGGL((block_attn_dkv_join_kernel<T, DP>), dim3((unsigned)blocks), dim3(BA_THREADS), 0, s, a);
     return tpu3_launch_status();
