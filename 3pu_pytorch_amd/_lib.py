@@ -131,7 +131,7 @@ SIGNATURES = {
     "tpu3_block_attn_fwd_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
     "tpu3_block_attn_bwd": (_i, [_vp, _i, _i, _i, _i, _i, _hp, _hp, _hp, _hp, _hp, _vp, _i, _f, _vp, _vp, _i, _vp, _vp, _vp,
                                  _vp, _vp, _vp, _sz]),
-    "tpu3_block_attn_bwd_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "tpu3_block_attn_bwd_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
 }
 
 TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}                                  # TPU3_TYPE_*

@@ -38,8 +38,9 @@ struct BaArgs {
     float *delta;                           // (b, hq, m): do . o
     float *gmax;                            // (b, hq, m): largest |do| of the row
     uint64_t *bits;                         // (b, hk, nb, mt): bit = query of the tile of 64 picked the block
-    float *part;                            // split forward: (rows, splits, d + 4); split dk / dv: (splits, blocks, 2, 64, d)
-    int32_t *used;                          // split dk / dv: (splits, blocks), the part holds something
+    float *part;                            // split forward: (rows, splits, d + 4); dk / dv in parts: (parts, 2, 64, d)
+    int32_t *picks, *first;                 // dk / dv in parts: queries that picked a block; first part of a block, and the end
+    int chunk;                              // queries of a part; 0: a workgroup per block
     int b, m, n, nb, mt, hq, hk, group, d, count, causal, splits, tiles, qt, cap;
     unsigned group_inverse;                 // ceil(2^32 / group): r / group = umulhi(r, it) for r * group < 2^32, group > 1
     float scale, scale2;                    // scale2 = scale * log2(e)
@@ -246,20 +247,28 @@ template <typename T, int DP> struct BaStage {
     }
 };
 
-// w, kw: waves a SIMD that the register allocation aims at (forward and dq, dk / dv).  A wave has 16 rows (keys): with 32,
-// every operand read from LDS feeds two matrix instructions, but half as many waves hide the latencies (attend clouds:
-// 188 us instead of 146).
-#ifndef BW64
-#define BW64 3
-#define BW128 2
-#define BK64 3
-#define BK128 2
+// How a kernel is laid out over registers and LDS; w: waves a SIMD that the register allocation aims at.  More waves hide
+// more of the chain scores -> maximum -> exponentials -> product, until the operands no longer fit: measured on clouds
+// of 5000 points (64 channels) and a sequence of 8192 (128), us with 2 / 3 / 4 waves: forward - / 144 / 129 and
+// 310 / 279 / -, dq - / 94 / 99 and 341 / 520 / -, dk and dv - / 63 / 92 and 346 / 900 / -.  A wave has 16 rows (keys):
+// with 32, every operand read from LDS feeds two matrix instructions, but half as many waves are there (188 for 146).
+// together: 16-row tiles whose row operands are read in one go; columns: 16-channel columns read in one go.
+#ifndef DQ_TOG
+#define DQ_TOG 2
+#define DQ_COL 8
 #endif
-template <typename T, int DP> struct BaShape {
-    static constexpr int w = sizeof(T) == 4 ? (DP == 128 ? 1 : DP == 64 ? 2 : 3) : DP == 128 ? BW128 : BW64;
-    static constexpr int kw = sizeof(T) == 4 ? (DP == 128 ? 1 : 2) : DP == 128 ? BK128 : BK64;
-    // 16-row tiles whose row operands are read together (fp32 rows are twice as wide)
-    static constexpr int TOGETHER = DP * sizeof(T) >= 512 ? 1 : DP * sizeof(T) >= 256 ? 2 : 4;
+template <typename T, int DP> struct BaFwd {
+    static constexpr bool F32 = sizeof(T) == 4;
+    static constexpr int w = F32 ? (DP == 128 ? 1 : DP == 64 ? 2 : 3) : DP == 128 ? 3 : 4;
+    static constexpr int together = F32 ? (DP == 32 ? 4 : DP == 64 ? 2 : 1) : DP == 128 ? 1 : 2;
+    static constexpr int columns = DP / 16 < 4 ? DP / 16 : 4;
+};
+template <typename T, int DP> struct BaBwd {
+    static constexpr bool F32 = sizeof(T) == 4;
+    static constexpr int w = F32 ? (DP == 128 ? 1 : DP == 64 ? 2 : 3) : DP == 128 ? 2 : 3;
+    static constexpr int together = F32 ? (DP == 32 ? 4 : DP == 64 ? 2 : 1) : DP == 128 ? DQ_TOG : 4;
+    static constexpr int columns = DP / 16 < DQ_COL ? DP / 16 : DQ_COL;
+    static constexpr int kw = F32 ? (DP == 128 ? 1 : 2) : DP == 128 ? 2 : 3;
 };
 // LDS reads above stay above: the compiler otherwise sinks each to its matrix instruction and waits for it there
 __device__ __forceinline__ void ba_issue() { __builtin_amdgcn_sched_barrier(0); }
@@ -410,11 +419,10 @@ struct BaRow {
 };
 
 // scores (keys x rows) of the tile: s[x] = 16 keys x 16 rows
-template <typename T, int DP>
+template <typename T, int DP, int TG>
 __device__ __forceinline__ void ba_scores(const T *tile, const typename hd_vec<T>::v8 *f, hd_f4 *s)
 {
     typedef BaLds<T, DP> L;
-    constexpr int TG = BaShape<T, DP>::TOGETHER;
     const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int x0 = 0; x0 < 4; x0 += TG) {
@@ -435,14 +443,125 @@ __device__ __forceinline__ void ba_scores(const T *tile, const typename hd_vec<T
                 s[x0 + x] = ba_mma<T>(kf[x][kk], f[kk], s[x0 + x]);
     }
 }
-// the tile's columns of 32 keys, all channels
-template <typename T, int DP> __device__ __forceinline__ void ba_columns(const T *tile, int r0, typename hd_vec<T>::v8 *f)
-{
+// acc[d] += (tile's columns) (f[0] for its first 32 rows, f[1] for the others): a group of columns is read while the matrix
+// instructions of the one before run.  start() reads the first group; before(j) runs ahead of half j's matrix instructions.
+template <typename T, int DP, int VG> struct BaColumns {
+    static constexpr int STEPS = 2 * (DP / 16) / VG;
+    typename hd_vec<T>::v8 c[2][VG];
+    __device__ __forceinline__ void read(const T *tile, int step)
+    {
 #pragma unroll
-    for (int d = 0; d < DP / 16; ++d)
-        f[d] = BaLds<T, DP>::column(tile, r0, d);
-}
+        for (int i = 0; i < VG; ++i)
+            c[step & 1][i] = BaLds<T, DP>::column(tile, step >= STEPS / 2 ? 32 : 0, (step % (STEPS / 2)) * VG + i);
+    }
+    __device__ __forceinline__ void start(const T *tile)
+    {
+        read(tile, 0);
+        ba_issue();
+    }
+    template <typename F> __device__ __forceinline__ void run(const T *tile, hd_f4 *acc, F &&before)
+    {
+        typename hd_vec<T>::v8 f;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            if (s % (STEPS / 2) == 0)
+                f = before(s / (STEPS / 2));
+            if (s + 1 < STEPS) {
+                read(tile, s + 1);
+                ba_issue();
+            }
+#pragma unroll
+            for (int i = 0; i < VG; ++i) {
+                hd_f4 &x = acc[(s % (STEPS / 2)) * VG + i];
+                x = ba_mma<T>(c[s & 1][i], f, x);
+            }
+        }
+    }
+};
 __device__ __forceinline__ bool ba_finite(float x) { return fabsf(x) <= 3.4028235e38f; }
+
+// one block of keys: Ks, with Vs behind it, in LDS; k0 = its first key; bit = this lane's row picked it
+template <typename T, int DP, bool CAREFUL>
+__device__ __forceinline__ void ba_fwd_block(const BaArgs &a, const BaRow &R, const typename hd_vec<T>::v8 *qf, const T *Ks, const T *V,
+                                             int k0, bool bit, const unsigned long long *odd, hd_f4 *acc, hd_f4 &sums, float &top)
+{
+    typedef typename hd_vec<T>::v8 V8;
+    const T *Vs = Ks + BA_ROWS * DP;
+    const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
+    if (!__any(bit))
+        return;                         // (wave-uniform)
+    hd_f4 s[4];
+    ba_scores<T, DP, BaFwd<T, DP>::together>(Ks, qf, s);
+    BaColumns<T, DP, BaFwd<T, DP>::columns> vc;
+    vc.start(Vs);
+    if (__any(bit && k0 + BA_BLOCK > R.limit)) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                s[x][r] = k0 + x * 16 + g * 4 + r < R.limit ? s[x][r] : -INFINITY;
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            mx = fmaxf(mx, s[x][r]);
+    mx = ba_col_max(mx) * a.scale2;
+    const float next = bit ? fmaxf(top, mx) : top;
+    const float base = next == -INFINITY ? 0.f : next;
+    const float keep = __builtin_amdgcn_exp2f(top - base);          // top = -inf: 0
+    top = next;
+    if (__any(keep != 1.f)) {
+        sums *= keep;
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d)
+            acc[d] *= keep;
+    }
+    // a row that did not pick the block: exp2(x - inf) = 0 (a score that is not finite is left to the careful pass)
+    const float off = bit ? base : INFINITY;
+    auto weight = [&](int x) __attribute__((always_inline)) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            s[x][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][r], a.scale2, -off));
+            if (CAREFUL)
+                s[x][r] = bit ? s[x][r] : 0.f;
+        }
+    };
+    vc.run(Vs, acc, [&](int j) __attribute__((always_inline)) {
+        weight(2 * j), weight(2 * j + 1);
+        const V8 pf = ba_pack<T>(s[2 * j], s[2 * j + 1]);
+        // the denominator: in the 16-bit types one more row of the product, ones times the probabilities, as rounded as they
+        // are there; in fp32, whose matrix instructions are the bound, this lane's share by additions
+        if constexpr (sizeof(T) == 2)
+            sums = ba_mma<T>(ba_ones<T>(), pf, sums);
+        else
+            sums += s[2 * j] + s[2 * j + 1];
+        return pf;
+    });
+    if constexpr (CAREFUL) {
+        for (unsigned long long left = *odd; left; left &= left - 1) {
+            const int kk = __ffsll(left) - 1;                   // the key's place in the block: score register and lane group
+            float p = 0.f;
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    p = (kk >> 4) == x && (kk & 3) == r ? s[x][r] : p;
+            p = __shfl(p, ((kk >> 2) & 3) * 16 + l15, 64);
+            const bool sees = bit && k0 + kk < R.limit;
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int ch = d * 16 + g * 4 + r;
+                    const float val = sees && ch < a.d ? (float)V[(int64_t)(k0 + kk) * a.v.sr + ch] : 0.f;
+                    if (!ba_finite(val))
+                        acc[d][r] = __builtin_fmaf(p, val, acc[d][r]);
+                }
+        }
+    }
+}
 
 // A value that is not finite, times the probability 0 of a row that does not see it, is not 0: in the matrix product it would
 // reach every row of the wave.  A workgroup that ends with such an output runs its blocks a second time, carefully: these
@@ -454,123 +573,48 @@ __device__ __forceinline__ void ba_fwd_pass(const BaArgs &a, const BaTile &t, co
 {
     typedef BaLds<T, DP> L;
     typedef BaStage<T, DP> S;
-    typedef typename hd_vec<T>::v8 V8;
-    T *Ks = (T *)smem, *Vs = (T *)(smem + L::TILE);
-    const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
     const T *K = (const T *)a.k.data + t.b * a.k.sb + t.h * a.k.sh, *V = (const T *)a.v.data + t.b * a.v.sb + t.h * a.v.sh;
     const T *Kl = S::lane(K, a.d), *Vl = S::lane(V, a.d);
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d)
         acc[d] = hd_f4{0.f, 0.f, 0.f, 0.f};
     top = -INFINITY, sums = hd_f4{0.f, 0.f, 0.f, 0.f};
+    // (a second tile buffer and one barrier less a block made no difference: 142 for 144 us)
     S kr, vr;
-    if (t.z < count) {
-        const int r0 = (int)list[t.z] * BA_BLOCK;
-        kr.load(Kl, a.k.sr, r0, t.live);
-        vr.load(Vl, a.v.sr, r0, t.live);
-    }
-    for (int u = t.z; u < count; u += a.splits) {
-        const int k0 = (int)list[u] * BA_BLOCK;
-        const bool bit = R.mine && ((mask[u] >> R.ql) & 1);
-        __syncthreads();
-        kr.store(Ks);
+    auto fetch = [&](int u) __attribute__((always_inline)) {
+        if (u < count) {
+            const int r0 = (int)list[u] * BA_BLOCK;
+            kr.load(Kl, a.k.sr, r0, t.live);
+            vr.load(Vl, a.v.sr, r0, t.live);
+        }
+    };
+    T *k = (T *)smem, *v = (T *)(smem + L::TILE);
+    auto put = [&]() __attribute__((always_inline)) {
+        kr.store(k);
         if constexpr (CAREFUL) {
             if (threadIdx.x == 0)
                 *odd = 0;
             __syncthreads();
-            vr.store_finite(Vs, odd);
+            vr.store_finite(v, odd);
         } else {
-            vr.store(Vs);
+            vr.store(v);
         }
+    };
+    fetch(t.z);
+    for (int u = t.z; u < count; u += a.splits) {
         __syncthreads();
-        if (u + a.splits < count) {
-            const int r0 = (int)list[u + a.splits] * BA_BLOCK;
-            kr.load(Kl, a.k.sr, r0, t.live);
-            vr.load(Vl, a.v.sr, r0, t.live);
-        }
-        if (!__any(bit))
-            continue;                       // (wave-uniform; the barriers are at the head of the loop)
-        hd_f4 s[4];
-        ba_scores<T, DP>(Ks, qf, s);
-        V8 vf[DP / 16];
-        ba_columns<T, DP>(Vs, 0, vf);
-        ba_issue();
-        if (__any(bit && k0 + BA_BLOCK > R.limit)) {
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    s[x][r] = k0 + x * 16 + g * 4 + r < R.limit ? s[x][r] : -INFINITY;
-        }
-        float mx = -INFINITY;
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                mx = fmaxf(mx, s[x][r]);
-        mx = ba_col_max(mx) * a.scale2;
-        const float next = bit ? fmaxf(top, mx) : top;
-        const float base = next == -INFINITY ? 0.f : next;
-        const float keep = __builtin_amdgcn_exp2f(top - base);          // top = -inf: 0
-        top = next;
-        if (__any(keep != 1.f)) {
-            sums *= keep;
-#pragma unroll
-            for (int d = 0; d < DP / 16; ++d)
-                acc[d] *= keep;
-        }
-        // a row that did not pick the block: exp2(x - inf) = 0 (a score that is not finite is left to the careful pass)
-        const float off = bit ? base : INFINITY;
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                s[x][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][r], a.scale2, -off));
-                if (CAREFUL)
-                    s[x][r] = bit ? s[x][r] : 0.f;
-            }
-        V8 vn[DP / 16];
-        ba_columns<T, DP>(Vs, 32, vn);
-        ba_issue();
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const V8 pf = ba_pack<T>(s[2 * j], s[2 * j + 1]);
-            // the denominator as one more row of the product: ones times the probabilities, as rounded as they are there
-            sums = ba_mma<T>(ba_ones<T>(), pf, sums);
-#pragma unroll
-            for (int d = 0; d < DP / 16; ++d)
-                acc[d] = ba_mma<T>(j ? vn[d] : vf[d], pf, acc[d]);
-        }
-        if constexpr (CAREFUL) {
-            for (unsigned long long left = *odd; left; left &= left - 1) {
-                const int kk = __ffsll(left) - 1;                   // the key's place in the block: score register and lane group
-                float p = 0.f;
-#pragma unroll
-                for (int x = 0; x < 4; ++x)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        p = (kk >> 4) == x && (kk & 3) == r ? s[x][r] : p;
-                p = __shfl(p, ((kk >> 2) & 3) * 16 + l15, 64);
-                const bool sees = bit && k0 + kk < R.limit;
-#pragma unroll
-                for (int d = 0; d < DP / 16; ++d)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int ch = d * 16 + g * 4 + r;
-                        const float val = sees && ch < a.d ? (float)V[(int64_t)(k0 + kk) * a.v.sr + ch] : 0.f;
-                        if (!ba_finite(val))
-                            acc[d][r] = __builtin_fmaf(p, val, acc[d][r]);
-                    }
-            }
-        }
+        put();
+        __syncthreads();
+        fetch(u + a.splits);
+        ba_fwd_block<T, DP, CAREFUL>(a, R, qf, k, V, (int)list[u] * BA_BLOCK, R.mine && ((mask[u] >> R.ql) & 1), odd, acc, sums, top);
     }
 }
 
 template <typename T, int DP>
-__global__ __launch_bounds__(BA_THREADS, (BaShape<T, DP>::w)) void block_attn_fwd_kernel(BaArgs a, int64_t all)
+__global__ __launch_bounds__(BA_THREADS, (BaFwd<T, DP>::w)) void block_attn_fwd_kernel(BaArgs a, int64_t all)
 {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    __shared__ unsigned long long odd;      // careful pass: rows of the tile that hold a value that is not finite
+    __shared__ unsigned long long odd;   // careful pass: rows of a tile that hold a value that is not finite
     typedef BaLds<T, DP> L;
     uint64_t *mask = (uint64_t *)(smem + 2 * L::TILE);
     uint32_t *list = (uint32_t *)(mask + a.cap), *words = list + a.cap, *before = words + (a.nb + 31) / 32;
@@ -583,10 +627,10 @@ __global__ __launch_bounds__(BA_THREADS, (BaShape<T, DP>::w)) void block_attn_fw
     ba_row_operand<T, DP>(R.at<T>(a.q, t.b), R.mine, a.d, qf);
     const int count = ba_union(a, t, list, mask, words, before);
 
-    hd_f4 acc[DP / 16], sums;               // sums: running sum of the row, in every register
+    hd_f4 acc[DP / 16], sums;               // sums: running sum of the row
     float top;                              // running maximum of the row, scaled
     ba_fwd_pass<T, DP, false>(a, t, R, qf, smem, mask, list, count, &odd, acc, sums, top);
-    bool finite = ba_finite(sums[0]);
+    bool finite = ba_finite(sums[0] + sums[1] + sums[2] + sums[3]);
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d)
 #pragma unroll
@@ -594,9 +638,10 @@ __global__ __launch_bounds__(BA_THREADS, (BaShape<T, DP>::w)) void block_attn_fw
             finite &= ba_finite(acc[d][r]);
     if (__syncthreads_or(!finite))
         ba_fwd_pass<T, DP, true>(a, t, R, qf, smem, mask, list, count, &odd, acc, sums, top);
+    const float total = ba_col_sum(sums[0] + sums[1] + sums[2] + sums[3]);
     if (!R.there)
         return;
-    const float sum = sums[0];
+    const float sum = sizeof(T) == 2 ? sums[0] : total;
     if (a.splits > 1) {
         float *P = a.part + (R.flat(a, t.b) * a.splits + t.z) * (DP + 4);
 #pragma unroll
@@ -662,6 +707,45 @@ __device__ __forceinline__ float ba_pow2_inverse(float x)
     return e == 0 || e >= 253 ? 1.f : __uint_as_float((uint32_t)(254 - e) << 23);
 }
 
+template <typename T, int DP>
+__device__ __forceinline__ void ba_dq_block(const BaArgs &a, const BaRow &R, const typename hd_vec<T>::v8 *qf, const typename hd_vec<T>::v8 *gf,
+                                            float lse, float delta, float up, const T *Ks, int k0, bool bit, hd_f4 *acc)
+{
+    typedef typename hd_vec<T>::v8 V8;
+    constexpr bool HALF = __is_same(T, _Float16);
+    const T *Vs = Ks + BA_ROWS * DP;
+    const int g = (threadIdx.x & 63) >> 4;
+    if (!__any(bit))
+        return;                             // (wave-uniform)
+    hd_f4 s[4], dp[4];
+    ba_scores<T, DP, BaBwd<T, DP>::together>(Ks, qf, s);
+    ba_scores<T, DP, BaBwd<T, DP>::together>(Vs, gf, dp);
+    BaColumns<T, DP, BaBwd<T, DP>::columns> kc;
+    kc.start(Ks);
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][r], a.scale2, -lse)) * (dp[x][r] - delta);
+            s[x][r] = HALF ? e * up : e;
+        }
+    if (__any(bit && k0 + BA_BLOCK > R.limit)) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                s[x][r] = k0 + x * 16 + g * 4 + r < R.limit ? s[x][r] : 0.f;
+    }
+    if (!__all(bit)) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                s[x][r] = bit ? s[x][r] : 0.f;
+    }
+    kc.run(Ks, acc, [&](int j) __attribute__((always_inline)) { return ba_pack<T>(s[2 * j], s[2 * j + 1]); });
+}
+
 // As in the forward kernel, CAREFUL is the second pass of a workgroup in which a key that is not finite may have reached rows
 // that do not see it; those that do are not numbers (poison).
 template <typename T, int DP, bool CAREFUL>
@@ -672,86 +756,47 @@ __device__ __forceinline__ void ba_dq_pass(const BaArgs &a, const BaTile &t, con
 {
     typedef BaLds<T, DP> L;
     typedef BaStage<T, DP> S;
-    typedef typename hd_vec<T>::v8 V8;
-    constexpr bool HALF = __is_same(T, _Float16);
-    T *Ks = (T *)smem, *Vs = (T *)(smem + L::TILE);
-    const int g = (threadIdx.x & 63) >> 4;
     const T *Kl = S::lane((const T *)a.k.data + t.b * a.k.sb + t.h * a.k.sh, a.d);
     const T *Vl = S::lane((const T *)a.v.data + t.b * a.v.sb + t.h * a.v.sh, a.d);
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d)
         acc[d] = hd_f4{0.f, 0.f, 0.f, 0.f};
     S kr, vr;
-    if (count > 0) {
-        const int r0 = (int)list[0] * BA_BLOCK;
-        kr.load(Kl, a.k.sr, r0, t.live);
-        vr.load(Vl, a.v.sr, r0, t.live);
-    }
-    for (int u = 0; u < count; ++u) {
-        const int k0 = (int)list[u] * BA_BLOCK;
-        const bool bit = R.mine && ((mask[u] >> R.ql) & 1);
-        __syncthreads();
-        vr.store(Vs);
+    auto fetch = [&](int u) __attribute__((always_inline)) {
+        if (u < count) {
+            const int r0 = (int)list[u] * BA_BLOCK;
+            kr.load(Kl, a.k.sr, r0, t.live);
+            vr.load(Vl, a.v.sr, r0, t.live);
+        }
+    };
+    T *k = (T *)smem, *v = (T *)(smem + L::TILE);
+    auto put = [&]() __attribute__((always_inline)) {
+        vr.store(v);
         if constexpr (CAREFUL) {
             if (threadIdx.x == 0)
                 *odd = 0;
             __syncthreads();
-            kr.store_finite(Ks, odd);
+            kr.store_finite(k, odd);
         } else {
-            kr.store(Ks);
+            kr.store(k);
         }
+    };
+    fetch(0);
+    for (int u = 0; u < count; ++u) {
         __syncthreads();
+        put();
+        __syncthreads();
+        fetch(u + 1);
+        const int k0 = (int)list[u] * BA_BLOCK;
+        const bool bit = R.mine && ((mask[u] >> R.ql) & 1);
         if constexpr (CAREFUL)
             poison |= bit && (*odd & (R.limit - k0 >= BA_BLOCK ? ~0ull : (1ull << max(0, R.limit - k0)) - 1)) != 0;
-        if (u + 1 < count) {
-            const int r0 = (int)list[u + 1] * BA_BLOCK;
-            kr.load(Kl, a.k.sr, r0, t.live);
-            vr.load(Vl, a.v.sr, r0, t.live);
-        }
-        if (!__any(bit))
-            continue;
-        hd_f4 s[4], dp[4];
-        ba_scores<T, DP>(Ks, qf, s);
-        ba_scores<T, DP>(Vs, gf, dp);
-        V8 kf[DP / 16];
-        ba_columns<T, DP>(Ks, 0, kf);
-        ba_issue();
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][r], a.scale2, -lse)) * (dp[x][r] - delta);
-                s[x][r] = HALF ? e * up : e;
-            }
-        if (__any(bit && k0 + BA_BLOCK > R.limit)) {
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    s[x][r] = k0 + x * 16 + g * 4 + r < R.limit ? s[x][r] : 0.f;
-        }
-        if (!__all(bit)) {
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    s[x][r] = bit ? s[x][r] : 0.f;
-        }
-        V8 kn[DP / 16];
-        ba_columns<T, DP>(Ks, 32, kn);
-        ba_issue();
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const V8 sf = ba_pack<T>(s[2 * j], s[2 * j + 1]);
-#pragma unroll
-            for (int d = 0; d < DP / 16; ++d)
-                acc[d] = ba_mma<T>(j ? kn[d] : kf[d], sf, acc[d]);
-        }
+        ba_dq_block<T, DP>(a, R, qf, gf, lse, delta, up, k, k0, bit, acc);
     }
 }
 
 template <typename T, int DP>
-__global__ __launch_bounds__(BA_THREADS, (BaShape<T, DP>::w)) void block_attn_dq_kernel(BaArgs a, int64_t all)
+__global__ __launch_bounds__(BA_THREADS, (BaBwd<T, DP>::w)) void block_attn_dq_kernel(BaArgs a, int64_t all)
 {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ unsigned long long odd;
@@ -845,16 +890,58 @@ __global__ __launch_bounds__(BA_THREADS) void block_pick_bits_kernel(BaArgs a)
     }
 }
 
+// Some blocks are picked by many more queries than others (a popular region, the start of a sequence), and where blocks are
+// few the chip would wait for the longest.  Their queries are then dealt into parts of `chunk` in order; a part is a
+// workgroup's work, and a block of several parts is added up in their order afterwards.
+__global__ __launch_bounds__(BA_THREADS) void block_picks_kernel(BaArgs a)
+{
+    __shared__ int s[4];
+    const uint64_t *bits = a.bits + (int64_t)blockIdx.x * a.mt;
+    int v = 0;
+    for (int w = threadIdx.x; w < a.mt; w += BA_THREADS)
+        v += __popcll(bits[w]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+        v += __shfl_xor(v, o, 64);
+    if ((threadIdx.x & 63) == 0)
+        s[threadIdx.x >> 6] = v;
+    __syncthreads();
+    if (threadIdx.x == 0)
+        a.picks[blockIdx.x] = s[0] + s[1] + s[2] + s[3];
+}
+// first[i] = number of parts of the blocks before i (a block nobody picked is one part: it writes zeros); at most 1024 blocks
+__global__ __launch_bounds__(1024) void block_parts_kernel(BaArgs a, int blocks)
+{
+    __shared__ int s[16];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int mine = t < blocks ? max(1, (a.picks[t] + a.chunk - 1) / a.chunk) : 0;
+    int inc = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int v = __shfl_up(inc, o, 64);
+        inc += lane >= o ? v : 0;
+    }
+    if (lane == 63)
+        s[wave] = inc;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w)
+        inc += s[w];
+    if (t < blocks)
+        a.first[t] = inc - mine;
+    if (t == blocks - 1)
+        a.first[blocks] = inc;
+}
+
 // ---- backward: dk, dv ----------------------------------------------------------------------------------------------------
 // A workgroup per block of keys; a wave owns 16 of its keys.  Scores are formed as rows x keys here, so that P and dS come
 // out with a key per lane: the B operand of dv^T = do^T P and dk^T = q^T dS.
 constexpr int BD_WORDS = 64;                // tiles of queries looked through at a time
 
 template <typename T, int DP>
-__global__ __launch_bounds__(BA_THREADS, (BaShape<T, DP>::kw)) void block_attn_dkv_kernel(BaArgs a, int64_t all)
+__global__ __launch_bounds__(BA_THREADS, (BaBwd<T, DP>::kw)) void block_attn_dkv_kernel(BaArgs a, int64_t all)
 {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    __shared__ int list_rows;
+    __shared__ int list_all;
     typedef BaLds<T, DP> L;
     typedef typename hd_vec<T>::v8 V8;
     constexpr bool HALF = __is_same(T, _Float16);
@@ -862,8 +949,27 @@ __global__ __launch_bounds__(BA_THREADS, (BaShape<T, DP>::kw)) void block_attn_d
     float *lse_s = (float *)(smem + 2 * L::TILE), *delta_s = lse_s + 64, *gmax_s = delta_s + 64;
     int *limit_s = (int *)(gmax_s + 64), *list = limit_s + 64;              // list: BD_WORDS * 64 queries
 
-    const int64_t id = ba_xcd(blockIdx.x, all);
-    const int z = (int)(id % a.splits), blk = (int)(id / a.splits % a.nb), bh = (int)(id / a.splits / a.nb), h = bh % a.hk, b = bh / a.hk;
+    int64_t id = ba_xcd(blockIdx.x, all), part = 0;
+    int skip = 0, take = 0x7FFFFFFF, parts = 1;                 // of the queries that picked the block, in order
+    if (a.chunk) {
+        const int blocks = a.b * a.hk * a.nb;
+        part = id;
+        if (part >= a.first[blocks])
+            return;
+        int lo = 0, hi = blocks - 1;        // the last block whose first part is not behind this one
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (a.first[mid] <= part)
+                lo = mid;
+            else
+                hi = mid - 1;
+        }
+        id = lo;
+        parts = a.first[lo + 1] - a.first[lo];
+        skip = (int)(part - a.first[lo]) * a.chunk;
+        take = a.chunk;
+    }
+    const int blk = (int)(id % a.nb), bh = (int)(id / a.nb), h = bh % a.hk, b = bh / a.hk;
     const int live = a.n_arr ? min(max(a.n_arr[b], 0), a.n) : a.n, lm = a.m_arr ? min(max(a.m_arr[b], 0), a.m) : a.m;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
     const int key = blk * BA_BLOCK + wave * 16 + l15;
@@ -875,9 +981,8 @@ __global__ __launch_bounds__(BA_THREADS, (BaShape<T, DP>::kw)) void block_attn_d
     for (int d = 0; d < DP / 16; ++d)
         dk[d] = dv[d] = hd_f4{0.f, 0.f, 0.f, 0.f};
     float up = 1.f;                         // fp16: dk is accumulated times this power of two
-    bool first = true, any = false;
+    bool first = true;
     const uint64_t *bits = a.bits + ((int64_t)bh * a.nb + blk) * a.mt;
-    const int per = (a.mt + a.splits - 1) / a.splits, end = min(a.mt, (z + 1) * per);
 
     typedef BaStage<T, DP> S;
     V8 qr[S::PER], gr[S::PER];
@@ -907,25 +1012,27 @@ __global__ __launch_bounds__(BA_THREADS, (BaShape<T, DP>::kw)) void block_attn_d
         }
     };
 
-    for (int w0 = z * per; w0 < end; w0 += BD_WORDS) {
-        // the queries of the next 64 tiles that picked this block, in order
+    for (int w0 = 0; w0 < a.mt && take > 0; w0 += BD_WORDS) {
+        // the queries of the next 64 tiles that picked this block, in order; `skip` of them are other parts', `take` are ours
         if (wave == 0) {
-            uint64_t word = w0 + lane < min(end, w0 + BD_WORDS) ? bits[w0 + lane] : 0ull;
+            uint64_t word = w0 + lane < a.mt ? bits[w0 + lane] : 0ull;
             int inc = __popcll(word), at = -inc;
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
                 const int v = __shfl_up(inc, o, 64);
                 inc += lane >= o ? v : 0;
             }
-            at += inc;
+            at += inc - skip;
             if (lane == 63)
-                list_rows = inc * a.group;
-            for (; word; word &= word - 1)
-                list[at++] = (w0 + lane) * 64 + __ffsll((unsigned long long)word) - 1;
+                list_all = inc;
+            for (; word; word &= word - 1, ++at)
+                if (at >= 0 && at < take)
+                    list[at] = (w0 + lane) * 64 + __ffsll((unsigned long long)word) - 1;
         }
         __syncthreads();
-        const int rows = list_rows;
-        any |= rows > 0;
+        const int here = min(take, max(0, list_all - skip)), rows = here * a.group;
+        skip = max(0, skip - list_all);
+        take -= here;
         if (rows > 0)
             fetch(0, rows);
         for (int r0 = 0; r0 < rows; r0 += BA_ROWS) {
@@ -1012,15 +1119,8 @@ __global__ __launch_bounds__(BA_THREADS, (BaShape<T, DP>::kw)) void block_attn_d
         __syncthreads();                    // the list is rebuilt
     }
     const float back = HALF ? a.scale / up : a.scale;
-    const int64_t tile = ((int64_t)z * a.b * a.hk + bh) * a.nb + blk;
-    if (a.splits > 1) {                     // a part of the queries: joined by block_attn_dkv_join_kernel
-        if (threadIdx.x == 0)
-            a.used[tile] = any;
-        if (!any)
-            return;
-    }
-    if (a.splits > 1) {
-        float *P = a.part + (tile * 2 * BA_BLOCK + wave * 16 + l15) * DP;
+    if (parts > 1) {                        // joined by block_attn_dkv_join_kernel
+        float *P = a.part + (part * 2 * BA_BLOCK + wave * 16 + l15) * DP;
 #pragma unroll
         for (int d = 0; d < DP / 16; ++d) {
             *(hd_f4 *)(P + d * 16 + g * 4) = dk[d] * back;
@@ -1043,15 +1143,16 @@ __global__ __launch_bounds__(BA_THREADS, (BaShape<T, DP>::kw)) void block_attn_d
 template <typename T, int DP> __global__ __launch_bounds__(BA_THREADS) void block_attn_dkv_join_kernel(BaArgs a)
 {
     const int blk = (int)(blockIdx.x % a.nb), bh = (int)(blockIdx.x / a.nb), h = bh % a.hk, b = bh / a.hk;
-    const int64_t parts = (int64_t)a.b * a.hk * a.nb, tile = (int64_t)bh * a.nb + blk;
+    const int p0 = a.first[blockIdx.x], p1 = a.first[blockIdx.x + 1];
+    if (p1 - p0 < 2)
+        return;
     for (int e = threadIdx.x; e < 2 * BA_BLOCK * DP / 4; e += BA_THREADS) {
         const int row = e / (DP / 4), c = (e % (DP / 4)) * 4, key = blk * BA_BLOCK + row % BA_BLOCK;
         if (key >= a.n || c >= a.d)
             continue;
         hd_f4 y = {0.f, 0.f, 0.f, 0.f};
-        for (int z = 0; z < a.splits; ++z)
-            if (a.used[z * parts + tile])
-                y += *(const hd_f4 *)(a.part + ((z * parts + tile) * 2 * BA_BLOCK + row) * DP + c);
+        for (int p = p0; p < p1; ++p)
+            y += *(const hd_f4 *)(a.part + ((int64_t)p * 2 * BA_BLOCK + row) * DP + c);
         T *O = (T *)(row < BA_BLOCK ? a.out : a.out2);
         ba_store4<T>(O + (((int64_t)b * a.n + key) * a.hk + h) * a.d + c, y);
     }
@@ -1085,7 +1186,7 @@ int ba_fill(BaArgs &a, int type, int b, int m, int n, int d, const tpu3_heads *q
     return 1;
 }
 
-// Splits of a tile's blocks: where the tiles alone do not fill the chip (two workgroups a compute unit).
+// Splits of a tile's blocks: where the tiles alone do not fill the chip (four workgroups a compute unit).
 int ba_splits(int b, int m, int n, int hq, int hk, int count)
 {
     if (b <= 0 || m <= 0 || n <= 0 || hk <= 0 || hq < hk || count <= 0)
@@ -1095,27 +1196,30 @@ int ba_splits(int b, int m, int n, int hq, int hk, int count)
         return 1;
     const int64_t tiles = (int64_t)b * hk * ((m - 1) / qt + 1);
     const int64_t used = (int64_t)(m < qt ? m : qt) * count, nb = (n - 1) / BA_BLOCK + 1;
-    int64_t s = 512 / tiles, most = used < nb ? used : nb;
+    int64_t s = 1024 / tiles, most = used < nb ? used : nb;
     s = s < most ? s : most;
     return s < 1 ? 1 : s > 64 ? 64 : (int)s;
 }
 
-// Parts of the queries for dk and dv: some blocks are picked by many more queries than others (the first of a sequence by
-// nearly all), and few blocks leave the chip waiting for the longest one.  A part holds 512 queries at least.
-int ba_dkv_splits(int b, int m, int hk, int nb)
+// Queries of a part of the dk / dv pass where blocks are few (0: a workgroup per block), and the most parts there can be.
+int ba_dkv_chunk(int b, int m, int hk, int nb, int count)
 {
     const int64_t blocks = (int64_t)b * hk * nb;
-    if (blocks <= 0 || blocks >= 1024)
-        return 1;
-    int64_t s = (2047 + blocks) / blocks;
-    const int64_t most = ((int64_t)m + 511) / 512;
-    s = s < most ? s : most;
-    return s > 8 ? 8 : s < 1 ? 1 : (int)s;
+    if (blocks <= 0 || blocks > 1024)
+        return 0;
+    const int64_t picks = (int64_t)b * hk * m * (count < nb ? count : nb);
+    const int64_t c = (picks / 1536 + 63) / 64 * 64;
+    return (int)(c < 128 ? 128 : c);
+}
+int64_t ba_dkv_parts(int b, int m, int hk, int nb, int count)
+{
+    const int64_t picks = (int64_t)b * hk * m * (count < nb ? count : nb);
+    return (int64_t)b * hk * nb + picks / ba_dkv_chunk(b, m, hk, nb, count);
 }
 
 int ba_dp(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 
-size_t ba_lds(const BaArgs &a, size_t tile) { return 2 * tile + (size_t)a.cap * 12 + (size_t)((a.nb + 31) / 32) * 8; }
+size_t ba_lds(const BaArgs &a, size_t tiles) { return tiles + (size_t)a.cap * 12 + (size_t)((a.nb + 31) / 32) * 8; }
 
 template <typename K> int ba_allow(K kernel, size_t lds)
 {
@@ -1125,7 +1229,7 @@ template <typename K> int ba_allow(K kernel, size_t lds)
 template <typename T, int DP> int ba_forward(const BaArgs &a, hipStream_t s)
 {
     const int64_t all = (int64_t)a.b * a.hk * a.tiles * a.splits;
-    const size_t lds = ba_lds(a, BaLds<T, DP>::TILE);
+    const size_t lds = ba_lds(a, 2 * BaLds<T, DP>::TILE);
     int rc = ba_allow(block_attn_fwd_kernel<T, DP>, lds);
     if (rc)
         return rc;
@@ -1142,7 +1246,7 @@ template <typename T, int DP> int ba_backward(BaArgs a, void *dq, void *dk, void
     int rc = TPU3_OK;
     // dq also leaves the rows' do . o for the pass over the keys
     const int64_t all = (int64_t)a.b * a.hk * a.tiles;
-    const size_t lds = ba_lds(a, BaLds<T, DP>::TILE);
+    const size_t lds = ba_lds(a, 2 * BaLds<T, DP>::TILE);
     rc = ba_allow(block_attn_dq_kernel<T, DP>, lds);
     if (rc)
         return rc;
@@ -1157,9 +1261,13 @@ template <typename T, int DP> int ba_backward(BaArgs a, void *dq, void *dk, void
         return rc;
     a.out = dk, a.out2 = dv;
     const int64_t blocks = (int64_t)a.b * a.hk * a.nb;
-    a.splits = ba_dkv_splits(a.b, a.m, a.hk, a.nb);
-    hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP>), dim3((unsigned)(blocks * a.splits)), dim3(BA_THREADS), lds2, s, a, blocks * a.splits);
-    if (a.splits > 1)
+    const int64_t all2 = a.chunk ? ba_dkv_parts(a.b, a.m, a.hk, a.nb, a.count) : blocks;
+    if (a.chunk) {
+        hipLaunchKernelGGL(block_picks_kernel, dim3((unsigned)blocks), dim3(BA_THREADS), 0, s, a);
+        hipLaunchKernelGGL(block_parts_kernel, dim3(1), dim3(1024), 0, s, a, (int)blocks);
+    }
+    hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP>), dim3((unsigned)all2), dim3(BA_THREADS), lds2, s, a, all2);
+    if (a.chunk)
         hipLaunchKernelGGL((block_attn_dkv_join_kernel<T, DP>), dim3((unsigned)blocks), dim3(BA_THREADS), 0, s, a);
     return tpu3_launch_status();
 }
@@ -1206,30 +1314,31 @@ extern "C" int tpu3_block_attn_fwd(tpu3_stream_t stream, int type, int b, int m,
 }
 
 namespace {
-// the parts of the backward workspace: bits, delta, gmax, used, part
+// the pieces of the backward workspace: bits, delta, gmax, picks, first, part
 struct BaBwdLayout {
-    size_t delta, gmax, used, part, bytes;
+    size_t delta, gmax, picks, first, part, bytes;
 };
-BaBwdLayout ba_bwd_layout(int b, int m, int n, int hq, int hk, int d)
+BaBwdLayout ba_bwd_layout(int b, int m, int n, int hq, int hk, int d, int count)
 {
     const size_t nb = n > 0 ? (size_t)(n - 1) / BA_BLOCK + 1 : 0, mt = ((size_t)m + 63) / 64, blocks = (size_t)b * hk * nb;
-    const size_t splits = (size_t)ba_dkv_splits(b, m, hk, (int)nb);
+    const bool parts = ba_dkv_chunk(b, m, hk, (int)nb, count) > 0;
     auto up = [](size_t x) { return (x + 15) / 16 * 16; };
     BaBwdLayout l;
     l.delta = up(blocks * mt * 8);
     l.gmax = l.delta + up((size_t)b * hq * m * 4);
-    l.used = l.gmax + up((size_t)b * hq * m * 4);
-    l.part = l.used + (splits > 1 ? up(splits * blocks * 4) : 0);
-    l.bytes = l.part + (splits > 1 ? splits * blocks * 2 * BA_BLOCK * ba_dp(d) * 4 : 0);
+    l.picks = l.gmax + up((size_t)b * hq * m * 4);
+    l.first = l.picks + (parts ? up(blocks * 4) : 0);
+    l.part = l.first + (parts ? up((blocks + 1) * 4) : 0);
+    l.bytes = l.part + (parts ? (size_t)ba_dkv_parts(b, m, hk, (int)nb, count) * 2 * BA_BLOCK * ba_dp(d) * 4 : 0);
     return l;
 }
 }  // namespace
 
-extern "C" size_t tpu3_block_attn_bwd_workspace_bytes(int b, int m, int n, int hq, int hk, int d)
+extern "C" size_t tpu3_block_attn_bwd_workspace_bytes(int b, int m, int n, int hq, int hk, int d, int count)
 {
-    if (b <= 0 || m <= 0 || hq <= 0 || hk <= 0 || d <= 0)
+    if (b <= 0 || m <= 0 || hq <= 0 || hk <= 0 || d <= 0 || count <= 0)
         return 0;
-    return ba_bwd_layout(b, m, n, hq, hk, d).bytes;
+    return ba_bwd_layout(b, m, n, hq, hk, d, count).bytes;
 }
 
 extern "C" int tpu3_block_attn_bwd(tpu3_stream_t stream, int type, int b, int m, int n, int d, const tpu3_heads *q,
@@ -1244,14 +1353,16 @@ extern "C" int tpu3_block_attn_bwd(tpu3_stream_t stream, int type, int b, int m,
         return rc;
     if (!hd_rows_ok(o, type) || !hd_rows_ok(go, type) || o->heads != a.hq || go->heads != a.hq || !lse || !dq || ((uintptr_t)rest & 15) ||
         ((uintptr_t)dq & 15) || (n > 0 && (!dk || !dv || ((uintptr_t)dk & 15) || ((uintptr_t)dv & 15))) || !workspace ||
-        ((uintptr_t)workspace & 15) || workspace_bytes < tpu3_block_attn_bwd_workspace_bytes(b, m, n, a.hq, a.hk, d))
+        ((uintptr_t)workspace & 15) || workspace_bytes < tpu3_block_attn_bwd_workspace_bytes(b, m, n, a.hq, a.hk, d, count))
         return TPU3_EINVAL;
     a.o = *o, a.go = *go, a.lse = (float *)lse, a.rest = type == TPU3_TYPE_F32 ? nullptr : (void *)rest;
-    const BaBwdLayout l = ba_bwd_layout(b, m, n, a.hq, a.hk, d);
+    const BaBwdLayout l = ba_bwd_layout(b, m, n, a.hq, a.hk, d, count);
+    a.chunk = ba_dkv_chunk(b, m, a.hk, a.nb, count);
     a.bits = (uint64_t *)workspace;
     a.delta = (float *)((char *)workspace + l.delta);
     a.gmax = (float *)((char *)workspace + l.gmax);
-    a.used = (int32_t *)((char *)workspace + l.used);
+    a.picks = (int32_t *)((char *)workspace + l.picks);
+    a.first = (int32_t *)((char *)workspace + l.first);
     a.part = (float *)((char *)workspace + l.part);
     const hipStream_t s = (hipStream_t)stream;
     return type == TPU3_TYPE_F32 ? ba_backward_d<float>(a, dq, dk, dv, s) : type == TPU3_TYPE_F16 ? ba_backward_d<_Float16>(a, dq, dk, dv, s) : ba_backward_d<__bf16>(a, dq, dk, dv, s);

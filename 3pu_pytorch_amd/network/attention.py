@@ -331,7 +331,7 @@ class _BlockAttention(torch.autograd.Function):
         dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         make = torch.zeros if m == 0 else torch.empty                # (no queries: the kernels do not run)
         dk, dv = (make(t.shape, dtype=t.dtype, device=t.device) for t in (k, v))
-        need = L.lib().tpu3_block_attn_bwd_workspace_bytes(b, m, n, hq, hk, d)
+        need = L.lib().tpu3_block_attn_bwd_workspace_bytes(b, m, n, hq, hk, d, count)
         ws = _workspace(need, q)
         _launch("tpu3_block_attn_bwd", q, L.TYPES[q.dtype], b, m, n, d, _heads(q), _heads(k), _heads(v), _heads(o), _heads(go),
                 blocks.data_ptr(), count, ctx.scale, L.ptr(n_arr), L.ptr(m_arr), ctx.causal, lse.data_ptr(), L.ptr(rest),

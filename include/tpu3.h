@@ -602,7 +602,7 @@ int tpu3_block_attn_bwd(tpu3_stream_t stream, int type, int b, int m, int n, int
                         const tpu3_heads *v, const tpu3_heads *o, const tpu3_heads *go, const int32_t *blocks, int count,
                         float scale, const int32_t *n_arr, const int32_t *m_arr, int causal, const float *lse,
                         const void *rest, void *dq, void *dk, void *dv, void *workspace, size_t workspace_bytes);
-size_t tpu3_block_attn_bwd_workspace_bytes(int b, int m, int n, int hq, int hk, int d);
+size_t tpu3_block_attn_bwd_workspace_bytes(int b, int m, int n, int hq, int hk, int d, int count);
 
 /* ---- measurement hooks (bench.py and tools/ only; a caller of the path never needs them) ------------
  * tpu3_debug_fps_bucket_events: the NEXT bucketed-FPS call (n beyond the register-resident limit)
