@@ -661,41 +661,51 @@ __global__ __launch_bounds__(BA_THREADS, (BaFwd<T, DP>::w)) void block_attn_fwd_
         a.lse[R.flat(a, t.b)] = sum > 0.f ? top + log2f(sum) : -INFINITY;
 }
 
-// Joins the splits of a row: 16 lanes a row, each a few channels.
+// Joins the splits of a row, a wave a row: a lane per split forms the splits' factors, then a lane per DP / 64 channels adds
+// the splits up, eight loads at a time.
 template <typename T, int DP>
 __global__ __launch_bounds__(BA_THREADS) void block_attn_join_kernel(BaArgs a, int64_t rows)
 {
-    const int64_t row = (int64_t)blockIdx.x * (BA_THREADS / 16) + (threadIdx.x >> 4);
+    constexpr int W = DP / 64 > 0 ? DP / 64 : 1;
+    __shared__ float factor[BA_THREADS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t row = (int64_t)blockIdx.x * (BA_THREADS / 64) + wave;
     if (row >= rows)
         return;
-    const int l = threadIdx.x & 15;
     const float *P = a.part + row * a.splits * (DP + 4);
-    float top = -INFINITY;
-    for (int z = 0; z < a.splits; ++z)
-        top = fmaxf(top, P[z * (DP + 4) + DP]);
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, y[DP / 16] = {};
-    for (int z = 0; z < a.splits; ++z) {
-        const float *Z = P + z * (DP + 4);
-        const float f = __builtin_amdgcn_exp2f(Z[DP] - base);
-        sum = __builtin_fmaf(Z[DP + 1], f, sum);
+    const float mine = lane < a.splits ? P[lane * (DP + 4) + DP] : -INFINITY, part = lane < a.splits ? P[lane * (DP + 4) + DP + 1] : 0.f;
+    float top = mine;
 #pragma unroll
-        for (int c = 0; c < DP / 16; ++c)
-            y[c] = __builtin_fmaf(Z[l * (DP / 16) + c], f, y[c]);
-    }
+    for (int o = 32; o > 0; o >>= 1)
+        top = fmaxf(top, __shfl_xor(top, o, 64));
+    const float base = top == -INFINITY ? 0.f : top, f = __builtin_amdgcn_exp2f(mine - base);
+    float sum = part * f;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+        sum += __shfl_xor(sum, o, 64);
+    factor[threadIdx.x] = f;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
     const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
     const int64_t i = row % a.m, bh = row / a.m, h = bh % a.hq, b = bh / a.hq;
-    T *O = (T *)a.out + ((b * a.m + i) * a.hq + h) * a.d;
-#pragma unroll
-    for (int c = 0; c < DP / 16; ++c)
-        if (l * (DP / 16) + c < a.d) {
-            const T v = (T)(y[c] * inv);
-            O[l * (DP / 16) + c] = v;
-            if (a.rest)
-                ((T *)a.rest)[O - (T *)a.out + l * (DP / 16) + c] = (T)(y[c] * inv - (float)v);
-        }
-    if (a.lse && l == 0)
+    const int64_t at = ((b * a.m + i) * a.hq + h) * a.d;
+    if (a.lse && lane == 0)
         a.lse[row] = sum > 0.f ? top + log2f(sum) : -INFINITY;
+    if (lane * W >= a.d)
+        return;
+    float y[W] = {};
+#pragma unroll 8
+    for (int z = 0; z < a.splits; ++z)
+#pragma unroll
+        for (int c = 0; c < W; ++c)
+            y[c] = __builtin_fmaf(P[z * (DP + 4) + lane * W + c], factor[wave * 64 + z], y[c]);
+#pragma unroll
+    for (int c = 0; c < W; ++c) {
+        const T v = (T)(y[c] * inv);
+        ((T *)a.out)[at + lane * W + c] = v;
+        if (a.rest)
+            ((T *)a.rest)[at + lane * W + c] = (T)(y[c] * inv - (float)v);
+    }
 }
 
 // ---- backward: dq, and the rows' do . o ----------------------------------------------------------------------------------
@@ -1196,7 +1206,7 @@ int ba_splits(int b, int m, int n, int hq, int hk, int count)
         return 1;
     const int64_t tiles = (int64_t)b * hk * ((m - 1) / qt + 1);
     const int64_t used = (int64_t)(m < qt ? m : qt) * count, nb = (n - 1) / BA_BLOCK + 1;
-    int64_t s = 1024 / tiles, most = used < nb ? used : nb;
+    int64_t s = (m <= 16 ? 512 : 1024) / tiles, most = used < nb ? used : nb;
     s = s < most ? s : most;
     return s < 1 ? 1 : s > 64 ? 64 : (int)s;
 }
@@ -1235,7 +1245,7 @@ template <typename T, int DP> int ba_forward(const BaArgs &a, hipStream_t s)
         return rc;
     hipLaunchKernelGGL((block_attn_fwd_kernel<T, DP>), dim3((unsigned)all), dim3(BA_THREADS), lds, s, a, all);
     if (a.splits > 1) {
-        const int64_t rows = (int64_t)a.b * a.hq * a.m, per = BA_THREADS / 16;
+        const int64_t rows = (int64_t)a.b * a.hq * a.m, per = BA_THREADS / 64;
         hipLaunchKernelGGL((block_attn_join_kernel<T, DP>), dim3((unsigned)((rows + per - 1) / per)), dim3(BA_THREADS), 0, s, a, rows);
     }
     return tpu3_launch_status();

@@ -78,72 +78,93 @@ struct BsArgs {
     const float *means;
     const int32_t *n_arr, *m_arr;
     int32_t *out;                           // (b, m, hk, count)
-    double *ws_score;                       // (b, hk, m, splits, count)
+    uint64_t *ws_key;                       // (b, hk, m, splits, count)
     int32_t *ws_id;
-    int32_t *todo, *todo_rows;              // queries that the approximate scores leave open: their number, their rows
+    uint64_t *open;                         // block_select_many_kernel: queries left open, a word of 64 a wave
     int b, m, n, nb, hk, group, d, count, causal, splits;
 };
 
 constexpr int BS_KEEP = 1024;               // candidates in LDS at a time
 constexpr int BS_MAX = TPU3_BLOCK_COUNT_MAX;
 
+// Scores as unsigned numbers of the same order (0 is below every score: no candidate).
+__device__ __forceinline__ uint64_t bs_key(double v)
+{
+    if (!(v == v))
+        v = -INFINITY;                      // not a number: behind every number
+    v += 0.0;                               // -0 is 0
+    const uint64_t u = (uint64_t)__double_as_longlong(v);
+    return u ^ ((u >> 63) ? ~0ull : 0x8000000000000000ull);
+}
+constexpr uint64_t BS_OWN = ~0ull;          // above every score: the block that a causal query always gets
+
 struct BsShared {
     double q[128];
-    double score[BS_KEEP];
+    uint64_t key[BS_KEEP];
     int id[BS_KEEP];
-    double wave_score[4 * BS_MAX];
+    uint64_t wave_key[4 * BS_MAX];
     int wave_id[4 * BS_MAX];
 };
 
-__device__ __forceinline__ bool bs_better(double a, int ia, double b, int ib) { return a > b || (a == b && ia < ib); }
+__device__ __forceinline__ bool bs_better(uint64_t a, int ia, uint64_t b, int ib) { return a > b || (a == b && ia < ib); }
 
-// The `count` best of the n candidates in s.score / s.id, best first, into their first places; the rest of these places is
-// filled with (-inf, INT_MAX).  Every wave extracts the best of a quarter one by one; their 4 * count meet by rank.
+// The `count` best of the n candidates in s.key / s.id, best first, into their first places; the rest of these places is
+// filled with (0, INT_MAX).  A lane sorts its four candidates once; its wave then takes the best head `count` times, by the
+// keys' upper halves and, only where these are equal, by the lower halves and the ids.  The waves' lists meet by rank.
 __device__ void bs_best(BsShared &s, int n, int count)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    double v[4];
+    uint64_t v[4];
     int id[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const int e = wave * 256 + j * 64 + lane;
-        v[j] = e < n ? s.score[e] : -INFINITY;
+        const int e = j * BS_THREADS + threadIdx.x;
+        v[j] = e < n ? s.key[e] : 0ull;
         id[j] = e < n ? s.id[e] : 0x7FFFFFFF;
     }
-    for (int r = 0; r < count; ++r) {
-        double bv = v[0];
-        int bi = id[0];
-#pragma unroll
-        for (int j = 1; j < 4; ++j)
-            if (bs_better(v[j], id[j], bv, bi))
-                bv = v[j], bi = id[j];
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            const double ov = __shfl_xor(bv, o, 64);
-            const int oi = __shfl_xor(bi, o, 64);
-            if (bs_better(ov, oi, bv, bi))
-                bv = ov, bi = oi;
+    auto order = [&](int x, int y) __attribute__((always_inline)) {
+        if (bs_better(v[y], id[y], v[x], id[x])) {
+            const uint64_t t = v[x];
+            const int u = id[x];
+            v[x] = v[y], id[x] = id[y];
+            v[y] = t, id[y] = u;
         }
-        if (lane == 0)
-            s.wave_score[wave * count + r] = bv, s.wave_id[wave * count + r] = bi;
+    };
+    order(0, 1), order(2, 3), order(0, 2), order(1, 3), order(1, 2);
+    for (int r = 0; r < count; ++r) {
+        const uint32_t hi = (uint32_t)(v[0] >> 32), lo = (uint32_t)v[0];
+        const uint32_t mh = tpu3_wave_max_u32(hi);
+        unsigned long long who = __ballot(hi == mh);
+        if (__popcll(who) > 1) {
+            const uint32_t ml = tpu3_wave_max_u32(hi == mh ? lo : 0u);
+            who = __ballot(hi == mh && lo == ml);
+            if (__popcll(who) > 1) {
+                const uint32_t mi = tpu3_wave_min_u32(hi == mh && lo == ml ? (uint32_t)id[0] : 0xFFFFFFFFu);
+                who = __ballot(hi == mh && lo == ml && (uint32_t)id[0] == mi);
+            }
+        }
+        if (lane == __ffsll(who) - 1) {
+            s.wave_key[wave * count + r] = v[0], s.wave_id[wave * count + r] = id[0];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (id[j] == bi)
-                v[j] = -INFINITY, id[j] = 0x7FFFFFFF;
+            for (int j = 0; j < 3; ++j)
+                v[j] = v[j + 1], id[j] = id[j + 1];
+            v[3] = 0ull, id[3] = 0x7FFFFFFF;
+        }
     }
     __syncthreads();
     const int c = threadIdx.x;              // 4 * count <= 256 candidates, one a thread
     if (c < 4 * count) {
-        const double cv = s.wave_score[c];
+        const uint64_t cv = s.wave_key[c];
         const int ci = s.wave_id[c];
         int rank = 0;
+#pragma unroll 8
         for (int o = 0; o < 4 * count; ++o) {
-            const double ov = s.wave_score[o];
+            const uint64_t ov = s.wave_key[o];
             const int oi = s.wave_id[o];
             rank += bs_better(ov, oi, cv, ci) || (ov == cv && oi == ci && o < c) ? 1 : 0;
         }
         if (rank < count)
-            s.score[rank] = cv, s.id[rank] = ci;
+            s.key[rank] = cv, s.id[rank] = ci;
     }
     __syncthreads();
 }
@@ -163,7 +184,7 @@ __device__ void bs_emit(const BsShared &s, int count, int32_t *out)
 
 // A workgroup per (query, key head, part of the blocks).  Eight lanes form a score: each adds up every eighth group of four
 // channels, three exchanges join them.
-template <typename T> __device__ void block_select_row(const BsArgs &a, BsShared &s, int64_t row, int z)
+template <typename T, int DP> __device__ void block_select_row(const BsArgs &a, BsShared &s, int64_t row, int z)
 {
     const int i = (int)(row % a.m);
     const int bh = (int)(row / a.m), h = bh % a.hk, b = bh / a.hk;
@@ -188,27 +209,43 @@ template <typename T> __device__ void block_select_row(const BsArgs &a, BsShared
     }
     __syncthreads();
     const int slot = threadIdx.x >> 3, part = threadIdx.x & 7;
+    constexpr int STEP = BS_THREADS / 8, VECS = DP / 32;
+    double q[VECS][4];
+#pragma unroll
+    for (int x = 0; x < VECS; ++x)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            q[x][j] = s.q[x * 32 + part * 4 + j];
+    const float *M = a.means + ((int64_t)b * a.nb * a.hk + h) * a.d + part * 4;
+    const int64_t stride = (int64_t)a.hk * a.d;
     int kept = 0;                                               // candidates in LDS
     for (int c0 = z0; c0 < z1 || c0 == z0;) {
         const int take = min(z1 - c0, BS_KEEP - kept);
-        for (int t0 = 0; t0 < take; t0 += BS_THREADS / 8) {
-            const int t = t0 + slot, blk = c0 + t;
-            double v = 0.0;
-            if (t < take) {
-                const float *M = a.means + (((int64_t)b * a.nb + blk) * a.hk + h) * a.d;
-                for (int c = part * 4; c < a.d; c += 32) {
-                    const hd_f4 x = *(const hd_f4 *)(M + c);
+        hd_f4 next[VECS];
+        auto fetch = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        v = __builtin_fma((double)x[j], s.q[c + j], v);
-                }
-            }
+            for (int x = 0; x < VECS; ++x)
+                next[x] = t < take && x * 32 + part * 4 < a.d ? *(const hd_f4 *)(M + (c0 + t) * stride + x * 32) : hd_f4{0.f, 0.f, 0.f, 0.f};
+        };
+        fetch(slot);
+        for (int t0 = 0; t0 < take; t0 += STEP) {
+            const int t = t0 + slot, blk = c0 + t;
+            hd_f4 m[VECS];
+#pragma unroll
+            for (int x = 0; x < VECS; ++x)
+                m[x] = next[x];
+            fetch(t + STEP);
+            double v = 0.0;
+#pragma unroll
+            for (int x = 0; x < VECS; ++x)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    v = __builtin_fma((double)m[x][j], q[x][j], v);
 #pragma unroll
             for (int o = 4; o > 0; o >>= 1)
                 v += __shfl_xor(v, o, 64);
             if (t < take && part == 0) {
-                v = v == v ? v : -INFINITY;                     // not a number: behind every number
-                s.score[kept + t] = blk == own ? INFINITY : v;
+                s.key[kept + t] = blk == own ? BS_OWN : bs_key(v);
                 s.id[kept + t] = blk;
             }
         }
@@ -223,24 +260,36 @@ template <typename T> __device__ void block_select_row(const BsArgs &a, BsShared
     }
     if ((int)threadIdx.x < a.count) {
         const int64_t at = (row * a.splits + z) * a.count + threadIdx.x;
-        a.ws_score[at] = s.score[threadIdx.x];
+        a.ws_key[at] = s.key[threadIdx.x];
         a.ws_id[at] = s.id[threadIdx.x];
     }
 }
 
-template <typename T>
-__global__ __launch_bounds__(BS_THREADS) void block_select_kernel(BsArgs a)
+template <typename T, int DP> __global__ __launch_bounds__(BS_THREADS) void block_select_kernel(BsArgs a)
 {
     __shared__ BsShared s;
-    if (a.todo) {                           // the rows of a list
-        const int all = *a.todo;
-        for (int r = blockIdx.x; r < all; r += gridDim.x) {
-            block_select_row<T>(a, s, a.todo_rows[r], 0);
-            __syncthreads();
-        }
-        return;
+    block_select_row<T, DP>(a, s, blockIdx.x / a.splits, (int)(blockIdx.x % a.splits));
+}
+
+// The queries that block_select_many_kernel left open: one word of 64 queries a wave of it.
+template <typename T, int DP> __global__ __launch_bounds__(BS_THREADS) void block_select_open_kernel(BsArgs a, int qtiles, int64_t waves)
+{
+    __shared__ BsShared s;
+    __shared__ uint64_t open[BS_THREADS];
+    for (int64_t w0 = (int64_t)blockIdx.x * BS_THREADS; w0 < waves; w0 += (int64_t)gridDim.x * BS_THREADS) {
+        const uint64_t mine = w0 + threadIdx.x < waves ? a.open[w0 + threadIdx.x] : 0ull;
+        if (!__syncthreads_or(mine != 0))
+            continue;
+        open[threadIdx.x] = mine;
+        __syncthreads();
+        for (int t = 0; t < BS_THREADS; ++t)
+            for (uint64_t left = open[t]; left; left &= left - 1) {
+                const int64_t w = w0 + t;
+                block_select_row<T, DP>(a, s, w / qtiles * a.m + w % qtiles * 64 + __ffsll((unsigned long long)left) - 1, 0);
+                __syncthreads();
+            }
+        __syncthreads();
     }
-    block_select_row<T>(a, s, blockIdx.x / a.splits, (int)(blockIdx.x % a.splits));
 }
 
 __global__ __launch_bounds__(BS_THREADS) void block_select_join_kernel(BsArgs a)
@@ -251,7 +300,7 @@ __global__ __launch_bounds__(BS_THREADS) void block_select_join_kernel(BsArgs a)
     const int bh = (int)(row / a.m), h = bh % a.hk, b = bh / a.hk;
     const int all = a.splits * a.count;                         // <= BS_KEEP by the host's choice of splits
     for (int t = threadIdx.x; t < all; t += BS_THREADS) {
-        s.score[t] = a.ws_score[row * all + t];
+        s.key[t] = a.ws_key[row * all + t];
         s.id[t] = a.ws_id[row * all + t];
     }
     __syncthreads();
@@ -266,8 +315,11 @@ __global__ __launch_bounds__(BS_THREADS) void block_select_join_kernel(BsArgs a)
 // for the sums, doubled for sums that cut off instead of rounding).  Pass 1 keeps the k + 1 largest scores of every query, a
 // chain of v_med3 (one instruction an entry).  Where the k-th is more than 2 eps above the next, the order of the exact
 // scores around that place is known, and pass 2, which forms the same scores again, lists the blocks above it in ascending
-// order.  The other queries (near ties, equal rows, values that are not finite; a few in a thousand) are put on a list
-// for block_select_kernel's exact scores.
+// order.  For the other queries (a few in a hundred) pass 2 also lists the blocks within 2 eps of the place, and the wave
+// forms their scores in 64 bits, one block at a time, to choose among them.  Only where these are too many for the list
+// (rows of equal means) or a value is not finite is the query left open to block_select_open_kernel.
+constexpr int BT_MORE = 16;                 // places behind `count` for blocks near the edge
+constexpr int BT_NEAR = 1 << 30;            // marks them
 constexpr int BT_STRIDE = 20;               // floats between two queries' 16 scores in LDS
 
 struct BtSplit {
@@ -291,7 +343,8 @@ __global__ __launch_bounds__(BS_THREADS) void block_select_many_kernel(BsArgs a,
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
     float *sc = (float *)smem + wave * (64 * BT_STRIDE);
-    int *found = (int *)((float *)smem + 4 * 64 * BT_STRIDE) + wave * 64 * a.count;          // (count, 64)
+    const int places = max(a.count, min(a.count + BT_MORE, 64));
+    int *found = (int *)((float *)smem + 4 * 64 * BT_STRIDE) + wave * 64 * places;          // (places, 64)
     const int64_t w = (int64_t)blockIdx.x * 4 + wave;
     if (w >= waves)
         return;                             // (no barriers below: a wave works by itself)
@@ -432,11 +485,14 @@ __global__ __launch_bounds__(BS_THREADS) void block_select_many_kernel(BsArgs a,
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1)
         mn = fmaxf(mn, __shfl_xor(mn, o, 64));
-    const float eps = 1.220703125e-4f * sqrtf(qn) * sqrtf(mn);
+    const float eps2 = 2.44140625e-4f * sqrtf(qn) * sqrtf(mn);         // 2 eps
     const bool any_odd = __any(odd);
-    const bool sure = everything || k == 0 || (!any_odd && best[NL - 2] - best[NL - 1] > 2.f * eps && best[NL - 2] < INFINITY);
-    const float above = everything ? -INFINITY : best[NL - 1];
-    int at = 0;
+    const float kth = best[NL - 2], after = best[NL - 1];
+    const bool plain = everything || k == 0 || (!any_odd && kth - after > eps2 && kth < INFINITY);
+    // blocks above `in` are picked, those from `near` on may be
+    const float in = everything ? -INFINITY : plain ? after : after + eps2, near = plain ? INFINITY : kth - eps2;
+    bool open = !plain && (any_odd || !(eps2 < INFINITY) || !(fabsf(kth) < INFINITY) || !(fabsf(after) < INFINITY));
+    int at = 0, certain = 0;
     if (k > 0) {
         if (most > 0)
             fetch(0);
@@ -444,19 +500,66 @@ __global__ __launch_bounds__(BS_THREADS) void block_select_many_kernel(BsArgs a,
             float x[16];
             scores(t0, false, x);
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-                if (t0 + e < end && (everything || x[e] > above) && at < k)
-                    found[at++ * 64 + lane] = t0 + e;
+            for (int e = 0; e < 16; ++e) {
+                const bool sure = everything || x[e] > in;
+                if (t0 + e < end && (sure || x[e] >= near)) {
+                    if (at < places)
+                        found[at * 64 + lane] = t0 + e + (sure ? 0 : BT_NEAR);
+                    ++at;
+                    certain += sure;
+                }
+            }
         }
     }
+    open |= !plain && at > places;
+    open &= i < lm;
+    for (unsigned long long left = __ballot(!plain && !open && i < lm); left; left &= left - 1) {
+        const int f = __ffsll(left) - 1, all = __shfl(at, f, 64), want = k - __shfl(certain, f, 64);
+        const int mine = lane < all ? found[lane * 64 + f] : 0;
+        const bool unsure = (mine & BT_NEAR) != 0;
+        const unsigned long long near_ones = __ballot(unsure);
+        double qv[DP / 64 > 0 ? DP / 64 : 1];
+#pragma unroll
+        for (int c = 0; c < (DP / 64 > 0 ? DP / 64 : 1); ++c) {
+            qv[c] = 0.0;
+            if (c * 64 + lane < a.d)
+                for (int e = 0; e < a.group; ++e)
+                    qv[c] += (double)(float)Q[(i0 + f) * a.q.sr + e * a.q.sh + c * 64 + lane];
+        }
+        uint64_t key = 0;
+        for (unsigned long long u = near_ones; u; u &= u - 1) {
+            const int e = __ffsll(u) - 1;
+            const float *p = M + (__shfl(mine, e, 64) & ~BT_NEAR) * mstride;
+            double v = 0.0;
+#pragma unroll
+            for (int c = 0; c < (DP / 64 > 0 ? DP / 64 : 1); ++c)
+                if (c * 64 + lane < a.d)
+                    v = __builtin_fma((double)p[c * 64 + lane], qv[c], v);
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1)
+                v += __shfl_xor(v, o, 64);
+            key = lane == e ? bs_key(v) : key;
+        }
+        int rank = 0;                       // (the list ascends: equal scores to the lower block)
+        for (unsigned long long u = near_ones; u; u &= u - 1) {
+            const int e = __ffsll(u) - 1;
+            const uint64_t other = __shfl((unsigned long long)key, e, 64);
+            rank += other > key || (other == key && e < lane) ? 1 : 0;
+        }
+        const bool stays = lane < all && (!unsure || rank < want);
+        const unsigned long long kept = __ballot(stays);
+        if (stays)
+            found[__popcll(kept & ((1ull << lane) - 1)) * 64 + f] = mine & ~BT_NEAR;
+        at = lane == f ? __popcll(kept) : at;
+    }
+    at = min(at, k);                        // (open queries may hold more)
     if (own >= 0)
         found[at++ * 64 + lane] = own;      // behind all others: they are earlier blocks
     for (; at < a.count; ++at)
         found[at * 64 + lane] = -1;
-    if (i < lm && !sure) {
-        const int slot = atomicAdd(a.todo, 1);
-        a.todo_rows[slot] = (int)((int64_t)bh * a.m + i);
-    }
+    const unsigned long long opened = __ballot(open);
+    if (lane == 0)
+        a.open[w] = opened;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     int32_t *out = a.out + (((int64_t)b * a.m + i0) * a.hk + h) * a.count;
@@ -486,7 +589,8 @@ template <typename T, int DP, bool LOQ> int bs_many_launch(const BsArgs &a, hipS
 {
     const int qtiles = (a.m + 63) / 64, k = a.count - a.causal;
     const int64_t waves = (int64_t)a.b * a.hk * qtiles;
-    const size_t lds = (size_t)4 * 64 * (BT_STRIDE + a.count) * 4;
+    const int places = a.count + BT_MORE < 64 ? a.count + BT_MORE : 64;
+    const size_t lds = (size_t)4 * 64 * (BT_STRIDE + (places > a.count ? places : a.count)) * 4;
     const dim3 grid((unsigned)((waves + 3) / 4));
     hipError_t e = hipSuccess;
 #define BT_GO(NL)                                                                                                        \
@@ -507,7 +611,11 @@ template <typename T, int DP, bool LOQ> int bs_many_launch(const BsArgs &a, hipS
     else
         BT_GO(65)
 #undef BT_GO
-    return e == hipSuccess ? tpu3_launch_status() : (int)e;
+    if (e != hipSuccess)
+        return (int)e;
+    const int64_t words = (waves + BS_THREADS - 1) / BS_THREADS;
+    hipLaunchKernelGGL((block_select_open_kernel<T, DP>), dim3((unsigned)(words < 1024 ? words : 1024)), dim3(BS_THREADS), 0, s, a, qtiles, waves);
+    return tpu3_launch_status();
 }
 template <typename T, bool LOQ> int bs_many_d(const BsArgs &a, hipStream_t s)
 {
@@ -551,7 +659,7 @@ extern "C" size_t tpu3_block_select_workspace_bytes(int b, int m, int n, int hk,
     if (b <= 0 || m <= 0 || n <= 0 || hk <= 0 || count <= 0 || count > BS_MAX)
         return 0;
     if (bs_many(b, m, hk))
-        return ((size_t)b * m * hk + 2) * 4;
+        return (size_t)b * hk * (((size_t)m + 63) / 64) * 8;
     const int splits = bs_splits(b, m, hk, (n - 1) / BS_BLOCK + 1, count);
     return splits == 1 ? 0 : (size_t)b * m * hk * splits * count * 12;
 }
@@ -581,34 +689,37 @@ extern "C" int tpu3_block_select(tpu3_stream_t stream, int type, int b, int m, i
         return TPU3_ELIMIT;
     const hipStream_t s = (hipStream_t)stream;
     if (many) {
-        if (!workspace || ((uintptr_t)workspace & 7) || workspace_bytes < ((size_t)rows + 2) * 4)
+        if (!workspace || ((uintptr_t)workspace & 7) || workspace_bytes < tpu3_block_select_workspace_bytes(b, m, n, hk, count))
             return TPU3_EINVAL;
-        a.todo = (int32_t *)workspace, a.todo_rows = a.todo + 2;
-        const hipError_t e = tpu3_fill_u32(a.todo, 0, 2, s);
-        if (e != hipSuccess)
-            return (int)e;
-        const bool bf16 = type == TPU3_TYPE_BF16;
-        const int rc = type == TPU3_TYPE_F32 ? bs_many_d<float, true>(a, s)
-                       : !bf16               ? bs_many_d<_Float16, true>(a, s)
-                       : a.group == 1        ? bs_many_d<__bf16, false>(a, s)
-                                             : bs_many_d<__bf16, true>(a, s);
-        if (rc)
-            return rc;
+        a.open = (uint64_t *)workspace;
+        // (bf16 queries of one head are their own first term)
+        return type == TPU3_TYPE_F32   ? bs_many_d<float, true>(a, s)
+               : type == TPU3_TYPE_F16 ? bs_many_d<_Float16, true>(a, s)
+               : a.group == 1          ? bs_many_d<__bf16, false>(a, s)
+                                       : bs_many_d<__bf16, true>(a, s);
     }
     if (a.splits > 1) {
         if (!workspace || ((uintptr_t)workspace & 7) || workspace_bytes < (size_t)rows * a.splits * count * 12)
             return TPU3_EINVAL;
-        a.ws_score = (double *)workspace;
-        a.ws_id = (int32_t *)(a.ws_score + rows * a.splits * count);
+        a.ws_key = (uint64_t *)workspace;
+        a.ws_id = (int32_t *)(a.ws_key + rows * a.splits * count);
     }
-    const dim3 grid((unsigned)(many ? (rows < 1024 ? rows : 1024) : rows * a.splits));
-#define BS_GO(T) hipLaunchKernelGGL(block_select_kernel<T>, grid, dim3(BS_THREADS), 0, s, a)
+    const dim3 grid((unsigned)(rows * a.splits));
+#define BS_GO(T)                                                                                                    \
+    {                                                                                                               \
+        if (d <= 32)                                                                                                \
+            hipLaunchKernelGGL((block_select_kernel<T, 32>), grid, dim3(BS_THREADS), 0, s, a);                      \
+        else if (d <= 64)                                                                                           \
+            hipLaunchKernelGGL((block_select_kernel<T, 64>), grid, dim3(BS_THREADS), 0, s, a);                      \
+        else                                                                                                        \
+            hipLaunchKernelGGL((block_select_kernel<T, 128>), grid, dim3(BS_THREADS), 0, s, a);                     \
+    }
     if (type == TPU3_TYPE_F32)
-        BS_GO(float);
+        BS_GO(float)
     else if (type == TPU3_TYPE_F16)
-        BS_GO(_Float16);
+        BS_GO(_Float16)
     else
-        BS_GO(__bf16);
+        BS_GO(__bf16)
 #undef BS_GO
     if (a.splits > 1)
         hipLaunchKernelGGL(block_select_join_kernel, dim3((unsigned)rows), dim3(BS_THREADS), 0, s, a);
