@@ -661,27 +661,27 @@ __global__ __launch_bounds__(BA_THREADS, (BaFwd<T, DP>::w)) void block_attn_fwd_
         a.lse[R.flat(a, t.b)] = sum > 0.f ? top + log2f(sum) : -INFINITY;
 }
 
-// Joins the splits of a row, a wave a row: a lane per split forms the splits' factors, then a lane per DP / 64 channels adds
-// the splits up, eight loads at a time.
-template <typename T, int DP>
+// Joins the splits of a row, RL lanes a row (16, or a wave for more splits): a lane per split forms the splits' factors, then a
+// lane per DP / RL channels adds the splits up, eight loads at a time.
+template <typename T, int DP, int RL>
 __global__ __launch_bounds__(BA_THREADS) void block_attn_join_kernel(BaArgs a, int64_t rows)
 {
-    constexpr int W = DP / 64 > 0 ? DP / 64 : 1;
+    constexpr int W = DP / RL > 0 ? DP / RL : 1;
     __shared__ float factor[BA_THREADS];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t row = (int64_t)blockIdx.x * (BA_THREADS / 64) + wave;
+    const int lane = threadIdx.x % RL, first = threadIdx.x - lane;
+    const int64_t row = (int64_t)blockIdx.x * (BA_THREADS / RL) + threadIdx.x / RL;
     if (row >= rows)
         return;
     const float *P = a.part + row * a.splits * (DP + 4);
     const float mine = lane < a.splits ? P[lane * (DP + 4) + DP] : -INFINITY, part = lane < a.splits ? P[lane * (DP + 4) + DP + 1] : 0.f;
     float top = mine;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1)
+    for (int o = RL / 2; o > 0; o >>= 1)
         top = fmaxf(top, __shfl_xor(top, o, 64));
     const float base = top == -INFINITY ? 0.f : top, f = __builtin_amdgcn_exp2f(mine - base);
     float sum = part * f;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1)
+    for (int o = RL / 2; o > 0; o >>= 1)
         sum += __shfl_xor(sum, o, 64);
     factor[threadIdx.x] = f;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -698,7 +698,7 @@ __global__ __launch_bounds__(BA_THREADS) void block_attn_join_kernel(BaArgs a, i
     for (int z = 0; z < a.splits; ++z)
 #pragma unroll
         for (int c = 0; c < W; ++c)
-            y[c] = __builtin_fmaf(P[z * (DP + 4) + lane * W + c], factor[wave * 64 + z], y[c]);
+            y[c] = __builtin_fmaf(P[z * (DP + 4) + lane * W + c], factor[first + z], y[c]);
 #pragma unroll
     for (int c = 0; c < W; ++c) {
         const T v = (T)(y[c] * inv);
@@ -1150,17 +1150,21 @@ __global__ __launch_bounds__(BA_THREADS, (BaBwd<T, DP>::kw)) void block_attn_dkv
 }
 
 // dk and dv of a block from its parts, in the parts' order
+constexpr int BJ_SLICES = 4;                // workgroups a block
 template <typename T, int DP> __global__ __launch_bounds__(BA_THREADS) void block_attn_dkv_join_kernel(BaArgs a)
 {
-    const int blk = (int)(blockIdx.x % a.nb), bh = (int)(blockIdx.x / a.nb), h = bh % a.hk, b = bh / a.hk;
-    const int p0 = a.first[blockIdx.x], p1 = a.first[blockIdx.x + 1];
+    const int id = (int)(blockIdx.x / BJ_SLICES), blk = id % a.nb, bh = id / a.nb, h = bh % a.hk, b = bh / a.hk;
+    const int p0 = a.first[id], p1 = a.first[id + 1];
     if (p1 - p0 < 2)
         return;
-    for (int e = threadIdx.x; e < 2 * BA_BLOCK * DP / 4; e += BA_THREADS) {
+    constexpr int EACH = 2 * BA_BLOCK * DP / 4 / BJ_SLICES;
+    const int e0 = (int)(blockIdx.x % BJ_SLICES) * EACH;
+    for (int e = e0 + threadIdx.x; e < e0 + EACH; e += BA_THREADS) {
         const int row = e / (DP / 4), c = (e % (DP / 4)) * 4, key = blk * BA_BLOCK + row % BA_BLOCK;
         if (key >= a.n || c >= a.d)
             continue;
         hd_f4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
         for (int p = p0; p < p1; ++p)
             y += *(const hd_f4 *)(a.part + ((int64_t)p * 2 * BA_BLOCK + row) * DP + c);
         T *O = (T *)(row < BA_BLOCK ? a.out : a.out2);
@@ -1218,7 +1222,7 @@ int ba_dkv_chunk(int b, int m, int hk, int nb, int count)
     if (blocks <= 0 || blocks > 1024)
         return 0;
     const int64_t picks = (int64_t)b * hk * m * (count < nb ? count : nb);
-    const int64_t c = (picks / 1536 + 63) / 64 * 64;
+    const int64_t c = (picks / 1024 + 63) / 64 * 64;
     return (int)(c < 128 ? 128 : c);
 }
 int64_t ba_dkv_parts(int b, int m, int hk, int nb, int count)
@@ -1245,8 +1249,12 @@ template <typename T, int DP> int ba_forward(const BaArgs &a, hipStream_t s)
         return rc;
     hipLaunchKernelGGL((block_attn_fwd_kernel<T, DP>), dim3((unsigned)all), dim3(BA_THREADS), lds, s, a, all);
     if (a.splits > 1) {
-        const int64_t rows = (int64_t)a.b * a.hq * a.m, per = BA_THREADS / 64;
-        hipLaunchKernelGGL((block_attn_join_kernel<T, DP>), dim3((unsigned)((rows + per - 1) / per)), dim3(BA_THREADS), 0, s, a, rows);
+        const int64_t rows = (int64_t)a.b * a.hq * a.m, per = BA_THREADS / (a.splits <= 16 ? 16 : 64);
+        const dim3 grid((unsigned)((rows + per - 1) / per));
+        if (a.splits <= 16)
+            hipLaunchKernelGGL((block_attn_join_kernel<T, DP, 16>), grid, dim3(BA_THREADS), 0, s, a, rows);
+        else
+            hipLaunchKernelGGL((block_attn_join_kernel<T, DP, 64>), grid, dim3(BA_THREADS), 0, s, a, rows);
     }
     return tpu3_launch_status();
 }
@@ -1278,7 +1286,7 @@ template <typename T, int DP> int ba_backward(BaArgs a, void *dq, void *dk, void
     }
     hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP>), dim3((unsigned)all2), dim3(BA_THREADS), lds2, s, a, all2);
     if (a.chunk)
-        hipLaunchKernelGGL((block_attn_dkv_join_kernel<T, DP>), dim3((unsigned)blocks), dim3(BA_THREADS), 0, s, a);
+        hipLaunchKernelGGL((block_attn_dkv_join_kernel<T, DP>), dim3((unsigned)(blocks * BJ_SLICES)), dim3(BA_THREADS), 0, s, a);
     return tpu3_launch_status();
 }
 

@@ -12,8 +12,8 @@
 // 64 bits (a position of 1e5 times a frequency of 1 leaves 7 of fp32's 24 bits for the fraction of a turn), the sine and
 // cosine of the fraction in 32.  Both pair orders use one expression, z[c] = y[c] C[c] + y[partner(c)] S[c], with the sign
 // folded into S and C = 1, S = 0 behind the pairs.  In the half-split order the partner sits in another lane: the normed row
-// goes through LDS with its first half stored a second time behind the second, so that the partner of channel c is
-// always c + P places from the start (P pairs) and every lane reads eight consecutive floats.
+// goes through LDS with its first half stored a second time behind the second, so that the partner of channel c is always
+// channel c + P (P pairs; lane exchanges where P is a multiple of eight).
 // The next row is requested before the current one is worked on (a wave otherwise has 1 KB in flight, and the chip 7 MB).
 #include "heads.h"
 
@@ -96,46 +96,52 @@ template <int LPR> __device__ __forceinline__ float nr_row_sum(float v)
     return v;
 }
 
-// floats of an exchange row: the channels, the first half again, and zeros up to the last place that is read
-__host__ __device__ __forceinline__ int nr_row(int d, int pairs, int interleaved) { return interleaved ? 0 : d + (pairs + 3) / 4 * 4 + 4; }
+// Exchange rows, for halves whose length is no multiple of eight: channel c of a row sits at (c % 8) * slots + c / 8, so that
+// the lanes of a wave, which hold channels 8 l .. 8 l + 7, meet different banks whatever the shift is; the first half is
+// stored a second time behind the second, and places behind that copy are zero (read by channels that do not turn, times
+// S = 0).
+__host__ __device__ __forceinline__ int nr_slots(int d, int pairs) { return (d + pairs + 7) / 8 + 1; }
+__host__ __device__ __forceinline__ bool nr_exchanges(int pairs, int interleaved) { return !interleaved && pairs % 8 != 0; }
 
-// eight channels from c0 on turned; `row` is this row's exchange slice
-__device__ __forceinline__ void nr_turn(const NrArgs &a, const float *cs, float *row, int c0, float *y)
+// eight channels from c0 on turned; `row` is this row's exchange slice.  Whole rows run it (LPR lanes each).
+template <int LPR> __device__ __forceinline__ void nr_turn(const NrArgs &a, const float *cs, float *row, int c0, bool live, float *y)
 {
+    const int P = a.total_pairs;
     float o[8];
     if (a.interleaved) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             o[i] = y[i ^ 1];
+    } else if (P % 8 == 0) {                // the partner is a whole number of lanes away
+        const int l = c0 >> 3, shift = P >> 3, from = l < shift ? l + shift : l < 2 * shift ? l - shift : l;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            o[i] = __shfl(y[i], from, LPR);
     } else {
-        const int P = a.total_pairs;
-        if (c0 + 8 <= 2 * P) {
-            *(hd_f4 *)(row + c0) = hd_f4{y[0], y[1], y[2], y[3]};
-            *(hd_f4 *)(row + c0 + 4) = hd_f4{y[4], y[5], y[6], y[7]};
-        } else if (c0 < 2 * P) {
+        const int slots = nr_slots(a.d, P);
+        if (c0 < 2 * P) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if (c0 + i < 2 * P)
-                    row[c0 + i] = y[i];
+                    row[i * slots + (c0 >> 3)] = y[i];
         }
-        if (c0 + 8 <= P) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                row[2 * P + c0 + i] = y[i];
-        } else if (c0 < P) {
+        if (c0 < P) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if (c0 + i < P)
-                    row[2 * P + c0 + i] = y[i];
+                    row[((2 * P + i) & 7) * slots + ((2 * P + c0 + i) >> 3)] = y[i];
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();    // the row's lanes are in one wave, whose LDS accesses complete in order
+        if (live)
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            o[i] = row[P + c0 + i];
+            for (int i = 0; i < 8; ++i)
+                o[i] = row[((P + i) & 7) * slots + ((P + c0 + i) >> 3)];
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
+    if (!live)
+        return;
     const hd_f4 c_0 = *(const hd_f4 *)(cs + c0), c_1 = *(const hd_f4 *)(cs + c0 + 4);
     const hd_f4 s_0 = *(const hd_f4 *)(cs + a.d + c0), s_1 = *(const hd_f4 *)(cs + a.d + c0 + 4);
 #pragma unroll
@@ -143,11 +149,20 @@ __device__ __forceinline__ void nr_turn(const NrArgs &a, const float *cs, float 
         y[i] = __builtin_fmaf(o[i], i < 4 ? s_0[i & 3] : s_1[i & 3], y[i] * (i < 4 ? c_0[i & 3] : c_1[i & 3]));
 }
 
-// the exchange rows' places behind the second half's copy stay zero (read by channels that do not turn, times S = 0)
 __device__ __forceinline__ void nr_clear(float *ex, int all)
 {
     for (int i = threadIdx.x; i < all; i += NR_THREADS)
         ex[i] = 0.f;
+}
+// where the tokens' rows start in the (strided) inputs: at[t] of x[0], x[1], g[0], g[1] for n of them
+__device__ __forceinline__ void nr_places(const NrArgs &a, int64_t t0, int count, int n, int64_t *at)
+{
+    for (int i = threadIdx.x; i < count * n; i += NR_THREADS) {
+        const int which = i / count, t = i - which * count;
+        const int64_t tok = t0 + t, e = tok / a.n, r = tok - e * a.n;
+        const tpu3_heads &x = which < 2 ? a.x[which] : a.g[which - 2];
+        at[which * a.tok + t] = e * x.sb + r * x.sr;
+    }
 }
 
 template <typename T, int LPR>
@@ -156,33 +171,35 @@ __global__ __launch_bounds__(NR_THREADS) void norm_rotate_kernel(NrArgs a)
     extern __shared__ __attribute__((aligned(16))) char smem[];
     constexpr int GROUPS = NR_THREADS / LPR;
     typedef typename hd_vec<T>::v8 V8;
-    const int len = nr_row(a.d, a.total_pairs, a.interleaved);
-    float *ex = (float *)smem, *cs = ex + GROUPS * len;         // (GROUPS, len) exchange rows, (tok, 2, d) turns
+    const int len = nr_exchanges(a.total_pairs, a.interleaved) ? 8 * nr_slots(a.d, a.total_pairs) : 0;
+    int64_t *at = (int64_t *)smem;                              // (2, tok) places of the tokens' rows
+    float *cs = (float *)(at + 2 * a.tok), *ex = cs + a.tok * 2 * a.d;      // (tok, 2, d) turns, (GROUPS, len) exchange rows
     const int64_t t0 = (int64_t)blockIdx.x * a.tok;
     const int count = (int)min((int64_t)a.tok, a.tokens - t0);
     const int grp = threadIdx.x / LPR, c0 = (threadIdx.x % LPR) * 8;
     const bool live = c0 < a.d;
     const int cr = live ? c0 : 0;           // (idle lanes of a row work on channel 0's addresses and write nothing)
     nr_clear(ex, GROUPS * len);
+    nr_places(a, t0, count, 2, at);
     nr_turns(a, t0, count, 1.f, cs);
     __syncthreads();
-    const int hq = a.x[0].heads, rows = count * (hq + a.x[1].heads);
+    const int hq = a.x[0].heads, hk = a.x[1].heads, rows = count * (hq + hk);
+    const float iq = 1.f / (float)hq, ik = hk ? 1.f / (float)hk : 0.f;
+    const T *X0 = (const T *)a.x[0].data + cr, *X1 = (const T *)a.x[1].data + cr;
+    T *Y0 = (T *)a.out[0] + t0 * hq * a.d + c0, *Y1 = (T *)a.out[1] + t0 * hk * a.d + c0;
+    // row r of the tile: queries first, token by token (r < 2^16, heads <= 1024: the rounded quotient is exact)
     auto place = [&](int r, int &side, int &t, int &h) __attribute__((always_inline)) {
-        side = r < count * hq ? 0 : 1;
-        const int heads = a.x[side].heads;
+        side = r >= count * hq;
         r -= side ? count * hq : 0;
-        t = r / heads;
-        h = r - t * heads;
+        t = (int)(((float)r + 0.5f) * (side ? ik : iq));
+        h = r - t * (side ? hk : hq);
     };
     auto load = [&](int r, V8 &v) __attribute__((always_inline)) {
-        if (r < rows && live) {
-            int side, t, h;
-            place(r, side, t, h);
-            const int64_t tok = t0 + t, e = tok / a.n, i = tok - e * a.n;
-            v = *(const V8 *)((const T *)a.x[side].data + e * a.x[side].sb + i * a.x[side].sr + h * a.x[side].sh + c0);
-        }
+        int side, t, h;
+        place(min(r, rows - 1), side, t, h);
+        v = *(const V8 *)((side ? X1 : X0) + at[side * a.tok + t] + h * (side ? a.x[1].sh : a.x[0].sh));
     };
-    V8 cur = {}, next = {};
+    V8 cur, next;
     load(grp, cur);
     for (int r = grp; r < rows; r += GROUPS) {
         load(r + GROUPS, next);
@@ -191,7 +208,7 @@ __global__ __launch_bounds__(NR_THREADS) void norm_rotate_kernel(NrArgs a)
         float y[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            y[j] = (float)cur[j];
+            y[j] = live ? (float)cur[j] : 0.f;
         float ss = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -202,10 +219,9 @@ __global__ __launch_bounds__(NR_THREADS) void norm_rotate_kernel(NrArgs a)
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             y[j] = y[j] * inv * w[j];
-        if (live) {
-            nr_turn(a, cs + t * 2 * a.d, ex + grp * len, c0, y);
-            hd_store8((T *)a.out[side] + ((t0 + t) * a.x[side].heads + h) * a.d + c0, y);
-        }
+        nr_turn<LPR>(a, cs + t * 2 * a.d, ex + grp * len, c0, live, y);
+        if (live)
+            hd_store8((side ? Y1 : Y0) + (t * (side ? hk : hq) + h) * a.d, y);
         cur = next;
     }
 }
@@ -220,13 +236,14 @@ __global__ __launch_bounds__(NR_THREADS) void norm_rotate_bwd_kernel(NrArgs a, i
     extern __shared__ __attribute__((aligned(16))) char smem[];
     constexpr int GROUPS = NR_THREADS / LPR, PER = 64 / LPR;
     typedef typename hd_vec<T>::v8 V8;
-    const int heads_all = a.x[0].heads + a.x[1].heads, len = nr_row(a.d, a.total_pairs, a.interleaved);
-    float *ex = (float *)smem;
-    float *acc = ex + GROUPS * len;                             // (units, d) per-head sums
+    const int heads_all = a.x[0].heads + a.x[1].heads;
+    const int len = nr_exchanges(a.total_pairs, a.interleaved) ? 8 * nr_slots(a.d, a.total_pairs) : 0;
+    int64_t *at = (int64_t *)smem;                              // (4, tok) places of the tokens' rows
+    float *cs = (float *)(at + 4 * a.tok), *acc = cs + a.tok * 2 * a.d;     // (tok, 2, d) turns; (units, d) per-head sums
     const bool per_head = (a.w[0] && a.w_head[0]) || (a.w[1] && a.w_head[1]);
     const bool want = a.want_w[0] || a.want_w[1];
     const int units = heads_all * split;
-    float *cs = acc + (want ? (per_head ? units : 8) * a.d : 0);
+    float *ex = acc + (want ? (per_head ? units : 8) * a.d : 0);            // (GROUPS, len) exchange rows
     const int grp = threadIdx.x / LPR, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c0 = (threadIdx.x % LPR) * 8;
     const bool live = c0 < a.d;
     const int cr = live ? c0 : 0;
@@ -239,26 +256,28 @@ __global__ __launch_bounds__(NR_THREADS) void norm_rotate_bwd_kernel(NrArgs a, i
     for (int64_t t0 = (int64_t)blockIdx.x * a.tok; t0 < a.tokens; t0 += (int64_t)gridDim.x * a.tok) {
         const int count = (int)min((int64_t)a.tok, a.tokens - t0);
         __syncthreads();
+        nr_places(a, t0, count, 4, at);
         nr_turns(a, t0, count, -1.f, cs);
         __syncthreads();
         for (int u = wave; u < units; u += 4) {
             const int hu = u / split, s = u - hu * split;
             const int side = hu < a.x[0].heads ? 0 : 1, h = side ? hu - a.x[0].heads : hu, heads = a.x[side].heads;
-            const T *X = (const T *)a.x[side].data + h * a.x[side].sh + c0;
-            const T *G = (const T *)a.g[side].data + h * a.g[side].sh + c0;
-            T *Y = (T *)a.out[side];
+            const T *X = (const T *)a.x[side].data + h * a.x[side].sh + cr;
+            const T *G = (const T *)a.g[side].data + h * a.g[side].sh + cr;
+            const int64_t *xa = at + side * a.tok, *ga = at + (2 + side) * a.tok;
+            T *Y = (T *)a.out[side] + (t0 * heads + h) * a.d + c0;
             const int last = min(count, (s + 1) * part_tok);
             float w[8], wg[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
             nr_weights(a.w[side], a.w_type, h * a.w_head[side] + cr, w);
             V8 xc = {}, gc = {}, xn = {}, gn = {};
             auto load = [&](int t, V8 &x, V8 &g) __attribute__((always_inline)) {
-                if (t < last && live) {
-                    const int64_t tok = t0 + t, e = tok / a.n, i = tok - e * a.n;
-                    x = *(const V8 *)(X + e * a.x[side].sb + i * a.x[side].sr);
-                    g = *(const V8 *)(G + e * a.g[side].sb + i * a.g[side].sr);
-                }
+                t = min(t, last - 1);
+                x = *(const V8 *)(X + xa[t]);
+                g = *(const V8 *)(G + ga[t]);
             };
             const int tl = lane / LPR;
+            if (s * part_tok >= last)
+                continue;
             load(s * part_tok + tl, xc, gc);
             // (whole waves run the loop: the lanes of a row exchange values inside)
             for (int tb = s * part_tok; tb < last; tb += PER) {
@@ -269,8 +288,7 @@ __global__ __launch_bounds__(NR_THREADS) void norm_rotate_bwd_kernel(NrArgs a, i
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     x[j] = row ? (float)xc[j] : 0.f, g[j] = row ? (float)gc[j] : 0.f;
-                if (live)
-                    nr_turn(a, cs + tc * 2 * a.d, ex + grp * len, c0, g);
+                nr_turn<LPR>(a, cs + tc * 2 * a.d, ex + grp * len, c0, live, g);
                 float ss = 0.f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
@@ -289,7 +307,7 @@ __global__ __launch_bounds__(NR_THREADS) void norm_rotate_bwd_kernel(NrArgs a, i
                 for (int j = 0; j < 8; ++j)
                     g[j] = inv * __builtin_fmaf(-x[j], dot, g[j]);
                 if (row)
-                    hd_store8(Y + ((t0 + t) * heads + h) * a.d + c0, g);
+                    hd_store8(Y + t * heads * a.d, g);
                 xc = xn, gc = gn;
             }
             if (!want)
@@ -381,7 +399,9 @@ NrPlan nr_plan(int64_t tokens, int heads, int d, int pairs, int interleaved, boo
     const int64_t tiles = (tokens + p.tok - 1) / p.tok;
     p.split = bwd && heads % 4 ? (p.tok >= 4 ? 4 : 1) : 1;
     p.wgs = bwd ? (int)(tiles < NR_MAX_WG ? tiles : NR_MAX_WG) : 0;
-    p.lds = (size_t)(NR_THREADS / p.lpr) * nr_row(d, pairs, interleaved) * 4 + (size_t)p.tok * d * 8;
+    p.lds = (size_t)p.tok * (d * 8 + (bwd ? 32 : 16));
+    if (nr_exchanges(pairs, interleaved))
+        p.lds += (size_t)(NR_THREADS / p.lpr) * 8 * nr_slots(d, pairs) * 4;
     if (bwd && want)
         p.lds += (size_t)(per_head ? heads * p.split : 8) * d * 4;
     return p;
