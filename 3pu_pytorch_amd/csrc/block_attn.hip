@@ -250,24 +250,21 @@ template <typename T, int DP> struct BaStage {
 // How a kernel is laid out over registers and LDS; w: waves a SIMD that the register allocation aims at.  More waves hide
 // more of the chain scores -> maximum -> exponentials -> product, until the operands no longer fit: measured on clouds
 // of 5000 points (64 channels) and a sequence of 8192 (128), us with 2 / 3 / 4 waves: forward - / 144 / 129 and
-// 310 / 279 / -, dq - / 94 / 99 and 341 / 520 / -, dk and dv - / 63 / 92 and 346 / 900 / -.  A wave has 16 rows (keys):
+// 310 / 279 / -, dq - / 94 / 99 and 341 / 520 / -, dk and dv - / 63 / 92 and 346 / 900 / -; fp32 of 24 channels,
+// forward, - / 59 / 49.  A wave has 16 rows (keys):
 // with 32, every operand read from LDS feeds two matrix instructions, but half as many waves are there (188 for 146).
 // together: 16-row tiles whose row operands are read in one go; columns: 16-channel columns read in one go.
-#ifndef DQ_TOG
-#define DQ_TOG 2
-#define DQ_COL 8
-#endif
 template <typename T, int DP> struct BaFwd {
     static constexpr bool F32 = sizeof(T) == 4;
-    static constexpr int w = F32 ? (DP == 128 ? 1 : DP == 64 ? 2 : 3) : DP == 128 ? 3 : 4;
+    static constexpr int w = F32 ? (DP == 128 ? 1 : DP == 64 ? 2 : 4) : DP == 128 ? 3 : 4;
     static constexpr int together = F32 ? (DP == 32 ? 4 : DP == 64 ? 2 : 1) : DP == 128 ? 1 : 2;
     static constexpr int columns = DP / 16 < 4 ? DP / 16 : 4;
 };
 template <typename T, int DP> struct BaBwd {
     static constexpr bool F32 = sizeof(T) == 4;
     static constexpr int w = F32 ? (DP == 128 ? 1 : DP == 64 ? 2 : 3) : DP == 128 ? 2 : 3;
-    static constexpr int together = F32 ? (DP == 32 ? 4 : DP == 64 ? 2 : 1) : DP == 128 ? DQ_TOG : 4;
-    static constexpr int columns = DP / 16 < DQ_COL ? DP / 16 : DQ_COL;
+    static constexpr int together = F32 ? (DP == 32 ? 4 : DP == 64 ? 2 : 1) : DP == 128 ? 2 : 4;
+    static constexpr int columns = DP / 16;
     static constexpr int kw = F32 ? (DP == 128 ? 1 : 2) : DP == 128 ? 2 : 3;
 };
 // LDS reads above stay above: the compiler otherwise sinks each to its matrix instruction and waits for it there

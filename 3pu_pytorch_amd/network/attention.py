@@ -64,14 +64,18 @@ def _heads(t):
                    stride[2] if size[2] > 1 else 0, size[2])
 
 
+# the stream handle without the Stream object around it (2 us of a call's 10)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
 def _launch(name, t, *args):
     """A C entry point on the current stream of the tensor's device (which is made the current device if it is not)."""
     dev = t.get_device()
     if torch.cuda.current_device() == dev:
-        rc = getattr(L.lib(), name)(torch.cuda.current_stream(dev).cuda_stream, *args)
+        rc = getattr(L.lib(), name)(_raw_stream(dev), *args)
     else:
         with torch.cuda.device(dev):
-            rc = getattr(L.lib(), name)(torch.cuda.current_stream(dev).cuda_stream, *args)
+            rc = getattr(L.lib(), name)(_raw_stream(dev), *args)
     if rc:
         L.check(rc, name)
 
