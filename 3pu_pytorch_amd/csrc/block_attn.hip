@@ -456,13 +456,18 @@ template <typename T, int DP, int VG> struct BaColumns {
         read(tile, 0);
         ba_issue();
     }
-    template <typename F> __device__ __forceinline__ void run(const T *tile, hd_f4 *acc, F &&before)
+    // before(j): the operand f[j]; REST adds a second term of it, after(j)
+    template <bool REST, typename F, typename G>
+    __device__ __forceinline__ void run(const T *tile, hd_f4 *acc, F &&before, G &&after)
     {
-        typename hd_vec<T>::v8 f;
+        typename hd_vec<T>::v8 f, f2;
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
             if (s % (STEPS / 2) == 0)
                 f = before(s / (STEPS / 2));
+            if constexpr (REST)
+                if (s % (STEPS / 2) == 0)
+                    f2 = after(s / (STEPS / 2), f);
             if (s + 1 < STEPS) {
                 read(tile, s + 1);
                 ba_issue();
@@ -471,6 +476,13 @@ template <typename T, int DP, int VG> struct BaColumns {
             for (int i = 0; i < VG; ++i) {
                 hd_f4 &x = acc[(s % (STEPS / 2)) * VG + i];
                 x = ba_mma<T>(c[s & 1][i], f, x);
+            }
+            if constexpr (REST) {
+#pragma unroll
+                for (int i = 0; i < VG; ++i) {
+                    hd_f4 &x = acc[(s % (STEPS / 2)) * VG + i];
+                    x = ba_mma<T>(c[s & 1][i], f2, x);
+                }
             }
         }
     }
@@ -525,7 +537,7 @@ __device__ __forceinline__ void ba_fwd_block(const BaArgs &a, const BaRow &R, co
                 s[x][r] = bit ? s[x][r] : 0.f;
         }
     };
-    vc.run(Vs, acc, [&](int j) __attribute__((always_inline)) {
+    const auto rounded = [&](int j) __attribute__((always_inline)) {
         weight(2 * j), weight(2 * j + 1);
         const V8 pf = ba_pack<T>(s[2 * j], s[2 * j + 1]);
         // the denominator: in the 16-bit types one more row of the product, ones times the probabilities, as rounded as they
@@ -535,7 +547,8 @@ __device__ __forceinline__ void ba_fwd_block(const BaArgs &a, const BaRow &R, co
         else
             sums += s[2 * j] + s[2 * j + 1];
         return pf;
-    });
+    };
+    vc.template run<false>(Vs, acc, rounded, rounded);
     if constexpr (CAREFUL) {
         for (unsigned long long left = *odd; left; left &= left - 1) {
             const int kk = __ffsll(left) - 1;                   // the key's place in the block: score register and lane group
@@ -750,7 +763,17 @@ __device__ __forceinline__ void ba_dq_block(const BaArgs &a, const BaRow &R, con
             for (int r = 0; r < 4; ++r)
                 s[x][r] = bit ? s[x][r] : 0.f;
     }
-    kc.run(Ks, acc, [&](int j) __attribute__((always_inline)) { return ba_pack<T>(s[2 * j], s[2 * j + 1]); });
+    // A row's ds add up to nothing, so its dq is what is left of large terms: ds enters in two terms of the 16-bit type (one
+    // alone: an error of twice the result's own rounding)
+    kc.template run<sizeof(T) == 2>(
+        Ks, acc, [&](int j) __attribute__((always_inline)) { return ba_pack<T>(s[2 * j], s[2 * j + 1]); },
+        [&](int j, const V8 &f) __attribute__((always_inline)) {
+            hd_f4 r0, r1;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                r0[r] = s[2 * j][r] - (float)f[r], r1[r] = s[2 * j + 1][r] - (float)f[4 + r];
+            return ba_pack<T>(r0, r1);
+        });
 }
 
 // As in the forward kernel, CAREFUL is the second pass of a workgroup in which a key that is not finite may have reached rows
