@@ -114,11 +114,12 @@ __device__ __forceinline__ bool bs_better(uint64_t a, int ia, uint64_t b, int ib
 __device__ void bs_best(BsShared &s, int n, int count)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const bool one = n <= 256;              // one wave holds them all
     uint64_t v[4];
     int id[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const int e = j * BS_THREADS + threadIdx.x;
+        const int e = one ? (wave ? n : j * 64 + lane) : j * BS_THREADS + threadIdx.x;
         v[j] = e < n ? s.key[e] : 0ull;
         id[j] = e < n ? s.id[e] : 0x7FFFFFFF;
     }
@@ -131,7 +132,7 @@ __device__ void bs_best(BsShared &s, int n, int count)
         }
     };
     order(0, 1), order(2, 3), order(0, 2), order(1, 3), order(1, 2);
-    for (int r = 0; r < count; ++r) {
+    for (int r = 0; r < (one && wave ? 0 : count); ++r) {
         const uint32_t hi = (uint32_t)(v[0] >> 32), lo = (uint32_t)v[0];
         const uint32_t mh = tpu3_wave_max_u32(hi);
         unsigned long long who = __ballot(hi == mh);
@@ -144,7 +145,10 @@ __device__ void bs_best(BsShared &s, int n, int count)
             }
         }
         if (lane == __ffsll(who) - 1) {
-            s.wave_key[wave * count + r] = v[0], s.wave_id[wave * count + r] = id[0];
+            if (one)
+                s.key[r] = v[0], s.id[r] = id[0];               // (all of them are in registers)
+            else
+                s.wave_key[wave * count + r] = v[0], s.wave_id[wave * count + r] = id[0];
 #pragma unroll
             for (int j = 0; j < 3; ++j)
                 v[j] = v[j + 1], id[j] = id[j + 1];
@@ -152,6 +156,8 @@ __device__ void bs_best(BsShared &s, int n, int count)
         }
     }
     __syncthreads();
+    if (one)
+        return;
     const int c = threadIdx.x;              // 4 * count <= 256 candidates, one a thread
     if (c < 4 * count) {
         const uint64_t cv = s.wave_key[c];
@@ -203,8 +209,13 @@ template <typename T, int DP> __device__ void block_select_row(const BsArgs &a, 
     for (int c = threadIdx.x; c < 128; c += BS_THREADS) {
         double v = 0.0;
         if (c < a.d && z1 > z0)
-            for (int g = 0; g < a.group; ++g)
-                v += (double)(float)Q[g * a.q.sh + c];
+            for (int g = 0; g < a.group; g += 4) {              // (loads of four heads in flight)
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    x[e] = g + e < a.group ? (float)Q[(g + e) * a.q.sh + c] : 0.f;
+                v += ((double)x[0] + (double)x[1]) + ((double)x[2] + (double)x[3]);
+            }
         s.q[c] = v;
     }
     __syncthreads();
@@ -221,32 +232,32 @@ template <typename T, int DP> __device__ void block_select_row(const BsArgs &a, 
     int kept = 0;                                               // candidates in LDS
     for (int c0 = z0; c0 < z1 || c0 == z0;) {
         const int take = min(z1 - c0, BS_KEEP - kept);
-        hd_f4 next[VECS];
-        auto fetch = [&](int t) __attribute__((always_inline)) {
+        constexpr int AHEAD = 16 / VECS > 4 ? 4 : 16 / VECS;     // blocks of a lane in flight
+        for (int t0 = 0; t0 < take; t0 += AHEAD * STEP) {
+            hd_f4 m[AHEAD][VECS];
 #pragma unroll
-            for (int x = 0; x < VECS; ++x)
-                next[x] = t < take && x * 32 + part * 4 < a.d ? *(const hd_f4 *)(M + (c0 + t) * stride + x * 32) : hd_f4{0.f, 0.f, 0.f, 0.f};
-        };
-        fetch(slot);
-        for (int t0 = 0; t0 < take; t0 += STEP) {
-            const int t = t0 + slot, blk = c0 + t;
-            hd_f4 m[VECS];
+            for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
-            for (int x = 0; x < VECS; ++x)
-                m[x] = next[x];
-            fetch(t + STEP);
-            double v = 0.0;
+                for (int x = 0; x < VECS; ++x)
+                    m[u][x] = t0 + u * STEP + slot < take && x * 32 + part * 4 < a.d
+                                  ? *(const hd_f4 *)(M + (c0 + t0 + u * STEP + slot) * stride + x * 32)
+                                  : hd_f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int x = 0; x < VECS; ++x)
+            for (int u = 0; u < AHEAD; ++u) {
+                const int t = t0 + u * STEP + slot, blk = c0 + t;
+                double v = 0.0;
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    v = __builtin_fma((double)m[x][j], q[x][j], v);
+                for (int x = 0; x < VECS; ++x)
 #pragma unroll
-            for (int o = 4; o > 0; o >>= 1)
-                v += __shfl_xor(v, o, 64);
-            if (t < take && part == 0) {
-                s.key[kept + t] = blk == own ? BS_OWN : bs_key(v);
-                s.id[kept + t] = blk;
+                    for (int j = 0; j < 4; ++j)
+                        v = __builtin_fma((double)m[u][x][j], q[x][j], v);
+#pragma unroll
+                for (int o = 4; o > 0; o >>= 1)
+                    v += __shfl_xor(v, o, 64);
+                if (t < take && part == 0) {
+                    s.key[kept + t] = blk == own ? BS_OWN : bs_key(v);
+                    s.id[kept + t] = blk;
+                }
             }
         }
         __syncthreads();

@@ -27,17 +27,18 @@ BLOCK = L.ATTN_BLOCK        # consecutive keys of a block
 
 
 def _rows(t, name, like=None):
-    """The checks of a (B, rows, heads, D) tensor; returned with strides that the kernels take (a copy if they do not)."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+    """The checks of a (B, rows, heads, D) tensor."""
+    if not isinstance(t, torch.Tensor) or t.get_device() < 0:
         raise RuntimeError("%s must be a CUDA tensor" % name)
     if t.dim() != 4:
         raise RuntimeError("%s must be (B, rows, heads, D), got %s" % (name, tuple(t.shape)))
     if t.dtype not in L.TYPES:
         raise RuntimeError("%s must be float32, float16 or bfloat16, got %s" % (name, t.dtype))
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+    if like is not None and (t.dtype != like.dtype or t.get_device() != like.get_device()):
         raise RuntimeError("%s must be %s on %s, got %s on %s" % (name, like.dtype, like.device, t.dtype, t.device))
-    if t.size(3) == 0 or t.size(3) % 8:
-        raise RuntimeError("%s: D must be a multiple of 8, got %d" % (name, t.size(3)))
+    d = t.shape[3]
+    if d == 0 or d % 8:
+        raise RuntimeError("%s: D must be a multiple of 8, got %d" % (name, d))
     return t
 
 
@@ -81,16 +82,16 @@ def _launch(name, t, *args):
 
 
 def _workspace(need, t):
-    return torch.empty((need,), dtype=torch.uint8, device=t.device) if need else None
+    return t.new_empty((need,), dtype=torch.uint8) if need else None
 
 
-def _lengths(t, name, b, device):
+def _lengths(t, name, b, like):
     if t is None:
         return None
     L.require_device(t, name)
     L.require_dtype(t, torch.int32, name)
-    if tuple(t.shape) != (b,) or t.device != device:
-        raise RuntimeError("%s must be (%d,) on %s, got %s on %s" % (name, b, device, tuple(t.shape), t.device))
+    if t.shape != (b,) or t.get_device() != like.get_device():
+        raise RuntimeError("%s must be (%d,) on %s, got %s on %s" % (name, b, like.device, tuple(t.shape), t.device))
     return t
 
 
@@ -115,8 +116,8 @@ def _weights(wq, wk, d):
 
 def _norm_rotate_forward(q, k, wq, wk, position, freq, eps, interleaved):
     q, k = _taken(q), _taken(k)
-    oq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ok = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    oq = q.new_empty(q.shape)
+    ok = None if k is None else k.new_empty(k.shape)
     b, n, _, d = q.shape
     _launch("tpu3_norm_rotate_fwd", q, L.TYPES[q.dtype], b, n, d, _heads(q), _heads(k), *_weights(wq, wk, d),
             _rotation(q, position, freq), eps, interleaved, oq.data_ptr(), L.ptr(ok))
@@ -182,11 +183,11 @@ def norm_rotate(q, k, q_weight, k_weight, position, freq, eps=1e-6, interleaved=
     weights = []
     for w, h, name in ((q_weight, hq, "q_weight"), (k_weight, 0 if k is None else k.size(2), "k_weight")):
         if w is not None:
-            if not w.is_cuda or w.device != q.device:
+            if w.get_device() != q.get_device():
                 raise RuntimeError("%s must be a CUDA tensor on %s" % (name, q.device))
             if w.dtype not in L.TYPES:
                 raise RuntimeError("%s must be float32, float16 or bfloat16, got %s" % (name, w.dtype))
-            if tuple(w.shape) not in ((d,), (h, d)):
+            if w.shape != (d,) and w.shape != (h, d):
                 raise RuntimeError("%s must be (%d,) or (%d, %d), got %s" % (name, d, h, d, tuple(w.shape)))
         weights.append(w)
     wq, wk = weights
@@ -196,7 +197,7 @@ def norm_rotate(q, k, q_weight, k_weight, position, freq, eps=1e-6, interleaved=
         if wq.dim() != wk.dim():
             wq, wk = wq.expand(hq, d), wk.expand(k.size(2), d)
     wq, wk = (w if w is None or (w.is_contiguous() and not w.data_ptr() & 15) else w.contiguous().clone() for w in (wq, wk))
-    if not position.is_cuda or not freq.is_cuda or position.device != q.device or freq.device != q.device:
+    if position.get_device() != q.get_device() or freq.get_device() != q.get_device():
         raise RuntimeError("position and freq must be CUDA tensors on %s" % q.device)
     if position.dtype not in L.POSITION_TYPES:
         raise RuntimeError("position must be float32, float64, int32 or int64, got %s" % position.dtype)
@@ -206,7 +207,7 @@ def norm_rotate(q, k, q_weight, k_weight, position, freq, eps=1e-6, interleaved=
         raise RuntimeError("norm_rotate: position and freq are constants: pass them detached")
     if position.dim() == 2:
         position = position.unsqueeze(2)
-    if position.dim() != 3 or freq.dim() != 2 or tuple(position.shape) != (b, n, freq.size(0)) or freq.size(0) == 0:
+    if position.dim() != 3 or freq.dim() != 2 or position.shape != (b, n, freq.shape[0]) or freq.shape[0] == 0:
         raise RuntimeError("norm_rotate: position %s and freq %s do not fit %d x %d rows"
                            % (tuple(position.shape), tuple(freq.shape), b, n))
     if 2 * freq.numel() > d:
@@ -245,7 +246,7 @@ def block_means(k, n_arr=None, out=None, last=None):
         raise RuntimeError("block_means: D must be at most 128, got %d" % d)
     if hk == 0:
         raise RuntimeError("block_means: k has no heads")
-    n_arr = _lengths(n_arr, "n_arr", b, k.device)
+    n_arr = _lengths(n_arr, "n_arr", b, k)
     shape = (b, (_keys(n) + BLOCK - 1) // BLOCK, hk, d)
     if out is None:
         if last is not None:
@@ -278,22 +279,22 @@ def select_blocks(q, means, keys, count, n_arr=None, m_arr=None, causal=False):
     q = _rows(q.detach() if isinstance(q, torch.Tensor) else q, "q")
     b, m, hq, d = q.shape
     count, keys = _count(count), _keys(int(keys))
-    if not isinstance(means, torch.Tensor) or not means.is_cuda:
+    if not isinstance(means, torch.Tensor) or means.get_device() < 0:
         raise RuntimeError("means must be a CUDA tensor")
     L.require_dtype(means, torch.float32, "means")
     if means.dim() != 4 or (means.size(0), means.size(1), means.size(3)) != (b, (keys + BLOCK - 1) // BLOCK, d) \
-            or means.device != q.device:
+            or means.get_device() != q.get_device():
         raise RuntimeError("means %s do not fit q %s and %d keys" % (tuple(means.shape), tuple(q.shape), keys))
     hk = means.size(2)
     if hk == 0 or hq == 0 or hq % hk:
         raise RuntimeError("select_blocks: %d query heads over %d key heads" % (hq, hk))
     if d > 128:
         raise RuntimeError("select_blocks: D must be at most 128, got %d" % d)
-    n_arr, m_arr = _lengths(n_arr, "n_arr", b, q.device), _lengths(m_arr, "m_arr", b, q.device)
+    n_arr, m_arr = _lengths(n_arr, "n_arr", b, q), _lengths(m_arr, "m_arr", b, q)
     means = means.detach().contiguous()
     if means.data_ptr() & 15:
         means = means.clone()
-    blocks = torch.empty((b, m, hk, count), dtype=torch.int32, device=q.device)
+    blocks = q.new_empty((b, m, hk, count), dtype=torch.int32)
     q = _taken(q)
     need = L.lib().tpu3_block_select_workspace_bytes(b, m, keys, hk, count)
     ws = _workspace(need, q)
@@ -307,9 +308,9 @@ def _attention_forward(q, k, v, blocks, scale, n_arr, m_arr, causal, grad=False)
     q, k, v = _taken(q), _taken(k), _taken(v)
     b, m, hq, d = q.shape
     n, hk, count = k.size(1), k.size(2), blocks.size(3)
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((b, hq, m), dtype=torch.float32, device=q.device) if grad else None
-    rest = torch.empty(q.shape, dtype=q.dtype, device=q.device) if grad and q.dtype != torch.float32 else None
+    o = q.new_empty(q.shape)
+    lse = q.new_empty((b, hq, m), dtype=torch.float32) if grad else None
+    rest = q.new_empty(q.shape) if grad and q.dtype != torch.float32 else None
     need = L.lib().tpu3_block_attn_fwd_workspace_bytes(b, m, n, hq, hk, d, count)
     ws = _workspace(need, q)
     _launch("tpu3_block_attn_fwd", q, L.TYPES[q.dtype], b, m, n, d, _heads(q), _heads(k), _heads(v), blocks.data_ptr(), count,
@@ -353,7 +354,7 @@ def _check_attention(q, k, v, scale, n_arr, m_arr):
     q = _rows(q, "q")
     k, v = _rows(k, "k", q), _rows(v, "v", q)
     b, m, hq, d = q.shape
-    if tuple(v.shape) != tuple(k.shape) or k.size(0) != b or k.size(3) != d:
+    if v.shape != k.shape or k.shape[0] != b or k.shape[3] != d:
         raise RuntimeError("q %s, k %s and v %s do not match" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
     hk = k.size(2)
     if hk == 0 or hq == 0 or hq % hk or hq // hk > 64:
@@ -364,7 +365,7 @@ def _check_attention(q, k, v, scale, n_arr, m_arr):
     scale = d ** -0.5 if scale is None else float(scale)
     if not (0.0 < scale < 1e30) or math.isinf(scale):
         raise RuntimeError("scale must be positive and finite, got %s" % scale)
-    return q, k, v, scale, _lengths(n_arr, "n_arr", b, q.device), _lengths(m_arr, "m_arr", b, q.device)
+    return q, k, v, scale, _lengths(n_arr, "n_arr", b, q), _lengths(m_arr, "m_arr", b, q)
 
 
 def block_attention(q, k, v, blocks, scale=None, n_arr=None, m_arr=None, causal=False):
@@ -379,7 +380,7 @@ def block_attention(q, k, v, blocks, scale=None, n_arr=None, m_arr=None, causal=
         (B, M, Hq, D) of q's type; a row that sees nothing (or is behind m_arr): 0
     Differentiable in q, k and v (keys behind n_arr: gradient 0)."""
     q, k, v, scale, n_arr, m_arr = _check_attention(q, k, v, scale, n_arr, m_arr)
-    if not isinstance(blocks, torch.Tensor) or not blocks.is_cuda or blocks.device != q.device:
+    if not isinstance(blocks, torch.Tensor) or blocks.get_device() != q.get_device():
         raise RuntimeError("blocks must be a CUDA tensor on %s" % q.device)
     if blocks.dtype not in (torch.int32, torch.int64):
         raise RuntimeError("blocks must be int32 or int64, got %s" % blocks.dtype)
