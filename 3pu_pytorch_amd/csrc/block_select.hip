@@ -282,21 +282,25 @@ template <typename T, int DP> __global__ __launch_bounds__(BS_THREADS) void bloc
     block_select_row<T, DP>(a, s, blockIdx.x / a.splits, (int)(blockIdx.x % a.splits));
 }
 
-// The queries that block_select_many_kernel left open: one word of 64 queries a wave of it.
+// The queries that block_select_many_kernel left open: one word of 64 queries a wave of it.  A workgroup looks at quarters of
+// words, 16 queries each, every gridDim.x-th: where all are open (equal means throughout) they still spread over the chip.
+constexpr int BO_PARTS = 4, BO_QUERIES = 64 / BO_PARTS;
 template <typename T, int DP> __global__ __launch_bounds__(BS_THREADS) void block_select_open_kernel(BsArgs a, int qtiles, int64_t waves)
 {
     __shared__ BsShared s;
-    __shared__ uint64_t open[BS_THREADS];
-    for (int64_t w0 = (int64_t)blockIdx.x * BS_THREADS; w0 < waves; w0 += (int64_t)gridDim.x * BS_THREADS) {
-        const uint64_t mine = w0 + threadIdx.x < waves ? a.open[w0 + threadIdx.x] : 0ull;
+    __shared__ uint32_t open[BS_THREADS];
+    const int64_t units = waves * BO_PARTS, step = gridDim.x;
+    for (int64_t u0 = blockIdx.x; u0 < units; u0 += step * BS_THREADS) {
+        const int64_t u = u0 + threadIdx.x * step;
+        const uint32_t mine = u < units ? (uint32_t)(a.open[u / BO_PARTS] >> (u % BO_PARTS * BO_QUERIES)) & ((1u << BO_QUERIES) - 1) : 0u;
         if (!__syncthreads_or(mine != 0))
             continue;
         open[threadIdx.x] = mine;
         __syncthreads();
         for (int t = 0; t < BS_THREADS; ++t)
-            for (uint64_t left = open[t]; left; left &= left - 1) {
-                const int64_t w = w0 + t;
-                block_select_row<T, DP>(a, s, w / qtiles * a.m + w % qtiles * 64 + __ffsll((unsigned long long)left) - 1, 0);
+            for (uint32_t left = open[t]; left; left &= left - 1) {
+                const int64_t at = u0 + t * step, w = at / BO_PARTS;
+                block_select_row<T, DP>(a, s, w / qtiles * a.m + w % qtiles * 64 + at % BO_PARTS * BO_QUERIES + __ffs(left) - 1, 0);
                 __syncthreads();
             }
         __syncthreads();
@@ -378,12 +382,12 @@ __global__ __launch_bounds__(BS_THREADS) void block_select_many_kernel(BsArgs a,
 
     // B operands: rows i0 + sub*16 + l15, channels kk*32 + g*8 .. +8, summed over the group's heads
     BtSplit q[4][DP / 32];
-    float qn = 0.f;                         // |q|^2 of query `lane`
+    float qn = 0.f, qp = 0.f;               // |q|^2 of query `lane`; the same of its heads before they are added up, together
     const T *Q = (const T *)a.q.data + b * a.q.sb + (int64_t)h * a.group * a.q.sh;
 #pragma unroll
     for (int sub = 0; sub < 4; ++sub) {
         const int r = i0 + sub * 16 + l15;
-        float n2 = 0.f;
+        float n2 = 0.f, parts = 0.f;
 #pragma unroll
         for (int kk = 0; kk < DP / 32; ++kk) {
             const int c = kk * 32 + g * 8;
@@ -393,8 +397,10 @@ __global__ __launch_bounds__(BS_THREADS) void block_select_many_kernel(BsArgs a,
                     float y[8];
                     hd_load8(Q + r * a.q.sr + e * a.q.sh + c, y);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
+                    for (int j = 0; j < 8; ++j) {
                         x[j] += y[j];
+                        parts = __builtin_fmaf(y[j], y[j], parts);
+                    }
                 }
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -404,6 +410,11 @@ __global__ __launch_bounds__(BS_THREADS) void block_select_many_kernel(BsArgs a,
         n2 += __shfl_xor(n2, 16, 64);
         n2 += __shfl_xor(n2, 32, 64);
         qn = g == sub ? n2 : qn;            // lane sub*16 + l15
+        if (a.group > 1) {
+            parts += __shfl_xor(parts, 16, 64);
+            parts += __shfl_xor(parts, 32, 64);
+            qp = g == sub ? parts : qp;
+        }
     }
 
     const float *M = a.means + ((int64_t)b * a.nb * a.hk + h) * a.d;
@@ -496,13 +507,16 @@ __global__ __launch_bounds__(BS_THREADS) void block_select_many_kernel(BsArgs a,
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1)
         mn = fmaxf(mn, __shfl_xor(mn, o, 64));
-    const float eps2 = 2.44140625e-4f * sqrtf(qn) * sqrtf(mn);         // 2 eps
-    const bool any_odd = __any(odd);
+    // 2 eps; the heads' fp32 sums: off by (group - 1) 2^-24 sum |q_h| <= (group - 1) 2^-24 sqrt(group sum |q_h|^2)
+    const float heads = (float)(a.group - 1) * 2.384185791015625e-7f * sqrtf((float)a.group * qp);
+    const float eps2 = (2.44140625e-4f * sqrtf(qn) + heads) * sqrtf(mn);
+    // (squares near the smallest numbers of fp32 say nothing)
+    const bool bounded = !__any(odd) && qn > 1e-30f && mn > 1e-30f && eps2 < INFINITY;
     const float kth = best[NL - 2], after = best[NL - 1];
-    const bool plain = everything || k == 0 || (!any_odd && kth - after > eps2 && kth < INFINITY);
+    const bool plain = everything || k == 0 || (bounded && kth - after > eps2 && kth < INFINITY);
     // blocks above `in` are picked, those from `near` on may be
     const float in = everything ? -INFINITY : plain ? after : after + eps2, near = plain ? INFINITY : kth - eps2;
-    bool open = !plain && (any_odd || !(eps2 < INFINITY) || !(fabsf(kth) < INFINITY) || !(fabsf(after) < INFINITY));
+    bool open = !plain && (!bounded || !(fabsf(kth) < INFINITY) || !(fabsf(after) < INFINITY));
     int at = 0, certain = 0;
     if (k > 0) {
         if (most > 0)
@@ -624,8 +638,8 @@ template <typename T, int DP, bool LOQ> int bs_many_launch(const BsArgs &a, hipS
 #undef BT_GO
     if (e != hipSuccess)
         return (int)e;
-    const int64_t words = (waves + BS_THREADS - 1) / BS_THREADS;
-    hipLaunchKernelGGL((block_select_open_kernel<T, DP>), dim3((unsigned)(words < 1024 ? words : 1024)), dim3(BS_THREADS), 0, s, a, qtiles, waves);
+    const int64_t units = waves * BO_PARTS;
+    hipLaunchKernelGGL((block_select_open_kernel<T, DP>), dim3((unsigned)(units < 1024 ? units : 1024)), dim3(BS_THREADS), 0, s, a, qtiles, waves);
     return tpu3_launch_status();
 }
 template <typename T, bool LOQ> int bs_many_d(const BsArgs &a, hipStream_t s)
