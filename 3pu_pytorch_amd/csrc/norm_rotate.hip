@@ -20,6 +20,7 @@
 namespace {
 
 constexpr int NR_THREADS = 256;
+constexpr size_t NR_LDS = 160 * 1024;
 constexpr int NR_MAX_WG = 1024;             // backward: persistent workgroups, one partial weight gradient each
 
 struct NrArgs {
@@ -402,6 +403,8 @@ NrPlan nr_plan(int64_t tokens, int heads, int d, int pairs, int interleaved, boo
     p.lds = (size_t)p.tok * (d * 8 + (bwd ? 32 : 16));
     if (nr_exchanges(pairs, interleaved))
         p.lds += (size_t)(NR_THREADS / p.lpr) * 8 * nr_slots(d, pairs) * 4;
+    if (bwd && want && per_head && p.lds + (size_t)heads * p.split * d * 4 > NR_LDS)
+        p.split = 1;
     if (bwd && want)
         p.lds += (size_t)(per_head ? heads * p.split : 8) * d * 4;
     return p;
@@ -529,7 +532,7 @@ extern "C" int tpu3_norm_rotate_bwd(tpu3_stream_t stream, int type, int b, int n
         return TPU3_EINVAL;
     a.part = (float *)workspace;
     const NrPlan p = nr_plan(a.tokens, heads, d, a.total_pairs, a.interleaved, true, per_head, want);
-    if (p.lds > 160 * 1024)
+    if (p.lds > NR_LDS)
         return TPU3_ELIMIT;
     a.tok = p.tok;
     const hipStream_t s = (hipStream_t)stream;

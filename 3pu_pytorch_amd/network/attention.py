@@ -159,7 +159,8 @@ def norm_rotate(q, k, q_weight, k_weight, position, freq, eps=1e-6, interleaved=
     :param
         q         (B, N, Hq, D); D <= 256
         k         (B, N, Hk, D) or None
-        q_weight, k_weight  (D,) for all heads, (heads, D), or None for ones
+        q_weight, k_weight  (D,) for all heads, (heads, D), or None for ones; (heads, D) with a gradient: (Hq + Hk) * D at
+                  most 24576
         position  (B, N) or (B, N, axes): places in a sequence (int32 / int64) or coordinates (float32 / float64)
         freq      (axes, pairs) float32 / float64, 2 * axes * pairs <= D: pair axis * pairs + f turns by
                   position[axis] * freq[axis, f], an angle formed in 64 bits
@@ -214,6 +215,9 @@ def norm_rotate(q, k, q_weight, k_weight, position, freq, eps=1e-6, interleaved=
         raise RuntimeError("norm_rotate: %d pairs need more than %d channels" % (freq.numel(), d))
     args = (q, k, wq, wk, position, freq.contiguous(), float(eps), int(bool(interleaved)))
     grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4])
+    if grad and any(w is not None and w.dim() == 2 and w.requires_grad for w in (wq, wk)) \
+            and (hq + (0 if k is None else k.size(2))) * d > 24576:
+        raise RuntimeError("norm_rotate: the gradient of weights for every head needs heads * D of at most 24576")
     return _NormRotate.apply(*args) if grad else _norm_rotate_forward(*args)
 
 
@@ -274,7 +278,7 @@ def select_blocks(q, means, keys, count, n_arr=None, m_arr=None, causal=False):
         count   blocks a query and key head, 1 to 64
     :return
         (B, M, Hk, count) int32, ascending, -1 behind the found ones.  The best `count` of (sum of the group's query
-        rows) . mean, scored in 64 bits, equal ones to the lowest block; causal: the block of the query's own position
+        rows) . mean, scored in 64 bits, equal ones to the lowest block, a score that is not a number last; causal: the block of the query's own position
         always, the others among those before it.  Queries behind m_arr: all -1.  No gradient."""
     q = _rows(q.detach() if isinstance(q, torch.Tensor) else q, "q")
     b, m, hq, d = q.shape
