@@ -40,6 +40,7 @@ struct BaArgs {
     uint64_t *bits;                         // (b, hk, nb, mt): bit = query of the tile of 64 picked the block
     float *part;                            // split forward: (rows, splits, d + 4); dk / dv in parts: (parts, 2, 64, d)
     int32_t *picks, *first;                 // dk / dv in parts: queries that picked a block; first part of a block, and the end
+    uint32_t *unclean;                      // dk / dv: a value that is not finite came out somewhere
     int chunk;                              // queries of a part; 0: a workgroup per block
     int b, m, n, nb, mt, hq, hk, group, d, count, causal, splits, tiles, qt, cap;
     unsigned group_inverse;                 // ceil(2^32 / group): r / group = umulhi(r, it) for r * group < 2^32, group > 1
@@ -727,6 +728,10 @@ __device__ __forceinline__ float ba_pow2_inverse(float x)
     return e == 0 || e >= 253 ? 1.f : __uint_as_float((uint32_t)(254 - e) << 23);
 }
 
+// Where ds still passes 65504 (|do . v - do . o| beyond that times the largest |do|), the pass is run again, with a power
+// smaller by BA_LOW for the rows (keys) that it reached: that quotient is at most 2 * 128 channels * 65504.
+constexpr float BA_LOW = 1.f / 4096.f;
+
 template <typename T, int DP>
 __device__ __forceinline__ void ba_dq_block(const BaArgs &a, const BaRow &R, const typename hd_vec<T>::v8 *qf, const typename hd_vec<T>::v8 *gf,
                                             float lse, float delta, float up, const T *Ks, int k0, bool bit, hd_f4 *acc)
@@ -875,14 +880,21 @@ __global__ __launch_bounds__(BA_THREADS, (BaBwd<T, DP>::w)) void block_attn_dq_k
     hd_f4 acc[DP / 16];
     bool poison = false;
     ba_dq_pass<T, DP, false>(a, t, R, qf, gf, lse, delta, up, smem, mask, list, count, &odd, acc, poison);
-    bool finite = true;
+    auto unclean = [&]() __attribute__((always_inline)) {       // this lane's row
+        bool finite = true;
 #pragma unroll
-    for (int d = 0; d < DP / 16; ++d)
+        for (int d = 0; d < DP / 16; ++d)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            finite &= ba_finite(acc[d][r]);
-    if (__syncthreads_or(!finite))
+            for (int r = 0; r < 4; ++r)
+                finite &= ba_finite(acc[d][r]);
+        return ba_col_max(finite || poison ? 0.f : 1.f) > 0.f;
+    };
+    bool bad = unclean();
+    for (int pass = 0; __syncthreads_or(bad) && pass < (HALF ? 2 : 1); ++pass) {
+        up *= pass && bad ? BA_LOW : 1.f;
         ba_dq_pass<T, DP, true>(a, t, R, qf, gf, lse, delta, up, smem, mask, list, count, &odd, acc, poison);
+        bad = unclean();
+    }
     if (!R.there)
         return;
     T *O = (T *)a.out + R.out(a, t.b);
@@ -902,6 +914,8 @@ __global__ __launch_bounds__(BA_THREADS) void block_pick_bits_kernel(BaArgs a)
     const int tile = (int)(blockIdx.x % a.mt), bh = (int)(blockIdx.x / a.mt), h = bh % a.hk, b = bh / a.hk;
     const int live = a.n_arr ? min(max(a.n_arr[b], 0), a.n) : a.n, lm = a.m_arr ? min(max(a.m_arr[b], 0), a.m) : a.m;
     const int i0 = tile * 64, entries = min(64, a.m - i0) * a.count;
+    if (blockIdx.x == 0 && threadIdx.x == 0)
+        *a.unclean = 0;                     // (for the kernels behind this one)
     const int32_t *idx = a.blocks + (((int64_t)b * a.m + i0) * a.hk + h) * a.count;
     for (int b0 = 0; b0 < a.nb; b0 += BP_WORDS) {
         const int words = min(BP_WORDS, a.nb - b0);
@@ -967,59 +981,41 @@ __global__ __launch_bounds__(1024) void block_parts_kernel(BaArgs a, int blocks)
 // out with a key per lane: the B operand of dv^T = do^T P and dk^T = q^T dS.
 constexpr int BD_WORDS = 64;                // tiles of queries looked through at a time
 
-template <typename T, int DP>
-__global__ __launch_bounds__(BA_THREADS, (BaBwd<T, DP>::kw)) void block_attn_dkv_kernel(BaArgs a, int64_t all)
+// What a workgroup of the dk / dv kernel has: its block, its part of the queries that picked it, in order
+struct BaKeys {
+    int b, h, live, lm, key;                // key: this lane's
+    int skip, take;
+    const uint64_t *bits;
+};
+
+// CAREFUL: values of q and do that are not finite stay out of the products, and the keys that a row with such a value sees are
+// not numbers (poison); low: 1 or BA_LOW.  A kernel of its own, which ends at once where the first has left only finite values
+// (within the first kernel its registers spill: 388 for 357 us on a sequence of 8192).
+template <typename T, int DP, bool CAREFUL>
+__device__ __forceinline__ void ba_dkv_pass(const BaArgs &a, const BaKeys &w, const typename hd_vec<T>::v8 *kf, const typename hd_vec<T>::v8 *vf,
+                                            char *smem, int *list_all, unsigned long long *odd, float low,
+                                            hd_f4 *dk, hd_f4 *dv, float &up, bool &poison)
 {
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    __shared__ int list_all;
     typedef BaLds<T, DP> L;
     typedef typename hd_vec<T>::v8 V8;
     constexpr bool HALF = __is_same(T, _Float16);
     T *Qs = (T *)smem, *Gs = (T *)(smem + L::TILE);
     float *lse_s = (float *)(smem + 2 * L::TILE), *delta_s = lse_s + 64, *gmax_s = delta_s + 64;
     int *limit_s = (int *)(gmax_s + 64), *list = limit_s + 64;              // list: BD_WORDS * 64 queries
-
-    int64_t id = ba_xcd(blockIdx.x, all), part = 0;
-    int skip = 0, take = 0x7FFFFFFF, parts = 1;                 // of the queries that picked the block, in order
-    if (a.chunk) {
-        const int blocks = a.b * a.hk * a.nb;
-        part = id;
-        if (part >= a.first[blocks])
-            return;
-        int lo = 0, hi = blocks - 1;        // the last block whose first part is not behind this one
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) / 2;
-            if (a.first[mid] <= part)
-                lo = mid;
-            else
-                hi = mid - 1;
-        }
-        id = lo;
-        parts = a.first[lo + 1] - a.first[lo];
-        skip = (int)(part - a.first[lo]) * a.chunk;
-        take = a.chunk;
-    }
-    const int blk = (int)(id % a.nb), bh = (int)(id / a.nb), h = bh % a.hk, b = bh / a.hk;
-    const int live = a.n_arr ? min(max(a.n_arr[b], 0), a.n) : a.n, lm = a.m_arr ? min(max(a.m_arr[b], 0), a.m) : a.m;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
-    const int key = blk * BA_BLOCK + wave * 16 + l15;
-    V8 kf[DP / 32], vf[DP / 32];
-    hd_f4 dk[DP / 16], dv[DP / 16];
-    ba_row_operand<T, DP>((const T *)a.k.data + b * a.k.sb + (int64_t)key * a.k.sr + h * a.k.sh, key < live, a.d, kf);
-    ba_row_operand<T, DP>((const T *)a.v.data + b * a.v.sb + (int64_t)key * a.v.sr + h * a.v.sh, key < live, a.d, vf);
+    int skip = w.skip, take = w.take;
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d)
         dk[d] = dv[d] = hd_f4{0.f, 0.f, 0.f, 0.f};
-    float up = 1.f;                         // fp16: dk is accumulated times this power of two
+    up = 1.f;                               // fp16: dk is accumulated times this power of two
     bool first = true;
-    const uint64_t *bits = a.bits + ((int64_t)bh * a.nb + blk) * a.mt;
 
     typedef BaStage<T, DP> S;
-    V8 qr[S::PER], gr[S::PER];
+    S qr, gr;
     float row_lse = 0.f, row_delta = 0.f, row_gmax = 0.f;
     int row_limit = 0;
-    const T *Q = S::lane((const T *)a.q.data + b * a.q.sb + (int64_t)h * a.group * a.q.sh, a.d);
-    const T *G = S::lane((const T *)a.go.data + b * a.go.sb + (int64_t)h * a.group * a.go.sh, a.d);
+    const T *Q = S::lane((const T *)a.q.data + w.b * a.q.sb + (int64_t)w.h * a.group * a.q.sh, a.d);
+    const T *G = S::lane((const T *)a.go.data + w.b * a.go.sb + (int64_t)w.h * a.group * a.go.sh, a.d);
     // rows r0 .. r0 + 63 of the list (query by query, all heads of the group) to registers; rows behind the last are its
     // copies that see nothing
     auto fetch = [&](int r0, int rows) __attribute__((always_inline)) {
@@ -1028,15 +1024,15 @@ __global__ __launch_bounds__(BA_THREADS, (BaBwd<T, DP>::kw)) void block_attn_dkv
             const int r = min(r0 + S::row(x), rows - 1);
             const int q = a.group == 1 ? r : (int)__umulhi((unsigned)r, a.group_inverse), e = r - q * a.group;
             const int64_t i = list[q];
-            qr[x] = *(const V8 *)(Q + i * a.q.sr + e * a.q.sh);
-            gr[x] = *(const V8 *)(G + i * a.go.sr + e * a.go.sh);
+            qr.r[x] = *(const V8 *)(Q + i * a.q.sr + e * a.q.sh);
+            gr.r[x] = *(const V8 *)(G + i * a.go.sr + e * a.go.sh);
         }
         row_lse = row_delta = row_gmax = 0.f;
         row_limit = 0;
         if (threadIdx.x < BA_ROWS && r0 + (int)threadIdx.x < rows) {
-            const int r = r0 + threadIdx.x, q = r / a.group, head = h * a.group + (r - q * a.group), i = list[q];
-            const int64_t p = ((int64_t)b * a.hq + head) * a.m + i;
-            row_lse = a.lse[p], row_delta = a.delta[p], row_limit = ba_limit(a, live, lm, i);
+            const int r = r0 + threadIdx.x, q = r / a.group, head = w.h * a.group + (r - q * a.group), i = list[q];
+            const int64_t p = ((int64_t)w.b * a.hq + head) * a.m + i;
+            row_lse = a.lse[p], row_delta = a.delta[p], row_limit = ba_limit(a, w.live, w.lm, i);
             if (HALF)
                 row_gmax = a.gmax[p];
         }
@@ -1045,7 +1041,7 @@ __global__ __launch_bounds__(BA_THREADS, (BaBwd<T, DP>::kw)) void block_attn_dkv
     for (int w0 = 0; w0 < a.mt && take > 0; w0 += BD_WORDS) {
         // the queries of the next 64 tiles that picked this block, in order; `skip` of them are other parts', `take` are ours
         if (wave == 0) {
-            uint64_t word = w0 + lane < a.mt ? bits[w0 + lane] : 0ull;
+            uint64_t word = w0 + lane < a.mt ? w.bits[w0 + lane] : 0ull;
             int inc = __popcll(word), at = -inc;
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
@@ -1054,23 +1050,28 @@ __global__ __launch_bounds__(BA_THREADS, (BaBwd<T, DP>::kw)) void block_attn_dkv
             }
             at += inc - skip;
             if (lane == 63)
-                list_all = inc;
+                *list_all = inc;
             for (; word; word &= word - 1, ++at)
                 if (at >= 0 && at < take)
                     list[at] = (w0 + lane) * 64 + __ffsll((unsigned long long)word) - 1;
         }
         __syncthreads();
-        const int here = min(take, max(0, list_all - skip)), rows = here * a.group;
-        skip = max(0, skip - list_all);
+        const int here = min(take, max(0, *list_all - skip)), rows = here * a.group;
+        skip = max(0, skip - *list_all);
         take -= here;
         if (rows > 0)
             fetch(0, rows);
         for (int r0 = 0; r0 < rows; r0 += BA_ROWS) {
             __syncthreads();                // the previous tile has been read
-#pragma unroll
-            for (int x = 0; x < S::PER; ++x) {
-                L::put8(Qs, S::row(x), S::part(x), qr[x]);
-                L::put8(Gs, S::row(x), S::part(x), gr[x]);
+            if constexpr (CAREFUL) {
+                if (threadIdx.x == 0)
+                    *odd = 0;
+                __syncthreads();
+                qr.store_finite(Qs, odd);
+                gr.store_finite(Gs, odd);
+            } else {
+                qr.store(Qs);
+                gr.store(Gs);
             }
             if (threadIdx.x < BA_ROWS) {
                 lse_s[threadIdx.x] = row_lse, delta_s[threadIdx.x] = row_delta, limit_s[threadIdx.x] = row_limit;
@@ -1080,13 +1081,16 @@ __global__ __launch_bounds__(BA_THREADS, (BaBwd<T, DP>::kw)) void block_attn_dkv
             __syncthreads();
             if (r0 + BA_ROWS < rows)
                 fetch(r0 + BA_ROWS, rows);
+            if constexpr (CAREFUL)
+                for (unsigned long long left = *odd; left; left &= left - 1)
+                    poison |= w.key < limit_s[__ffsll(left) - 1];
             if (HALF) {
                 // the largest |do| of the rows so far decides the power of two (every wave finds the same)
                 float m = gmax_s[lane];
 #pragma unroll
                 for (int o = 32; o > 0; o >>= 1)
                     m = fmaxf(m, __shfl_xor(m, o, 64));
-                const float want = ba_pow2_inverse(m);
+                const float want = ba_pow2_inverse(m) * low;
                 if (m > 0.f && (first || want < up)) {
                     if (!first)
 #pragma unroll
@@ -1120,7 +1124,7 @@ __global__ __launch_bounds__(BA_THREADS, (BaBwd<T, DP>::kw)) void block_attn_dkv
                     }
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const bool see = key < lim[r];
+                        const bool see = w.key < lim[r];
                         const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.scale2, -le[r]));
                         const float f = e * (dp[r] - de[r]);
                         p[x][r] = see ? e : 0.f;
@@ -1147,6 +1151,73 @@ __global__ __launch_bounds__(BA_THREADS, (BaBwd<T, DP>::kw)) void block_attn_dkv
             }
         }
         __syncthreads();                    // the list is rebuilt
+    }
+}
+
+template <typename T, int DP, bool CAREFUL>
+__global__ __launch_bounds__(BA_THREADS, (BaBwd<T, DP>::kw)) void block_attn_dkv_kernel(BaArgs a, int64_t all)
+{
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    __shared__ int list_all;
+    __shared__ unsigned long long odd;
+    typedef typename hd_vec<T>::v8 V8;
+    constexpr bool HALF = __is_same(T, _Float16);
+    if (CAREFUL && !*a.unclean)
+        return;
+    int64_t id = ba_xcd(blockIdx.x, all), part = 0;
+    int skip = 0, take = 0x7FFFFFFF, parts = 1;                 // of the queries that picked the block, in order
+    if (a.chunk) {
+        const int blocks = a.b * a.hk * a.nb;
+        part = id;
+        if (part >= a.first[blocks])
+            return;
+        int lo = 0, hi = blocks - 1;        // the last block whose first part is not behind this one
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (a.first[mid] <= part)
+                lo = mid;
+            else
+                hi = mid - 1;
+        }
+        id = lo;
+        parts = a.first[lo + 1] - a.first[lo];
+        skip = (int)(part - a.first[lo]) * a.chunk;
+        take = a.chunk;
+    }
+    const int blk = (int)(id % a.nb), bh = (int)(id / a.nb), h = bh % a.hk, b = bh / a.hk;
+    const int live = a.n_arr ? min(max(a.n_arr[b], 0), a.n) : a.n, lm = a.m_arr ? min(max(a.m_arr[b], 0), a.m) : a.m;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
+    const int key = blk * BA_BLOCK + wave * 16 + l15;
+    V8 kf[DP / 32], vf[DP / 32];
+    ba_row_operand<T, DP>((const T *)a.k.data + b * a.k.sb + (int64_t)key * a.k.sr + h * a.k.sh, key < live, a.d, kf);
+    ba_row_operand<T, DP>((const T *)a.v.data + b * a.v.sb + (int64_t)key * a.v.sr + h * a.v.sh, key < live, a.d, vf);
+    hd_f4 dk[DP / 16], dv[DP / 16];
+    const BaKeys w = {b, h, live, lm, key, skip, take, a.bits + ((int64_t)bh * a.nb + blk) * a.mt};
+    float up;
+    bool poison = false;
+    auto reached = [&]() __attribute__((always_inline)) {       // this lane's key holds what is not finite
+        bool finite = true;
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                finite &= ba_finite(dk[d][r]) && ba_finite(dv[d][r]);
+        return ba_col_max(finite || poison ? 0.f : 1.f) > 0.f;
+    };
+    ba_dkv_pass<T, DP, CAREFUL>(a, w, kf, vf, smem, &list_all, &odd, 1.f, dk, dv, up, poison);
+    if constexpr (CAREFUL) {
+        poison = ba_col_max(poison ? 1.f : 0.f) > 0.f;
+        const bool bad = HALF && reached();
+        if (HALF && __syncthreads_or(bad)) {
+            ba_dkv_pass<T, DP, true>(a, w, kf, vf, smem, &list_all, &odd, bad ? BA_LOW : 1.f, dk, dv, up, poison);
+            poison = ba_col_max(poison ? 1.f : 0.f) > 0.f;
+        }
+        if (poison)
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d)
+                dk[d] = dv[d] = hd_f4{NAN, NAN, NAN, NAN};
+    } else if (reached()) {
+        atomicOr(a.unclean, 1u);
     }
     const float back = HALF ? a.scale / up : a.scale;
     if (parts > 1) {                        // joined by block_attn_dkv_join_kernel
@@ -1294,7 +1365,9 @@ template <typename T, int DP> int ba_backward(BaArgs a, void *dq, void *dk, void
         return tpu3_launch_status();
     hipLaunchKernelGGL(block_pick_bits_kernel, dim3((unsigned)(a.b * a.hk * a.mt)), dim3(BA_THREADS), 0, s, a);
     const size_t lds2 = 2 * BaLds<T, DP>::TILE + 4 * 64 * 4 + (size_t)BD_WORDS * 64 * 4;
-    rc = ba_allow(block_attn_dkv_kernel<T, DP>, lds2);
+    rc = ba_allow(block_attn_dkv_kernel<T, DP, false>, lds2);
+    if (!rc)
+        rc = ba_allow(block_attn_dkv_kernel<T, DP, true>, lds2);
     if (rc)
         return rc;
     a.out = dk, a.out2 = dv;
@@ -1304,7 +1377,8 @@ template <typename T, int DP> int ba_backward(BaArgs a, void *dq, void *dk, void
         hipLaunchKernelGGL(block_picks_kernel, dim3((unsigned)blocks), dim3(BA_THREADS), 0, s, a);
         hipLaunchKernelGGL(block_parts_kernel, dim3(1), dim3(1024), 0, s, a, (int)blocks);
     }
-    hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP>), dim3((unsigned)all2), dim3(BA_THREADS), lds2, s, a, all2);
+    hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP, false>), dim3((unsigned)all2), dim3(BA_THREADS), lds2, s, a, all2);
+    hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP, true>), dim3((unsigned)all2), dim3(BA_THREADS), lds2, s, a, all2);
     if (a.chunk)
         hipLaunchKernelGGL((block_attn_dkv_join_kernel<T, DP>), dim3((unsigned)(blocks * BJ_SLICES)), dim3(BA_THREADS), 0, s, a);
     return tpu3_launch_status();
@@ -1352,9 +1426,9 @@ extern "C" int tpu3_block_attn_fwd(tpu3_stream_t stream, int type, int b, int m,
 }
 
 namespace {
-// the pieces of the backward workspace: bits, delta, gmax, picks, first, part
+// the pieces of the backward workspace: bits, delta, gmax, unclean, picks, first, part
 struct BaBwdLayout {
-    size_t delta, gmax, picks, first, part, bytes;
+    size_t delta, gmax, unclean, picks, first, part, bytes;
 };
 BaBwdLayout ba_bwd_layout(int b, int m, int n, int hq, int hk, int d, int count)
 {
@@ -1364,7 +1438,8 @@ BaBwdLayout ba_bwd_layout(int b, int m, int n, int hq, int hk, int d, int count)
     BaBwdLayout l;
     l.delta = up(blocks * mt * 8);
     l.gmax = l.delta + up((size_t)b * hq * m * 4);
-    l.picks = l.gmax + up((size_t)b * hq * m * 4);
+    l.unclean = l.gmax + up((size_t)b * hq * m * 4);
+    l.picks = l.unclean + 16;
     l.first = l.picks + (parts ? up(blocks * 4) : 0);
     l.part = l.first + (parts ? up((blocks + 1) * 4) : 0);
     l.bytes = l.part + (parts ? (size_t)ba_dkv_parts(b, m, hk, (int)nb, count) * 2 * BA_BLOCK * ba_dp(d) * 4 : 0);
@@ -1399,6 +1474,7 @@ extern "C" int tpu3_block_attn_bwd(tpu3_stream_t stream, int type, int b, int m,
     a.bits = (uint64_t *)workspace;
     a.delta = (float *)((char *)workspace + l.delta);
     a.gmax = (float *)((char *)workspace + l.gmax);
+    a.unclean = (uint32_t *)((char *)workspace + l.unclean);
     a.picks = (int32_t *)((char *)workspace + l.picks);
     a.first = (int32_t *)((char *)workspace + l.first);
     a.part = (float *)((char *)workspace + l.part);

@@ -43,6 +43,7 @@ NORM = [  # b, n, hq, hk, d, axes, pairs, weights, interleaved, position
     (1, 40, 2, 1, 200, 3, 33, "one", True, "f32"),
     (2, 2000, 7, 1, 64, 3, 10, "head", False, "f32"),
     (4, 1500, 2, 2, 64, 3, 10, "one", False, "f32"),
+    (1, 70, 127, 2, 128, 1, 64, "head", False, "i32"),
 ]
 
 
@@ -245,6 +246,27 @@ def test_select_blocks_ties_and_not_numbers(dev, m):
     assert torch.equal(ops.select_blocks(q, nan, n, 100 % 65)[..., :3], torch.arange(3, device=dev, dtype=torch.int32).expand(2, m, 1, 3))
 
 
+@pytest.mark.parametrize("kind", ["tiny queries", "tiny means", "heads that cancel", "far apart"])
+def test_select_blocks_at_the_ends_of_the_range(dev, kind):
+    """Squares that leave fp32's range, and heads whose sum is far smaller than they are: what the approximate scores are off
+    by must not be taken for less than it is."""
+    ops = pkg("network.operations")
+    gen = _gen(dev, 18)
+    q, mean = _randn(gen, 1, 600, 2, 40), _randn(gen, 1, 90, 1, 40)
+    if kind == "tiny queries":
+        q *= 1e-24
+    elif kind == "tiny means":
+        mean *= 1e-27
+    elif kind == "heads that cancel":
+        q[:, :, 1] = 1e-3 * q[:, :, 1] - 1e4 * q[:, :, 0]
+        q[:, :, 0] *= 1e4
+    else:
+        q[:, ::2] *= 1e15
+        mean[:, 1::3] *= 1e-18
+    got = ops.select_blocks(q, mean, 90 * 64, 6)
+    assert torch.equal(got.cpu(), orc64.select(q, mean, 90 * 64, 6))
+
+
 # ---- attention ---------------------------------------------------------------------------------------------------------
 ATTEND = [  # b, m, n, hq, hk, d, count, causal, ragged
     (1, 1, 1, 1, 1, 8, 1, False, False),
@@ -261,6 +283,9 @@ ATTEND = [  # b, m, n, hq, hk, d, count, causal, ragged
     (1, 70, 4300, 2, 2, 32, 64, False, False),
     (2, 1, 3000, 8, 2, 128, 16, True, True),
     (1, 1000, 300, 2, 2, 64, 2, False, False),
+    (1, 4500, 130, 1, 1, 8, 2, False, False),
+    (1, 4300, 200, 2, 1, 64, 3, True, False),
+    (2, 70, 4160, 8, 8, 32, 5, False, True),
 ]
 
 
@@ -421,6 +446,45 @@ def test_not_numbers_stay_where_they_are_seen(dev, dtype):
             assert not torch.isfinite(dq[0, sees_v]).all(dim=-1).any()
         if bad_k is not None:
             assert not torch.isfinite(dq[0, see[:, bad_k]]).all(dim=-1).any()
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_not_numbers_of_queries_reach_the_keys_they_see(dev, dtype):
+    """dk and dv: a query or an output gradient that is not finite reaches the keys that its query sees, not the later ones of
+    the same block under a causal mask."""
+    ops = pkg("network.operations")
+    q, k, v, go, _, _, _ = _attend_inputs(dev, (1, 128, 192, 2, 1, 64, 2, True, False), TYPES[dtype], 62)
+    blocks = torch.zeros((1, 128, 1, 2), dtype=torch.int32, device=dev)
+    blocks[:, ::2, :, 1] = 1
+    blocks[:, 1::2, :, 1] = 2
+    see = orc64.seen(1, 128, 192, 1, blocks, causal=True)[0, 0]
+    for which in (0, 1):
+        for i in (20, 101):
+            pair = [q.clone(), go.clone()]
+            pair[which][0, i, 1, 7] = math.nan
+            bad = [t.clone().requires_grad_() for t in (pair[0], k, v)]
+            _, dk, dv = torch.autograd.grad(ops.block_attention(*bad, blocks, causal=True), bad, pair[1])
+            pair[which][0, i, 1, 7] = 0
+            clean = [t.clone().requires_grad_() for t in (pair[0], k, v)]
+            _, dk2, dv2 = torch.autograd.grad(ops.block_attention(*clean, blocks, causal=True), clean, pair[1])
+            hit = see[i]
+            assert hit.any() and not hit.all() and not hit[(hit.nonzero().max() // 64 * 64):].all()
+            assert torch.equal(dk[0, ~hit], dk2[0, ~hit]) and torch.equal(dv[0, ~hit], dv2[0, ~hit])
+            assert dk[0, hit].isnan().any(dim=-1).all() and dv[0, hit].isnan().any(dim=-1).all()
+
+
+def test_score_gradients_beyond_half_precision(dev):
+    """fp16: do . v passes 65504 many times over although every input and every result is far below it."""
+    ops = pkg("network.operations")
+    q, k, v, go, blocks, _, _ = _attend_inputs(dev, (1, 150, 512, 2, 1, 128, 6, False, False), torch.float16, 33)
+    gen = _gen(dev, 34)
+    v = (8000 * torch.sign(_randn(gen, 1, 512, 1, 1)) + 100 * _randn(gen, 1, 512, 1, 128)).half()
+    go = (1e-3 * (1 + 0.1 * _randn(gen, *go.shape))).half()
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    o = ops.block_attention(*leaves, blocks, 0.01)
+    ref = orc64.attention(q, k, v, blocks, 0.01, go=go)
+    for nm, t in zip(("o", "dq", "dk", "dv"), (o,) + torch.autograd.grad(o, leaves, go)):
+        _within(t, ref[nm], ref["t_" + nm], nm)
 
 
 def test_keys_behind_2_to_the_31_elements(dev):
@@ -618,6 +682,8 @@ def test_refusals(dev):
         lambda: ops.norm_rotate(x, None, None, None, pos.detach(), ops.rotation_frequencies(1, 9, device=dev)),
         lambda: ops.norm_rotate(x, None, None, None, pos.detach(), ops.rotation_frequencies(2, 2, device=dev)),
         lambda: ops.norm_rotate(x, None, None, None, pos.detach(), freq, eps=-1.0),
+        lambda: ops.norm_rotate(torch.zeros((1, 4, 200, 128), device=dev), None, torch.ones((200, 128), device=dev, requires_grad=True),
+                                None, pos.detach(), freq),
     ]
     k = torch.zeros((1, 130, 1, 16), device=dev)
     blocks = torch.zeros((1, 4, 1, 2), dtype=torch.int32, device=dev)
