@@ -1291,7 +1291,10 @@ int ba_fill(BaArgs &a, int type, int b, int m, int n, int d, const tpu3_heads *q
     return 1;
 }
 
-// Splits of a tile's blocks: where the tiles alone do not fill the chip (four workgroups a compute unit).
+// Splits of a tile's blocks where the tiles alone do not fill the chip: up to four workgroups a compute unit, two for single
+// tokens (their blocks are few, and the join reads every split), and about one block a split.  Measured, us with / without:
+// 8 sequences, one token of 32 over 8 heads of 128 channels, 16 blocks: 15 / 25; the same for 8 tokens: 18 / 26; 312 tiles
+// of 32 queries whose picks differ (24 channels, 5 blocks each): 55 / 87.  From 512 tiles on it does not pay: 42 / 27.
 int ba_splits(int b, int m, int n, int hq, int hk, int count)
 {
     if (b <= 0 || m <= 0 || n <= 0 || hk <= 0 || hq < hk || count <= 0)
@@ -1299,22 +1302,30 @@ int ba_splits(int b, int m, int n, int hq, int hk, int count)
     const int qt = BA_ROWS / (hq / hk);
     if (qt < 1)
         return 1;
-    const int64_t tiles = (int64_t)b * hk * ((m - 1) / qt + 1);
-    const int64_t used = (int64_t)(m < qt ? m : qt) * count, nb = (n - 1) / BA_BLOCK + 1;
-    int64_t s = (m <= 16 ? 512 : 1024) / tiles, most = used < nb ? used : nb;
-    s = s < most ? s : most;
+    const int64_t tiles = (int64_t)b * hk * ((m - 1) / qt + 1), used = (int64_t)(m < qt ? m : qt) * count, nb = (n - 1) / BA_BLOCK + 1;
+    if (tiles >= 512)
+        return 1;
+    int64_t s = (m <= 16 ? 512 : 1024) / tiles;
+    s = s < used ? s : used;
+    s = s < nb ? s : nb;
+    s = s < 2 * count ? s : 2 * count;
     return s < 1 ? 1 : s > 64 ? 64 : (int)s;
 }
 
 // Queries of a part of the dk / dv pass where blocks are few (0: a workgroup per block), and the most parts there can be.
+// Measured, us for forward and backward with parts / a workgroup per block: 128 blocks (2048 queries, 8 heads over 2, 64
+// channels, 8 blocks each): 82 / 116, and 82 / 215 where all pick the first; 1024 blocks (8192 queries, 8 heads): 182 / 147,
+// and 186 / 256 where all pick the first, which is what the parts are for.  Where no block can have more than four parts, and
+// there are enough blocks for the chip, they only cost: 960 blocks (48 sequences of 312, 4 heads): 99 / 73.
 int ba_dkv_chunk(int b, int m, int hk, int nb, int count)
 {
     const int64_t blocks = (int64_t)b * hk * nb;
     if (blocks <= 0 || blocks > 1024)
         return 0;
     const int64_t picks = (int64_t)b * hk * m * (count < nb ? count : nb);
-    const int64_t c = (picks / 1024 + 63) / 64 * 64;
-    return (int)(c < 128 ? 128 : c);
+    int64_t c = (picks / 1024 + 63) / 64 * 64;
+    c = c < 128 ? 128 : c;
+    return blocks > 256 && m <= 4 * c ? 0 : (int)c;
 }
 int64_t ba_dkv_parts(int b, int m, int hk, int nb, int count)
 {

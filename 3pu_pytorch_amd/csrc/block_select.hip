@@ -595,7 +595,8 @@ __global__ __launch_bounds__(BS_THREADS) void block_select_many_kernel(BsArgs a,
     }
 }
 
-// Parts of the blocks: enough workgroups for the chip when there are few queries (a part holds 64 blocks at least).
+// Parts of the blocks: enough workgroups for the chip when there are few queries (a part holds 64 blocks at least; 64 queries
+// over 2048 blocks of 128 channels: 26 us, 170 in one part).
 int bs_splits(int b, int m, int hk, int nb, int count)
 {
     const int64_t rows = (int64_t)b * m * hk;
@@ -607,8 +608,11 @@ int bs_splits(int b, int m, int hk, int nb, int count)
     return s < 1 ? 1 : (int)s;
 }
 
-// A lane per query once there are enough of them.
-bool bs_many(int b, int m, int hk) { return m >= 16 && (int64_t)b * m * hk >= 512; }
+// A lane per query once there are enough of them to fill the chip with waves of 64: its time hardly depends on the number of
+// queries below that (64 channels, 80 blocks: 24 - 30 us), a workgroup per query costs more with each (10 us for 256 queries,
+// 12 for 2048, 22 for 4096, 36 for 8192, 43 for 10000).  More blocks lengthen the lane's chain: at 500 blocks 4096 queries take
+// 89 us against 45, 8192 take 90 against 81 (128 channels: 121 against 140) and 12000 take 90 against 116.
+bool bs_many(int b, int m, int hk, int nb) { return m >= 16 && (int64_t)b * m * hk >= (nb <= 128 ? 4096 : 8192); }
 
 template <typename T, int DP, bool LOQ> int bs_many_launch(const BsArgs &a, hipStream_t s)
 {
@@ -683,7 +687,7 @@ extern "C" size_t tpu3_block_select_workspace_bytes(int b, int m, int n, int hk,
 {
     if (b <= 0 || m <= 0 || n <= 0 || hk <= 0 || count <= 0 || count > BS_MAX)
         return 0;
-    if (bs_many(b, m, hk))
+    if (bs_many(b, m, hk, (n - 1) / BS_BLOCK + 1))
         return (size_t)b * hk * (((size_t)m + 63) / 64) * 8;
     const int splits = bs_splits(b, m, hk, (n - 1) / BS_BLOCK + 1, count);
     return splits == 1 ? 0 : (size_t)b * m * hk * splits * count * 12;
@@ -707,7 +711,7 @@ extern "C" int tpu3_block_select(tpu3_stream_t stream, int type, int b, int m, i
     a.count = count, a.causal = causal != 0;
     a.splits = a.nb ? bs_splits(b, m, hk, a.nb, count) : 1;
     const int64_t rows = (int64_t)b * m * hk;
-    const bool many = a.nb > 0 && bs_many(b, m, hk);
+    const bool many = a.nb > 0 && bs_many(b, m, hk, a.nb);
     if (many)
         a.splits = 1;
     if (rows * a.splits > 0x7FFFFFFFLL)

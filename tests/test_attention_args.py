@@ -92,7 +92,7 @@ SELECT = [
     (dict(type=-1), EINVAL), (dict(b=-1), EINVAL), (dict(m=-1), EINVAL), (dict(n=-1), EINVAL), (dict(d=0), EINVAL), (dict(hk=0), EINVAL),
     (dict(hk=3), EINVAL), (dict(count=0), EINVAL), (dict(count=65), ELIMIT), (dict(d=136), ELIMIT), (dict(n=2**31 - 1), ELIMIT),
     (dict(q=dict(data=0)), EINVAL), (dict(q=dict(sr=2)), EINVAL), (dict(means=0), EINVAL), (dict(means=8), EINVAL), (dict(blocks=0), EINVAL),
-    (dict(m=600), EINVAL), (dict(n=64 * 640), EINVAL), (dict(m=0), 0), (dict(b=0), 0),
+    (dict(m=5000), EINVAL), (dict(n=64 * 640), EINVAL), (dict(m=0), 0), (dict(b=0), 0),
 ]
 
 
