@@ -197,6 +197,11 @@ SELECT = [  # b, m, n, hq, hk, d, count, causal, ragged
     (1, 200, 4200, 2, 2, 64, 64, False, True),
     (1, 700, 5000, 4, 2, 64, 8, False, False),
     (2, 2100, 5000, 2, 1, 24, 13, True, True),
+    (9, 500, 300, 1, 1, 8, 3, False, False),
+    (1, 2100, 1500, 8, 2, 128, 16, True, False),
+    (1, 2200, 4200, 2, 2, 64, 64, False, True),
+    (3, 710, 2000, 6, 2, 40, 30, True, True),
+    (2, 1100, 9000, 4, 4, 96, 6, False, True),
 ]
 
 
@@ -220,7 +225,7 @@ def test_select_blocks(dev, case, dtype):
     assert got.dtype == torch.int32 and torch.equal(got.cpu(), want)
 
 
-@pytest.mark.parametrize("m", [1, 3, 400])
+@pytest.mark.parametrize("m", [1, 3, 400, 2200])
 def test_select_blocks_ties_and_not_numbers(dev, m):
     """Equal means, equal scores of opposite signs, zero queries: the lowest block wins; NaN ranks behind every number and
     infinities rank as such; means whose scores differ by less than an fp32 rounding keep their order."""
@@ -252,7 +257,7 @@ def test_select_blocks_at_the_ends_of_the_range(dev, kind):
     by must not be taken for less than it is."""
     ops = pkg("network.operations")
     gen = _gen(dev, 18)
-    q, mean = _randn(gen, 1, 600, 2, 40), _randn(gen, 1, 90, 1, 40)
+    q, mean = _randn(gen, 1, 4200, 2, 40), _randn(gen, 1, 90, 1, 40)
     if kind == "tiny queries":
         q *= 1e-24
     elif kind == "tiny means":
