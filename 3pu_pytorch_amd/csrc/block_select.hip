@@ -335,6 +335,7 @@ __global__ __launch_bounds__(BS_THREADS) void block_select_join_kernel(BsArgs a)
 // (rows of equal means) or a value is not finite is the query left open to block_select_open_kernel.
 constexpr int BT_MORE = 16;                 // places behind `count` for blocks near the edge
 constexpr int BT_NEAR = 1 << 30;            // marks them
+constexpr int BT_EXTRA = 4;                 // with numbers: places behind the k + 1st
 constexpr int BT_STRIDE = 20;               // floats between two queries' 16 scores in LDS
 
 struct BtSplit {
@@ -352,13 +353,14 @@ __device__ __forceinline__ BtSplit bt_split(const float *x)
     return r;
 }
 
-template <typename T, int DP, int NL, bool LOQ>
+template <typename T, int DP, int NL, bool LOQ, bool IDS>
 __global__ __launch_bounds__(BS_THREADS) void block_select_many_kernel(BsArgs a, int qtiles, int64_t waves)
 {
+    constexpr int EXTRA = IDS ? BT_EXTRA : 0;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
     float *sc = (float *)smem + wave * (64 * BT_STRIDE);
-    const int places = max(a.count, min(a.count + BT_MORE, 64));
+    const int places = IDS ? max(NL, a.count) : max(a.count, min(a.count + BT_MORE, 64));
     int *found = (int *)((float *)smem + 4 * 64 * BT_STRIDE) + wave * 64 * places;          // (places, 64)
     const int64_t w = (int64_t)blockIdx.x * 4 + wave;
     if (w >= waves)
@@ -483,10 +485,11 @@ __global__ __launch_bounds__(BS_THREADS) void block_select_many_kernel(BsArgs a,
         __builtin_amdgcn_wave_barrier();
     };
 
-    float best[NL];                         // descending; the first NL - 1 - k places are held by infinities
+    float best[NL];                         // descending; the first NL - 1 - EXTRA - k places are held by infinities
 #pragma unroll
     for (int j = 0; j < NL; ++j)
-        best[j] = j < NL - 1 - k ? INFINITY : -INFINITY;
+        best[j] = j < NL - 1 - EXTRA - k ? INFINITY : -INFINITY;
+    const uint32_t low = IDS ? 0xFFFFFFFFu >> __clz(a.nb | 1) : 0u;     // the bits of a block's number
     const bool everything = end <= k;
     if (__any(!everything)) {
         if (most > 0)
@@ -496,7 +499,10 @@ __global__ __launch_bounds__(BS_THREADS) void block_select_many_kernel(BsArgs a,
             scores(t0, true, x);
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                const float v = t0 + e < end ? x[e] : -INFINITY;
+                float v = x[e];
+                if constexpr (IDS)
+                    v = __uint_as_float((__float_as_uint(v) & ~low) | (uint32_t)(t0 + e));
+                v = t0 + e < end ? v : -INFINITY;
 #pragma unroll
                 for (int j = NL - 1; j > 0; --j)
                     best[j] = __builtin_amdgcn_fmed3f(best[j - 1], best[j], v);
@@ -509,16 +515,32 @@ __global__ __launch_bounds__(BS_THREADS) void block_select_many_kernel(BsArgs a,
         mn = fmaxf(mn, __shfl_xor(mn, o, 64));
     // 2 eps; the heads' fp32 sums: off by (group - 1) 2^-24 sum |q_h| <= (group - 1) 2^-24 sqrt(group sum |q_h|^2)
     const float heads = (float)(a.group - 1) * 2.384185791015625e-7f * sqrtf((float)a.group * qp);
-    const float eps2 = (2.44140625e-4f * sqrtf(qn) + heads) * sqrtf(mn);
+    // (a number in the score's lowest bits moves it by at most `low` 2^-23 of itself)
+    const float eps2 = ((2.44140625e-4f + 2.384185791015625e-7f * (float)low) * sqrtf(qn) + heads) * sqrtf(mn);
     // (squares near the smallest numbers of fp32 say nothing)
-    const bool bounded = !__any(odd) && qn > 1e-30f && mn > 1e-30f && eps2 < INFINITY;
-    const float kth = best[NL - 2], after = best[NL - 1];
+    const bool bounded = !__any(odd) && qn > 1e-30f && mn > 1e-30f && qn < 1e37f && mn < 1e37f;
+    const float kth = best[NL - 2 - EXTRA], after = best[NL - 1 - EXTRA];
     const bool plain = everything || k == 0 || (bounded && kth - after > eps2 && kth < INFINITY);
     // blocks above `in` are picked, those from `near` on may be
     const float in = everything ? -INFINITY : plain ? after : after + eps2, near = plain ? INFINITY : kth - eps2;
     bool open = !plain && (!bounded || !(fabsf(kth) < INFINITY) || !(fabsf(after) < INFINITY));
     int at = 0, certain = 0;
-    if (k > 0) {
+    if constexpr (IDS) {
+        // the list holds them; it holds all near ones if its end is not one of them
+        open |= !plain && best[NL - 1] >= near;
+#pragma unroll
+        for (int j = 0; j < NL; ++j) {
+            const bool sure = best[j] > in, here = best[j] < INFINITY && (sure || best[j] >= near) && !everything;
+            const int id = (int)(__float_as_uint(best[j]) & low);
+            if (here)
+                found[at * 64 + lane] = id + (sure ? 0 : BT_NEAR);
+            at += here;
+            certain += here && sure;
+        }
+        if (everything)
+            for (at = 0; at < end; ++at)
+                found[at * 64 + lane] = at;
+    } else if (k > 0) {
         if (most > 0)
             fetch(0);
         for (int t0 = 0; t0 < most; t0 += 16) {
@@ -565,11 +587,11 @@ __global__ __launch_bounds__(BS_THREADS) void block_select_many_kernel(BsArgs a,
                 v += __shfl_xor(v, o, 64);
             key = lane == e ? bs_key(v) : key;
         }
-        int rank = 0;                       // (the list ascends: equal scores to the lower block)
+        int rank = 0;
         for (unsigned long long u = near_ones; u; u &= u - 1) {
             const int e = __ffsll(u) - 1;
             const uint64_t other = __shfl((unsigned long long)key, e, 64);
-            rank += other > key || (other == key && e < lane) ? 1 : 0;
+            rank += other > key || (other == key && __shfl(mine, e, 64) < mine) ? 1 : 0;
         }
         const bool stays = lane < all && (!unsure || rank < want);
         const unsigned long long kept = __ballot(stays);
@@ -578,6 +600,23 @@ __global__ __launch_bounds__(BS_THREADS) void block_select_many_kernel(BsArgs a,
         at = lane == f ? __popcll(kept) : at;
     }
     at = min(at, k);                        // (open queries may hold more)
+    if constexpr (IDS) {                    // ascending
+        int id[NL - 1 - EXTRA];
+#pragma unroll
+        for (int j = 0; j < NL - 1 - EXTRA; ++j)
+            id[j] = j < at ? found[j * 64 + lane] & ~BT_NEAR : 0x7FFFFFFF;
+#pragma unroll
+        for (int x = 0; x < NL - 1 - EXTRA; ++x)
+#pragma unroll
+            for (int j = x & 1; j + 1 < NL - 1 - EXTRA; j += 2) {
+                const int lo = min(id[j], id[j + 1]), hi = max(id[j], id[j + 1]);
+                id[j] = lo, id[j + 1] = hi;
+            }
+#pragma unroll
+        for (int j = 0; j < NL - 1 - EXTRA; ++j)
+            if (j < at)
+                found[j * 64 + lane] = id[j];
+    }
     if (own >= 0)
         found[at++ * 64 + lane] = own;      // behind all others: they are earlier blocks
     for (; at < a.count; ++at)
@@ -618,27 +657,31 @@ template <typename T, int DP, bool LOQ> int bs_many_launch(const BsArgs &a, hipS
 {
     const int qtiles = (a.m + 63) / 64, k = a.count - a.causal;
     const int64_t waves = (int64_t)a.b * a.hk * qtiles;
-    const int places = a.count + BT_MORE < 64 ? a.count + BT_MORE : 64;
-    const size_t lds = (size_t)4 * 64 * (BT_STRIDE + (places > a.count ? places : a.count)) * 4;
+    size_t lds;
     const dim3 grid((unsigned)((waves + 3) / 4));
     hipError_t e = hipSuccess;
-#define BT_GO(NL)                                                                                                        \
+#define BT_GO(NL, IDS)                                                                                                   \
     {                                                                                                                    \
-        e = hipFuncSetAttribute((const void *)block_select_many_kernel<T, DP, NL, LOQ>,                                  \
+        const int places = IDS ? (NL > a.count ? NL : a.count) : a.count + BT_MORE < 64 ? a.count + BT_MORE : 64;        \
+        lds = (size_t)4 * 64 * (BT_STRIDE + (places > a.count ? places : a.count)) * 4;                                  \
+        e = hipFuncSetAttribute((const void *)block_select_many_kernel<T, DP, NL, LOQ, IDS>,                             \
                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);                                   \
         if (e == hipSuccess)                                                                                             \
-            hipLaunchKernelGGL((block_select_many_kernel<T, DP, NL, LOQ>), grid, dim3(BS_THREADS), lds, s, a, qtiles, waves); \
+            hipLaunchKernelGGL((block_select_many_kernel<T, DP, NL, LOQ, IDS>), grid, dim3(BS_THREADS), lds, s, a, qtiles, waves); \
     }
-    if (k < 5)
-        BT_GO(5)
-    else if (k < 9)
-        BT_GO(9)
-    else if (k < 17)
-        BT_GO(17)
-    else if (k < 33)
-        BT_GO(33)
+    const bool ids = a.nb <= 1024;
+    if (ids && k <= 4)
+        BT_GO(4 + 1 + BT_EXTRA, true)
+    else if (ids && k <= 8)
+        BT_GO(8 + 1 + BT_EXTRA, true)
+    else if (ids && k <= 16)
+        BT_GO(16 + 1 + BT_EXTRA, true)
+    else if (k <= 16)
+        BT_GO(17, false)
+    else if (k <= 32)
+        BT_GO(33, false)
     else
-        BT_GO(65)
+        BT_GO(65, false)
 #undef BT_GO
     if (e != hipSuccess)
         return (int)e;
