@@ -326,13 +326,17 @@ __global__ __launch_bounds__(BS_THREADS) void block_select_join_kernel(BsArgs a)
 // ---- selection for many queries ------------------------------------------------------------------------------------------
 // A lane per query, 64 queries of one key head a wave.  The scores come from the matrix cores, approximately, with a bound:
 // queries and means as two bf16 terms each (hi + lo, |x - hi - lo| <= 2^-18 |x|), three of the four partial products, fp32
-// sums: off by at most  eps = 2^-13 |q| max_b |mean_b|  (3 * 2^-18 for the terms left out, 3 d * 2^-24 = 2^-15.4 at d = 128
-// for the sums, doubled for sums that cut off instead of rounding).  Pass 1 keeps the k + 1 largest scores of every query, a
-// chain of v_med3 (one instruction an entry).  Where the k-th is more than 2 eps above the next, the order of the exact
-// scores around that place is known, and pass 2, which forms the same scores again, lists the blocks above it in ascending
-// order.  For the other queries (a few in a hundred) pass 2 also lists the blocks within 2 eps of the place, and the wave
-// forms their scores in 64 bits, one block at a time, to choose among them.  Only where these are too many for the list
-// (rows of equal means) or a value is not finite is the query left open to block_select_open_kernel.
+// sums: off by at most  eps = (3 * 2^-18 + 3 d 2^-23) |q| max_b |mean_b|  (the terms left out; every addition cut off at
+// 2^-23 of what it adds up).  bf16 queries of one head are their own first term: (2^-18 + 2 d 2^-23).  The kernel keeps the
+// k + 1 largest scores of every query, a chain of v_med3 (one instruction an entry).  Where the k-th is more than 2 eps above
+// the next, the order of the exact scores around that place is known.  For the other queries (a few in a hundred) the wave
+// forms the scores of the blocks within 2 eps of the place in 64 bits, one block at a time, to choose among them.  Only where
+// these are too many for the list (rows of equal means) or a value is not finite is the query left open to
+// block_select_open_kernel.
+// IDS, for up to 16 places among up to 1024 blocks: the block's number stands in the score's lowest bits, and the list holds
+// four places more, for near ones.  Otherwise a second pass forms the same scores again and lists what is above the place or
+// near it (8 clouds of 5000 points, 8 heads of 64 channels, 8 of 79 blocks: 60 us in two passes, 52 in one; 46 since the
+// bound counts the channels instead of standing at 2^-13).
 constexpr int BT_MORE = 16;                 // places behind `count` for blocks near the edge
 constexpr int BT_NEAR = 1 << 30;            // marks them
 constexpr int BT_EXTRA = 4;                 // with numbers: places behind the k + 1st
@@ -516,7 +520,8 @@ __global__ __launch_bounds__(BS_THREADS) void block_select_many_kernel(BsArgs a,
     // 2 eps; the heads' fp32 sums: off by (group - 1) 2^-24 sum |q_h| <= (group - 1) 2^-24 sqrt(group sum |q_h|^2)
     const float heads = (float)(a.group - 1) * 2.384185791015625e-7f * sqrtf((float)a.group * qp);
     // (a number in the score's lowest bits moves it by at most `low` 2^-23 of itself)
-    const float eps2 = ((2.44140625e-4f + 2.384185791015625e-7f * (float)low) * sqrtf(qn) + heads) * sqrtf(mn);
+    constexpr float OUT = (LOQ ? 3.f : 1.f) / 262144.f, ADD = (LOQ ? 3.f : 2.f) / 8388608.f;
+    const float eps2 = (2.f * (OUT + ADD * (float)a.d + (float)low / 8388608.f) * sqrtf(qn) + heads) * sqrtf(mn);
     // (squares near the smallest numbers of fp32 say nothing)
     const bool bounded = !__any(odd) && qn > 1e-30f && mn > 1e-30f && qn < 1e37f && mn < 1e37f;
     const float kth = best[NL - 2 - EXTRA], after = best[NL - 1 - EXTRA];

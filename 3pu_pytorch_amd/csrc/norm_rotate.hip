@@ -357,28 +357,37 @@ __global__ __launch_bounds__(NR_THREADS) void norm_rotate_bwd_kernel(NrArgs a, i
     }
 }
 
-// out[i] = sum over the workgroups' partial sums of column i, in 64 bits and in a fixed order
-__global__ __launch_bounds__(1024) void norm_rotate_wsum_kernel(int wgs, int cols, int first, int count, int w_type,
-                                                               const float *__restrict__ part, void *__restrict__ out)
+// Sums over the workgroups' partial sums of every column, in 64 bits and in a fixed order: the first nq columns to out0, the
+// others to out1 (either may be absent).  Bound by latency: a thread has eight loads in flight (13 us a set, one set at a time,
+// with one).
+constexpr int NW_COLS = 16, NW_PARTS = 64;
+__global__ __launch_bounds__(NW_COLS * NW_PARTS) void norm_rotate_wsum_kernel(int wgs, int cols, int nq, int w_type, const float *__restrict__ part,
+                                                                               void *__restrict__ out0, void *__restrict__ out1)
 {
-    __shared__ double s[32][33];
-    const int c = threadIdx.x & 31, g = threadIdx.x >> 5, i = blockIdx.x * 32 + c;
+    __shared__ double s[NW_PARTS][NW_COLS + 1];
+    const int c = threadIdx.x % NW_COLS, g = threadIdx.x / NW_COLS, i = blockIdx.x * NW_COLS + c;
     double v = 0.0;
-    if (i < count)
-        for (int r = g; r < wgs; r += 32)
-            v += (double)part[(int64_t)r * cols + first + i];
+    if (i < cols)
+#pragma unroll 8
+        for (int r = g; r < wgs; r += NW_PARTS)
+            v += (double)part[(int64_t)r * cols + i];
     s[g][c] = v;
     __syncthreads();
-    if (g == 0 && i < count) {
+    if (g == 0 && i < cols) {
         v = 0.0;
-        for (int r = 0; r < 32; ++r)
+#pragma unroll 8
+        for (int r = 0; r < NW_PARTS; ++r)
             v += s[r][c];
+        void *out = i < nq ? out0 : out1;
+        const int at = i < nq ? i : i - nq;
+        if (!out)
+            return;
         if (w_type == TPU3_TYPE_F32)
-            ((float *)out)[i] = (float)v;
+            ((float *)out)[at] = (float)v;
         else if (w_type == TPU3_TYPE_F16)
-            ((_Float16 *)out)[i] = (_Float16)(float)v;
+            ((_Float16 *)out)[at] = (_Float16)(float)v;
         else
-            ((__bf16 *)out)[i] = (__bf16)(float)v;
+            ((__bf16 *)out)[at] = (__bf16)(float)v;
     }
 }
 
@@ -540,10 +549,8 @@ extern "C" int tpu3_norm_rotate_bwd(tpu3_stream_t stream, int type, int b, int n
     if (st || !want)
         return st;
     // columns of a partial row: per head, all query heads' weights then all key heads'; else one set each
-    const int cols = (per_head ? heads : 2) * d, nq = (per_head ? q->heads : 1) * d, nk = (per_head ? k->heads : 1) * d;
-    if (a.want_w[0])
-        hipLaunchKernelGGL(norm_rotate_wsum_kernel, dim3((nq + 31) / 32), dim3(1024), 0, s, p.wgs, cols, 0, nq, w_type, a.part, dwq);
-    if (a.want_w[1])
-        hipLaunchKernelGGL(norm_rotate_wsum_kernel, dim3((nk + 31) / 32), dim3(1024), 0, s, p.wgs, cols, nq, nk, w_type, a.part, dwk);
+    const int cols = (per_head ? heads : 2) * d, nq = (per_head ? q->heads : 1) * d;
+    hipLaunchKernelGGL(norm_rotate_wsum_kernel, dim3((cols + NW_COLS - 1) / NW_COLS), dim3(NW_COLS * NW_PARTS), 0, s, p.wgs, cols, nq, w_type,
+                       a.part, a.want_w[0] ? dwq : nullptr, a.want_w[1] ? dwk : nullptr);
     return tpu3_launch_status();
 }
