@@ -98,10 +98,10 @@ template <int LPR> __device__ __forceinline__ float nr_row_sum(float v)
 }
 
 // Exchange rows, for halves whose length is no multiple of eight: channel c of a row sits at (c % 8) * slots + c / 8, so that
-// the lanes of a wave, which hold channels 8 l .. 8 l + 7, meet different banks whatever the shift is; the first half is
-// stored a second time behind the second, and places behind that copy are zero (read by channels that do not turn, times
-// S = 0).
-__host__ __device__ __forceinline__ int nr_slots(int d, int pairs) { return (d + pairs + 7) / 8 + 1; }
+// the lanes of a wave, which hold channels 8 l .. 8 l + 7, meet different banks whatever the shift is.  Lanes write whole
+// groups of eight: what lies behind the second half is written over by the copy of the first, which is written after it, and
+// what a channel behind the pairs reads is not used.
+__host__ __device__ __forceinline__ int nr_slots(int d, int pairs) { return (d + pairs + 15) / 8 + 1; }
 __host__ __device__ __forceinline__ bool nr_exchanges(int pairs, int interleaved) { return !interleaved && pairs % 8 != 0; }
 
 // eight channels from c0 on turned; `row` is this row's exchange slice.  Whole rows run it (LPR lanes each).
@@ -120,24 +120,22 @@ template <int LPR> __device__ __forceinline__ void nr_turn(const NrArgs &a, cons
             o[i] = __shfl(y[i], from, LPR);
     } else {
         const int slots = nr_slots(a.d, P);
-        if (c0 < 2 * P) {
+        if (live)
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (c0 + i < 2 * P)
-                    row[i * slots + (c0 >> 3)] = y[i];
-        }
-        if (c0 < P) {
+                row[i * slots + (c0 >> 3)] = y[i];
+        if (c0 < P)
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (c0 + i < P)
-                    row[((2 * P + i) & 7) * slots + ((2 * P + c0 + i) >> 3)] = y[i];
-        }
+                row[((2 * P + i) & 7) * slots + ((2 * P + c0 + i) >> 3)] = y[i];
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();    // the row's lanes are in one wave, whose LDS accesses complete in order
         if (live)
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                o[i] = row[((P + i) & 7) * slots + ((P + c0 + i) >> 3)];
+            for (int i = 0; i < 8; ++i) {
+                const float x = row[((P + i) & 7) * slots + ((P + c0 + i) >> 3)];
+                o[i] = c0 + i < 2 * P ? x : 0.f;
+            }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
@@ -150,11 +148,6 @@ template <int LPR> __device__ __forceinline__ void nr_turn(const NrArgs &a, cons
         y[i] = __builtin_fmaf(o[i], i < 4 ? s_0[i & 3] : s_1[i & 3], y[i] * (i < 4 ? c_0[i & 3] : c_1[i & 3]));
 }
 
-__device__ __forceinline__ void nr_clear(float *ex, int all)
-{
-    for (int i = threadIdx.x; i < all; i += NR_THREADS)
-        ex[i] = 0.f;
-}
 // where the tokens' rows start in the (strided) inputs: at[t] of x[0], x[1], g[0], g[1] for n of them
 __device__ __forceinline__ void nr_places(const NrArgs &a, int64_t t0, int count, int n, int64_t *at)
 {
@@ -180,7 +173,6 @@ __global__ __launch_bounds__(NR_THREADS) void norm_rotate_kernel(NrArgs a)
     const int grp = threadIdx.x / LPR, c0 = (threadIdx.x % LPR) * 8;
     const bool live = c0 < a.d;
     const int cr = live ? c0 : 0;           // (idle lanes of a row work on channel 0's addresses and write nothing)
-    nr_clear(ex, GROUPS * len);
     nr_places(a, t0, count, 2, at);
     nr_turns(a, t0, count, 1.f, cs);
     __syncthreads();
@@ -250,7 +242,6 @@ __global__ __launch_bounds__(NR_THREADS) void norm_rotate_bwd_kernel(NrArgs a, i
     const int cr = live ? c0 : 0;
     const int part_tok = (a.tok + split - 1) / split;
     float ws[2][8] = {};
-    nr_clear(ex, GROUPS * len);
     if (want && per_head)
         for (int i = threadIdx.x; i < units * a.d; i += NR_THREADS)
             acc[i] = 0.f;
