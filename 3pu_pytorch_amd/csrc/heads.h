@@ -40,6 +40,21 @@ template <> __device__ __forceinline__ void hd_store8<float>(float *p, const flo
     *(hd_f4 *)(p + 4) = hd_f4{x[4], x[5], x[6], x[7]};
 }
 
+// the same, past the caches
+template <typename T> __device__ __forceinline__ void hd_stream8(T *p, const float *x)
+{
+    if constexpr (sizeof(T) == 4) {
+        __builtin_nontemporal_store(hd_f4{x[0], x[1], x[2], x[3]}, (hd_f4 *)p);
+        __builtin_nontemporal_store(hd_f4{x[4], x[5], x[6], x[7]}, (hd_f4 *)(p + 4));
+    } else {
+        typename hd_vec<T>::v8 v;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = (T)x[i];
+        __builtin_nontemporal_store(v, (typename hd_vec<T>::v8 *)p);
+    }
+}
+
 static inline int hd_type_size(int type) { return type == TPU3_TYPE_F32 ? 4 : 2; }
 static inline bool hd_type_ok(int type) { return type == TPU3_TYPE_F32 || type == TPU3_TYPE_F16 || type == TPU3_TYPE_BF16; }
 // a (b, rows, heads, d) argument: every row of d channels starts on 16 bytes

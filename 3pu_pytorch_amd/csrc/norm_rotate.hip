@@ -15,6 +15,9 @@
 // goes through LDS with its first half stored a second time behind the second, so that the partner of channel c is always
 // channel c + P (P pairs; lane exchanges where P is a multiple of eight).
 // The next row is requested before the current one is worked on (a wave otherwise has 1 KB in flight, and the chip 7 MB).
+// Results are stored past the caches, so that the inputs stay there for the backward pass: a cloud of 80000 points (8 + 8
+// heads of 64 channels, fp16) 92 -> 67 us where they do; rotation and attention over it together 343 -> 339, over 4 clouds of
+// 5000 78 -> 77, over 16 297 -> 310, over 32 579 -> 580.
 #include "heads.h"
 
 namespace {
@@ -214,7 +217,7 @@ __global__ __launch_bounds__(NR_THREADS) void norm_rotate_kernel(NrArgs a)
             y[j] = y[j] * inv * w[j];
         nr_turn<LPR>(a, cs + t * 2 * a.d, ex + grp * len, c0, live, y);
         if (live)
-            hd_store8((side ? Y1 : Y0) + (t * (side ? hk : hq) + h) * a.d, y);
+            hd_stream8((side ? Y1 : Y0) + (t * (side ? hk : hq) + h) * a.d, y);
         cur = next;
     }
 }
@@ -299,7 +302,7 @@ __global__ __launch_bounds__(NR_THREADS) void norm_rotate_bwd_kernel(NrArgs a, i
                 for (int j = 0; j < 8; ++j)
                     g[j] = inv * __builtin_fmaf(-x[j], dot, g[j]);
                 if (row)
-                    hd_store8(Y + t * heads * a.d, g);
+                    hd_stream8(Y + t * heads * a.d, g);
                 xc = xn, gc = gn;
             }
             if (!want)
