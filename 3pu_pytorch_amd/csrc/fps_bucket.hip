@@ -779,10 +779,9 @@ __global__ __launch_bounds__(NW * 64, ((R <= 7 && NW == 16) ? 8 : 4)) void rl_ma
         return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i));
     };
 
-    // One sample folded into the lane's R running distances.  (r6) The distance chain runs on PACKED fp32 -- two points per
-    // v_pk_add_f32 / v_pk_mul_f32 / v_pk_fma_f32, each half the IEEE operation of the scalar instruction (same bits):
-    // 3 R + R minima instead of 6 R + R instructions per sample and lane; the update is the phase in which the four waves
-    // of a SIMD queue for its VALU (docs/kernels/fps_register_resident_levels.md).
+    // One sample folded into the lane's R running distances, two points at a time.  (The pairs were meant for packed fp32
+    // instructions, 3 R + R minima instead of 6 R + R per sample and lane; the library is built without them, so they are
+    // scalar ones: same bits.  docs/kernels/fps_register_resident_levels.md)
     typedef float rl_f2 __attribute__((ext_vector_type(2)));
     auto fold_sample = [&](float qx, float qy, float qz) __attribute__((always_inline)) {
         const rl_f2 qx2 = {qx, qx}, qy2 = {qy, qy}, qz2 = {qz, qz};

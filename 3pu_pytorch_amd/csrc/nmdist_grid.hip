@@ -280,10 +280,9 @@ __device__ __forceinline__ float nmg_point_box(float x, float y, float z, const 
 // update of the eight runs only when some lane may take one of them.
 // (First version: the rows through SCALAR loads straight from memory -- zero vector traffic, but eight dependent
 // round trips per tile with nothing to hide them behind at 2.4 waves per SIMD: 7.6 us per tile, 671 us per 80 000^2.)
-// (r6b) PACKED: the wave's LDS slice holds the tile as candidate PAIRS -- eight words per pair: x0 x1 y0 y1 z0 z1 i0 i1 --
-// so that two ds_read_b128 deliver register pairs v_pk_add_f32 / v_pk_mul_f32 / v_pk_fma_f32 can take as they are: the
-// three subtractions and the mul / fma / fma of the reference's expression run on TWO candidates per instruction (each
-// half is the IEEE operation of the scalar instruction: same bits), 3 + 0.5 instructions per pair instead of 6.6.
+// (r6b) The wave's LDS slice holds the tile as candidate PAIRS -- eight words per pair: x0 x1 y0 y1 z0 z1 i0 i1 -- so that two
+// ds_read_b128 deliver two candidates.  (Meant for packed fp32 instructions, two candidates each; the library is built
+// without them, so the subtractions and the mul / fma / fma of the reference's expression are scalar: same bits.)
 typedef float nmg_f2 __attribute__((ext_vector_type(2)));
 typedef float nmg_f4 __attribute__((ext_vector_type(4)));
 

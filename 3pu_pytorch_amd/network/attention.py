@@ -14,8 +14,14 @@ heads shares a key head and its blocks).  n_arr / m_arr: int32 device tensors of
 in the ragged point-set calls.  causal: query i stands at key position n - m + i (live lengths) and sees the keys up to it.
 Rows near each other should hold points near each other (a space-filling order, a sequence): a block is then a neighbourhood.
 
-Device tensors only; everything runs on the current stream of the tensors' device and can be captured into a graph.  Results
-do not depend on the order in which workgroups run."""
+Device tensors only; everything runs on the current stream of the tensors' device and can be captured into a graph (a backward
+pass: torch.autograd.grad, or backward() while no eager graph of the same leaves is alive, which torch itself cannot capture).
+Results do not depend on the order in which workgroups run.
+
+A key, query, value or output gradient that is not finite reaches what its masks let it reach and nothing else; a gradient that
+it reaches is not a number as a whole row.  Scores, softmax statistics, sums and norms are held in 32 bits or more; the 16-bit
+types round probabilities and score gradients to their own type before the second matrix product (score gradients of dq in two
+terms), float32 rounds nothing.  Means of blocks and scores of blocks are formed in 64 bits."""
 import math
 
 import torch
