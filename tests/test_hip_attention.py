@@ -202,6 +202,8 @@ SELECT = [  # b, m, n, hq, hk, d, count, causal, ragged
     (1, 2200, 4200, 2, 2, 64, 64, False, True),
     (3, 710, 2000, 6, 2, 40, 30, True, True),
     (2, 1100, 9000, 4, 4, 96, 6, False, True),
+    (1, 4200, 4200, 1, 1, 16, 1, True, False),
+    (1, 8300, 66000, 1, 1, 32, 5, False, False),
 ]
 
 
@@ -270,6 +272,26 @@ def test_select_blocks_at_the_ends_of_the_range(dev, kind):
         mean[:, 1::3] *= 1e-18
     got = ops.select_blocks(q, mean, 90 * 64, 6)
     assert torch.equal(got.cpu(), orc64.select(q, mean, 90 * 64, 6))
+
+
+@pytest.mark.parametrize("m", [7, 4300])
+def test_select_blocks_zeros_and_queries_that_are_not_numbers(dev, m):
+    """Queries and means with one channel each: most scores are exactly 0, of either sign.  Rows of NaN and infinities: the
+    scores that are numbers first."""
+    ops = pkg("network.operations")
+    gen = _gen(dev, 28)
+    q, mean = torch.zeros((1, m, 1, 24), device=dev), torch.zeros((1, 70, 1, 24), device=dev)
+    q[0, torch.arange(m), 0, torch.randint(0, 24, (m,), device=dev, generator=gen)] = 1.0
+    mean[0, torch.arange(70), 0, torch.randint(0, 24, (70,), device=dev, generator=gen)] = torch.randn(70, device=dev, generator=gen)
+    mean[0, ::5] *= -1
+    q[0, 3] = math.nan
+    q[0, 5, 0, 1] = math.inf
+    if m > 100:
+        q[0, 70:90] = math.nan
+        q[0, 200:210] = 0
+    for count in (3, 20):
+        got = ops.select_blocks(q, mean, 70 * 64, count)
+        assert torch.equal(got.cpu(), orc64.select(q, mean, 70 * 64, count))
 
 
 # ---- attention ---------------------------------------------------------------------------------------------------------
@@ -606,16 +628,17 @@ def test_on_side_streams_at_once(dev):
             assert all(torch.equal(a, c) for a, c in zip(r, want[i] + (few[i],)))
 
 
-def test_captured_and_replayed(dev):
+@pytest.mark.parametrize("n", [200, 2100])
+def test_captured_and_replayed(dev, n):
     """norm_rotate, selection, attention and their gradients in one graph; replayed with other inputs and the program's own
     eager calls in between, two graphs of the same operators at once."""
     ops = pkg("network.operations")
     freq = ops.rotation_frequencies(1, 16, device=dev)
-    position = torch.arange(200, device=dev).expand(2, 200)
+    position = torch.arange(n, device=dev).expand(2, n)
 
     def make(seed):
         gen = _gen(dev, seed)
-        return [_randn(gen, 2, 200, h, 32, dtype=torch.float16) for h in (4, 2, 2)] + [1 + 0.1 * _randn(gen, 32), _randn(gen, 2, 200, 4, 32, dtype=torch.float16)]
+        return [_randn(gen, 2, n, h, 32, dtype=torch.float16) for h in (4, 2, 2)] + [1 + 0.1 * _randn(gen, 32), _randn(gen, 2, n, 4, 32, dtype=torch.float16)]
 
     def step(q, k, v, w, go):
         q, k, v, w = (t.detach().requires_grad_() for t in (q, k, v, w))
