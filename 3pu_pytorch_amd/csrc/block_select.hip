@@ -639,15 +639,17 @@ __global__ __launch_bounds__(BS_THREADS) void block_select_many_kernel(BsArgs a,
     }
 }
 
-// Parts of the blocks: enough workgroups for the chip when there are few queries (a part holds 64 blocks at least; 64 queries
-// over 2048 blocks of 128 channels: 26 us, 170 in one part).
+// Parts of the blocks where there are few queries.  Up to 256 blocks one workgroup is faster than parts and the launch that joins
+// them (64 channels, 80 blocks, 1 / 64 / 512 queries: 5.6 / 5.8 / 6.6 us for 8.8 / 9.3 / 11.6; 256 blocks: 6.8 / 7.1 / 8.3 for 8.8 /
+// 9.4 / 12.0); beyond, parts of 128 blocks up to four workgroups a compute unit, two for up to 64 queries (2048 blocks of 128
+// channels, 64 queries: 18 for 20; 256: 35 with four, 48 with two; 1000 blocks, 64: 11.5 for 15.3).
 int bs_splits(int b, int m, int hk, int nb, int count)
 {
     const int64_t rows = (int64_t)b * m * hk;
-    if (rows <= 0)
+    if (rows <= 0 || nb <= 256)
         return 1;
-    int64_t s = 1024 / rows;
-    s = s < (nb + 63) / 64 ? s : (nb + 63) / 64;
+    int64_t s = (rows <= 64 ? 512 : 1024) / rows;
+    s = s < (nb + 127) / 128 ? s : (nb + 127) / 128;
     s = s < BS_KEEP / count ? s : BS_KEEP / count;
     return s < 1 ? 1 : (int)s;
 }

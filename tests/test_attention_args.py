@@ -27,7 +27,8 @@ def test_workspace_sizes(abi):
     assert lib.tpu3_block_select_workspace_bytes(1, 5, 0, 1, 4) == 0
     assert lib.tpu3_block_select_workspace_bytes(1, 5, 100, 1, 65) == 0
     assert lib.tpu3_block_select_workspace_bytes(2, 4096, 4096, 8, 16) == 2 * 8 * 64 * 8         # a word a 64 queries
-    assert lib.tpu3_block_select_workspace_bytes(1, 1, 64 * 640, 1, 16) == 10 * 16 * 12          # ten parts of 64 blocks
+    assert lib.tpu3_block_select_workspace_bytes(1, 1, 64 * 256, 1, 16) == 0
+    assert lib.tpu3_block_select_workspace_bytes(1, 1, 64 * 640, 1, 16) == 5 * 16 * 12           # five parts of 128 blocks
     assert lib.tpu3_block_attn_fwd_workspace_bytes(4, 4096, 4096, 8, 8, 64, 16) == 0
     one = lib.tpu3_block_attn_fwd_workspace_bytes(1, 1, 4096, 8, 2, 128, 16)
     assert one > 0 and one % (8 * (128 + 4) * 4) == 0
