@@ -151,6 +151,16 @@ template <typename T> __device__ __forceinline__ typename hd_vec<T>::v8 ba_pack(
     return f;
 }
 
+// what rounding a and b to f took
+template <typename T> __device__ __forceinline__ typename hd_vec<T>::v8 ba_rest(const hd_f4 &a, const hd_f4 &b, const typename hd_vec<T>::v8 &f)
+{
+    hd_f4 r0, r1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        r0[i] = a[i] - (float)f[i], r1[i] = b[i] - (float)f[4 + i];
+    return ba_pack<T>(r0, r1);
+}
+
 template <typename T> __device__ __forceinline__ typename hd_vec<T>::v8 ba_ones()
 {
     typename hd_vec<T>::v8 f;
@@ -251,8 +261,8 @@ template <typename T, int DP> struct BaStage {
 // How a kernel is laid out over registers and LDS; w: waves a SIMD that the register allocation aims at.  More waves hide
 // more of the chain scores -> maximum -> exponentials -> product, until the operands no longer fit: measured on clouds
 // of 5000 points (64 channels) and a sequence of 8192 (128), us with 2 / 3 / 4 waves: forward - / 144 / 129 and
-// 310 / 279 / -, dq - / 94 / 99 and 341 / 520 / -, dk and dv - / 63 / 92 and 346 / 900 / -; fp32 of 24 channels,
-// forward, - / 59 / 49.  A wave has 16 rows (keys):
+// 310 / 279 / -, dq - / 94 / 99 and 341 / 520 / -, dk and dv - / 63 / 92 and 346 / 900 / - (both before their
+// second terms); fp32 of 24 channels, forward, - / 59 / 49.  A wave has 16 rows (keys):
 // with 32, every operand read from LDS feeds two matrix instructions, but half as many waves are there (188 for 146).
 // together: 16-row tiles whose row operands are read in one go; columns: 16-channel columns read in one go.
 template <typename T, int DP> struct BaFwd {
@@ -772,13 +782,7 @@ __device__ __forceinline__ void ba_dq_block(const BaArgs &a, const BaRow &R, con
     // alone: an error of twice the result's own rounding)
     kc.template run<sizeof(T) == 2>(
         Ks, acc, [&](int j) __attribute__((always_inline)) { return ba_pack<T>(s[2 * j], s[2 * j + 1]); },
-        [&](int j, const V8 &f) __attribute__((always_inline)) {
-            hd_f4 r0, r1;
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                r0[r] = s[2 * j][r] - (float)f[r], r1[r] = s[2 * j + 1][r] - (float)f[4 + r];
-            return ba_pack<T>(r0, r1);
-        });
+        [&](int j, const V8 &f) __attribute__((always_inline)) { return ba_rest<T>(s[2 * j], s[2 * j + 1], f); });
 }
 
 // As in the forward kernel, CAREFUL is the second pass of a workgroup in which a key that is not finite may have reached rows
@@ -1132,6 +1136,11 @@ __device__ __forceinline__ void ba_dkv_pass(const BaArgs &a, const BaKeys &w, co
                     }
                 }
                 const V8 pf = ba_pack<T>(p[0], p[1]), sf = ba_pack<T>(ds[0], ds[1]);
+                // 16-bit types: what their rounding took, as a second term (one term alone: gradients off by 1.4 - 1.6 times
+                // what the plain form in 32 bits and its last rounding are off; 72 -> 82 and 365 -> 400 us)
+                V8 pr, sr;
+                if constexpr (sizeof(T) == 2)
+                    pr = ba_rest<T>(p[0], p[1], pf), sr = ba_rest<T>(ds[0], ds[1], sf);
                 constexpr int TG = DP / 16 < 4 ? DP / 16 : 4;
 #pragma unroll
                 for (int d0 = 0; d0 < DP / 16; d0 += TG) {
@@ -1146,6 +1155,13 @@ __device__ __forceinline__ void ba_dkv_pass(const BaArgs &a, const BaKeys &w, co
                     for (int d = 0; d < TG; ++d) {
                         dv[d0 + d] = ba_mma<T>(gc[d], pf, dv[d0 + d]);
                         dk[d0 + d] = ba_mma<T>(qc[d], sf, dk[d0 + d]);
+                    }
+                    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                        for (int d = 0; d < TG; ++d) {
+                            dv[d0 + d] = ba_mma<T>(gc[d], pr, dv[d0 + d]);
+                            dk[d0 + d] = ba_mma<T>(qc[d], sr, dk[d0 + d]);
+                        }
                     }
                 }
             }
