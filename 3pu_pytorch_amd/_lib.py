@@ -127,9 +127,9 @@ SIGNATURES = {
     "tpu3_block_means": (_i, [_vp, _i, _i, _i, _i, _hp, _vp, _i, _vp]),
     "tpu3_block_select": (_i, [_vp, _i, _i, _i, _i, _i, _hp, _i, _vp, _vp, _vp, _i, _i, _vp, _vp, _sz]),
     "tpu3_block_select_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
-    "tpu3_block_attn_fwd": (_i, [_vp, _i, _i, _i, _i, _i, _hp, _hp, _hp, _vp, _i, _f, _vp, _vp, _i, _vp, _vp, _vp, _vp, _sz]),
+    "tpu3_block_attn_fwd": (_i, [_vp, _i, _i, _i, _i, _i, _hp, _hp, _hp, _vp, _i, ctypes.c_double, _vp, _vp, _i, _vp, _vp, _vp, _vp, _sz]),
     "tpu3_block_attn_fwd_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
-    "tpu3_block_attn_bwd": (_i, [_vp, _i, _i, _i, _i, _i, _hp, _hp, _hp, _hp, _hp, _vp, _i, _f, _vp, _vp, _i, _vp, _vp, _vp,
+    "tpu3_block_attn_bwd": (_i, [_vp, _i, _i, _i, _i, _i, _hp, _hp, _hp, _hp, _hp, _vp, _i, ctypes.c_double, _vp, _vp, _i, _vp, _vp, _vp,
                                  _vp, _vp, _vp, _sz]),
     "tpu3_block_attn_bwd_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
 }

@@ -44,7 +44,7 @@ struct BaArgs {
     int chunk;                              // queries of a part; 0: a workgroup per block
     int b, m, n, nb, mt, hq, hk, group, d, count, causal, splits, tiles, qt, cap;
     unsigned group_inverse;                 // ceil(2^32 / group): r / group = umulhi(r, it) for r * group < 2^32, group > 1
-    float scale, scale2;                    // scale2 = scale * log2(e)
+    float scale, scale2, scale2_rest;       // scale * log2(e) in two terms
 };
 
 typedef short ba_s4 __attribute__((ext_vector_type(4)));
@@ -65,6 +65,23 @@ template <> __device__ __forceinline__ hd_f4 ba_mma<float>(const hd_f8 &a, const
     for (int i = 0; i < 8; ++i)
         c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], c, 0, 0, 0);
     return c;
+}
+// The same for scores.  fp32: the 32 products in two sums of 16 of their own, so that only the last addition rounds at the
+// score's size: with one chain of D such roundings the output of 96 channels was off by twice the plain form's error (1.3e-6
+// against 6e-7; 4e-7 with these).
+template <typename T> __device__ __forceinline__ hd_f4 ba_score_mma(const typename hd_vec<T>::v8 &a, const typename hd_vec<T>::v8 &b, hd_f4 c)
+{
+    if constexpr (sizeof(T) == 2) {
+        return ba_mma<T>(a, b, c);
+    } else {
+        hd_f4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], x, 0, 0, 0);
+            y = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[4 + i], b.v[4 + i], y, 0, 0, 0);
+        }
+        return c + (x + y);
+    }
 }
 
 template <typename T> __device__ __forceinline__ typename hd_vec<T>::v8 ba_zero()
@@ -448,7 +465,7 @@ __device__ __forceinline__ void ba_scores(const T *tile, const typename hd_vec<T
         for (int kk = 0; kk < DP / 32; ++kk)
 #pragma unroll
             for (int x = 0; x < TG; ++x)
-                s[x0 + x] = ba_mma<T>(kf[x][kk], f[kk], s[x0 + x]);
+                s[x0 + x] = ba_score_mma<T>(kf[x][kk], f[kk], s[x0 + x]);
     }
 }
 // acc[d] += (tile's columns) (f[0] for its first 32 rows, f[1] for the others): a group of columns is read while the matrix
@@ -498,6 +515,15 @@ template <typename T, int DP, int VG> struct BaColumns {
         }
     }
 };
+// 2^(scaled score - off).  The rounding of the scale moves all scores of a row alike, by as much as all of an fp32 result's other
+// roundings where scores reach 20 (96 channels): fp32 takes its second term too.
+template <typename T> __device__ __forceinline__ float ba_power(const BaArgs &a, float s, float off)
+{
+    float e = __builtin_fmaf(s, a.scale2, -off);
+    if constexpr (sizeof(T) == 4)
+        e = __builtin_fmaf(s, a.scale2_rest, e);
+    return __builtin_amdgcn_exp2f(e);
+}
 __device__ __forceinline__ bool ba_finite(float x) { return fabsf(x) <= 3.4028235e38f; }
 
 // one block of keys: Ks, with Vs behind it, in LDS; k0 = its first key; bit = this lane's row picked it
@@ -543,7 +569,7 @@ __device__ __forceinline__ void ba_fwd_block(const BaArgs &a, const BaRow &R, co
     auto weight = [&](int x) __attribute__((always_inline)) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            s[x][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][r], a.scale2, -off));
+            s[x][r] = ba_power<T>(a, s[x][r], off);
             if (CAREFUL)
                 s[x][r] = bit ? s[x][r] : 0.f;
         }
@@ -761,7 +787,7 @@ __device__ __forceinline__ void ba_dq_block(const BaArgs &a, const BaRow &R, con
     for (int x = 0; x < 4; ++x)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][r], a.scale2, -lse)) * (dp[x][r] - delta);
+            const float e = ba_power<T>(a, s[x][r], lse) * (dp[x][r] - delta);
             s[x][r] = HALF ? e * up : e;
         }
     if (__any(bit && k0 + BA_BLOCK > R.limit)) {
@@ -1123,13 +1149,13 @@ __device__ __forceinline__ void ba_dkv_pass(const BaArgs &a, const BaKeys &w, co
                     hd_f4 s = {0.f, 0.f, 0.f, 0.f}, dp = s;
 #pragma unroll
                     for (int kk = 0; kk < DP / 32; ++kk) {
-                        s = ba_mma<T>(qa[kk], kf[kk], s);
-                        dp = ba_mma<T>(ga[kk], vf[kk], dp);
+                        s = ba_score_mma<T>(qa[kk], kf[kk], s);
+                        dp = ba_score_mma<T>(ga[kk], vf[kk], dp);
                     }
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const bool see = w.key < lim[r];
-                        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.scale2, -le[r]));
+                        const float e = ba_power<T>(a, s[r], le[r]);
                         const float f = e * (dp[r] - de[r]);
                         p[x][r] = see ? e : 0.f;
                         ds[x][r] = see ? (HALF ? f * up : f) : 0.f;
@@ -1281,10 +1307,10 @@ template <typename T, int DP> __global__ __launch_bounds__(BA_THREADS) void bloc
 
 // ---- host --------------------------------------------------------------------------------------------------------------
 int ba_fill(BaArgs &a, int type, int b, int m, int n, int d, const tpu3_heads *q, const tpu3_heads *k, const tpu3_heads *v,
-            const int32_t *blocks, int count, float scale, const int32_t *n_arr, const int32_t *m_arr, int causal)
+            const int32_t *blocks, int count, double scale, const int32_t *n_arr, const int32_t *m_arr, int causal)
 {
     if (b < 0 || m < 0 || n < 0 || d <= 0 || !hd_type_ok(type) || !q || !k || !v || q->heads <= 0 || k->heads <= 0 ||
-        q->heads % k->heads || v->heads != k->heads || count <= 0 || !(scale > 0.f) || scale > 3e38f)
+        q->heads % k->heads || v->heads != k->heads || count <= 0 || !(scale >= 1e-30) || scale > 1e30)
         return TPU3_EINVAL;
     if (d % 8 || d > 128 || count > TPU3_BLOCK_COUNT_MAX || q->heads / k->heads > BA_ROWS ||
         (n > 0 && (n - 1) / BA_BLOCK + 1 > TPU3_ATTN_BLOCKS_MAX))
@@ -1292,7 +1318,10 @@ int ba_fill(BaArgs &a, int type, int b, int m, int n, int d, const tpu3_heads *q
     a.q = *q, a.k = *k, a.v = *v, a.blocks = blocks, a.n_arr = n_arr, a.m_arr = m_arr;
     a.b = b, a.m = m, a.n = n, a.nb = n > 0 ? (n - 1) / BA_BLOCK + 1 : 0, a.mt = (m + 63) / 64;
     a.hq = q->heads, a.hk = k->heads, a.group = a.hq / a.hk, a.d = d, a.count = count, a.causal = causal != 0;
-    a.scale = scale, a.scale2 = scale * 1.44269504088896340736f;
+    a.scale = (float)scale, a.scale2 = (float)(scale * 1.44269504088896340736);
+    if (type == TPU3_TYPE_F32 && (double)a.scale2 >= scale * 1.44269504088896340736)
+        a.scale2 = nextafterf(a.scale2, 0.f);                   // (the rest above 0: a masked score times it stays -infinity)
+    a.scale2_rest = (float)(scale * 1.44269504088896340736 - (double)a.scale2);
     a.group_inverse = a.group > 1 ? (unsigned)(((1ull << 32) + a.group - 1) / a.group) : 0u;
     a.qt = BA_ROWS / a.group;
     a.tiles = m > 0 ? (m - 1) / a.qt + 1 : 0;
@@ -1431,7 +1460,7 @@ extern "C" size_t tpu3_block_attn_fwd_workspace_bytes(int b, int m, int n, int h
 }
 
 extern "C" int tpu3_block_attn_fwd(tpu3_stream_t stream, int type, int b, int m, int n, int d, const tpu3_heads *q,
-                                   const tpu3_heads *k, const tpu3_heads *v, const int32_t *blocks, int count, float scale,
+                                   const tpu3_heads *k, const tpu3_heads *v, const int32_t *blocks, int count, double scale,
                                    const int32_t *n_arr, const int32_t *m_arr, int causal, void *out, float *lse,
                                    void *rest, void *workspace, size_t workspace_bytes)
 {
@@ -1483,7 +1512,7 @@ extern "C" size_t tpu3_block_attn_bwd_workspace_bytes(int b, int m, int n, int h
 
 extern "C" int tpu3_block_attn_bwd(tpu3_stream_t stream, int type, int b, int m, int n, int d, const tpu3_heads *q,
                                    const tpu3_heads *k, const tpu3_heads *v, const tpu3_heads *o, const tpu3_heads *go,
-                                   const int32_t *blocks, int count, float scale, const int32_t *n_arr, const int32_t *m_arr,
+                                   const int32_t *blocks, int count, double scale, const int32_t *n_arr, const int32_t *m_arr,
                                    int causal, const float *lse, const void *rest, void *dq, void *dk, void *dv,
                                    void *workspace, size_t workspace_bytes)
 {

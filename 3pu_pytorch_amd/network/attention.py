@@ -373,8 +373,8 @@ def _check_attention(q, k, v, scale, n_arr, m_arr):
         raise RuntimeError("D must be at most 128, got %d" % d)
     _keys(k.size(1))
     scale = d ** -0.5 if scale is None else float(scale)
-    if not (0.0 < scale < 1e30) or math.isinf(scale):
-        raise RuntimeError("scale must be positive and finite, got %s" % scale)
+    if not 1e-30 <= scale <= 1e30:
+        raise RuntimeError("scale must be 1e-30 to 1e30, got %s" % scale)
     return q, k, v, scale, _lengths(n_arr, "n_arr", b, q), _lengths(m_arr, "m_arr", b, q)
 
 

@@ -591,7 +591,7 @@ size_t tpu3_block_select_workspace_bytes(int b, int m, int n, int hk, int count)
  * (b, q->heads, m) f32, log2 of the denominator, and rest, like out, what the rounding of a 16-bit out took.
  * q->heads / k->heads <= 64, d <= 128; workspace = tpu3_block_attn_fwd_workspace_bytes bytes, 16-byte aligned (0: NULL). */
 int tpu3_block_attn_fwd(tpu3_stream_t stream, int type, int b, int m, int n, int d, const tpu3_heads *q, const tpu3_heads *k,
-                        const tpu3_heads *v, const int32_t *blocks, int count, float scale, const int32_t *n_arr,
+                        const tpu3_heads *v, const int32_t *blocks, int count, double scale, const int32_t *n_arr,
                         const int32_t *m_arr, int causal, void *out, float *lse, void *rest, void *workspace,
                         size_t workspace_bytes);
 size_t tpu3_block_attn_fwd_workspace_bytes(int b, int m, int n, int hq, int hk, int d, int count);
@@ -600,7 +600,7 @@ size_t tpu3_block_attn_fwd_workspace_bytes(int b, int m, int n, int hq, int hk, 
  * tpu3_block_attn_bwd_workspace_bytes bytes, 16-byte aligned. */
 int tpu3_block_attn_bwd(tpu3_stream_t stream, int type, int b, int m, int n, int d, const tpu3_heads *q, const tpu3_heads *k,
                         const tpu3_heads *v, const tpu3_heads *o, const tpu3_heads *go, const int32_t *blocks, int count,
-                        float scale, const int32_t *n_arr, const int32_t *m_arr, int causal, const float *lse,
+                        double scale, const int32_t *n_arr, const int32_t *m_arr, int causal, const float *lse,
                         const void *rest, void *dq, void *dk, void *dv, void *workspace, size_t workspace_bytes);
 size_t tpu3_block_attn_bwd_workspace_bytes(int b, int m, int n, int hq, int hk, int d, int count);
 
