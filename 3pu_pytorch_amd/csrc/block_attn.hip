@@ -32,7 +32,7 @@ struct BaArgs {
     tpu3_heads q, k, v, o, go;              // o, go: backward
     const int32_t *blocks;                  // (b, m, hk, count)
     const int32_t *n_arr, *m_arr;
-    void *out, *out2;                       // forward: o; dq pass: dq; dk / dv pass: dk, dv (contiguous)
+    void *out, *out2, *dq;                  // forward: o; backward: dk, dv, dq (contiguous)
     void *rest;                             // 16-bit types, contiguous like o: what the rounding of o took, for do . o
     float *lse;                             // (b, hq, m): log2 of the softmax denominator, scaled scores in base 2
     float *delta;                           // (b, hq, m): do . o
@@ -40,7 +40,7 @@ struct BaArgs {
     uint64_t *bits;                         // (b, hk, nb, mt): bit = query of the tile of 64 picked the block
     float *part;                            // split forward: (rows, splits, d + 4); dk / dv in parts: (parts, 2, 64, d)
     int32_t *picks, *first;                 // dk / dv in parts: queries that picked a block; first part of a block, and the end
-    uint32_t *unclean;                      // dk / dv: a value that is not finite came out somewhere
+    uint32_t *unclean;                      // backward: a value that is not finite came out somewhere
     int chunk;                              // queries of a part; 0: a workgroup per block
     int b, m, n, nb, mt, hq, hk, group, d, count, causal, splits, tiles, qt, cap;
     unsigned group_inverse;                 // ceil(2^32 / group): r / group = umulhi(r, it) for r * group < 2^32, group > 1
@@ -811,8 +811,8 @@ __device__ __forceinline__ void ba_dq_block(const BaArgs &a, const BaRow &R, con
         [&](int j, const V8 &f) __attribute__((always_inline)) { return ba_rest<T>(s[2 * j], s[2 * j + 1], f); });
 }
 
-// As in the forward kernel, CAREFUL is the second pass of a workgroup in which a key that is not finite may have reached rows
-// that do not see it; those that do are not numbers (poison).
+// As in the forward kernel, CAREFUL is for tiles in which a key that is not finite may have reached rows that do not see it;
+// those that do are not numbers (poison).
 template <typename T, int DP, bool CAREFUL>
 __device__ __forceinline__ void ba_dq_pass(const BaArgs &a, const BaTile &t, const BaRow &R, const typename hd_vec<T>::v8 *qf,
                                            const typename hd_vec<T>::v8 *gf, float lse, float delta, float up, char *smem,
@@ -860,18 +860,14 @@ __device__ __forceinline__ void ba_dq_pass(const BaArgs &a, const BaTile &t, con
     }
 }
 
-template <typename T, int DP>
-__global__ __launch_bounds__(BA_THREADS, (BaBwd<T, DP>::w)) void block_attn_dq_kernel(BaArgs a, int64_t all)
+template <typename T, int DP, bool CAREFUL> __device__ __forceinline__ void ba_dq_tile(const BaArgs &a, int64_t id, char *smem, unsigned long long *odd)
 {
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    __shared__ unsigned long long odd;
     typedef BaLds<T, DP> L;
     typedef typename hd_vec<T>::v8 V8;
     constexpr bool HALF = __is_same(T, _Float16);
     uint64_t *mask = (uint64_t *)(smem + 2 * L::TILE);
     uint32_t *list = (uint32_t *)(mask + a.cap), *words = list + a.cap, *before = words + (a.nb + 31) / 32;
 
-    const int64_t id = ba_xcd(blockIdx.x, all);
     const BaTile t = ba_tile(a, id);
     const int g = (threadIdx.x & 63) >> 4;
     const BaRow R(a, t);
@@ -909,8 +905,8 @@ __global__ __launch_bounds__(BA_THREADS, (BaBwd<T, DP>::w)) void block_attn_dq_k
     const int count = ba_union(a, t, list, mask, words, before);
     hd_f4 acc[DP / 16];
     bool poison = false;
-    ba_dq_pass<T, DP, false>(a, t, R, qf, gf, lse, delta, up, smem, mask, list, count, &odd, acc, poison);
-    auto unclean = [&]() __attribute__((always_inline)) {       // this lane's row
+    ba_dq_pass<T, DP, CAREFUL>(a, t, R, qf, gf, lse, delta, up, smem, mask, list, count, odd, acc, poison);
+    auto reached = [&]() __attribute__((always_inline)) {       // this lane's row holds what is not finite
         bool finite = true;
 #pragma unroll
         for (int d = 0; d < DP / 16; ++d)
@@ -919,20 +915,30 @@ __global__ __launch_bounds__(BA_THREADS, (BaBwd<T, DP>::w)) void block_attn_dq_k
                 finite &= ba_finite(acc[d][r]);
         return ba_col_max(finite || poison ? 0.f : 1.f) > 0.f;
     };
-    bool bad = unclean();
-    for (int pass = 0; __syncthreads_or(bad) && pass < (HALF ? 2 : 1); ++pass) {
-        up *= pass && bad ? BA_LOW : 1.f;
-        ba_dq_pass<T, DP, true>(a, t, R, qf, gf, lse, delta, up, smem, mask, list, count, &odd, acc, poison);
-        bad = unclean();
+    if constexpr (CAREFUL) {
+        const bool bad = HALF && reached();
+        if (HALF && __syncthreads_or(bad)) {
+            up *= bad ? BA_LOW : 1.f;
+            ba_dq_pass<T, DP, true>(a, t, R, qf, gf, lse, delta, up, smem, mask, list, count, odd, acc, poison);
+        }
+    } else if (reached()) {
+        atomicOr(a.unclean, 1u);
     }
     if (!R.there)
         return;
-    T *O = (T *)a.out + R.out(a, t.b);
+    T *O = (T *)a.dq + R.out(a, t.b);
     const float back = poison ? NAN : HALF ? a.scale / up : a.scale;
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d)
         if (d * 16 + g * 4 < a.d)
             ba_store4<T>(O + d * 16 + g * 4, acc[d] * back);
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(BA_THREADS, (BaBwd<T, DP>::w)) void block_attn_dq_kernel(BaArgs a, int64_t all)
+{
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    ba_dq_tile<T, DP, false>(a, ba_xcd(blockIdx.x, all), smem, nullptr);
 }
 
 // ---- backward: which queries picked a block ------------------------------------------------------------------------------
@@ -1019,8 +1025,7 @@ struct BaKeys {
 };
 
 // CAREFUL: values of q and do that are not finite stay out of the products, and the keys that a row with such a value sees are
-// not numbers (poison); low: 1 or BA_LOW.  A kernel of its own, which ends at once where the first has left only finite values
-// (within the first kernel its registers spill: 388 for 357 us on a sequence of 8192).
+// not numbers (poison); low: 1 or BA_LOW.
 template <typename T, int DP, bool CAREFUL>
 __device__ __forceinline__ void ba_dkv_pass(const BaArgs &a, const BaKeys &w, const typename hd_vec<T>::v8 *kf, const typename hd_vec<T>::v8 *vf,
                                             char *smem, int *list_all, unsigned long long *odd, float low,
@@ -1197,16 +1202,11 @@ __device__ __forceinline__ void ba_dkv_pass(const BaArgs &a, const BaKeys &w, co
 }
 
 template <typename T, int DP, bool CAREFUL>
-__global__ __launch_bounds__(BA_THREADS, (BaBwd<T, DP>::kw)) void block_attn_dkv_kernel(BaArgs a, int64_t all)
+__device__ __forceinline__ void ba_dkv_part(const BaArgs &a, int64_t id, char *smem, int *list_all, unsigned long long *odd)
 {
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    __shared__ int list_all;
-    __shared__ unsigned long long odd;
     typedef typename hd_vec<T>::v8 V8;
     constexpr bool HALF = __is_same(T, _Float16);
-    if (CAREFUL && !*a.unclean)
-        return;
-    int64_t id = ba_xcd(blockIdx.x, all), part = 0;
+    int64_t part = 0;
     int skip = 0, take = 0x7FFFFFFF, parts = 1;                 // of the queries that picked the block, in order
     if (a.chunk) {
         const int blocks = a.b * a.hk * a.nb;
@@ -1246,12 +1246,12 @@ __global__ __launch_bounds__(BA_THREADS, (BaBwd<T, DP>::kw)) void block_attn_dkv
                 finite &= ba_finite(dk[d][r]) && ba_finite(dv[d][r]);
         return ba_col_max(finite || poison ? 0.f : 1.f) > 0.f;
     };
-    ba_dkv_pass<T, DP, CAREFUL>(a, w, kf, vf, smem, &list_all, &odd, 1.f, dk, dv, up, poison);
+    ba_dkv_pass<T, DP, CAREFUL>(a, w, kf, vf, smem, list_all, odd, 1.f, dk, dv, up, poison);
     if constexpr (CAREFUL) {
         poison = ba_col_max(poison ? 1.f : 0.f) > 0.f;
         const bool bad = HALF && reached();
         if (HALF && __syncthreads_or(bad)) {
-            ba_dkv_pass<T, DP, true>(a, w, kf, vf, smem, &list_all, &odd, bad ? BA_LOW : 1.f, dk, dv, up, poison);
+            ba_dkv_pass<T, DP, true>(a, w, kf, vf, smem, list_all, odd, bad ? BA_LOW : 1.f, dk, dv, up, poison);
             poison = ba_col_max(poison ? 1.f : 0.f) > 0.f;
         }
         if (poison)
@@ -1280,6 +1280,29 @@ __global__ __launch_bounds__(BA_THREADS, (BaBwd<T, DP>::kw)) void block_attn_dkv
             ba_store4<T>((T *)a.out + at + d * 16 + g * 4, dk[d] * back);
             ba_store4<T>((T *)a.out2 + at + d * 16 + g * 4, dv[d]);
         }
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(BA_THREADS, (BaBwd<T, DP>::kw)) void block_attn_dkv_kernel(BaArgs a, int64_t all)
+{
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    __shared__ int list_all;
+    ba_dkv_part<T, DP, false>(a, ba_xcd(blockIdx.x, all), smem, &list_all, nullptr);
+}
+
+// Both once more, carefully, where anything came out that is not finite (a launch that ends at once where nothing did: 4.6 us;
+// inside the two kernels above the careful passes cost registers, and with them 388 for 357 us).
+template <typename T, int DP> __global__ __launch_bounds__(BA_THREADS) void block_attn_careful_kernel(BaArgs a, int64_t tiles, int64_t parts)
+{
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    __shared__ int list_all;
+    __shared__ unsigned long long odd;
+    if (!*a.unclean)
+        return;
+    if (blockIdx.x < tiles)
+        ba_dq_tile<T, DP, true>(a, blockIdx.x, smem, &odd);
+    else
+        ba_dkv_part<T, DP, true>(a, blockIdx.x - tiles, smem, &list_all, &odd);
 }
 
 // dk and dv of a block from its parts, in the parts' order
@@ -1331,7 +1354,8 @@ int ba_fill(BaArgs &a, int type, int b, int m, int n, int d, const tpu3_heads *q
         return TPU3_OK;
     if (!hd_rows_ok(q, type) || !blocks || (n > 0 && (!hd_rows_ok(k, type) || !hd_rows_ok(v, type))))
         return TPU3_EINVAL;
-    if ((int64_t)b * a.hk * a.tiles > 0x7FFFFFFFLL / 64 || (int64_t)b * a.hk * a.nb > 0x7FFFFFFFLL || (int64_t)b * a.hk * a.mt > 0x7FFFFFFFLL)
+    const int64_t most = (1 << 23) - 1;     // workgroups of 256 threads: 2^32 threads a launch, two kinds of them in one
+    if ((int64_t)b * a.hk * a.tiles > most || (int64_t)b * a.hk * a.nb > most || (int64_t)b * a.hk * a.mt > most)
         return TPU3_ELIMIT;
     return 1;
 }
@@ -1408,33 +1432,29 @@ template <typename T, int DP> int ba_forward(const BaArgs &a, hipStream_t s)
 
 template <typename T, int DP> int ba_backward(BaArgs a, void *dq, void *dk, void *dv, hipStream_t s)
 {
-    int rc = TPU3_OK;
-    // dq also leaves the rows' do . o for the pass over the keys
-    const int64_t all = (int64_t)a.b * a.hk * a.tiles;
-    const size_t lds = ba_lds(a, 2 * BaLds<T, DP>::TILE);
-    rc = ba_allow(block_attn_dq_kernel<T, DP>, lds);
+    const int64_t tiles = (int64_t)a.b * a.hk * a.tiles, blocks = (int64_t)a.b * a.hk * a.nb;
+    const int64_t parts = a.chunk ? ba_dkv_parts(a.b, a.m, a.hk, a.nb, a.count) : blocks;
+    const size_t lds = ba_lds(a, 2 * BaLds<T, DP>::TILE), lds2 = 2 * BaLds<T, DP>::TILE + 4 * 64 * 4 + (size_t)BD_WORDS * 64 * 4;
+    const size_t most = lds > lds2 ? lds : lds2;
+    int rc = ba_allow(block_attn_dq_kernel<T, DP>, lds);
+    if (!rc)
+        rc = ba_allow(block_attn_dkv_kernel<T, DP>, lds2);
+    if (!rc)
+        rc = ba_allow(block_attn_careful_kernel<T, DP>, most);
     if (rc)
         return rc;
-    a.out = dq;
-    hipLaunchKernelGGL((block_attn_dq_kernel<T, DP>), dim3((unsigned)all), dim3(BA_THREADS), lds, s, a, all);
+    a.dq = dq, a.out = dk, a.out2 = dv;
+    hipLaunchKernelGGL(block_pick_bits_kernel, dim3((unsigned)(a.b * a.hk * a.mt)), dim3(BA_THREADS), 0, s, a);
+    // dq also leaves the rows' do . o for the pass over the keys
+    hipLaunchKernelGGL((block_attn_dq_kernel<T, DP>), dim3((unsigned)tiles), dim3(BA_THREADS), lds, s, a, tiles);
     if (a.nb == 0)
         return tpu3_launch_status();
-    hipLaunchKernelGGL(block_pick_bits_kernel, dim3((unsigned)(a.b * a.hk * a.mt)), dim3(BA_THREADS), 0, s, a);
-    const size_t lds2 = 2 * BaLds<T, DP>::TILE + 4 * 64 * 4 + (size_t)BD_WORDS * 64 * 4;
-    rc = ba_allow(block_attn_dkv_kernel<T, DP, false>, lds2);
-    if (!rc)
-        rc = ba_allow(block_attn_dkv_kernel<T, DP, true>, lds2);
-    if (rc)
-        return rc;
-    a.out = dk, a.out2 = dv;
-    const int64_t blocks = (int64_t)a.b * a.hk * a.nb;
-    const int64_t all2 = a.chunk ? ba_dkv_parts(a.b, a.m, a.hk, a.nb, a.count) : blocks;
     if (a.chunk) {
         hipLaunchKernelGGL(block_picks_kernel, dim3((unsigned)blocks), dim3(BA_THREADS), 0, s, a);
         hipLaunchKernelGGL(block_parts_kernel, dim3(1), dim3(1024), 0, s, a, (int)blocks);
     }
-    hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP, false>), dim3((unsigned)all2), dim3(BA_THREADS), lds2, s, a, all2);
-    hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP, true>), dim3((unsigned)all2), dim3(BA_THREADS), lds2, s, a, all2);
+    hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP>), dim3((unsigned)parts), dim3(BA_THREADS), lds2, s, a, parts);
+    hipLaunchKernelGGL((block_attn_careful_kernel<T, DP>), dim3((unsigned)(tiles + parts)), dim3(BA_THREADS), most, s, a, tiles, parts);
     if (a.chunk)
         hipLaunchKernelGGL((block_attn_dkv_join_kernel<T, DP>), dim3((unsigned)(blocks * BJ_SLICES)), dim3(BA_THREADS), 0, s, a);
     return tpu3_launch_status();

@@ -718,7 +718,7 @@ extern "C" int tpu3_block_means(tpu3_stream_t stream, int type, int b, int n, in
     int blocks = nb;
     if (last > 0 && (last - 1) / BS_BLOCK + 2 < blocks)
         blocks = (last - 1) / BS_BLOCK + 2;
-    if ((int64_t)b * blocks > 0x7FFFFFFFLL)
+    if ((int64_t)b * blocks >= 1 << 24)     // (2^32 threads a launch)
         return TPU3_ELIMIT;
     const hipStream_t s = (hipStream_t)stream;
     const dim3 grid((unsigned)(b * blocks));
@@ -764,7 +764,7 @@ extern "C" int tpu3_block_select(tpu3_stream_t stream, int type, int b, int m, i
     const bool many = a.nb > 0 && bs_many(b, m, hk, a.nb);
     if (many)
         a.splits = 1;
-    if (rows * a.splits > 0x7FFFFFFFLL)
+    if (rows * a.splits > 0x7FFFFFFFLL || (!many && rows * a.splits >= 1 << 24))
         return TPU3_ELIMIT;
     const hipStream_t s = (hipStream_t)stream;
     if (many) {

@@ -496,7 +496,7 @@ extern "C" int tpu3_norm_rotate_fwd(tpu3_stream_t stream, int type, int b, int n
         return TPU3_EINVAL;
     a.out[0] = oq, a.out[1] = ok;
     const NrPlan p = nr_plan(a.tokens, q->heads + k->heads, d, a.total_pairs, a.interleaved, false, false, false);
-    if ((a.tokens + p.tok - 1) / p.tok > 0x7FFFFFFFLL)
+    if ((a.tokens + p.tok - 1) / p.tok >= 1 << 24)              // (2^32 threads a launch)
         return TPU3_ELIMIT;
     a.tok = p.tok;
     const hipStream_t s = (hipStream_t)stream;
