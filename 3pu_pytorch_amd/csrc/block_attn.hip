@@ -178,18 +178,6 @@ template <typename T> __device__ __forceinline__ typename hd_vec<T>::v8 ba_rest(
     return ba_pack<T>(r0, r1);
 }
 
-template <typename T> __device__ __forceinline__ typename hd_vec<T>::v8 ba_ones()
-{
-    typename hd_vec<T>::v8 f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if constexpr (sizeof(T) == 4)
-            f.v[i] = 1.f;
-        else
-            f[i] = (T)1.f;
-    return f;
-}
-
 template <typename T> __device__ __forceinline__ void ba_store4(T *p, const hd_f4 &x)
 {
     typename hd_vec<T>::v4 y;
@@ -574,18 +562,16 @@ __device__ __forceinline__ void ba_fwd_block(const BaArgs &a, const BaRow &R, co
                 s[x][r] = bit ? s[x][r] : 0.f;
         }
     };
-    const auto rounded = [&](int j) __attribute__((always_inline)) {
-        weight(2 * j), weight(2 * j + 1);
-        const V8 pf = ba_pack<T>(s[2 * j], s[2 * j + 1]);
-        // the denominator: in the 16-bit types one more row of the product, ones times the probabilities, as rounded as they
-        // are there; in fp32, whose matrix instructions are the bound, this lane's share by additions
-        if constexpr (sizeof(T) == 2)
-            sums = ba_mma<T>(ba_ones<T>(), pf, sums);
-        else
+    // the denominator: this lane's share by additions, of the probabilities as they are; the product takes them in two terms of a
+    // 16-bit type (in one, the output was off by 1.25 times what its last rounding takes: bf16 0.0021 for 0.0017)
+    vc.template run<sizeof(T) == 2>(
+        Vs, acc,
+        [&](int j) __attribute__((always_inline)) {
+            weight(2 * j), weight(2 * j + 1);
             sums += s[2 * j] + s[2 * j + 1];
-        return pf;
-    };
-    vc.template run<false>(Vs, acc, rounded, rounded);
+            return ba_pack<T>(s[2 * j], s[2 * j + 1]);
+        },
+        [&](int j, const V8 &f) __attribute__((always_inline)) { return ba_rest<T>(s[2 * j], s[2 * j + 1], f); });
     if constexpr (CAREFUL) {
         for (unsigned long long left = *odd; left; left &= left - 1) {
             const int kk = __ffsll(left) - 1;                   // the key's place in the block: score register and lane group
@@ -685,10 +671,9 @@ __global__ __launch_bounds__(BA_THREADS, (BaFwd<T, DP>::w)) void block_attn_fwd_
             finite &= ba_finite(acc[d][r]);
     if (__syncthreads_or(!finite))
         ba_fwd_pass<T, DP, true>(a, t, R, qf, smem, mask, list, count, &odd, acc, sums, top);
-    const float total = ba_col_sum(sums[0] + sums[1] + sums[2] + sums[3]);
+    const float sum = ba_col_sum(sums[0] + sums[1] + sums[2] + sums[3]);
     if (!R.there)
         return;
-    const float sum = sizeof(T) == 2 ? sums[0] : total;
     if (a.splits > 1) {
         float *P = a.part + (R.flat(a, t.b) * a.splits + t.z) * (DP + 4);
 #pragma unroll

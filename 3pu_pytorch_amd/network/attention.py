@@ -20,8 +20,8 @@ Results do not depend on the order in which workgroups run.
 
 A key, query, value or output gradient that is not finite reaches what its masks let it reach and nothing else; a gradient that
 it reaches is not a number as a whole row.  Scores, softmax statistics, sums and norms are held in 32 bits or more; the 16-bit
-types round the probabilities of the output to their own type before the second matrix product (those of the gradients, and the
-score gradients, to two terms of it), float32 rounds nothing.  Means of blocks and scores of blocks are formed in 64 bits."""
+types take probabilities and score gradients into the second matrix products in two terms of their own type, which together hold
+2^-17 (bfloat16) or 2^-22 (float16) of a value; float32 rounds nothing.  Means of blocks and scores of blocks are formed in 64 bits."""
 import math
 
 import torch
