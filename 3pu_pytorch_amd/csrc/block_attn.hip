@@ -34,7 +34,7 @@ struct BaArgs {
     const int32_t *n_arr, *m_arr;
     void *out, *out2, *dq;                  // forward: o; backward: dk, dv, dq (contiguous)
     void *rest;                             // 16-bit types, contiguous like o: what the rounding of o took, for do . o
-    float *lse;                             // (b, hq, m): log2 of the softmax denominator, scaled scores in base 2
+    float *lse;                             // (b, hq, m, 2): a row's largest score, log2 of its sum of ba_power(score - largest)
     float *delta;                           // (b, hq, m): do . o
     float *gmax;                            // (b, hq, m): largest |do| of the row
     uint64_t *bits;                         // (b, hk, nb, mt): bit = query of the tile of 64 picked the block
@@ -503,14 +503,28 @@ template <typename T, int DP, int VG> struct BaColumns {
         }
     }
 };
-// 2^(scaled score - off).  The rounding of the scale moves all scores of a row alike, by as much as all of an fp32 result's other
-// roundings where scores reach 20 (96 channels): fp32 takes its second term too.
-template <typename T> __device__ __forceinline__ float ba_power(const BaArgs &a, float s, float off)
+// 2^(scaled d + shift), d = a score less its row's largest.  The difference comes first: near the largest score, where the weight
+// is, it is exact however large the scores are (scaled ones of 2^31 and more had no or infinite weight when the difference was of
+// their rounded products, and the gradients' probabilities were off by half a step of the largest score).  fp32 takes the
+// scale's second term too: its rounding moves a difference of 20 by as much as all of an fp32 result's other roundings.
+template <typename T> __device__ __forceinline__ float ba_power(const BaArgs &a, float d, float shift)
 {
-    float e = __builtin_fmaf(s, a.scale2, -off);
+    float e = __builtin_fmaf(d, a.scale2, shift);
     if constexpr (sizeof(T) == 4)
-        e = __builtin_fmaf(s, a.scale2_rest, e);
+        e = __builtin_fmaf(d, a.scale2_rest, e);
     return __builtin_amdgcn_exp2f(e);
+}
+// what the backward pass takes of a row's softmax
+struct BaStat {
+    float top, shift;                       // p = ba_power(score - top, shift)
+};
+__device__ __forceinline__ void ba_put_row(const BaArgs &a, int64_t row, float top, float sum)
+{
+    a.lse[2 * row] = top, a.lse[2 * row + 1] = sum > 0.f ? log2f(sum) : -INFINITY;
+}
+__device__ __forceinline__ BaStat ba_get_row(const BaArgs &a, int64_t row)
+{
+    return {a.lse[2 * row], -a.lse[2 * row + 1]};
 }
 __device__ __forceinline__ bool ba_finite(float x) { return fabsf(x) <= 3.4028235e38f; }
 
@@ -541,10 +555,10 @@ __device__ __forceinline__ void ba_fwd_block(const BaArgs &a, const BaRow &R, co
 #pragma unroll
         for (int r = 0; r < 4; ++r)
             mx = fmaxf(mx, s[x][r]);
-    mx = ba_col_max(mx) * a.scale2;
+    mx = ba_col_max(mx);
     const float next = bit ? fmaxf(top, mx) : top;
     const float base = next == -INFINITY ? 0.f : next;
-    const float keep = __builtin_amdgcn_exp2f(top - base);          // top = -inf: 0
+    const float keep = ba_power<T>(a, top - base, 0.f);             // top = -inf: 0
     top = next;
     if (__any(keep != 1.f)) {
         sums *= keep;
@@ -552,12 +566,12 @@ __device__ __forceinline__ void ba_fwd_block(const BaArgs &a, const BaRow &R, co
         for (int d = 0; d < DP / 16; ++d)
             acc[d] *= keep;
     }
-    // a row that did not pick the block: exp2(x - inf) = 0 (a score that is not finite is left to the careful pass)
+    // a row that did not pick the block: 2^(x - inf) = 0 (a score that is not finite is left to the careful pass)
     const float off = bit ? base : INFINITY;
     auto weight = [&](int x) __attribute__((always_inline)) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            s[x][r] = ba_power<T>(a, s[x][r], off);
+            s[x][r] = ba_power<T>(a, s[x][r] - off, 0.f);
             if (CAREFUL)
                 s[x][r] = bit ? s[x][r] : 0.f;
         }
@@ -661,7 +675,7 @@ __global__ __launch_bounds__(BA_THREADS, (BaFwd<T, DP>::w)) void block_attn_fwd_
     const int count = ba_union(a, t, list, mask, words, before);
 
     hd_f4 acc[DP / 16], sums;               // sums: running sum of the row
-    float top;                              // running maximum of the row, scaled
+    float top;                              // running maximum of the row's scores
     ba_fwd_pass<T, DP, false>(a, t, R, qf, smem, mask, list, count, &odd, acc, sums, top);
     bool finite = ba_finite(sums[0] + sums[1] + sums[2] + sums[3]);
 #pragma unroll
@@ -690,7 +704,7 @@ __global__ __launch_bounds__(BA_THREADS, (BaFwd<T, DP>::w)) void block_attn_fwd_
         if (d * 16 + g * 4 < a.d)
             ba_store_rest<T>((T *)a.out + at, (T *)a.rest + at, a.rest != nullptr, d * 16 + g * 4, acc[d] * inv);
     if (a.lse && g == 0)
-        a.lse[R.flat(a, t.b)] = sum > 0.f ? top + log2f(sum) : -INFINITY;
+        ba_put_row(a, R.flat(a, t.b), top, sum);
 }
 
 // Joins the splits of a row, RL lanes a row (16, or a wave for more splits): a lane per split forms the splits' factors, then a
@@ -710,7 +724,7 @@ __global__ __launch_bounds__(BA_THREADS) void block_attn_join_kernel(BaArgs a, i
 #pragma unroll
     for (int o = RL / 2; o > 0; o >>= 1)
         top = fmaxf(top, __shfl_xor(top, o, 64));
-    const float base = top == -INFINITY ? 0.f : top, f = __builtin_amdgcn_exp2f(mine - base);
+    const float base = top == -INFINITY ? 0.f : top, f = ba_power<T>(a, mine - base, 0.f);
     float sum = part * f;
 #pragma unroll
     for (int o = RL / 2; o > 0; o >>= 1)
@@ -722,7 +736,7 @@ __global__ __launch_bounds__(BA_THREADS) void block_attn_join_kernel(BaArgs a, i
     const int64_t i = row % a.m, bh = row / a.m, h = bh % a.hq, b = bh / a.hq;
     const int64_t at = ((b * a.m + i) * a.hq + h) * a.d;
     if (a.lse && lane == 0)
-        a.lse[row] = sum > 0.f ? top + log2f(sum) : -INFINITY;
+        ba_put_row(a, row, top, sum);
     if (lane * W >= a.d)
         return;
     float y[W] = {};
@@ -755,7 +769,7 @@ constexpr float BA_LOW = 1.f / 4096.f;
 
 template <typename T, int DP>
 __device__ __forceinline__ void ba_dq_block(const BaArgs &a, const BaRow &R, const typename hd_vec<T>::v8 *qf, const typename hd_vec<T>::v8 *gf,
-                                            float lse, float delta, float up, const T *Ks, int k0, bool bit, hd_f4 *acc)
+                                            const BaStat &stat, float delta, float up, const T *Ks, int k0, bool bit, hd_f4 *acc)
 {
     typedef typename hd_vec<T>::v8 V8;
     constexpr bool HALF = __is_same(T, _Float16);
@@ -772,7 +786,7 @@ __device__ __forceinline__ void ba_dq_block(const BaArgs &a, const BaRow &R, con
     for (int x = 0; x < 4; ++x)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const float e = ba_power<T>(a, s[x][r], lse) * (dp[x][r] - delta);
+            const float e = ba_power<T>(a, s[x][r] - stat.top, stat.shift) * (dp[x][r] - delta);
             s[x][r] = HALF ? e * up : e;
         }
     if (__any(bit && k0 + BA_BLOCK > R.limit)) {
@@ -800,7 +814,7 @@ __device__ __forceinline__ void ba_dq_block(const BaArgs &a, const BaRow &R, con
 // those that do are not numbers (poison).
 template <typename T, int DP, bool CAREFUL>
 __device__ __forceinline__ void ba_dq_pass(const BaArgs &a, const BaTile &t, const BaRow &R, const typename hd_vec<T>::v8 *qf,
-                                           const typename hd_vec<T>::v8 *gf, float lse, float delta, float up, char *smem,
+                                           const typename hd_vec<T>::v8 *gf, const BaStat &stat, float delta, float up, char *smem,
                                            const uint64_t *mask, const uint32_t *list, int count, unsigned long long *odd,
                                            hd_f4 *acc, bool &poison)
 {
@@ -841,7 +855,7 @@ __device__ __forceinline__ void ba_dq_pass(const BaArgs &a, const BaTile &t, con
         const bool bit = R.mine && ((mask[u] >> R.ql) & 1);
         if constexpr (CAREFUL)
             poison |= bit && (*odd & (R.limit - k0 >= BA_BLOCK ? ~0ull : (1ull << max(0, R.limit - k0)) - 1)) != 0;
-        ba_dq_block<T, DP>(a, R, qf, gf, lse, delta, up, k, k0, bit, acc);
+        ba_dq_block<T, DP>(a, R, qf, gf, stat, delta, up, k, k0, bit, acc);
     }
 }
 
@@ -859,7 +873,8 @@ template <typename T, int DP, bool CAREFUL> __device__ __forceinline__ void ba_d
     V8 qf[DP / 32], gf[DP / 32];
     ba_row_operand<T, DP>(R.at<T>(a.q, t.b), R.mine, a.d, qf);
     ba_row_operand<T, DP>(R.at<T>(a.go, t.b), R.mine, a.d, gf);
-    float delta = 0.f, gmax = 0.f, lse = 0.f, up = 1.f;
+    float delta = 0.f, gmax = 0.f, up = 1.f;
+    BaStat stat = {0.f, 0.f};
     {
         // the rounding of o, times a gradient, would move all of a row's ds one way: it goes back in
         V8 of[DP / 32], rf[DP / 32];
@@ -879,7 +894,7 @@ template <typename T, int DP, bool CAREFUL> __device__ __forceinline__ void ba_d
         }
         if (R.mine) {
             const int64_t at = R.flat(a, t.b);
-            lse = a.lse[at];
+            stat = ba_get_row(a, at);
             if (g == 0) {
                 a.delta[at] = delta;
                 if (HALF)
@@ -890,7 +905,7 @@ template <typename T, int DP, bool CAREFUL> __device__ __forceinline__ void ba_d
     const int count = ba_union(a, t, list, mask, words, before);
     hd_f4 acc[DP / 16];
     bool poison = false;
-    ba_dq_pass<T, DP, CAREFUL>(a, t, R, qf, gf, lse, delta, up, smem, mask, list, count, odd, acc, poison);
+    ba_dq_pass<T, DP, CAREFUL>(a, t, R, qf, gf, stat, delta, up, smem, mask, list, count, odd, acc, poison);
     auto reached = [&]() __attribute__((always_inline)) {       // this lane's row holds what is not finite
         bool finite = true;
 #pragma unroll
@@ -904,7 +919,7 @@ template <typename T, int DP, bool CAREFUL> __device__ __forceinline__ void ba_d
         const bool bad = HALF && reached();
         if (HALF && __syncthreads_or(bad)) {
             up *= bad ? BA_LOW : 1.f;
-            ba_dq_pass<T, DP, true>(a, t, R, qf, gf, lse, delta, up, smem, mask, list, count, odd, acc, poison);
+            ba_dq_pass<T, DP, true>(a, t, R, qf, gf, stat, delta, up, smem, mask, list, count, odd, acc, poison);
         }
     } else if (reached()) {
         atomicOr(a.unclean, 1u);
@@ -1020,7 +1035,7 @@ __device__ __forceinline__ void ba_dkv_pass(const BaArgs &a, const BaKeys &w, co
     typedef typename hd_vec<T>::v8 V8;
     constexpr bool HALF = __is_same(T, _Float16);
     T *Qs = (T *)smem, *Gs = (T *)(smem + L::TILE);
-    float *lse_s = (float *)(smem + 2 * L::TILE), *delta_s = lse_s + 64, *gmax_s = delta_s + 64;
+    float *top_s = (float *)(smem + 2 * L::TILE), *shift_s = top_s + 64, *delta_s = shift_s + 64, *gmax_s = delta_s + 64;
     int *limit_s = (int *)(gmax_s + 64), *list = limit_s + 64;              // list: BD_WORDS * 64 queries
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
     int skip = w.skip, take = w.take;
@@ -1032,7 +1047,8 @@ __device__ __forceinline__ void ba_dkv_pass(const BaArgs &a, const BaKeys &w, co
 
     typedef BaStage<T, DP> S;
     S qr, gr;
-    float row_lse = 0.f, row_delta = 0.f, row_gmax = 0.f;
+    BaStat row_stat = {0.f, 0.f};
+    float row_delta = 0.f, row_gmax = 0.f;
     int row_limit = 0;
     const T *Q = S::lane((const T *)a.q.data + w.b * a.q.sb + (int64_t)w.h * a.group * a.q.sh, a.d);
     const T *G = S::lane((const T *)a.go.data + w.b * a.go.sb + (int64_t)w.h * a.group * a.go.sh, a.d);
@@ -1047,12 +1063,13 @@ __device__ __forceinline__ void ba_dkv_pass(const BaArgs &a, const BaKeys &w, co
             qr.r[x] = *(const V8 *)(Q + i * a.q.sr + e * a.q.sh);
             gr.r[x] = *(const V8 *)(G + i * a.go.sr + e * a.go.sh);
         }
-        row_lse = row_delta = row_gmax = 0.f;
+        row_stat = {0.f, 0.f};
+        row_delta = row_gmax = 0.f;
         row_limit = 0;
         if (threadIdx.x < BA_ROWS && r0 + (int)threadIdx.x < rows) {
             const int r = r0 + threadIdx.x, q = r / a.group, head = w.h * a.group + (r - q * a.group), i = list[q];
             const int64_t p = ((int64_t)w.b * a.hq + head) * a.m + i;
-            row_lse = a.lse[p], row_delta = a.delta[p], row_limit = ba_limit(a, w.live, w.lm, i);
+            row_stat = ba_get_row(a, p), row_delta = a.delta[p], row_limit = ba_limit(a, w.live, w.lm, i);
             if (HALF)
                 row_gmax = a.gmax[p];
         }
@@ -1094,7 +1111,8 @@ __device__ __forceinline__ void ba_dkv_pass(const BaArgs &a, const BaKeys &w, co
                 gr.store(Gs);
             }
             if (threadIdx.x < BA_ROWS) {
-                lse_s[threadIdx.x] = row_lse, delta_s[threadIdx.x] = row_delta, limit_s[threadIdx.x] = row_limit;
+                top_s[threadIdx.x] = row_stat.top, shift_s[threadIdx.x] = row_stat.shift;
+                delta_s[threadIdx.x] = row_delta, limit_s[threadIdx.x] = row_limit;
                 if (HALF)
                     gmax_s[threadIdx.x] = row_gmax;
             }
@@ -1132,7 +1150,7 @@ __device__ __forceinline__ void ba_dkv_pass(const BaArgs &a, const BaKeys &w, co
                         ga[kk] = L::row8(Gs, j * 32 + x * 16 + l15, kk * 4 + g);
                     }
                     const int r4 = j * 32 + x * 16 + g * 4;
-                    const hd_f4 le = *(const hd_f4 *)(lse_s + r4), de = *(const hd_f4 *)(delta_s + r4);
+                    const hd_f4 to = *(const hd_f4 *)(top_s + r4), sh = *(const hd_f4 *)(shift_s + r4), de = *(const hd_f4 *)(delta_s + r4);
                     const int4 li = *(const int4 *)(limit_s + r4);
                     const int lim[4] = {li.x, li.y, li.z, li.w};
                     ba_issue();
@@ -1145,7 +1163,7 @@ __device__ __forceinline__ void ba_dkv_pass(const BaArgs &a, const BaKeys &w, co
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const bool see = w.key < lim[r];
-                        const float e = ba_power<T>(a, s[r], le[r]);
+                        const float e = ba_power<T>(a, s[r] - to[r], sh[r]);
                         const float f = e * (dp[r] - de[r]);
                         p[x][r] = see ? e : 0.f;
                         ds[x][r] = see ? (HALF ? f * up : f) : 0.f;
@@ -1419,7 +1437,7 @@ template <typename T, int DP> int ba_backward(BaArgs a, void *dq, void *dk, void
 {
     const int64_t tiles = (int64_t)a.b * a.hk * a.tiles, blocks = (int64_t)a.b * a.hk * a.nb;
     const int64_t parts = a.chunk ? ba_dkv_parts(a.b, a.m, a.hk, a.nb, a.count) : blocks;
-    const size_t lds = ba_lds(a, 2 * BaLds<T, DP>::TILE), lds2 = 2 * BaLds<T, DP>::TILE + 4 * 64 * 4 + (size_t)BD_WORDS * 64 * 4;
+    const size_t lds = ba_lds(a, 2 * BaLds<T, DP>::TILE), lds2 = 2 * BaLds<T, DP>::TILE + 5 * 64 * 4 + (size_t)BD_WORDS * 64 * 4;
     const size_t most = lds > lds2 ? lds : lds2;
     int rc = ba_allow(block_attn_dq_kernel<T, DP>, lds);
     if (!rc)
@@ -1473,7 +1491,7 @@ extern "C" int tpu3_block_attn_fwd(tpu3_stream_t stream, int type, int b, int m,
     const int rc = ba_fill(a, type, b, m, n, d, q, k, v, blocks, count, scale, n_arr, m_arr, causal);
     if (rc <= 0)
         return rc;
-    if (!out || ((uintptr_t)out & 15) || ((uintptr_t)rest & 15))
+    if (!out || ((uintptr_t)out & 15) || ((uintptr_t)rest & 15) || ((uintptr_t)lse & 7))
         return TPU3_EINVAL;
     a.out = out, a.lse = lse, a.rest = type == TPU3_TYPE_F32 ? nullptr : rest;
     a.splits = ba_splits(b, m, n, a.hq, a.hk, count);
@@ -1525,7 +1543,7 @@ extern "C" int tpu3_block_attn_bwd(tpu3_stream_t stream, int type, int b, int m,
     const int rc = ba_fill(a, type, b, m, n, d, q, k, v, blocks, count, scale, n_arr, m_arr, causal);
     if (rc <= 0)
         return rc;
-    if (!hd_rows_ok(o, type) || !hd_rows_ok(go, type) || o->heads != a.hq || go->heads != a.hq || !lse || !dq || ((uintptr_t)rest & 15) ||
+    if (!hd_rows_ok(o, type) || !hd_rows_ok(go, type) || o->heads != a.hq || go->heads != a.hq || !lse || ((uintptr_t)lse & 7) || !dq || ((uintptr_t)rest & 15) ||
         ((uintptr_t)dq & 15) || (n > 0 && (!dk || !dv || ((uintptr_t)dk & 15) || ((uintptr_t)dv & 15))) || !workspace ||
         ((uintptr_t)workspace & 15) || workspace_bytes < tpu3_block_attn_bwd_workspace_bytes(b, m, n, a.hq, a.hk, d, count))
         return TPU3_EINVAL;

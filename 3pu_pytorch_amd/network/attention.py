@@ -319,7 +319,7 @@ def _attention_forward(q, k, v, blocks, scale, n_arr, m_arr, causal, grad=False)
     b, m, hq, d = q.shape
     n, hk, count = k.size(1), k.size(2), blocks.size(3)
     o = q.new_empty(q.shape)
-    lse = q.new_empty((b, hq, m), dtype=torch.float32) if grad else None
+    lse = q.new_empty((b, hq, m, 2), dtype=torch.float32) if grad else None
     rest = q.new_empty(q.shape) if grad and q.dtype != torch.float32 else None
     need = L.lib().tpu3_block_attn_fwd_workspace_bytes(b, m, n, hq, hk, d, count)
     ws = _workspace(need, q)

@@ -80,3 +80,52 @@ def test_errors_of_16_bit_types_are_their_last_rounding(dev, b, m, n, hq, hk, d,
         here, there = _error(x, z), _error(y.to(q.dtype), z)
         print("%s: %.3g, plain %.3g" % (name, here, there))
         assert here <= 1.05 * there, (name, here, there)
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("queries", [200, 2])
+def test_scores_far_beyond_the_exponents_range(dev, dtype, queries):
+    """Scores of up to 2^33 (fp16) and 2^87, all exact in fp32 and far apart: the largest key has all the weight, so the output is its
+    value, dv the sum of the gradients of the rows that chose it, and ds, dq, dk are 0, all exactly."""
+    ops = pkg("network.operations")
+    gen = torch.Generator(device=dev).manual_seed(5)
+    dt, n, d = TYPES[dtype], 128, 64
+    big = 2.0 ** (13 if dt == torch.float16 else 40)
+    pattern = torch.sign(_randn(gen, d))
+    w = 1 + torch.randperm(n, device=dev, generator=gen).float() / 128
+    side = torch.tensor([1.0, -1.0], device=dev).repeat(queries // 2)                           # odd rows want the smallest
+    row = side * (1 + torch.arange(queries, device=dev) % 128 / 128)
+    q = (big * row[:, None] * pattern).to(dt).view(1, queries, 1, d)
+    k = (big * w[:, None] * pattern).to(dt).view(1, n, 1, d)
+    v = torch.randint(-8, 9, (1, n, 1, d), device=dev, generator=gen).to(dt)
+    go = torch.randint(-1, 2, (1, queries, 1, d), device=dev, generator=gen).to(dt)
+    blocks = torch.tensor([0, 1], dtype=torch.int32, device=dev).expand(1, queries, 1, 2)
+    o, dq, dk, dv = _run(ops, (q, k, v), go, blocks)
+    best, worst = w.argmax(), w.argmin()
+    assert torch.equal(o, torch.where((side > 0).view(1, -1, 1, 1), v[:, best:best + 1], v[:, worst:worst + 1]))
+    want = torch.zeros_like(v)
+    want[0, best], want[0, worst] = go[0, side > 0].sum(dim=0), go[0, side < 0].sum(dim=0)
+    assert torch.equal(dv, want) and (dq == 0).all() and (dk == 0).all()
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_gradients_of_scores_with_a_large_common_part(dev, dtype):
+    """Scores of 2^20 + {0 .. 7}, exact in fp32: the probabilities are those of 0 .. 7.  A probability is off by the rounding of the
+    exponent, of exp2 and of the sum, together below 2^-19, and by its two terms in the 16-bit types (2^-17): 2^-15 of the sum
+    of magnitudes, and the last rounding."""
+    ops = pkg("network.operations")
+    gen = torch.Generator(device=dev).manual_seed(6)
+    dt, n, m, d = TYPES[dtype], 256, 150, 32
+    q, k = torch.zeros((1, m, 1, d), device=dev), torch.zeros((1, n, 1, d), device=dev)
+    q[..., 0], k[..., 0] = 1024, 1024
+    q[..., 1] = 1
+    k[..., 1] = torch.randint(0, 8, (1, n, 1), device=dev, generator=gen).float()
+    q, k = q.to(dt), k.to(dt)
+    v, go = _randn(gen, 1, n, 1, d, dtype=dt), _randn(gen, 1, m, 1, d, dtype=dt)
+    blocks = torch.arange(4, dtype=torch.int32, device=dev).expand(1, m, 1, 4)
+    o, _, _, dv = _run(ops, (q, k, v), go, blocks, 1.0)
+    p = torch.softmax(k[0, :, 0, 1].double(), dim=0)
+    u = torch.finfo(dt).eps / 2
+    for got, want, size in ((o, p @ v[0, :, 0].double(), p @ v[0, :, 0].double().abs()),
+                            (dv, p[:, None] * go[0, :, 0].double().sum(dim=0), p[:, None] * go[0, :, 0].double().abs().sum(dim=0))):
+        assert ((got[0, :, 0].double() - want).abs() <= u * want.abs() + 2.0 ** -15 * size + 2.0 ** -25).all()
