@@ -520,11 +520,14 @@ struct BaStat {
 };
 __device__ __forceinline__ void ba_put_row(const BaArgs &a, int64_t row, float top, float sum)
 {
-    a.lse[2 * row] = top, a.lse[2 * row + 1] = sum > 0.f ? log2f(sum) : -INFINITY;
+    a.lse[2 * row] = top, a.lse[2 * row + 1] = log2f(sum);          // nothing seen, or scores of -infinity only: -infinity; NaN: NaN
 }
 __device__ __forceinline__ BaStat ba_get_row(const BaArgs &a, int64_t row)
 {
-    return {a.lse[2 * row], -a.lse[2 * row + 1]};
+    const float top = a.lse[2 * row], log = a.lse[2 * row + 1];
+    if (log == -INFINITY)                   // no weights (its output is 0): 2^(score - inf) = 0, also for scores of -infinity
+        return {0.f, -INFINITY};
+    return {top, -log};
 }
 __device__ __forceinline__ bool ba_finite(float x) { return fabsf(x) <= 3.4028235e38f; }
 

@@ -129,3 +129,51 @@ def test_gradients_of_scores_with_a_large_common_part(dev, dtype):
     for got, want, size in ((o, p @ v[0, :, 0].double(), p @ v[0, :, 0].double().abs()),
                             (dv, p[:, None] * go[0, :, 0].double().sum(dim=0), p[:, None] * go[0, :, 0].double().abs().sum(dim=0))):
         assert ((got[0, :, 0].double() - want).abs() <= u * want.abs() + 2.0 ** -15 * size + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_keys_and_values_that_are_not_numbers_in_the_gradients_of_keys(dev, dtype):
+    """A key that is NaN: the rows that see it have no probabilities, so dk and dv of every key that one of them sees are not
+    numbers, as whole rows.  A value that is NaN: the same for dk; dv does not depend on it.  All others have the bits of a
+    call without them."""
+    ops = pkg("network.operations")
+    q, k, v, go, _ = _inputs(dev, 1, 128, 192, 2, 1, 64, 1, TYPES[dtype], 61)
+    blocks = torch.zeros((1, 128, 1, 2), dtype=torch.int32, device=dev)
+    blocks[:, ::2, :, 1] = 1
+    blocks[:, 1::2, :, 1] = 2
+    see = orc64.seen(1, 128, 192, 1, blocks, causal=True)[0, 0]
+    _, _, dk2, dv2 = _run(ops, (q, k, v), go, blocks, causal=True)
+    for bad in (70, 100, 150):
+        hit = see[see[:, bad]].any(dim=0)
+        assert hit.any() and not hit.all()
+        kk = k.clone()
+        kk[0, bad, 0, 3] = math.nan
+        _, _, dk, dv = _run(ops, (q, kk, v), go, blocks, causal=True)
+        assert dk[0, hit].isnan().all() and dv[0, hit].isnan().all()
+        assert torch.equal(dk[0, ~hit], dk2[0, ~hit]) and torch.equal(dv[0, ~hit], dv2[0, ~hit])
+        vv = v.clone()
+        vv[0, bad, 0, 5] = math.nan
+        _, _, dk, dv = _run(ops, (q, k, vv), go, blocks, causal=True)
+        assert dk[0, hit].isnan().all() and torch.equal(dv, dv2)
+        assert torch.equal(dk[0, ~hit], dk2[0, ~hit])
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("queries", [130, 2])
+def test_rows_whose_scores_are_all_minus_infinity(dev, dtype, queries):
+    """Such a row is 0 and passes no gradient on to the keys and values it sees; its own gradient is 0 where the keys are finite
+    (scores that overflow), not a number where they are not."""
+    ops = pkg("network.operations")
+    q, k, v, go, _ = _inputs(dev, 1, queries, 128, 2, 1, 64, 1, TYPES[dtype], 62)
+    blocks = (torch.arange(queries, device=dev) % 2).to(torch.int32).view(1, -1, 1, 1)
+    infinite = TYPES[dtype] == torch.float16
+    q[..., 0] = 1000 if infinite else 1e25
+    k[..., 0] = 0
+    k[0, 64:, 0, 0] = -math.inf if infinite else -1e25
+    o, dq, dk, dv = _run(ops, (q, k, v), go, blocks)
+    assert (o[0, 1::2] == 0).all() and (dk[0, 64:] == 0).all() and (dv[0, 64:] == 0).all()
+    assert dq[0, 1::2].isnan().all() if infinite else (dq[0, 1::2] == 0).all()
+    keep = slice(0, None, 2)
+    alone = _run(ops, (q[:, keep], k, v), go[:, keep], blocks[:, keep])
+    assert torch.equal(o[:, keep], alone[0]) and torch.isfinite(dk[0, :64]).all() and torch.isfinite(dv[0, :64]).all()
+    assert torch.isfinite(dq[:, keep]).all()
