@@ -33,10 +33,9 @@ struct BaArgs {
     const int32_t *blocks;                  // (b, m, hk, count)
     const int32_t *n_arr, *m_arr;
     void *out, *out2, *dq;                  // forward: o; backward: dk, dv, dq (contiguous)
-    void *rest;                             // 16-bit types, contiguous like o: what the rounding of o took, for do . o
-    float *lse;                             // (b, hq, m, 2): a row's largest score, log2 of its sum of ba_power(score - largest)
-    float *delta;                           // (b, hq, m): do . o
-    float *gmax;                            // (b, hq, m): largest |do| of the row
+    void *rest;                             // 16-bit types, contiguous like o: what the rounding of o took (ba_rest_scale), for do . o
+    float *lse;                             // (b, hq, m, 2): BaStat of the row
+    float *row;                             // (b, hq, m, 2): for dk, dv: shift of the row there, and do . o
     uint64_t *bits;                         // (b, hk, nb, mt): bit = query of the tile of 64 picked the block
     float *part;                            // split forward: (rows, splits, d + 4); dk / dv in parts: (parts, 2, 64, d)
     int32_t *picks, *first;                 // dk / dv in parts: queries that picked a block; first part of a block, and the end
@@ -187,6 +186,10 @@ template <typename T> __device__ __forceinline__ void ba_store4(T *p, const hd_f
     *(typename hd_vec<T>::v4 *)p = y;
 }
 
+// What the rounding of o took, as it is stored: fp16 times 2^11 (at most 2^15, and a step of 2^-35 where o itself is below the
+// normal numbers).
+template <typename T> __device__ __forceinline__ constexpr float ba_rest_scale() { return __is_same(T, _Float16) ? 2048.f : 1.f; }
+
 // the same, and what the rounding took
 template <typename T> __device__ __forceinline__ void ba_store_rest(T *p, T *rest, bool want, int at, const hd_f4 &x)
 {
@@ -195,7 +198,7 @@ template <typename T> __device__ __forceinline__ void ba_store_rest(T *p, T *res
         hd_f4 r;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            r[i] = x[i] - (float)(T)x[i];
+            r[i] = (x[i] - (float)(T)x[i]) * ba_rest_scale<T>();
         ba_store4<T>(rest + at, r);
     }
 }
@@ -516,18 +519,13 @@ template <typename T> __device__ __forceinline__ float ba_power(const BaArgs &a,
 }
 // what the backward pass takes of a row's softmax
 struct BaStat {
-    float top, shift;                       // p = ba_power(score - top, shift)
+    float top, shift;                       // p = ba_power(score - top, shift): the largest score, minus log2 of the sum
 };
+// A row without weights (nothing seen, or scores of -infinity only; its output is 0): 2^(score - inf) = 0, also for scores of
+// -infinity.  A sum that is not a number: no more is p.
 __device__ __forceinline__ void ba_put_row(const BaArgs &a, int64_t row, float top, float sum)
 {
-    a.lse[2 * row] = top, a.lse[2 * row + 1] = log2f(sum);          // nothing seen, or scores of -infinity only: -infinity; NaN: NaN
-}
-__device__ __forceinline__ BaStat ba_get_row(const BaArgs &a, int64_t row)
-{
-    const float top = a.lse[2 * row], log = a.lse[2 * row + 1];
-    if (log == -INFINITY)                   // no weights (its output is 0): 2^(score - inf) = 0, also for scores of -infinity
-        return {0.f, -INFINITY};
-    return {top, -log};
+    a.lse[2 * row] = sum == 0.f ? 0.f : top, a.lse[2 * row + 1] = sum == 0.f ? -INFINITY : -log2f(sum);
 }
 __device__ __forceinline__ bool ba_finite(float x) { return fabsf(x) <= 3.4028235e38f; }
 
@@ -753,26 +751,41 @@ __global__ __launch_bounds__(BA_THREADS) void block_attn_join_kernel(BaArgs a, i
         const T v = (T)(y[c] * inv);
         ((T *)a.out)[at + lane * W + c] = v;
         if (a.rest)
-            ((T *)a.rest)[at + lane * W + c] = (T)(y[c] * inv - (float)v);
+            ((T *)a.rest)[at + lane * W + c] = (T)((y[c] * inv - (float)v) * ba_rest_scale<T>());
     }
 }
 
 // ---- backward: dq, and the rows' do . o ----------------------------------------------------------------------------------
-// fp16: ds is scaled by a power of two that brings the row's largest |do| to [1, 2) before it is rounded, and the
-// accumulated row is scaled back: ds of a small gradient would fall below fp16's normal numbers otherwise.
-__device__ __forceinline__ float ba_pow2_inverse(float x)
+// fp16: two terms of the type hold a number to 2^-22 of it only from 2^-3 on, and to 2^-25 at best, and ds may be of any size.  Its
+// row (in dk: its key) is therefore taken times a power of two, `up`, that starts high and is lowered, with what has been added
+// up, whenever the largest |ds| so far would pass 2^15: to where that is 2^10 .. 2^11, so that it is seldom lowered twice.  (A power
+// from the largest |do| alone left ds of small values or small probabilities below fp16's normal numbers: values of 1e-3, |do| of
+// 256: errors of dq and dk 9 times the last rounding's.)  Rows (keys) do not share powers: none loses digits to another's ds.
+constexpr float BA_UP = 1.2676506002282294e30f;                 // 2^100
+constexpr float BA_P_SHIFT = 15.f;                              // fp16, dk and dv: probabilities times 2^15
+
+// brings x to [2^10, 2^11), within 2^-100 .. 2^100
+__device__ __forceinline__ float ba_pow2_to_1024(float x)
 {
     const int e = (int)((__float_as_uint(x) >> 23) & 255u);
-    return e == 0 || e >= 253 ? 1.f : __uint_as_float((uint32_t)(254 - e) << 23);
+    return __uint_as_float((uint32_t)min(max(264 - e, 27), 227) << 23);
 }
-
-// Where ds still passes 65504 (|do . v - do . o| beyond that times the largest |do|), the pass is run again, with a power
-// smaller by BA_LOW for the rows (keys) that it reached: that quotient is at most 2 * 128 channels * 65504.
-constexpr float BA_LOW = 1.f / 4096.f;
+// lowers up, and sums with it, where big * up would pass 2^15; big: the lane's column's largest |ds|
+template <int N> __device__ __forceinline__ void ba_lower(float big, float &up, hd_f4 (&sums)[N])
+{
+    const bool passes = big * up > 32768.f;
+    if (!__any(passes))
+        return;
+    const float next = passes ? ba_pow2_to_1024(big) : up, keep = next / up;
+    up = next;
+#pragma unroll
+    for (int d = 0; d < N; ++d)
+        sums[d] *= keep;
+}
 
 template <typename T, int DP>
 __device__ __forceinline__ void ba_dq_block(const BaArgs &a, const BaRow &R, const typename hd_vec<T>::v8 *qf, const typename hd_vec<T>::v8 *gf,
-                                            const BaStat &stat, float delta, float up, const T *Ks, int k0, bool bit, hd_f4 *acc)
+                                            const BaStat &stat, float delta, float &up, const T *Ks, int k0, bool bit, hd_f4 (&acc)[DP / 16])
 {
     typedef typename hd_vec<T>::v8 V8;
     constexpr bool HALF = __is_same(T, _Float16);
@@ -788,10 +801,8 @@ __device__ __forceinline__ void ba_dq_block(const BaArgs &a, const BaRow &R, con
 #pragma unroll
     for (int x = 0; x < 4; ++x)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float e = ba_power<T>(a, s[x][r] - stat.top, stat.shift) * (dp[x][r] - delta);
-            s[x][r] = HALF ? e * up : e;
-        }
+        for (int r = 0; r < 4; ++r)
+            s[x][r] = ba_power<T>(a, s[x][r] - stat.top, stat.shift) * (dp[x][r] - delta);
     if (__any(bit && k0 + BA_BLOCK > R.limit)) {
 #pragma unroll
         for (int x = 0; x < 4; ++x)
@@ -806,6 +817,18 @@ __device__ __forceinline__ void ba_dq_block(const BaArgs &a, const BaRow &R, con
             for (int r = 0; r < 4; ++r)
                 s[x][r] = bit ? s[x][r] : 0.f;
     }
+    if constexpr (HALF) {
+        float big = 0.f;
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                big = fmaxf(big, fabsf(s[x][r]));
+        ba_lower(ba_col_max(big), up, acc);
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            s[x] *= up;
+    }
     // A row's ds add up to nothing, so its dq is what is left of large terms: ds enters in two terms of the 16-bit type (one
     // alone: an error of twice the result's own rounding)
     kc.template run<sizeof(T) == 2>(
@@ -817,12 +840,13 @@ __device__ __forceinline__ void ba_dq_block(const BaArgs &a, const BaRow &R, con
 // those that do are not numbers (poison).
 template <typename T, int DP, bool CAREFUL>
 __device__ __forceinline__ void ba_dq_pass(const BaArgs &a, const BaTile &t, const BaRow &R, const typename hd_vec<T>::v8 *qf,
-                                           const typename hd_vec<T>::v8 *gf, const BaStat &stat, float delta, float up, char *smem,
+                                           const typename hd_vec<T>::v8 *gf, const BaStat &stat, float delta, float &up, char *smem,
                                            const uint64_t *mask, const uint32_t *list, int count, unsigned long long *odd,
-                                           hd_f4 *acc, bool &poison)
+                                           hd_f4 (&acc)[DP / 16], bool &poison)
 {
     typedef BaLds<T, DP> L;
     typedef BaStage<T, DP> S;
+    up = BA_UP;
     const T *Kl = S::lane((const T *)a.k.data + t.b * a.k.sb + t.h * a.k.sh, a.d);
     const T *Vl = S::lane((const T *)a.v.data + t.b * a.v.sb + t.h * a.v.sh, a.d);
 #pragma unroll
@@ -876,7 +900,7 @@ template <typename T, int DP, bool CAREFUL> __device__ __forceinline__ void ba_d
     V8 qf[DP / 32], gf[DP / 32];
     ba_row_operand<T, DP>(R.at<T>(a.q, t.b), R.mine, a.d, qf);
     ba_row_operand<T, DP>(R.at<T>(a.go, t.b), R.mine, a.d, gf);
-    float delta = 0.f, gmax = 0.f, up = 1.f;
+    float delta = 0.f, up;
     BaStat stat = {0.f, 0.f};
     {
         // the rounding of o, times a gradient, would move all of a row's ds one way: it goes back in
@@ -886,23 +910,14 @@ template <typename T, int DP, bool CAREFUL> __device__ __forceinline__ void ba_d
 #pragma unroll
         for (int kk = 0; kk < DP / 32; ++kk)
 #pragma unroll
-            for (int x = 0; x < 8; ++x) {
-                delta = __builtin_fmaf((float)gf[kk][x], (float)of[kk][x] + (float)rf[kk][x], delta);
-                gmax = fmaxf(gmax, fabsf((float)gf[kk][x]));
-            }
+            for (int x = 0; x < 8; ++x)
+                delta = __builtin_fmaf((float)gf[kk][x], __builtin_fmaf((float)rf[kk][x], 1.f / ba_rest_scale<T>(), (float)of[kk][x]), delta);
         delta = ba_col_sum(delta);
-        if (HALF) {
-            gmax = ba_col_max(gmax);
-            up = ba_pow2_inverse(gmax);
-        }
         if (R.mine) {
-            const int64_t at = R.flat(a, t.b);
-            stat = ba_get_row(a, at);
-            if (g == 0) {
-                a.delta[at] = delta;
-                if (HALF)
-                    a.gmax[at] = gmax;
-            }
+            const int64_t at = 2 * R.flat(a, t.b);
+            stat = {a.lse[at], a.lse[at + 1]};
+            if (g == 0)
+                a.row[at] = stat.shift + (HALF ? BA_P_SHIFT : 0.f), a.row[at + 1] = delta;
         }
     }
     const int count = ba_union(a, t, list, mask, words, before);
@@ -918,23 +933,16 @@ template <typename T, int DP, bool CAREFUL> __device__ __forceinline__ void ba_d
                 finite &= ba_finite(acc[d][r]);
         return ba_col_max(finite || poison ? 0.f : 1.f) > 0.f;
     };
-    if constexpr (CAREFUL) {
-        const bool bad = HALF && reached();
-        if (HALF && __syncthreads_or(bad)) {
-            up *= bad ? BA_LOW : 1.f;
-            ba_dq_pass<T, DP, true>(a, t, R, qf, gf, stat, delta, up, smem, mask, list, count, odd, acc, poison);
-        }
-    } else if (reached()) {
+    if (!CAREFUL && reached())
         atomicOr(a.unclean, 1u);
-    }
     if (!R.there)
         return;
     T *O = (T *)a.dq + R.out(a, t.b);
-    const float back = poison ? NAN : HALF ? a.scale / up : a.scale;
+    const float down = poison ? NAN : HALF ? 1.f / up : 1.f;
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d)
         if (d * 16 + g * 4 < a.d)
-            ba_store4<T>(O + d * 16 + g * 4, acc[d] * back);
+            ba_store4<T>(O + d * 16 + g * 4, acc[d] * down * a.scale);
 }
 
 template <typename T, int DP>
@@ -1028,30 +1036,28 @@ struct BaKeys {
 };
 
 // CAREFUL: values of q and do that are not finite stay out of the products, and the keys that a row with such a value sees are
-// not numbers (poison); low: 1 or BA_LOW.
+// not numbers (poison).
 template <typename T, int DP, bool CAREFUL>
 __device__ __forceinline__ void ba_dkv_pass(const BaArgs &a, const BaKeys &w, const typename hd_vec<T>::v8 *kf, const typename hd_vec<T>::v8 *vf,
-                                            char *smem, int *list_all, unsigned long long *odd, float low,
-                                            hd_f4 *dk, hd_f4 *dv, float &up, bool &poison)
+                                            char *smem, int *list_all, unsigned long long *odd,
+                                            hd_f4 (&dk)[DP / 16], hd_f4 (&dv)[DP / 16], float &up, bool &poison)
 {
     typedef BaLds<T, DP> L;
     typedef typename hd_vec<T>::v8 V8;
     constexpr bool HALF = __is_same(T, _Float16);
     T *Qs = (T *)smem, *Gs = (T *)(smem + L::TILE);
-    float *top_s = (float *)(smem + 2 * L::TILE), *shift_s = top_s + 64, *delta_s = shift_s + 64, *gmax_s = delta_s + 64;
-    int *limit_s = (int *)(gmax_s + 64), *list = limit_s + 64;              // list: BD_WORDS * 64 queries
+    float *top_s = (float *)(smem + 2 * L::TILE), *shift_s = top_s + 64, *delta_s = shift_s + 64;
+    int *limit_s = (int *)(delta_s + 64), *list = limit_s + 64;              // list: BD_WORDS * 64 queries
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
     int skip = w.skip, take = w.take;
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d)
         dk[d] = dv[d] = hd_f4{0.f, 0.f, 0.f, 0.f};
-    up = 1.f;                               // fp16: dk is accumulated times this power of two
-    bool first = true;
+    up = BA_UP;                             // fp16: this lane's key's ds are taken times this power of two
 
     typedef BaStage<T, DP> S;
     S qr, gr;
-    BaStat row_stat = {0.f, 0.f};
-    float row_delta = 0.f, row_gmax = 0.f;
+    float row_top = 0.f, row_shift = 0.f, row_delta = 0.f;
     int row_limit = 0;
     const T *Q = S::lane((const T *)a.q.data + w.b * a.q.sb + (int64_t)w.h * a.group * a.q.sh, a.d);
     const T *G = S::lane((const T *)a.go.data + w.b * a.go.sb + (int64_t)w.h * a.group * a.go.sh, a.d);
@@ -1066,15 +1072,13 @@ __device__ __forceinline__ void ba_dkv_pass(const BaArgs &a, const BaKeys &w, co
             qr.r[x] = *(const V8 *)(Q + i * a.q.sr + e * a.q.sh);
             gr.r[x] = *(const V8 *)(G + i * a.go.sr + e * a.go.sh);
         }
-        row_stat = {0.f, 0.f};
-        row_delta = row_gmax = 0.f;
+        row_top = row_shift = row_delta = 0.f;
         row_limit = 0;
         if (threadIdx.x < BA_ROWS && r0 + (int)threadIdx.x < rows) {
             const int r = r0 + threadIdx.x, q = r / a.group, head = w.h * a.group + (r - q * a.group), i = list[q];
             const int64_t p = ((int64_t)w.b * a.hq + head) * a.m + i;
-            row_stat = ba_get_row(a, p), row_delta = a.delta[p], row_limit = ba_limit(a, w.live, w.lm, i);
-            if (HALF)
-                row_gmax = a.gmax[p];
+            row_top = a.lse[2 * p], row_shift = a.row[2 * p], row_delta = a.row[2 * p + 1];
+            row_limit = ba_limit(a, w.live, w.lm, i);
         }
     };
 
@@ -1114,10 +1118,8 @@ __device__ __forceinline__ void ba_dkv_pass(const BaArgs &a, const BaKeys &w, co
                 gr.store(Gs);
             }
             if (threadIdx.x < BA_ROWS) {
-                top_s[threadIdx.x] = row_stat.top, shift_s[threadIdx.x] = row_stat.shift;
+                top_s[threadIdx.x] = row_top, shift_s[threadIdx.x] = row_shift;
                 delta_s[threadIdx.x] = row_delta, limit_s[threadIdx.x] = row_limit;
-                if (HALF)
-                    gmax_s[threadIdx.x] = row_gmax;
             }
             __syncthreads();
             if (r0 + BA_ROWS < rows)
@@ -1125,22 +1127,6 @@ __device__ __forceinline__ void ba_dkv_pass(const BaArgs &a, const BaKeys &w, co
             if constexpr (CAREFUL)
                 for (unsigned long long left = *odd; left; left &= left - 1)
                     poison |= w.key < limit_s[__ffsll(left) - 1];
-            if (HALF) {
-                // the largest |do| of the rows so far decides the power of two (every wave finds the same)
-                float m = gmax_s[lane];
-#pragma unroll
-                for (int o = 32; o > 0; o >>= 1)
-                    m = fmaxf(m, __shfl_xor(m, o, 64));
-                const float want = ba_pow2_inverse(m) * low;
-                if (m > 0.f && (first || want < up)) {
-                    if (!first)
-#pragma unroll
-                        for (int d = 0; d < DP / 16; ++d)
-                            dk[d] *= want / up;
-                    up = want;
-                    first = false;
-                }
-            }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {   // 32 rows at a time
                 hd_f4 p[2], ds[2];
@@ -1169,8 +1155,18 @@ __device__ __forceinline__ void ba_dkv_pass(const BaArgs &a, const BaKeys &w, co
                         const float e = ba_power<T>(a, s[r] - to[r], sh[r]);
                         const float f = e * (dp[r] - de[r]);
                         p[x][r] = see ? e : 0.f;
-                        ds[x][r] = see ? (HALF ? f * up : f) : 0.f;
+                        ds[x][r] = see ? f : 0.f;
                     }
+                }
+                if constexpr (HALF) {
+                    float big = 0.f;
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            big = fmaxf(big, fabsf(ds[x][r]));
+                    ba_lower(ba_col_max(big), up, dk);
+                    ds[0] *= up, ds[1] *= up;
                 }
                 const V8 pf = ba_pack<T>(p[0], p[1]), sf = ba_pack<T>(ds[0], ds[1]);
                 // 16-bit types: what their rounding took, as a second term (one term alone: gradients off by 1.4 - 1.6 times
@@ -1252,14 +1248,9 @@ __device__ __forceinline__ void ba_dkv_part(const BaArgs &a, int64_t id, char *s
                 finite &= ba_finite(dk[d][r]) && ba_finite(dv[d][r]);
         return ba_col_max(finite || poison ? 0.f : 1.f) > 0.f;
     };
-    ba_dkv_pass<T, DP, CAREFUL>(a, w, kf, vf, smem, list_all, odd, 1.f, dk, dv, up, poison);
+    ba_dkv_pass<T, DP, CAREFUL>(a, w, kf, vf, smem, list_all, odd, dk, dv, up, poison);
     if constexpr (CAREFUL) {
         poison = ba_col_max(poison ? 1.f : 0.f) > 0.f;
-        const bool bad = HALF && reached();
-        if (HALF && __syncthreads_or(bad)) {
-            ba_dkv_pass<T, DP, true>(a, w, kf, vf, smem, list_all, odd, bad ? BA_LOW : 1.f, dk, dv, up, poison);
-            poison = ba_col_max(poison ? 1.f : 0.f) > 0.f;
-        }
         if (poison)
 #pragma unroll
             for (int d = 0; d < DP / 16; ++d)
@@ -1267,12 +1258,20 @@ __device__ __forceinline__ void ba_dkv_part(const BaArgs &a, int64_t id, char *s
     } else if (reached()) {
         atomicOr(a.unclean, 1u);
     }
-    const float back = HALF ? a.scale / up : a.scale;
+    // (fp16: probabilities came times 2^BA_P_SHIFT)
+    constexpr float P_DOWN = HALF ? 1.f / 32768.f : 1.f;
+    const float down = HALF ? P_DOWN / up : 1.f;
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) {
+        dk[d] = dk[d] * down * a.scale;
+        if (HALF)
+            dv[d] *= P_DOWN;
+    }
     if (parts > 1) {                        // joined by block_attn_dkv_join_kernel
         float *P = a.part + (part * 2 * BA_BLOCK + wave * 16 + l15) * DP;
 #pragma unroll
         for (int d = 0; d < DP / 16; ++d) {
-            *(hd_f4 *)(P + d * 16 + g * 4) = dk[d] * back;
+            *(hd_f4 *)(P + d * 16 + g * 4) = dk[d];
             *(hd_f4 *)(P + BA_BLOCK * DP + d * 16 + g * 4) = dv[d];
         }
         return;
@@ -1283,7 +1282,7 @@ __device__ __forceinline__ void ba_dkv_part(const BaArgs &a, int64_t id, char *s
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d)
         if (d * 16 + g * 4 < a.d) {
-            ba_store4<T>((T *)a.out + at + d * 16 + g * 4, dk[d] * back);
+            ba_store4<T>((T *)a.out + at + d * 16 + g * 4, dk[d]);
             ba_store4<T>((T *)a.out2 + at + d * 16 + g * 4, dv[d]);
         }
 }
@@ -1440,7 +1439,7 @@ template <typename T, int DP> int ba_backward(BaArgs a, void *dq, void *dk, void
 {
     const int64_t tiles = (int64_t)a.b * a.hk * a.tiles, blocks = (int64_t)a.b * a.hk * a.nb;
     const int64_t parts = a.chunk ? ba_dkv_parts(a.b, a.m, a.hk, a.nb, a.count) : blocks;
-    const size_t lds = ba_lds(a, 2 * BaLds<T, DP>::TILE), lds2 = 2 * BaLds<T, DP>::TILE + 5 * 64 * 4 + (size_t)BD_WORDS * 64 * 4;
+    const size_t lds = ba_lds(a, 2 * BaLds<T, DP>::TILE), lds2 = 2 * BaLds<T, DP>::TILE + 4 * 64 * 4 + (size_t)BD_WORDS * 64 * 4;
     const size_t most = lds > lds2 ? lds : lds2;
     int rc = ba_allow(block_attn_dq_kernel<T, DP>, lds);
     if (!rc)
@@ -1508,9 +1507,9 @@ extern "C" int tpu3_block_attn_fwd(tpu3_stream_t stream, int type, int b, int m,
 }
 
 namespace {
-// the pieces of the backward workspace: bits, delta, gmax, unclean, picks, first, part
+// the pieces of the backward workspace: bits, row, unclean, picks, first, part
 struct BaBwdLayout {
-    size_t delta, gmax, unclean, picks, first, part, bytes;
+    size_t row, unclean, picks, first, part, bytes;
 };
 BaBwdLayout ba_bwd_layout(int b, int m, int n, int hq, int hk, int d, int count)
 {
@@ -1518,9 +1517,8 @@ BaBwdLayout ba_bwd_layout(int b, int m, int n, int hq, int hk, int d, int count)
     const bool parts = ba_dkv_chunk(b, m, hk, (int)nb, count) > 0;
     auto up = [](size_t x) { return (x + 15) / 16 * 16; };
     BaBwdLayout l;
-    l.delta = up(blocks * mt * 8);
-    l.gmax = l.delta + up((size_t)b * hq * m * 4);
-    l.unclean = l.gmax + up((size_t)b * hq * m * 4);
+    l.row = up(blocks * mt * 8);
+    l.unclean = l.row + up((size_t)b * hq * m * 8);
     l.picks = l.unclean + 16;
     l.first = l.picks + (parts ? up(blocks * 4) : 0);
     l.part = l.first + (parts ? up((blocks + 1) * 4) : 0);
@@ -1554,8 +1552,7 @@ extern "C" int tpu3_block_attn_bwd(tpu3_stream_t stream, int type, int b, int m,
     const BaBwdLayout l = ba_bwd_layout(b, m, n, a.hq, a.hk, d, count);
     a.chunk = ba_dkv_chunk(b, m, a.hk, a.nb, count);
     a.bits = (uint64_t *)workspace;
-    a.delta = (float *)((char *)workspace + l.delta);
-    a.gmax = (float *)((char *)workspace + l.gmax);
+    a.row = (float *)((char *)workspace + l.row);
     a.unclean = (uint32_t *)((char *)workspace + l.unclean);
     a.picks = (int32_t *)((char *)workspace + l.picks);
     a.first = (int32_t *)((char *)workspace + l.first);

@@ -177,3 +177,61 @@ def test_rows_whose_scores_are_all_minus_infinity(dev, dtype, queries):
     alone = _run(ops, (q[:, keep], k, v), go[:, keep], blocks[:, keep])
     assert torch.equal(o[:, keep], alone[0]) and torch.isfinite(dk[0, :64]).all() and torch.isfinite(dv[0, :64]).all()
     assert torch.isfinite(dq[:, keep]).all()
+
+
+@pytest.mark.parametrize("size", [1.0, 1e-3, 1e-5])
+def test_fp16_gradients_of_small_values(dev, size):
+    """Values far below 1 (down to where the output itself is below fp16's normal numbers) and gradients of 256: score gradients
+    small against |do|, results that are normal numbers."""
+    ops = pkg("network.operations")
+    q, k, v, go, blocks = _inputs(dev, 1, 260, 1024, 2, 1, 128, 16, torch.float16, 21)
+    v, go = (size * v.float()).half(), 256 * go
+    scale = 128 ** -0.5
+    want = _formula(q, k, v, blocks, scale, False, go, torch.float64)
+    plain = _formula(q, k, v, blocks, scale, False, go, torch.float32)
+    got = _run(ops, (q, k, v), go, blocks)
+    for i, name in ((1, "dq"), (2, "dk"), (3, "dv")):
+        rows = want[i].shape[1]
+        worst = max((_error(got[i][:, r], want[i][:, r]) / _error(plain[i][:, r].half(), want[i][:, r]) for r in range(rows)))
+        here, there = _error(got[i], want[i]), _error(plain[i].half(), want[i])
+        print("%s: %.3g, plain %.3g, worst row %.3g of the plain form's" % (name, here, there, worst))
+        assert here <= 1.05 * there, (name, here, there)
+
+
+def test_fp16_gradients_of_keys_with_little_weight(dev):
+    """Every fourth key has e^-14 of the others' weight: its gradients are as exact, relative to them, as the others'."""
+    ops = pkg("network.operations")
+    q, k, v, go, blocks = _inputs(dev, 1, 300, 1024, 1, 1, 64, 16, torch.float16, 22)
+    q[..., 0] = 4
+    k[..., 0] = 0
+    k[:, ::4, :, 0] = -28
+    go = 256 * go
+    want = _formula(q, k, v, blocks, 0.125, False, go, torch.float64)
+    plain = _formula(q, k, v, blocks, 0.125, False, go, torch.float32)
+    got = _run(ops, (q, k, v), go, blocks)
+    few = torch.zeros((1, 1024), dtype=torch.bool, device=dev)
+    few[:, ::4] = True
+    for i, name in ((2, "dk"), (3, "dv")):
+        here, there = _error(got[i], want[i], few), _error(plain[i].half(), want[i], few)
+        print("%s: %.3g, plain %.3g" % (name, here, there))
+        assert here <= 1.05 * there, (name, here, there)
+
+
+@pytest.mark.parametrize("large", [60000.0, math.inf])
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_a_large_gradient_leaves_unseeing_keys_alone(dev, dtype, large):
+    """One query's output gradient is very large, or infinite, beside gradients of 1e-4: the keys that it does not see have the
+    gradients they have without it, to the bit."""
+    ops = pkg("network.operations")
+    q, k, v, go, _ = _inputs(dev, 1, 256, 256, 2, 1, 64, 1, TYPES[dtype], 23)
+    go = 1e-4 * go
+    blocks = torch.arange(4, dtype=torch.int32, device=dev).expand(1, 256, 1, 4)
+    for i in (20, 150):
+        pair = [go.clone(), go.clone()]
+        pair[0][0, i, 1] = large
+        pair[1][0, i, 1] = 0
+        _, dq, dk, dv = _run(ops, (q, k, v), pair[0], blocks, causal=True)
+        _, dq2, dk2, dv2 = _run(ops, (q, k, v), pair[1], blocks, causal=True)
+        assert torch.equal(dk[0, i + 1:], dk2[0, i + 1:]) and torch.equal(dv[0, i + 1:], dv2[0, i + 1:])
+        others = torch.arange(256, device=dev) != i
+        assert torch.equal(dq[0, others], dq2[0, others])
