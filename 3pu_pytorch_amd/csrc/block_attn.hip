@@ -517,15 +517,20 @@ template <typename T> __device__ __forceinline__ float ba_power(const BaArgs &a,
         e = __builtin_fmaf(d, a.scale2_rest, e);
     return __builtin_amdgcn_exp2f(e);
 }
+// The forward's weights are 2^shift at the most.  2^-13: a row adds up at most 64 blocks of 64 keys, so that no sum of weighted
+// values leaves the range that the values are in (at 1, 20 blocks of values of 3e38 came out infinite).  fp16, whose sums are
+// far from fp32's ends: 2^15, for the terms' sake (2^-14 is its last normal number).
+template <typename T> __device__ __forceinline__ constexpr float ba_weight_shift() { return __is_same(T, _Float16) ? 15.f : -13.f; }
+
 // what the backward pass takes of a row's softmax
 struct BaStat {
     float top, shift;                       // p = ba_power(score - top, shift): the largest score, minus log2 of the sum
 };
 // A row without weights (nothing seen, or scores of -infinity only; its output is 0): 2^(score - inf) = 0, also for scores of
 // -infinity.  A sum that is not a number: no more is p.
-__device__ __forceinline__ void ba_put_row(const BaArgs &a, int64_t row, float top, float sum)
+template <typename T> __device__ __forceinline__ void ba_put_row(const BaArgs &a, int64_t row, float top, float sum)
 {
-    a.lse[2 * row] = sum == 0.f ? 0.f : top, a.lse[2 * row + 1] = sum == 0.f ? -INFINITY : -log2f(sum);
+    a.lse[2 * row] = sum == 0.f ? 0.f : top, a.lse[2 * row + 1] = sum == 0.f ? -INFINITY : ba_weight_shift<T>() - log2f(sum);
 }
 __device__ __forceinline__ bool ba_finite(float x) { return fabsf(x) <= 3.4028235e38f; }
 
@@ -572,7 +577,7 @@ __device__ __forceinline__ void ba_fwd_block(const BaArgs &a, const BaRow &R, co
     auto weight = [&](int x) __attribute__((always_inline)) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            s[x][r] = ba_power<T>(a, s[x][r] - off, 0.f);
+            s[x][r] = ba_power<T>(a, s[x][r] - off, ba_weight_shift<T>());
             if (CAREFUL)
                 s[x][r] = bit ? s[x][r] : 0.f;
         }
@@ -705,7 +710,7 @@ __global__ __launch_bounds__(BA_THREADS, (BaFwd<T, DP>::w)) void block_attn_fwd_
         if (d * 16 + g * 4 < a.d)
             ba_store_rest<T>((T *)a.out + at, (T *)a.rest + at, a.rest != nullptr, d * 16 + g * 4, acc[d] * inv);
     if (a.lse && g == 0)
-        ba_put_row(a, R.flat(a, t.b), top, sum);
+        ba_put_row<T>(a, R.flat(a, t.b), top, sum);
 }
 
 // Joins the splits of a row, RL lanes a row (16, or a wave for more splits): a lane per split forms the splits' factors, then a
@@ -737,7 +742,7 @@ __global__ __launch_bounds__(BA_THREADS) void block_attn_join_kernel(BaArgs a, i
     const int64_t i = row % a.m, bh = row / a.m, h = bh % a.hq, b = bh / a.hq;
     const int64_t at = ((b * a.m + i) * a.hq + h) * a.d;
     if (a.lse && lane == 0)
-        ba_put_row(a, row, top, sum);
+        ba_put_row<T>(a, row, top, sum);
     if (lane * W >= a.d)
         return;
     float y[W] = {};

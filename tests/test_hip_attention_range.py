@@ -235,3 +235,19 @@ def test_a_large_gradient_leaves_unseeing_keys_alone(dev, dtype, large):
         assert torch.equal(dk[0, i + 1:], dk2[0, i + 1:]) and torch.equal(dv[0, i + 1:], dv2[0, i + 1:])
         others = torch.arange(256, device=dev) != i
         assert torch.equal(dq[0, others], dq2[0, others])
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("queries", [70, 1])
+def test_values_at_the_types_end(dev, dtype, queries):
+    """A mean of values near the largest number of the type is near it, and no sum on the way to it leaves the range."""
+    ops = pkg("network.operations")
+    dt = TYPES[dtype]
+    q, k, _, _, blocks = _inputs(dev, 1, queries, 2000, 2, 1, 64, 20, dt, 8)
+    top = 65504.0 if dt == torch.float16 else 3e38
+    v = torch.full((1, 2000, 1, 64), top, device=dev).to(dt)
+    v[..., ::2] *= -1
+    o = ops.block_attention(q, k, v, blocks).double()
+    want = v[:, :1].double()
+    # the denominator and the numerator add up the same terms: (2000 + 2) 2^-24 each at the most, 2^-17 for the terms, the last rounding
+    assert ((o - want).abs() <= (torch.finfo(dt).eps + 2.0 ** -12) * want.abs()).all()
