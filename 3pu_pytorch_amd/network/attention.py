@@ -14,7 +14,8 @@ heads shares a key head and its blocks).  n_arr / m_arr: int32 device tensors of
 in the ragged point-set calls.  causal: query i stands at key position n - m + i (live lengths) and sees the keys up to it.
 Rows near each other should hold points near each other (a space-filling order, a sequence): a block is then a neighbourhood.
 
-Device tensors only; everything runs on the current stream of the tensors' device and can be captured into a graph (a backward
+Gradients are those of reverse mode, once; where there are any, an input with a tangent of forward mode is refused.  Device
+tensors only; everything runs on the current stream of the tensors' device and can be captured into a graph (a backward
 pass: torch.autograd.grad, or backward() while no eager graph of the same leaves is alive, which torch itself cannot capture).
 Results do not depend on the order in which workgroups run.
 
@@ -25,6 +26,7 @@ types take probabilities and score gradients into the second matrix products in 
 import math
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import _lib as L
@@ -46,6 +48,15 @@ def _rows(t, name, like=None):
     if d == 0 or d % 8:
         raise RuntimeError("%s: D must be a multiple of 8, got %d" % (name, d))
     return t
+
+
+def _no_tangents(*tensors):
+    """There is no forward-mode derivative: the kernels' results would carry none, which means 0."""
+    if getattr(forward_ad, "_current_level", 0) < 0:
+        return                                          # (no dual level is open: no tensor has a tangent)
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("forward-mode derivatives are not offered: an input carries a tangent")
 
 
 def _taken(t):
@@ -140,6 +151,7 @@ class _NormRotate(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, gq, gk):
+        _no_tangents(gq, gk)
         q, k, wq, wk, position, freq = ctx.saved_tensors
         q, k, gq = _taken(q), _taken(k), _taken(gq)
         gk = None if k is None else _taken(gk)
@@ -217,6 +229,7 @@ def norm_rotate(q, k, q_weight, k_weight, position, freq, eps=1e-6, interleaved=
     if position.dim() != 3 or freq.dim() != 2 or position.shape != (b, n, freq.shape[0]) or freq.shape[0] == 0:
         raise RuntimeError("norm_rotate: position %s and freq %s do not fit %d x %d rows"
                            % (tuple(position.shape), tuple(freq.shape), b, n))
+    _no_tangents(q, k, q_weight, k_weight, position, freq)
     if 2 * freq.numel() > d:
         raise RuntimeError("norm_rotate: %d pairs need more than %d channels" % (freq.numel(), d))
     args = (q, k, wq, wk, position, freq.contiguous(), float(eps), int(bool(interleaved)))
@@ -339,6 +352,7 @@ class _BlockAttention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, go):
+        _no_tangents(go)
         q, k, v, o, lse, rest, blocks, n_arr, m_arr = ctx.saved_tensors
         q, k, v, o, go = (_taken(t) for t in (q, k, v, o, go))
         b, m, hq, d = q.shape
@@ -363,6 +377,7 @@ def _attention(q, k, v, *args):
 def _check_attention(q, k, v, scale, n_arr, m_arr):
     q = _rows(q, "q")
     k, v = _rows(k, "k", q), _rows(v, "v", q)
+    _no_tangents(q, k, v)
     b, m, hq, d = q.shape
     if v.shape != k.shape or k.shape[0] != b or k.shape[3] != d:
         raise RuntimeError("q %s, k %s and v %s do not match" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))

@@ -251,3 +251,33 @@ def test_values_at_the_types_end(dev, dtype, queries):
     want = v[:, :1].double()
     # the denominator and the numerator add up the same terms: (2000 + 2) 2^-24 each at the most, 2^-17 for the terms, the last rounding
     assert ((o - want).abs() <= (torch.finfo(dt).eps + 2.0 ** -12) * want.abs()).all()
+
+
+def test_forward_mode_derivatives_are_refused(dev):
+    """The kernels have no forward-mode derivative: an input that carries a tangent is refused, not taken for a constant."""
+    import torch.autograd.forward_ad as fw
+    ops = pkg("network.operations")
+    gen = torch.Generator(device=dev).manual_seed(1)
+    q, k, v = _randn(gen, 1, 4, 2, 16), _randn(gen, 1, 130, 1, 16), _randn(gen, 1, 130, 1, 16)
+    kq, w = _randn(gen, 1, 4, 1, 16), _randn(gen, 16)
+    pos, freq = torch.arange(4.0, device=dev).view(1, 4), ops.rotation_frequencies(1, 8, device=dev)
+    blocks = torch.zeros((1, 4, 1, 2), dtype=torch.int32, device=dev)
+    calls = [(lambda *a: ops.norm_rotate(*a)[0], (q, kq, w, w, pos, freq)),
+             (lambda *a: ops.block_attention(*a, blocks), (q, k, v)),
+             (lambda *a: ops.sparse_attention(*a, 2), (q, k, v))]
+    for call, args in calls:
+        plain = call(*args)
+        with fw.dual_level():
+            assert torch.equal(call(*args), plain)                          # (no tangents: as ever)
+            for i in range(len(args)):
+                some = [fw.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(args)]
+                with pytest.raises(RuntimeError, match="tangent|forward"):
+                    call(*some)
+    # a tangent in the gradient that a backward pass starts from
+    for call, args in calls[:2]:
+        leaf = args[0].clone().requires_grad_()
+        out = call(leaf, *args[1:])
+        with fw.dual_level():
+            go = fw.make_dual(torch.ones_like(out), torch.ones_like(out))
+            with pytest.raises(RuntimeError, match="tangent|forward"):
+                torch.autograd.grad(out, leaf, go)
