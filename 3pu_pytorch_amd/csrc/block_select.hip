@@ -26,9 +26,9 @@ __global__ __launch_bounds__(BS_THREADS) void block_means_kernel(int n, int d, i
     __shared__ double red[BS_THREADS * 8];
     const int b = blockIdx.x / blocks, j = blockIdx.x - b * blocks;
     const int live = n_arr ? min(max(n_arr[b], 0), n) : n;
-    // all blocks, or from the block of the first of the `last` newest rows on
+    // all blocks, or those that hold one of the `last` newest rows
     const int blk = j + (last >= 0 ? max(0, live - last) / BS_BLOCK : 0);
-    if (blk >= nb)
+    if (blk >= nb || (last >= 0 && blk * BS_BLOCK >= live))
         return;
     const int rows = min(BS_BLOCK, live - blk * BS_BLOCK);
     const int chunks = k.heads * (d / 8);

@@ -281,3 +281,20 @@ def test_forward_mode_derivatives_are_refused(dev):
             go = fw.make_dual(torch.ones_like(out), torch.ones_like(out))
             with pytest.raises(RuntimeError, match="tangent|forward"):
                 torch.autograd.grad(out, leaf, go)
+
+
+def test_kept_means_behind_the_newest_rows_are_left(dev):
+    """block_means(out=, last=) forms the blocks that hold the newest rows; those before and behind them keep what they hold."""
+    ops = pkg("network.operations")
+    gen = torch.Generator(device=dev).manual_seed(3)
+    k = _randn(gen, 5, 400, 2, 32)
+    live = [64, 100, 65, 400, 0]
+    lens = torch.tensor(live, dtype=torch.int32, device=dev)
+    for last in (1, 2, 64, 65, 130, 1000):
+        out = torch.full((5, 7, 2, 32), 7.0, device=dev)
+        ops.block_means(k, lens, out=out, last=last)
+        want = orc64.means(k, lens).float()
+        for e, n in enumerate(live):
+            first, end = max(0, n - last) // 64, -(-n // 64)
+            assert torch.equal(out[e, first:end], want[e, first:end])
+            assert (out[e, :first] == 7).all() and (out[e, end:] == 7).all()
