@@ -764,7 +764,9 @@ extern "C" int tpu3_block_select(tpu3_stream_t stream, int type, int b, int m, i
     const bool many = a.nb > 0 && bs_many(b, m, hk, a.nb);
     if (many)
         a.splits = 1;
-    if (rows * a.splits > 0x7FFFFFFFLL || (!many && rows * a.splits >= 1 << 24))
+    // (2^32 threads a launch)
+    const int64_t workgroups = many ? ((int64_t)b * hk * ((m - 1) / 64 + 1) + 3) / 4 : rows * a.splits;
+    if (rows > 0x7FFFFFFFLL || workgroups >= 1 << 24)
         return TPU3_ELIMIT;
     const hipStream_t s = (hipStream_t)stream;
     if (many) {
