@@ -1416,16 +1416,22 @@ int ba_dp(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 
 size_t ba_lds(const BaArgs &a, size_t tiles) { return tiles + (size_t)a.cap * 12 + (size_t)((a.nb + 31) / 32) * 8; }
 
-template <typename K> int ba_allow(K kernel, size_t lds)
+// The most that a launch of any size needs, the same in every call: calls from several threads do not change each other's limit
+// between setting it and launching.
+template <typename T, int DP> constexpr size_t ba_lds_most()
 {
-    return (int)hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    return 2 * BaLds<T, DP>::TILE + (size_t)BA_ROWS * TPU3_BLOCK_COUNT_MAX * 12 + TPU3_ATTN_BLOCKS_MAX / 32 * 8;
+}
+template <typename T, int DP, typename K> int ba_allow(K kernel)
+{
+    return (int)hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)ba_lds_most<T, DP>());
 }
 
 template <typename T, int DP> int ba_forward(const BaArgs &a, hipStream_t s)
 {
     const int64_t all = (int64_t)a.b * a.hk * a.tiles * a.splits;
     const size_t lds = ba_lds(a, 2 * BaLds<T, DP>::TILE);
-    int rc = ba_allow(block_attn_fwd_kernel<T, DP>, lds);
+    int rc = ba_allow<T, DP>(block_attn_fwd_kernel<T, DP>);
     if (rc)
         return rc;
     hipLaunchKernelGGL((block_attn_fwd_kernel<T, DP>), dim3((unsigned)all), dim3(BA_THREADS), lds, s, a, all);
@@ -1446,11 +1452,12 @@ template <typename T, int DP> int ba_backward(BaArgs a, void *dq, void *dk, void
     const int64_t parts = a.chunk ? ba_dkv_parts(a.b, a.m, a.hk, a.nb, a.count) : blocks;
     const size_t lds = ba_lds(a, 2 * BaLds<T, DP>::TILE), lds2 = 2 * BaLds<T, DP>::TILE + 4 * 64 * 4 + (size_t)BD_WORDS * 64 * 4;
     const size_t most = lds > lds2 ? lds : lds2;
-    int rc = ba_allow(block_attn_dq_kernel<T, DP>, lds);
+    static_assert(2 * BaLds<T, DP>::TILE + 4 * 64 * 4 + (size_t)BD_WORDS * 64 * 4 <= ba_lds_most<T, DP>(), "");
+    int rc = ba_allow<T, DP>(block_attn_dq_kernel<T, DP>);
     if (!rc)
-        rc = ba_allow(block_attn_dkv_kernel<T, DP>, lds2);
+        rc = ba_allow<T, DP>(block_attn_dkv_kernel<T, DP>);
     if (!rc)
-        rc = ba_allow(block_attn_careful_kernel<T, DP>, most);
+        rc = ba_allow<T, DP>(block_attn_careful_kernel<T, DP>);
     if (rc)
         return rc;
     a.dq = dq, a.out = dk, a.out2 = dv;

@@ -665,6 +665,7 @@ template <typename T, int DP, bool LOQ> int bs_many_launch(const BsArgs &a, hipS
     const int qtiles = (a.m + 63) / 64, k = a.count - a.causal;
     const int64_t waves = (int64_t)a.b * a.hk * qtiles;
     size_t lds;
+    const int most = 4 * 64 * (BT_STRIDE + 64) * 4;             // the same in every call: another thread's does not lower it
     const dim3 grid((unsigned)((waves + 3) / 4));
     hipError_t e = hipSuccess;
 #define BT_GO(NL, IDS)                                                                                                   \
@@ -672,7 +673,7 @@ template <typename T, int DP, bool LOQ> int bs_many_launch(const BsArgs &a, hipS
         const int places = IDS ? (NL > a.count ? NL : a.count) : a.count + BT_MORE < 64 ? a.count + BT_MORE : 64;        \
         lds = (size_t)4 * 64 * (BT_STRIDE + (places > a.count ? places : a.count)) * 4;                                  \
         e = hipFuncSetAttribute((const void *)block_select_many_kernel<T, DP, NL, LOQ, IDS>,                             \
-                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);                                   \
+                                hipFuncAttributeMaxDynamicSharedMemorySize, most);                                       \
         if (e == hipSuccess)                                                                                             \
             hipLaunchKernelGGL((block_select_many_kernel<T, DP, NL, LOQ, IDS>), grid, dim3(BS_THREADS), lds, s, a, qtiles, waves); \
     }

@@ -466,7 +466,8 @@ template <typename T> int nr_backward(const NrArgs &a, const NrPlan &p, hipStrea
                     : p.lpr == 8 ? (const void *)norm_rotate_bwd_kernel<T, 8>
                     : p.lpr == 16 ? (const void *)norm_rotate_bwd_kernel<T, 16>
                                   : (const void *)norm_rotate_bwd_kernel<T, 32>;
-    const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds);
+    // (the same in every call: another thread's does not lower it)
+    const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)NR_LDS);
     if (e != hipSuccess)
         return (int)e;
 #define NR_GO(L) hipLaunchKernelGGL((norm_rotate_bwd_kernel<T, L>), dim3(p.wgs), dim3(NR_THREADS), p.lds, s, a, p.split)

@@ -298,3 +298,29 @@ def test_kept_means_behind_the_newest_rows_are_left(dev):
             first, end = max(0, n - last) // 64, -(-n // 64)
             assert torch.equal(out[e, first:end], want[e, first:end])
             assert (out[e, :first] == 7).all() and (out[e, end:] == 7).all()
+
+
+def test_from_two_threads(dev):
+    """Calls of the same kernels with small and large workgroup memory from two threads, each on its own stream."""
+    ops = pkg("network.operations")
+    few = _inputs(dev, 1, 64, 4096, 1, 1, 64, 1, torch.bfloat16, 70)
+    many = _inputs(dev, 1, 64, 4096, 1, 1, 64, 64, torch.bfloat16, 71)
+    want = [_run(ops, s[:3], s[3], s[4]) for s in (few, many)]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i, s):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(300):
+                    got = _run(ops, s[:3], s[3], s[4])
+                torch.cuda.current_stream().synchronize()
+                wrong.extend(i for a, c in zip(got, want[i]) if not torch.equal(a, c))
+        except RuntimeError as e:
+            wrong.append(e)
+    threads = [threading.Thread(target=work, args=x) for x in enumerate((few, many))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
