@@ -342,6 +342,13 @@ constexpr int BT_NEAR = 1 << 30;            // marks them
 constexpr int BT_EXTRA = 4;                 // with numbers: places behind the k + 1st
 constexpr int BT_STRIDE = 20;               // floats between two queries' 16 scores in LDS
 
+// LDS accesses above and below stay there: between the lanes of one wave nothing more is needed (they complete in order)
+__device__ __forceinline__ void bt_exchange()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 struct BtSplit {
     hd_bf8 hi, lo;
 };
@@ -476,8 +483,7 @@ __global__ __launch_bounds__(BS_THREADS) void block_select_many_kernel(BsArgs a,
             }
             *(hd_f4 *)(sc + (sub * 16 + l15) * BT_STRIDE + g * 4) = c;
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();    // (one wave: its LDS accesses complete in order)
+        bt_exchange();
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const hd_f4 v = *(const hd_f4 *)(sc + lane * BT_STRIDE + j * 4);
@@ -485,8 +491,7 @@ __global__ __launch_bounds__(BS_THREADS) void block_select_many_kernel(BsArgs a,
             for (int r = 0; r < 4; ++r)
                 x[j * 4 + r] = v[r];
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        bt_exchange();
     };
 
     float best[NL];                         // descending; the first NL - 1 - EXTRA - k places are held by infinities
@@ -565,6 +570,7 @@ __global__ __launch_bounds__(BS_THREADS) void block_select_many_kernel(BsArgs a,
     }
     open |= !plain && at > places;
     open &= i < lm;
+    bt_exchange();                          // lanes read what others found
     for (unsigned long long left = __ballot(!plain && !open && i < lm); left; left &= left - 1) {
         const int f = __ffsll(left) - 1, all = __shfl(at, f, 64), want = k - __shfl(certain, f, 64);
         const int mine = lane < all ? found[lane * 64 + f] : 0;
@@ -604,6 +610,7 @@ __global__ __launch_bounds__(BS_THREADS) void block_select_many_kernel(BsArgs a,
             found[__popcll(kept & ((1ull << lane) - 1)) * 64 + f] = mine & ~BT_NEAR;
         at = lane == f ? __popcll(kept) : at;
     }
+    bt_exchange();                          // and this lane's list as others left it
     at = min(at, k);                        // (open queries may hold more)
     if constexpr (IDS) {                    // ascending
         int id[NL - 1 - EXTRA];
@@ -629,8 +636,7 @@ __global__ __launch_bounds__(BS_THREADS) void block_select_many_kernel(BsArgs a,
     const unsigned long long opened = __ballot(open);
     if (lane == 0)
         a.open[w] = opened;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    bt_exchange();
     int32_t *out = a.out + (((int64_t)b * a.m + i0) * a.hk + h) * a.count;
     const int rows = min(64, a.m - i0);
     for (int e = lane; e < rows * a.count; e += 64) {
