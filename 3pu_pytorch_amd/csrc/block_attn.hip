@@ -7,13 +7,16 @@
 //
 // Forward and dq: a workgroup takes 64 rows = 64 / group queries of one key head with all heads of the group (they share
 // the picked blocks), forms the UNION of the rows' blocks in LDS with one bit per query, and runs over it once, with the
-// running maximum and sum of the softmax.  A block that no row of a wave picked is skipped by that wave; the mask of the
-// others costs a select a score.  Queries that are near each other pick nearly the same blocks -- points in a spatial
-// order, tokens in a sequence, the heads of a group always -- so the union is a few blocks larger than one query's set,
-// and a block's keys and values are read once for 64 rows.
-// dk, dv: a workgroup per block of keys gathers the rows that picked it (a bit matrix, blocks by queries, written by
-// block_pick_bits_kernel) and runs over them densely.  Nothing is added up with atomics: results do not depend on the order
-// in which workgroups run.
+// running maximum and sum of the softmax.  A block that no row of a wave picked is skipped by that wave; in the others a row
+// that did not pick it subtracts infinity from its scores (forward; no instruction more a score) or takes zeros (dq; a select a
+// score).  A block's keys and values are read once for 64 rows.  What that costs is the union: queries that are near each other
+// pick some of the same blocks -- points in a spatial order, tokens in a sequence, the heads of a group always.  Blocks a query /
+// of a wave's 16 rows / of the 64: clouds of 5000 points in the order of a space-filling curve 8 / 16 / 24, rows of a level over
+// another's merged cloud 5 / 11 / 20, a causal sequence of 8192 rows 16 / 23 / 30.  Where neighbouring rows are far apart (the
+// same clouds shuffled: 8 / 58 / 76 of 79) all is worked on, and a call takes 2.2 times as long.
+// dk, dv: a workgroup per block of keys, or, up to 1024 blocks, per part of its queries (ba_dkv_chunk), gathers the rows that
+// picked it (a bit matrix, blocks by queries, written by block_pick_bits_kernel) and runs over them densely.  Nothing is added
+// up with atomics: results do not depend on the order in which workgroups run.
 //
 // Matrix instructions: 16x16x32 on the 16-bit types, 16x16x4 on fp32 (eight of them per 32 channels); accumulators, the
 // softmax and all sums in fp32.  Scores are formed transposed (keys x rows): a lane then holds 16 scores of ONE row, the
@@ -269,7 +272,7 @@ template <typename T, int DP> struct BaStage {
 // How a kernel is laid out over registers and LDS; w: waves a SIMD that the register allocation aims at.  More waves hide
 // more of the chain scores -> maximum -> exponentials -> product, until the operands no longer fit: measured on clouds
 // of 5000 points (64 channels) and a sequence of 8192 (128), us with 2 / 3 / 4 waves: forward - / 144 / 129 and
-// 310 / 279 / -, dq - / 94 / 99 and 341 / 520 / -, dk and dv - / 63 / 92 and 346 / 900 / - (both before their
+// 310 / 279 / -, dq - / 94 / 99 and 341 / 520 / -, dk and dv - / 63 / 92 and 346 / 900 / - (all before their
 // second terms); fp32 of 24 channels, forward, - / 59 / 49.  A wave has 16 rows (keys):
 // with 32, every operand read from LDS feeds two matrix instructions, but half as many waves are there (188 for 146).
 // together: 16-row tiles whose row operands are read in one go; columns: 16-channel columns read in one go.
@@ -1029,7 +1032,7 @@ __global__ __launch_bounds__(1024) void block_parts_kernel(BaArgs a, int blocks)
 }
 
 // ---- backward: dk, dv ----------------------------------------------------------------------------------------------------
-// A workgroup per block of keys; a wave owns 16 of its keys.  Scores are formed as rows x keys here, so that P and dS come
+// A workgroup per block of keys, or per part of the queries that picked it; a wave owns 16 of its keys.  Scores are formed as rows x keys here, so that P and dS come
 // out with a key per lane: the B operand of dv^T = do^T P and dk^T = q^T dS.
 constexpr int BD_WORDS = 64;                // tiles of queries looked through at a time
 

@@ -15,9 +15,10 @@
 // goes through LDS with its first half stored a second time behind the second, so that the partner of channel c is always
 // channel c + P (P pairs; lane exchanges where P is a multiple of eight).
 // The next row is requested before the current one is worked on (a wave otherwise has 1 KB in flight, and the chip 7 MB).
-// Results are stored past the caches, so that the inputs stay there for the backward pass: a cloud of 80000 points (8 + 8
-// heads of 64 channels, fp16) 92 -> 67 us where they do; rotation and attention over it together 343 -> 339, over 4 clouds of
-// 5000 78 -> 77, over 16 297 -> 310, over 32 579 -> 580.
+// Results are stored past the caches: this kernel alone is faster for it, a program hardly, since who reads the results next
+// finds fewer of them cached.  us with ordinary stores / with these, 8 + 8 heads of 64 channels, bf16: a cloud of 80000 points,
+// rotation 101 / 76, with attention behind it 387 / 386, forward and backward 1953 / 1941; 16 clouds of 5000 100 / 73, 352 / 357,
+// 1290 / 1312; 8 clouds 41 / 40, 164 / 162, 668 / 679; 2 clouds 17 / 15, 55 / 54, 226 / 225.
 #include "heads.h"
 
 namespace {
@@ -101,7 +102,8 @@ template <int LPR> __device__ __forceinline__ float nr_row_sum(float v)
 }
 
 // Exchange rows, for halves whose length is no multiple of eight: channel c of a row sits at (c % 8) * slots + c / 8, so that
-// the lanes of a wave, which hold channels 8 l .. 8 l + 7, meet different banks whatever the shift is.  Lanes write whole
+// the lanes of a row, which hold channels 8 l .. 8 l + 7, meet different banks whatever the shift is.  The rows of a wave, 8 *
+// slots apart, may still share theirs (64 channels, 30 pairs: 112 words, so the rows four apart do).  Lanes write whole
 // groups of eight: what lies behind the second half is written over by the copy of the first, which is written after it, and
 // what a channel behind the pairs reads is not used.
 __host__ __device__ __forceinline__ int nr_slots(int d, int pairs) { return (d + pairs + 15) / 8 + 1; }
