@@ -1352,7 +1352,7 @@ int ba_fill(BaArgs &a, int type, int b, int m, int n, int d, const tpu3_heads *q
         (n > 0 && (n - 1) / BA_BLOCK + 1 > TPU3_ATTN_BLOCKS_MAX))
         return TPU3_ELIMIT;
     a.q = *q, a.k = *k, a.v = *v, a.blocks = blocks, a.n_arr = n_arr, a.m_arr = m_arr;
-    a.b = b, a.m = m, a.n = n, a.nb = n > 0 ? (n - 1) / BA_BLOCK + 1 : 0, a.mt = (m + 63) / 64;
+    a.b = b, a.m = m, a.n = n, a.nb = n > 0 ? (n - 1) / BA_BLOCK + 1 : 0, a.mt = m > 0 ? (m - 1) / 64 + 1 : 0;
     a.hq = q->heads, a.hk = k->heads, a.group = a.hq / a.hk, a.d = d, a.count = count, a.causal = causal != 0;
     a.scale = (float)scale, a.scale2 = (float)(scale * 1.44269504088896340736);
     if (type == TPU3_TYPE_F32 && (double)a.scale2 >= scale * 1.44269504088896340736)

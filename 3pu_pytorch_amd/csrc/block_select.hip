@@ -668,7 +668,7 @@ bool bs_many(int b, int m, int hk, int nb) { return m >= 16 && (int64_t)b * m * 
 
 template <typename T, int DP, bool LOQ> int bs_many_launch(const BsArgs &a, hipStream_t s)
 {
-    const int qtiles = (a.m + 63) / 64, k = a.count - a.causal;
+    const int qtiles = (a.m - 1) / 64 + 1, k = a.count - a.causal;
     const int64_t waves = (int64_t)a.b * a.hk * qtiles;
     size_t lds;
     const int most = 4 * 64 * (BT_STRIDE + 64) * 4;             // the same in every call: another thread's does not lower it
@@ -715,7 +715,7 @@ extern "C" int tpu3_block_means(tpu3_stream_t stream, int type, int b, int n, in
 {
     if (b < 0 || n < 0 || d <= 0 || !hd_type_ok(type) || !k || k->heads <= 0)
         return TPU3_EINVAL;
-    if (d % 8 || d > 128)
+    if (d % 8 || d > 128 || (int64_t)k->heads * d > 0x7FFFFFFF)
         return TPU3_ELIMIT;
     if (b == 0 || n == 0 || last == 0)
         return TPU3_OK;
@@ -773,7 +773,7 @@ extern "C" int tpu3_block_select(tpu3_stream_t stream, int type, int b, int m, i
         a.splits = 1;
     // (2^32 threads a launch)
     const int64_t workgroups = many ? ((int64_t)b * hk * ((m - 1) / 64 + 1) + 3) / 4 : rows * a.splits;
-    if (rows > 0x7FFFFFFFLL || workgroups >= 1 << 24)
+    if (rows > 0x7FFFFFFFLL || m > 0x7FFFFFFF - 63 || workgroups >= 1 << 24)
         return TPU3_ELIMIT;
     const hipStream_t s = (hipStream_t)stream;
     if (many) {

@@ -36,6 +36,8 @@ BLOCK = L.ATTN_BLOCK        # consecutive keys of a block
 
 def _rows(t, name, like=None):
     """The checks of a (B, rows, heads, D) tensor."""
+    if isinstance(t, torch.Tensor) and t.dim() and max(t.shape) > 0x7FFFFFFF:
+        raise RuntimeError("%s: dimensions of at most 2^31 - 1, got %s" % (name, tuple(t.shape)))
     if not isinstance(t, torch.Tensor) or t.get_device() < 0:
         raise RuntimeError("%s must be a CUDA tensor" % name)
     if t.dim() != 4:
