@@ -184,7 +184,7 @@ def norm_rotate(q, k, q_weight, k_weight, position, freq, eps=1e-6, interleaved=
         position  (B, N) or (B, N, axes): places in a sequence (int32 / int64) or coordinates (float32 / float64)
         freq      (axes, pairs) float32 / float64, 2 * axes * pairs <= D: pair axis * pairs + f turns by
                   position[axis] * freq[axis, f], an angle formed in 64 bits
-        eps       y = x / sqrt(mean(x^2) + eps) * weight
+        eps       y = x / sqrt(mean(x^2) + eps) * weight, the mean in float32: rows with elements beyond 1e19 come out as 0
         interleaved   partners of pair p are channels (2p, 2p + 1) instead of (p, p + axes * pairs)
     :return
         (q, k) of the inputs' shapes and types (k None if it was None)
