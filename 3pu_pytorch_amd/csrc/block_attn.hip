@@ -38,7 +38,7 @@ struct BaArgs {
     void *out, *out2, *dq;                  // forward: o; backward: dk, dv, dq (contiguous)
     void *rest;                             // 16-bit types, contiguous like o: what the rounding of o took (ba_rest_scale), for do . o
     float *lse;                             // (b, hq, m, 2): BaStat of the row
-    float *row;                             // (b, hq, m, 2): for dk, dv: shift of the row there, and do . o
+    float *row;                             // (b, hq, m, 2): for dk, dv: BaStat::by of the row there, and do . o
     uint64_t *bits;                         // (b, hk, nb, mt): bit = query of the tile of 64 picked the block
     float *part;                            // split forward: (rows, splits, d + 4); dk / dv in parts: (parts, 2, 64, d)
     int32_t *picks, *first;                 // dk / dv in parts: queries that picked a block; first part of a block, and the end
@@ -525,15 +525,23 @@ template <typename T> __device__ __forceinline__ float ba_power(const BaArgs &a,
 // far from fp32's ends: 2^15, for the terms' sake (2^-14 is its last normal number).
 template <typename T> __device__ __forceinline__ constexpr float ba_weight_shift() { return __is_same(T, _Float16) ? 15.f : -13.f; }
 
-// what the backward pass takes of a row's softmax
+// What the backward pass takes of a row's softmax: the largest score, and of the sum minus its log2, or in fp32, where the rounding
+// of a log2 of up to 12 is as much as all other roundings together (dq of 24 channels off by 1.9 times the plain form's), its
+// reciprocal.  A row without weights (nothing seen, or scores of -infinity only; its output is 0) has p = 0 whatever its scores
+// are; a sum that is not a number: no more is p.
 struct BaStat {
-    float top, shift;                       // p = ba_power(score - top, shift): the largest score, minus log2 of the sum
+    float top, by;
 };
-// A row without weights (nothing seen, or scores of -infinity only; its output is 0): 2^(score - inf) = 0, also for scores of
-// -infinity.  A sum that is not a number: no more is p.
+template <typename T> __device__ __forceinline__ float ba_probability(const BaArgs &a, float score, float top, float by)
+{
+    return sizeof(T) == 4 ? ba_power<T>(a, score - top, 0.f) * by : ba_power<T>(a, score - top, by);
+}
 template <typename T> __device__ __forceinline__ void ba_put_row(const BaArgs &a, int64_t row, float top, float sum)
 {
-    a.lse[2 * row] = sum == 0.f ? 0.f : top, a.lse[2 * row + 1] = sum == 0.f ? -INFINITY : ba_weight_shift<T>() - log2f(sum);
+    constexpr bool F32 = sizeof(T) == 4;
+    a.lse[2 * row] = sum == 0.f ? (F32 ? INFINITY : 0.f) : top;
+    a.lse[2 * row + 1] = F32 ? (sum == 0.f ? 0.f : 0x1p-13f / sum) : sum == 0.f ? -INFINITY : ba_weight_shift<T>() - log2f(sum);
+    static_assert(!F32 || ba_weight_shift<T>() == -13.f, "");
 }
 __device__ __forceinline__ bool ba_finite(float x) { return fabsf(x) <= 3.4028235e38f; }
 
@@ -810,7 +818,7 @@ __device__ __forceinline__ void ba_dq_block(const BaArgs &a, const BaRow &R, con
     for (int x = 0; x < 4; ++x)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-            s[x][r] = ba_power<T>(a, s[x][r] - stat.top, stat.shift) * (dp[x][r] - delta);
+            s[x][r] = ba_probability<T>(a, s[x][r], stat.top, stat.by) * (dp[x][r] - delta);
     if (__any(bit && k0 + BA_BLOCK > R.limit)) {
 #pragma unroll
         for (int x = 0; x < 4; ++x)
@@ -925,7 +933,7 @@ template <typename T, int DP, bool CAREFUL> __device__ __forceinline__ void ba_d
             const int64_t at = 2 * R.flat(a, t.b);
             stat = {a.lse[at], a.lse[at + 1]};
             if (g == 0)
-                a.row[at] = stat.shift + (HALF ? BA_P_SHIFT : 0.f), a.row[at + 1] = delta;
+                a.row[at] = stat.by + (HALF ? BA_P_SHIFT : 0.f), a.row[at + 1] = delta;
         }
     }
     const int count = ba_union(a, t, list, mask, words, before);
@@ -1032,8 +1040,8 @@ __global__ __launch_bounds__(1024) void block_parts_kernel(BaArgs a, int blocks)
 }
 
 // ---- backward: dk, dv ----------------------------------------------------------------------------------------------------
-// A workgroup per block of keys, or per part of the queries that picked it; a wave owns 16 of its keys.  Scores are formed as rows x keys here, so that P and dS come
-// out with a key per lane: the B operand of dv^T = do^T P and dk^T = q^T dS.
+// A workgroup per block of keys, or per part of the queries that picked it; a wave owns 16 of its keys.  Scores are formed as
+// rows x keys here, so that P and dS come out with a key per lane: the B operand of dv^T = do^T P and dk^T = q^T dS.
 constexpr int BD_WORDS = 64;                // tiles of queries looked through at a time
 
 // What a workgroup of the dk / dv kernel has: its block, its part of the queries that picked it, in order
@@ -1054,7 +1062,7 @@ __device__ __forceinline__ void ba_dkv_pass(const BaArgs &a, const BaKeys &w, co
     typedef typename hd_vec<T>::v8 V8;
     constexpr bool HALF = __is_same(T, _Float16);
     T *Qs = (T *)smem, *Gs = (T *)(smem + L::TILE);
-    float *top_s = (float *)(smem + 2 * L::TILE), *shift_s = top_s + 64, *delta_s = shift_s + 64;
+    float *top_s = (float *)(smem + 2 * L::TILE), *by_s = top_s + 64, *delta_s = by_s + 64;
     int *limit_s = (int *)(delta_s + 64), *list = limit_s + 64;              // list: BD_WORDS * 64 queries
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
     int skip = w.skip, take = w.take;
@@ -1065,7 +1073,7 @@ __device__ __forceinline__ void ba_dkv_pass(const BaArgs &a, const BaKeys &w, co
 
     typedef BaStage<T, DP> S;
     S qr, gr;
-    float row_top = 0.f, row_shift = 0.f, row_delta = 0.f;
+    float row_top = 0.f, row_by = 0.f, row_delta = 0.f;
     int row_limit = 0;
     const T *Q = S::lane((const T *)a.q.data + w.b * a.q.sb + (int64_t)w.h * a.group * a.q.sh, a.d);
     const T *G = S::lane((const T *)a.go.data + w.b * a.go.sb + (int64_t)w.h * a.group * a.go.sh, a.d);
@@ -1080,12 +1088,12 @@ __device__ __forceinline__ void ba_dkv_pass(const BaArgs &a, const BaKeys &w, co
             qr.r[x] = *(const V8 *)(Q + i * a.q.sr + e * a.q.sh);
             gr.r[x] = *(const V8 *)(G + i * a.go.sr + e * a.go.sh);
         }
-        row_top = row_shift = row_delta = 0.f;
+        row_top = row_by = row_delta = 0.f;
         row_limit = 0;
         if (threadIdx.x < BA_ROWS && r0 + (int)threadIdx.x < rows) {
             const int r = r0 + threadIdx.x, q = r / a.group, head = w.h * a.group + (r - q * a.group), i = list[q];
             const int64_t p = ((int64_t)w.b * a.hq + head) * a.m + i;
-            row_top = a.lse[2 * p], row_shift = a.row[2 * p], row_delta = a.row[2 * p + 1];
+            row_top = a.lse[2 * p], row_by = a.row[2 * p], row_delta = a.row[2 * p + 1];
             row_limit = ba_limit(a, w.live, w.lm, i);
         }
     };
@@ -1126,7 +1134,7 @@ __device__ __forceinline__ void ba_dkv_pass(const BaArgs &a, const BaKeys &w, co
                 gr.store(Gs);
             }
             if (threadIdx.x < BA_ROWS) {
-                top_s[threadIdx.x] = row_top, shift_s[threadIdx.x] = row_shift;
+                top_s[threadIdx.x] = row_top, by_s[threadIdx.x] = row_by;
                 delta_s[threadIdx.x] = row_delta, limit_s[threadIdx.x] = row_limit;
             }
             __syncthreads();
@@ -1147,7 +1155,7 @@ __device__ __forceinline__ void ba_dkv_pass(const BaArgs &a, const BaKeys &w, co
                         ga[kk] = L::row8(Gs, j * 32 + x * 16 + l15, kk * 4 + g);
                     }
                     const int r4 = j * 32 + x * 16 + g * 4;
-                    const hd_f4 to = *(const hd_f4 *)(top_s + r4), sh = *(const hd_f4 *)(shift_s + r4), de = *(const hd_f4 *)(delta_s + r4);
+                    const hd_f4 to = *(const hd_f4 *)(top_s + r4), by = *(const hd_f4 *)(by_s + r4), de = *(const hd_f4 *)(delta_s + r4);
                     const int4 li = *(const int4 *)(limit_s + r4);
                     const int lim[4] = {li.x, li.y, li.z, li.w};
                     ba_issue();
@@ -1160,7 +1168,7 @@ __device__ __forceinline__ void ba_dkv_pass(const BaArgs &a, const BaKeys &w, co
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const bool see = w.key < lim[r];
-                        const float e = ba_power<T>(a, s[r] - to[r], sh[r]);
+                        const float e = ba_probability<T>(a, s[r], to[r], by[r]);
                         const float f = e * (dp[r] - de[r]);
                         p[x][r] = see ? e : 0.f;
                         ds[x][r] = see ? f : 0.f;

@@ -588,8 +588,9 @@ size_t tpu3_block_select_workspace_bytes(int b, int m, int n, int hk, int count)
 /* out (b, m, q->heads, d) contiguous = softmax(scale q k^T) v over the live keys of the blocks (b, m, k->heads, count) that a
  * query names (shared by the heads of a group; an index outside the live blocks, or behind what the query may see, counts
  * for nothing, one named twice counts once); a row that sees nothing: 0.  For the backward pass, or NULL: lse
- * (b, q->heads, m, 2) f32, 8-byte aligned, a row's largest score (not scaled) and minus log2 of its sum of exp(scale (score -
- * largest)) (0 and -infinity: no weights), and rest, like out, what the rounding of a 16-bit out took (fp16: times 2^11).
+ * (b, q->heads, m, 2) f32, 8-byte aligned, a row's largest score (not scaled) and, of its sum of exp(scale (score - largest)), in
+ * fp32 the reciprocal, in the 16-bit types minus the log2 (no weights: infinity and 0; 0 and -infinity), and rest, like out, what
+ * the rounding of a 16-bit out took (fp16: times 2^11).
  * q->heads / k->heads <= 64, d <= 128; workspace = tpu3_block_attn_fwd_workspace_bytes bytes, 16-byte aligned (0: NULL). */
 int tpu3_block_attn_fwd(tpu3_stream_t stream, int type, int b, int m, int n, int d, const tpu3_heads *q, const tpu3_heads *k,
                         const tpu3_heads *v, const int32_t *blocks, int count, double scale, const int32_t *n_arr,

@@ -324,3 +324,57 @@ def test_from_two_threads(dev):
     for t in threads:
         t.join()
     assert not wrong
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("m,n,hq,hk,d,causal", [(200, 300, 4, 2, 64, False), (150, 150, 2, 2, 128, True), (100, 500, 3, 1, 24, False)])
+def test_large_scores_that_are_rounded(dev, dtype, m, n, hq, hk, d, causal):
+    """Random scores of 2^29 (fp16) to 2^62: the passes over queries and over keys form the same rounded scores, so that the largest
+    key's probability is 1 in all of them: the output is its value, dv the sum of the gradients of the rows that chose it."""
+    ops = pkg("network.operations")
+    gen = torch.Generator(device=dev).manual_seed(7)
+    dt = TYPES[dtype]
+    big = 2.0 ** (12 if dt == torch.float16 else 30)
+    q, k = (big * _randn(gen, 1, m, hq, d)).to(dt), (big * _randn(gen, 1, n, hk, d)).to(dt)
+    v = torch.randint(-8, 9, (1, n, hk, d), device=dev, generator=gen).to(dt)
+    go = torch.randint(-1, 2, (1, m, hq, d), device=dev, generator=gen).to(dt)
+    blocks = torch.arange(-(-n // 64), dtype=torch.int32, device=dev).expand(1, m, hk, -1)
+    o, _, _, dv = _run(ops, (q, k, v), go, blocks, 1.0, causal=causal)
+    x = q.double().transpose(1, 2) @ k.double().transpose(1, 2).transpose(2, 3).contiguous().repeat_interleave(hq // hk, dim=1)
+    if causal:
+        x = torch.where(torch.arange(n, device=dev) <= torch.arange(m, device=dev)[:, None], x, torch.full_like(x, -math.inf))
+    two, best = x.topk(2, dim=3) if not causal else x[:, :, 1:].topk(2, dim=3)
+    # d + 8 roundings of at most d big^2 16 in both scores: the nearest two keys of a row are further apart than that
+    assert ((two[..., 0] - two[..., 1]) > 2 * (d + 8) * 2.0 ** -24 * d * 16 * big * big).float().mean() > 0.99
+    sure = (two[..., 0] - two[..., 1]) > 2 * (d + 8) * 2.0 ** -24 * d * 16 * big * big                          # (1,Hq,M)
+    if causal:
+        best = torch.cat((torch.zeros_like(best[:, :, :1]), best), dim=2)
+        sure = torch.cat((torch.ones_like(sure[:, :, :1]), sure), dim=2)
+    best = best[..., 0]
+    for h in range(hq):
+        want = v[0, best[0, h], h // (hq // hk)]
+        assert torch.equal(o[0, sure[0, h], h], want[sure[0, h]])
+    if bool(sure.all()):
+        want = torch.zeros((1, n, hk, d), device=dev, dtype=torch.float64)
+        for h in range(hq):
+            want[0, :, h // (hq // hk)].index_add_(0, best[0, h], go[0, :, h].double())
+        assert torch.equal(dv.double(), want)
+    assert torch.isfinite(dv).all()
+
+
+@pytest.mark.parametrize("b,m,n,hq,hk,d,count,causal", [(3, 400, 700, 2, 2, 24, 3, False), (2, 300, 1024, 4, 2, 64, 6, False),
+                                                        (1, 600, 600, 6, 2, 128, 4, True)])
+def test_errors_of_fp32(dev, b, m, n, hq, hk, d, count, causal):
+    """Both forms round every score, difference, exponential, product and sum in fp32, the kernels a probability twice (its power, its
+    quotient): the errors are of one size.  (With the log2 of the sum inside the exponent, half a step of 8 is a probability's whole
+    error and more: gradients off by 1.9 times the plain form's.)"""
+    ops = pkg("network.operations")
+    q, k, v, go, blocks = _inputs(dev, b, m, n, hq, hk, d, count, torch.float32, 11)
+    if causal:
+        blocks[..., 0] = 0
+    want = _formula(q, k, v, blocks, d ** -0.5, causal, go, torch.float64)
+    plain = _formula(q, k, v, blocks, d ** -0.5, causal, go, torch.float32)
+    for name, x, y, z in zip(("o", "dq", "dk", "dv"), _run(ops, (q, k, v), go, blocks, causal=causal), plain, want):
+        here, there = _error(x, z), _error(y, z)
+        print("%s: %.3g, plain %.3g" % (name, here, there))
+        assert here <= 1.5 * there, (name, here, there)
