@@ -378,3 +378,38 @@ def test_errors_of_fp32(dev, b, m, n, hq, hk, d, count, causal):
         here, there = _error(x, z), _error(y, z)
         print("%s: %.3g, plain %.3g" % (name, here, there))
         assert here <= 1.5 * there, (name, here, there)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("kind", ["places", "coordinates"])
+def test_errors_of_fp32_rotations(dev, kind, interleaved):
+    """Against the plain form: angles, cosines and sines in 64 bits, everything else in fp32.  The kernel rounds its cosines and sines
+    as the plain form does (a turn's last bits behind fp32 go in to first order), its products once less: the errors are of one
+    size.  (With the turn alone in fp32 the angle was off by up to 2 pi 2^-26: outputs by 1.2 times the plain form's.)"""
+    ops = pkg("network.operations")
+    gen = torch.Generator(device=dev).manual_seed(9)
+    b, n, h, d = 2, 900, 4, 64
+    x, g, w = _randn(gen, b, n, h, d).requires_grad_(), _randn(gen, b, n, h, d), 1 + 0.2 * _randn(gen, d)
+    if kind == "places":
+        pos, freq = torch.randint(0, 100000, (b, n), device=dev, generator=gen), ops.rotation_frequencies(1, 32, device=dev)
+    else:
+        pos, freq = _randn(gen, b, n, 3), 2.0 ** torch.arange(10, device=dev, dtype=torch.float64).mul(0.6).repeat(3, 1)
+    y, _ = ops.norm_rotate(x, None, w, None, pos, freq, interleaved=interleaved)
+    dx, = torch.autograd.grad(y, x, g)
+    ref = orc64.norm_rotate(x, w, pos, freq, 1e-6, interleaved, g)
+    p = pos.double() if pos.dim() == 3 else pos.double().unsqueeze(2)
+    a = (p.unsqueeze(3) * freq).flatten(2).unsqueeze(2)
+    c, s, r = torch.cos(a).float(), torch.sin(a).float(), a.size(3)
+
+    def turn(t, s):
+        one, two = (t[..., 0:2 * r:2], t[..., 1:2 * r:2]) if interleaved else (t[..., :r], t[..., r:2 * r])
+        pair = one * c - two * s, one * s + two * c
+        return torch.cat((torch.stack(pair, dim=4).flatten(3) if interleaved else torch.cat(pair, dim=3), t[..., 2 * r:]), dim=3)
+    xf = x.detach()
+    inv = torch.rsqrt((xf * xf).mean(dim=3, keepdim=True) + 1e-6)
+    unit, back = xf * inv, turn(g, -s) * w
+    for name, got, plain, want in (("y", y, turn(unit * w, s), ref["y"]),
+                                   ("dx", dx, inv * (back - unit * (back * unit).mean(dim=3, keepdim=True)), ref["dx"])):
+        here, there = _error(got, want), _error(plain, want)
+        print("%s: %.3g, plain %.3g" % (name, here, there))
+        assert here <= 1.1 * there, (name, here, there)
