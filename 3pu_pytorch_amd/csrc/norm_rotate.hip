@@ -82,9 +82,9 @@ __device__ __forceinline__ void nr_turns(const NrArgs &a, int64_t t0, int count,
         sincospif(2.f * (float)turn, &s, &c);
         // what the rounding of the turn took, to first order: an angle of up to 2 pi 2^-26 (fp32 outputs off by 7.8e-8 without it,
         // 7.0e-8 with it; the plain form 6.5e-8)
-        const float rest = 6.2831853f * (float)(turn - (double)(float)turn), s0 = s;
-        s = __builtin_fmaf(c, rest, s);
-        c = __builtin_fmaf(-s0, rest, c);
+        const float more = 6.2831853f * (float)(turn - (double)(float)turn), s0 = s;
+        s = __builtin_fmaf(c, more, s);
+        c = __builtin_fmaf(-s0, more, c);
         const int one = a.interleaved ? 2 * p : p, two = a.interleaved ? 2 * p + 1 : p + P;
         float *C = cs + t * 2 * a.d, *S = C + a.d;
         C[one] = C[two] = c;
